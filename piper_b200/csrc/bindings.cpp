@@ -415,6 +415,7 @@ int64_t attn_bwd_parts(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t sm
 
 #include "bindings_moe.inc"
 #include "bindings_fused.inc"
+#include "bindings_tuning.inc"
 #include "bindings_ops.inc"
 
 TORCH_LIBRARY(piper_c, m) {
@@ -450,5 +451,6 @@ TORCH_LIBRARY(piper_c, m) {
   m.def("attn_bwd_floats", &attn_bwd_floats);
   register_moe_ops(m);
   register_fused_ops(m);
+  register_tuning_ops(m);
   register_native_ops(m);
 }

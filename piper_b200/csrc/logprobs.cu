@@ -1,0 +1,494 @@
+// Log probabilities of given tokens, the entropy and the most probable alternatives of every row of logits, and their
+// gradient.  With z = x / temperature, M = max x, S = sum exp((x - M) / temperature):
+//
+//   log p_j = (x_j - M) / temperature - log S
+//   H       = log S - sum_j exp((x_j - M) / temperature) (x_j - M) / temperature / S
+//   dx_j    = [ g_j - p_j (sum_i g_i + dH (log p_j + H)) ] / temperature
+//
+// where g is the gradient of the log probabilities: of the token's and of the alternatives', zero elsewhere.  M and log S
+// are kept apart for the backward pass: their sum would lose the digits that small differences of logits are in.
+#include "logprobs.h"
+
+#include <cuda_bf16.h>
+
+#include <cfloat>
+#include <cmath>
+#include <cstdint>
+
+#include "ptx.cuh"
+
+namespace piper {
+namespace {
+
+constexpr int THREADS = 512;
+constexpr int WARPS = THREADS / 32;
+constexpr int MAX_PARTS = 8;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FAR_BELOW = -1e30f;      // in place of -inf behind a subtraction: exp() of it is 0, and so is 0 times it
+
+template <class T>
+constexpr int VEC = 16 / sizeof(T);
+
+// NaN where one of the two is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x to two units of the last place; results below the normal numbers are 0.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_float(float v, float& o) { o = v; }
+__device__ __forceinline__ void from_float(float v, __nv_bfloat16& o) { o = __float2bfloat16(v); }
+
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[4], float) {
+  f[0] = __uint_as_float(u.x);
+  f[1] = __uint_as_float(u.y);
+  f[2] = __uint_as_float(u.z);
+  f[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[8], __nv_bfloat16) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[4], float) {
+  return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&f)[8], __nv_bfloat16) {
+  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+}
+
+// ------------------------------------------------------------------ running maximum and sums
+// s = sum exp((x - m) / temperature), t = sum exp((x - m) / temperature) (x - m); every term of t has one sign, so the entropy
+// is a sum without cancellation.  m is -inf until something finite has come; `from` is what is subtracted.
+struct Sums {
+  float m, from, s, t;
+
+  __device__ __forceinline__ static Sums none() { return {-INFINITY, -FLT_MAX, 0.f, 0.f}; }
+
+  __device__ __forceinline__ void raise(float to, float c2) {
+    const float base = fmaxf(to, -FLT_MAX);
+    const float d = max_nan(from - base, FAR_BELOW), f = ex2(d * c2);
+    t = f * fmaf(s, d, t);
+    s *= f;
+    m = to;
+    from = base;
+  }
+  __device__ __forceinline__ void add(float x, float c2) {
+    const float d = max_nan(x - from, FAR_BELOW), w = ex2(d * c2);
+    s += w;
+    t = fmaf(w, d, t);
+  }
+  __device__ __forceinline__ void merge(const Sums& o, float c2) {
+    if (o.m > m) raise(o.m, c2);
+    const float d = max_nan(o.from - from, FAR_BELOW), f = ex2(d * c2);
+    s = fmaf(f, o.s, s);
+    t = fmaf(f, fmaf(o.s, d, o.t), t);
+  }
+};
+
+// ------------------------------------------------------------------ the largest of many keys
+// Value and index of an element as one integer that grows with the value and, among equal values, with a falling index, so no two
+// elements of a row have the same key and the order of ties is the order of ids.  0 is below every key.  A NaN counts as
+// -inf here (its row has no numbers to report anyway); -0 and 0 are equal.
+__device__ __forceinline__ uint64_t make_key(float x, uint32_t index) {
+  const float v = x == x ? x + 0.f : -INFINITY;
+  const uint32_t b = __float_as_uint(v);
+  const uint32_t ordered = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+  return static_cast<uint64_t>(ordered) << 32 | (0xFFFFFFFFu - index);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t o = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xFFFFFFFFu - static_cast<uint32_t>(k); }
+
+// One compare-exchange step of a bitonic network over the warp: lanes `mask` apart, the larger key to the lane whose bit of
+// `up` is clear.
+__device__ __forceinline__ uint64_t exchange(uint64_t k, int mask, bool larger) {
+  const uint64_t o = __shfl_xor_sync(0xffffffffu, k, mask);
+  return (k > o) == larger ? k : o;
+}
+
+// The warp's keys, falling by lane.
+__device__ __forceinline__ uint64_t sort_falling(uint64_t k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int mask = size / 2; mask > 0; mask /= 2) k = exchange(k, mask, ((lane & mask) == 0) == ((lane & size) == 0 || size == 32));
+  return k;
+}
+
+// The 32 largest of two falling lists, falling: lane by lane the larger of one list and the other reversed are they, first
+// rising and then falling or the other way round, which five exchanges put in order.
+__device__ __forceinline__ uint64_t merge_falling(uint64_t a, uint64_t b, int lane) {
+  const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  uint64_t k = a > r ? a : r;
+#pragma unroll
+  for (int mask = 16; mask > 0; mask /= 2) k = exchange(k, mask, (lane & mask) == 0);
+  return k;
+}
+
+// A key into a falling list, its last one out.
+__device__ __forceinline__ uint64_t insert_falling(uint64_t list, uint64_t key, int lane) {
+  const int at = __popc(__ballot_sync(0xffffffffu, list > key));
+  const uint64_t before = __shfl_up_sync(0xffffffffu, list, 1);
+  return lane < at ? list : lane == at ? key : before;
+}
+
+// The 32 largest of the lists of `n` warps (a power of two), in lists[0]; every thread of the CTA calls it with its own.
+__device__ __forceinline__ void merge_lists(uint64_t own, uint64_t (*lists)[32], int n, int warp, int lane) {
+  lists[warp][lane] = own;
+  for (int half = n / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (warp < half) {
+      own = merge_falling(own, lists[warp + half][lane], lane);
+      lists[warp][lane] = own;
+    }
+  }
+  __syncthreads();
+}
+
+struct Shared {
+  Sums sums[WARPS];
+  Sums parts[MAX_PARTS];
+  uint64_t lists[WARPS][32];
+  uint64_t part_lists[MAX_PARTS][32];
+};
+
+__device__ __forceinline__ void merge_lanes(Sums& v, float c2) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Sums w;
+    w.m = __shfl_xor_sync(0xffffffffu, v.m, o);
+    w.from = __shfl_xor_sync(0xffffffffu, v.from, o);
+    w.s = __shfl_xor_sync(0xffffffffu, v.s, o);
+    w.t = __shfl_xor_sync(0xffffffffu, v.t, o);
+    v.merge(w, c2);
+  }
+}
+
+// Where a part of a row begins, how many single elements stand in front of its first 16-byte boundary, how many vectors and
+// single elements follow.  Thread i takes single element i of the head and of the tail, and vectors i, i + THREADS, ...
+struct Span {
+  long long first;       // element of the row
+  int head, vecs, tail;
+
+  template <class T>
+  __device__ __forceinline__ static Span of(const T* row, int V, int part, int parts) {
+    const int len = ((V + parts - 1) / parts + 63) / 64 * 64;
+    const long long lo = static_cast<long long>(part) * len, hi = min(static_cast<long long>(V), lo + len);
+    const int n = hi > lo ? static_cast<int>(hi - lo) : 0;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row + lo) & 15u) / static_cast<int>(sizeof(T));
+    Span s;
+    s.first = lo;
+    s.head = min(n, (VEC<T> - off) % VEC<T>);
+    s.vecs = (n - s.head) / VEC<T>;
+    s.tail = n - s.head - s.vecs * VEC<T>;
+    return s;
+  }
+};
+
+// One CTA per row, or a cluster of `parts` CTAs where there are few rows, whose sums and lists meet in the shared memory of the
+// first.  One pass over the row: every thread keeps the running sums of its elements and the place of its largest.  For
+// the alternatives, the top-th largest of the threads' largest keys is a bound that at least so many elements reach; the elements
+// that reach it belong to the `top` threads whose largest does, so only those threads' elements, a 512th of the row each, are looked
+// at again.
+template <class T, bool TOP>
+__global__ void __launch_bounds__(THREADS, 2)
+logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
+                    float* __restrict__ entropy, float* __restrict__ top_logprob, long long* __restrict__ top_id,
+                    float* __restrict__ stats, int V, long long ld, long long ignore_index, int top, int parts, float inv_t) {
+  if (parts > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  grid_begin(logits, tokens);
+  __shared__ Shared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = blockIdx.x / parts;
+  const int part = static_cast<int>(blockIdx.x - row * parts);
+  const T* x = logits + row * ld;
+  const Span sp = Span::of(x, V, part, parts);
+  const T* head = x + sp.first;
+  const T* body = head + sp.head;
+  const T* tail = body + static_cast<long long>(sp.vecs) * VEC<T>;
+  const float c2 = inv_t * LOG2E;
+
+  Sums v = Sums::none();
+  uint32_t place = 0;                  // of the thread's largest; behind an -inf, of its first element
+  bool any = false;
+  auto single = [&](const T* p) {
+    const float f = to_float(*p);
+    if (f > v.m) {
+      v.raise(f, c2);
+      place = static_cast<uint32_t>(p - x);
+    } else if (!any) {
+      place = static_cast<uint32_t>(p - x);
+    }
+    any = true;
+    v.add(f, c2);
+  };
+  if (static_cast<int>(threadIdx.x) < sp.head) single(head + threadIdx.x);
+  constexpr int AHEAD = 4;
+  for (int i = threadIdx.x; i < sp.vecs; i += AHEAD * THREADS) {
+    uint4 u[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (i + j * THREADS < sp.vecs) u[j] = __ldcs(reinterpret_cast<const uint4*>(body) + i + j * THREADS);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (i + j * THREADS >= sp.vecs) break;
+      float f[VEC<T>];
+      unpack(u[j], f, T());
+      float lm = f[0];
+#pragma unroll
+      for (int q = 1; q < VEC<T>; ++q) lm = fmaxf(lm, f[q]);
+      if (lm > v.m || (TOP && !any)) {
+        if (TOP) {
+          const uint32_t at = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(i + j * THREADS) * VEC<T>;
+          int q0 = 0;
+          if (lm > v.m)
+#pragma unroll
+            for (int q = VEC<T> - 1; q >= 0; --q)
+              if (f[q] == lm) q0 = q;
+          place = at + q0;
+          any = true;
+        }
+        if (lm > v.m) v.raise(lm, c2);
+      }
+#pragma unroll
+      for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
+    }
+  }
+  if (static_cast<int>(threadIdx.x) < sp.tail) single(tail + threadIdx.x);
+  const uint64_t mine = TOP && any ? make_key(v.m, place) : 0;
+
+  merge_lanes(v, c2);
+  if (lane == 0) sh.sums[warp] = v;
+
+  uint64_t list = 0;
+  if (TOP) {
+    merge_lists(sort_falling(mine, lane), sh.lists, WARPS, warp, lane);
+    const uint64_t largest = sh.lists[0][lane];
+    const uint64_t bound = __shfl_sync(0xffffffffu, largest, top - 1);
+    __syncthreads();                   // the lists are read before they are written again
+    for (int o = warp; o < top; o += WARPS) {
+      const uint64_t k = __shfl_sync(0xffffffffu, largest, o);
+      if (k == 0) break;               // fewer threads than that have elements
+      const int rel = static_cast<int>(static_cast<long long>(key_index(k)) - sp.first);
+      const int owner = rel < sp.head ? rel
+                        : rel < sp.head + sp.vecs * VEC<T> ? (rel - sp.head) / VEC<T> % THREADS
+                                                           : rel - sp.head - sp.vecs * VEC<T>;
+      auto offer = [&](bool has, float f, uint32_t index) {
+        const uint64_t key = has ? make_key(f, index) : 0;
+        unsigned waiting = __ballot_sync(0xffffffffu, key >= bound && key != 0);
+        while (waiting != 0) {
+          const int from = __ffs(waiting) - 1;
+          waiting &= waiting - 1;
+          list = insert_falling(list, __shfl_sync(0xffffffffu, key, from), lane);
+        }
+      };
+      const bool at_head = lane == 0 && owner < sp.head, at_tail = lane == 1 && owner < sp.tail;
+      const T* s = at_head ? head + owner : tail + owner;
+      offer(at_head || at_tail, at_head || at_tail ? to_float(*s) : 0.f, static_cast<uint32_t>(s - x));
+      for (int i0 = owner; i0 < sp.vecs; i0 += 32 * THREADS) {
+        const int i = i0 + lane * THREADS;
+        const bool has = i < sp.vecs;
+        float f[VEC<T>];
+        unpack(has ? reinterpret_cast<const uint4*>(body)[i] : make_uint4(0, 0, 0, 0), f, T());
+        const uint32_t at = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(i) * VEC<T>;
+#pragma unroll
+        for (int q = 0; q < VEC<T>; ++q) offer(has, f[q], at + q);
+      }
+    }
+    merge_lists(list, sh.lists, WARPS, warp, lane);
+    list = sh.lists[0][lane];
+  } else {
+    __syncthreads();
+  }
+  if (warp == 0) {
+    v = lane < WARPS ? sh.sums[lane] : Sums::none();
+    merge_lanes(v, c2);
+  }
+  if (parts > 1) {
+    // the sums and the list of every part into the first CTA of the cluster, which has started by now
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (warp == 0) {
+      const uint32_t sums = mapa_u32(smem_u32(&sh.parts[part]), 0);
+      if (lane == 0)
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(sums), "f"(v.m), "f"(v.from), "f"(v.s), "f"(v.t)
+                     : "memory");
+      if (TOP)
+        asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(mapa_u32(smem_u32(&sh.part_lists[part][lane]), 0)), "l"(list)
+                     : "memory");
+    }
+    cluster_sync();
+    if (part != 0 || warp != 0) return;
+    v = lane < parts ? sh.parts[lane] : Sums::none();
+    merge_lanes(v, c2);
+    if (TOP)
+      for (int p = 1; p < parts; ++p) list = merge_falling(list, sh.part_lists[p][lane], lane);
+  } else if (warp != 0) {
+    return;
+  }
+  const bool empty = v.s == 0.f;       // nothing left: every probability is 0
+  const float log_s = empty ? -INFINITY : logf(v.s);
+  auto log_p = [&](float f) { return empty ? -INFINITY : fmaf(f - v.from, inv_t, -log_s); };
+  if (lane == 0) {
+    const long long y = tokens[row];
+    const bool counted = y != ignore_index && y >= 0 && y < V;
+    logprob[row] = counted ? log_p(to_float(x[y])) : 0.f;
+    entropy[row] = empty ? 0.f : fmaf(-v.t / v.s, inv_t, log_s);
+    stats[2 * row] = v.from;
+    stats[2 * row + 1] = log_s;
+  }
+  if (TOP && lane < top) {
+    top_logprob[row * top + lane] = log_p(key_value(list));
+    top_id[row * top + lane] = key_index(list);
+  }
+}
+
+// dx of one part of a row by one CTA, then the elements of the token and of the alternatives again with their g.
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS, 2)
+logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, const float* __restrict__ stats,
+                    const float* __restrict__ entropy, const long long* __restrict__ top_id,
+                    const float* __restrict__ d_logprob, const float* __restrict__ d_entropy, const float* __restrict__ d_top,
+                    T* __restrict__ d, int V, long long ld, long long ignore_index, int top, int parts, float inv_t) {
+  grid_begin(logits, tokens, stats, entropy, top_id, d_logprob, d_entropy, d_top);
+  const long long row = blockIdx.x / parts;
+  const int part = static_cast<int>(blockIdx.x - row * parts);
+  const T* x = logits + row * ld;
+  T* o = d + row * V;
+  const Span sp = Span::of(x, V, part, parts);
+  const long long y = tokens[row];
+  const bool counted = y != ignore_index && y >= 0 && y < V;
+  const float from = stats[2 * row], log_s = stats[2 * row + 1], h = entropy[row];
+  const float gy = counted && d_logprob != nullptr ? d_logprob[row] : 0.f;
+  const float gh = d_entropy != nullptr ? d_entropy[row] : 0.f;
+  float g = gy;
+  if (d_top != nullptr)
+    for (int i = 0; i < top; ++i) g += d_top[row * top + i];
+  const bool empty = log_s == -INFINITY;
+  // dx = -exp(u) (a + b u) with u = log p
+  const float a = (g + gh * h) * inv_t, b = gh * inv_t;
+  auto grad = [&](float f) {
+    const float u = fmaf(max_nan(f - from, FAR_BELOW), inv_t, -log_s);
+    return empty ? 0.f : -ex2(u * LOG2E) * fmaf(b, u, a);
+  };
+  const long long begin = sp.first, end = begin + sp.head + static_cast<long long>(sp.vecs) * VEC<T> + sp.tail;
+  if (ALIGNED) {                       // x and o have the same offset to a 16-byte boundary
+    const long long body = begin + sp.head, tail = end - sp.tail;
+    const int t = threadIdx.x;
+    if (t < sp.head) from_float(grad(to_float(x[begin + t])), o[begin + t]);
+    if (t < sp.tail) from_float(grad(to_float(x[tail + t])), o[tail + t]);
+    constexpr int AHEAD = 4;
+    for (int i = t; i < sp.vecs; i += AHEAD * THREADS) {
+      uint4 u[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (i + j * THREADS < sp.vecs) u[j] = __ldcs(reinterpret_cast<const uint4*>(x + body) + i + j * THREADS);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i + j * THREADS >= sp.vecs) break;
+        float f[VEC<T>];
+        unpack(u[j], f, T());
+#pragma unroll
+        for (int q = 0; q < VEC<T>; ++q) f[q] = grad(f[q]);
+        __stcs(reinterpret_cast<uint4*>(o + body) + i + j * THREADS, pack(f, T()));
+      }
+    }
+  } else {
+    for (long long i = begin + threadIdx.x; i < end; i += THREADS) from_float(grad(to_float(x[i])), o[i]);
+  }
+  __syncthreads();
+  // the token may be one of the alternatives: whoever writes a place has all that belongs to it
+  const int who = static_cast<int>(threadIdx.x);
+  const int listed = d_top != nullptr ? top : 0;
+  if (who > listed || (who == listed && !counted) || empty) return;
+  auto id = [&](int i) { return i < listed ? top_id[row * top + i] : y; };
+  const long long at = id(who);
+  if (at < begin || at >= end) return;
+  float sum = 0.f;
+  for (int i = 0; i <= listed; ++i)
+    if (i < listed ? id(i) == at : counted && y == at) sum += i < listed ? d_top[row * top + i] : gy;
+  from_float(fmaf(sum, inv_t, grad(to_float(x[at]))), o[at]);
+}
+
+// CTAs per row: with fewer rows than SMs have room for, a row is cut into up to eight pieces of at least 4,096 elements.
+int row_parts(long long T, int V, int num_sms) {
+  int parts = 1;
+  while (parts < MAX_PARTS && T * parts * 2 <= 2ll * num_sms && V / (parts * 2) >= 4096) parts *= 2;
+  return parts;
+}
+
+template <class... P, class... A>
+int launch_clusters(void (*kernel)(P...), long long grid, int cluster, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...) == cudaSuccess ? 0 : -3;
+}
+
+template <class T>
+int fwd(const LogprobArgs& a, float* logprob, float* entropy, float* top_logprob, long long* top_id, float* stats, int num_sms,
+        cudaStream_t st) {
+  const int parts = row_parts(a.T, a.V, num_sms);
+  auto kernel = a.top > 0 ? logprobs_fwd_kernel<T, true> : logprobs_fwd_kernel<T, false>;
+  return launch_clusters(kernel, a.T * parts, parts, st, static_cast<const T*>(a.logits), a.tokens, logprob, entropy, top_logprob,
+                         top_id, stats, a.V, a.ld, a.ignore_index, a.top, parts, a.inv_temperature);
+}
+
+template <class T>
+int bwd(const LogprobArgs& a, const float* stats, const float* entropy, const long long* top_id, const float* d_logprob,
+        const float* d_entropy, const float* d_top, void* d, int num_sms, cudaStream_t st) {
+  const int parts = row_parts(a.T, a.V, num_sms);
+  const uintptr_t apart = reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(d);
+  const bool aligned = (apart & 15u) == 0 && (a.T <= 1 || (a.ld - a.V) * sizeof(T) % 16 == 0);
+  auto kernel = aligned ? logprobs_bwd_kernel<T, true> : logprobs_bwd_kernel<T, false>;
+  return launch_clusters(kernel, a.T * parts, 1, st, static_cast<const T*>(a.logits), a.tokens, stats, entropy, top_id, d_logprob,
+                         d_entropy, d_top, static_cast<T*>(d), a.V, a.ld, a.ignore_index, a.top, parts, a.inv_temperature);
+}
+
+bool sound(const LogprobArgs& a) {
+  return a.T >= 0 && a.T <= (1ll << 27) && a.V > 0 && a.top >= 0 && a.top <= kMaxTopTokens && a.top <= a.V;
+}
+
+}  // namespace
+
+int logprobs_fwd(const LogprobArgs& a, float* logprob, float* entropy, float* top_logprob, long long* top_id, float* stats,
+                 int num_sms, cudaStream_t st) {
+  if (!sound(a)) return -1;
+  if (a.T == 0) return 0;
+  return a.f32 ? fwd<float>(a, logprob, entropy, top_logprob, top_id, stats, num_sms, st)
+               : fwd<__nv_bfloat16>(a, logprob, entropy, top_logprob, top_id, stats, num_sms, st);
+}
+
+int logprobs_bwd(const LogprobArgs& a, const float* stats, const float* entropy, const long long* top_id,
+                 const float* d_logprob, const float* d_entropy, const float* d_top, void* d, int num_sms, cudaStream_t st) {
+  if (!sound(a)) return -1;
+  if (a.T == 0) return 0;
+  return a.f32 ? bwd<float>(a, stats, entropy, top_id, d_logprob, d_entropy, d_top, d, num_sms, st)
+               : bwd<__nv_bfloat16>(a, stats, entropy, top_id, d_logprob, d_entropy, d_top, d, num_sms, st);
+}
+
+}  // namespace piper

@@ -14,8 +14,9 @@ from .core import (
     swiglu,
     wgrad_store,
 )
+from .logprobs import TokenLogprobs, token_logprobs
 
 __all__ = [
     "native", "linear", "rmsnorm", "add_rmsnorm", "qk_rope", "residual_add", "rope_tables", "attention", "swiglu",
-    "embedding", "cross_entropy", "grad_sinks", "wgrad_store",
+    "embedding", "cross_entropy", "token_logprobs", "TokenLogprobs", "grad_sinks", "wgrad_store",
 ]

@@ -1,0 +1,280 @@
+"""Log probabilities of tokens, entropy and alternatives against their definition in 64 bits.
+
+Tolerances.  Sums run over a thread's V / 512 elements (all V in a plain sum on the CPU) and about twenty merges; a term's
+relative error is a few 2^-23 and that of its exponent.  So log S is off by less than 2^-24 (depth + 40), a log probability by
+that and three roundings of its own size, the entropy by the same relative to its largest term.  A gradient is
+-p (a + b log p), whose two addends may cancel: its error is 2^-20 of their absolute sum, and half a step of its type."""
+import math
+
+import pytest
+import torch
+
+from piper_b200 import ops
+
+INF = float("inf")
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _definition(x, tokens, top, temperature, ignore_index=-100):
+    """In 64 bits, row by row of the formulas; ids by sorting (value falling, id rising)."""
+    x = x.detach().double().cpu()
+    tokens = tokens.cpu()
+    V = x.shape[-1]
+    left = torch.isfinite(x).any(-1, keepdim=True)
+    z = torch.where(left, x - x.amax(-1, keepdim=True), x) / temperature
+    logp = torch.where(left, z - torch.logsumexp(z, -1, keepdim=True), torch.full_like(z, -INF))
+    p = logp.exp()
+    H = -torch.where(p > 0, p * logp, torch.zeros_like(p)).sum(-1)
+    on = (tokens != ignore_index) & (tokens >= 0) & (tokens < V)
+    lp = torch.where(on, logp.gather(-1, tokens.clamp(0, V - 1).unsqueeze(-1)).squeeze(-1), 0.0)
+    ids = torch.sort(x, dim=-1, descending=True, stable=True).indices[..., :top]
+    return logp, p, H, on, lp, ids, left
+
+
+def _gradient(x, tokens, top, temperature, dlp, dH, dtop):
+    logp, p, H, on, _lp, ids, left = _definition(x, tokens, top, temperature)
+    up = torch.zeros_like(p)
+    V = p.shape[-1]
+    up.scatter_add_(-1, tokens.cpu().clamp(0, V - 1).unsqueeze(-1), (dlp.double().cpu() * on).unsqueeze(-1))
+    if top:
+        up.scatter_add_(-1, ids, dtop.double().cpu())
+    u = torch.where(p > 0, logp, torch.zeros_like(p))
+    dh = dH.double().cpu().unsqueeze(-1)
+    g = up.sum(-1, keepdim=True)
+    d = (up - p * g - dh * p * (u + H.unsqueeze(-1))) / temperature
+    size = (up.abs() + p * (up.abs().sum(-1, keepdim=True) + dh.abs() * (u.abs() + H.unsqueeze(-1)))) / temperature
+    return torch.where(left, d, torch.zeros_like(d)), size
+
+
+def _check(x, tokens, top, temperature, out, d=None, gradients=None):
+    V = x.shape[-1]
+    eps = 2.0 ** -24
+    depth = (V if not x.is_cuda else V / 512 + 20) + 40
+    logp, p, H, on, lp, ids, left = _definition(x, tokens, top, temperature)
+    row = eps * depth
+
+    def close(got, want, tol):
+        got = got.double().cpu()
+        same = (got == want) | ((got - want).abs() <= tol)
+        assert bool(same.all()), (got[~same][:5], want[~same][:5])
+
+    close(out.logprob, lp, row + 6 * eps * lp.abs().nan_to_num(posinf=0))
+    close(out.entropy, H, row * (1 + H) + 8 * eps * math.log(V + 1))
+    assert torch.equal(out.top_id.cpu(), ids)
+    want = logp.gather(-1, ids)
+    close(out.top_logprob, want, row + 6 * eps * want.abs().nan_to_num(posinf=0))
+    if d is not None:
+        want, size = _gradient(x, tokens, top, temperature, *gradients)
+        half = torch.finfo(x.dtype).eps / 2
+        tiny = torch.finfo(x.dtype).tiny
+        close(d, want, half * want.abs() + (2.0 ** -20 + 2 * row) * size + tiny)
+
+
+def _logits(T, V, dtype, device, seed, std=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(T, V, generator=g) * std).to(dtype)
+    tokens = torch.randint(0, V, (T,), generator=g)
+    return x.to(device), tokens.to(device)
+
+
+SHAPES = [(1, 1, 0), (1, 1, 1), (3, 7, 7), (2, 31, 20), (5, 33, 32), (4, 257, 5), (2, 4099, 32), (3, 8191, 3), (1, 128256, 20),
+          (2, 40000, 32), (300, 2048, 4), (40, 32003, 6), (0, 50, 3)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,top", SHAPES)
+def test_values_and_gradients(T, V, top, dtype, device):
+    for temperature in (1.0, 0.7):
+        x, tokens = _logits(T, V, dtype, device, 3 * T + V)
+        if T > 2:
+            tokens[1], tokens[2] = -100, V
+        x.requires_grad_(True)
+        out = ops.token_logprobs(x, tokens, top=top, temperature=temperature)
+        g = torch.Generator().manual_seed(5)
+        gradients = [torch.randn(s, generator=g).to(device) for s in ((T,), (T,), (T, top))]
+        (d,) = torch.autograd.grad([out.logprob, out.entropy, out.top_logprob], x, gradients)
+        assert d.dtype == dtype and d.shape == x.shape
+        _check(x, tokens, top, temperature, out, d, gradients)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [9, 600, 10007])
+def test_rows_that_are_special(V, dtype, device):
+    low = torch.finfo(dtype).min
+    x, tokens = _logits(8, V, dtype, device, V)
+    x[0] = -INF                                   # nothing left
+    x[1] = low                                    # all equal, at the type's lowest value
+    x[2] = low
+    x[2, V - 1] = 2.0                             # one token has all
+    x[3, ::2] = -INF
+    x[4] = -INF
+    x[4, V // 2] = -7.0                           # a single one left
+    x[5] = 0.0
+    x[5, 1::2] = -0.0                             # equal numbers of two signs
+    x[6] = x[6].round()                           # many ties
+    x[7, 0] = low
+    tokens[2], tokens[3], tokens[4] = 0, 0, V // 2
+    x.requires_grad_(True)
+    top = min(V, 8)
+    out = ops.token_logprobs(x, tokens, top=top)
+    gradients = [torch.ones(8, device=device), torch.full((8,), 0.5, device=device), torch.full((8, top), 0.1, device=device)]
+    (d,) = torch.autograd.grad([out.logprob, out.entropy, out.top_logprob], x, gradients)
+    assert bool(torch.isfinite(d).all())
+    _check(x, tokens, top, 1.0, out, d, gradients)
+    assert out.entropy[0] == 0 and out.logprob[0] == -INF and not d[0].any()
+    assert out.top_id[0].tolist() == list(range(top))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_without_numbers_are_nan(device):
+    for bad in (float("nan"), INF):
+        x, tokens = _logits(3, 700, torch.float32, device, 1)
+        x[1, 300] = bad
+        out = ops.token_logprobs(x, tokens, top=3)
+        for t in (out.logprob, out.entropy, out.top_logprob):
+            assert bool(torch.isnan(t[1]).all()) and not bool(torch.isnan(t[0]).any()) and not bool(torch.isnan(t[2]).any())
+        assert bool((out.top_id >= 0).all()) and bool((out.top_id < 700).all())
+        assert len(set(out.top_id[1].tolist())) == 3
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_largest_values_in_one_threads_elements(device):
+    """The alternatives all at one place of the pattern in which threads take vectors, and in an order that keeps replacing them."""
+    V = 65536
+    for dtype, vec in ((torch.bfloat16, 8), (torch.float32, 4)):
+        x = torch.zeros(1, V, dtype=dtype, device=device)
+        at = torch.arange(0, V, 512 * vec, device=device)
+        x[0, at] = torch.arange(1, len(at) + 1, device=device).to(dtype)
+        x[0, at + 1] = torch.arange(1, len(at) + 1, device=device).to(dtype)
+        tokens = torch.zeros(1, dtype=torch.int64, device=device)
+        _check(x, tokens, 20, 1.0, ops.token_logprobs(x, tokens, top=20))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_strides_offsets_and_shapes(device):
+    base = torch.randn(6, 1003, generator=torch.Generator().manual_seed(2)).to(device)
+    for dtype in (torch.bfloat16, torch.float32):
+        wide = base.to(dtype)
+        tokens = torch.tensor([0, 5, 900, -100, 1, 2], device=device)
+        for x in (wide[:, 1:], wide[:, 3:904], wide[:, :1000], wide.t().contiguous().t(), wide[:, 17:18].expand(6, 40)):
+            leaf = x.detach().requires_grad_(True)
+            out = ops.token_logprobs(leaf, tokens, top=4)
+            _check(x, tokens, 4, 1.0, out)
+            (d,) = torch.autograd.grad(out.logprob.sum(), leaf)
+            want, size = _gradient(x, tokens, 0, 1.0, torch.ones(6), torch.zeros(6), torch.zeros(6, 0))
+            assert bool(((d.double().cpu() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2 ** -18 * size).all())
+    x = base.view(2, 3, 1003)
+    out = ops.token_logprobs(x, tokens.view(2, 3), top=2)
+    assert out.logprob.shape == (2, 3) and out.top_id.shape == (2, 3, 2)
+    one = ops.token_logprobs(base[0], tokens[0], top=2)
+    assert one.logprob.shape == () and torch.equal(one.top_id, out.top_id[0, 0])
+    assert torch.equal(one.logprob, out.logprob[0, 0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_that_do_not_arrive(device):
+    x, tokens = _logits(4, 500, torch.float32, device, 9)
+    x.requires_grad_(True)
+    zero = [torch.zeros(4), torch.zeros(4), torch.zeros(4, 3)]
+    for which in range(3):
+        out = ops.token_logprobs(x, tokens, top=3)
+        picked = [out.logprob, out.entropy, out.top_logprob][which]
+        (d,) = torch.autograd.grad(picked.sum(), x)
+        gradients = list(zero)
+        gradients[which] = torch.ones_like(gradients[which])
+        _check(x, tokens, 3, 1.0, out, d, gradients)
+    with torch.no_grad():
+        assert not ops.token_logprobs(x, tokens).logprob.requires_grad
+
+
+def test_gradient_against_differences():
+    x, tokens = _logits(3, 11, torch.float32, "cpu", 4, std=1.0)
+    x = x.double().requires_grad_(True)
+    weights = torch.linspace(0.5, 1.5, 3)
+
+    def loss(v):
+        out = ops.token_logprobs(v, tokens, top=2, temperature=0.8)
+        return (weights * (out.logprob + 0.3 * out.entropy + out.top_logprob.sum(-1))).sum().double()
+
+    (d,) = torch.autograd.grad(loss(x), x)
+    h = 2.0 ** -9                                # error h^2 of the difference, 2^-22 / h of the loss in fp32
+    for i in range(3):
+        for j in range(11):
+            e = torch.zeros_like(x)
+            e[i, j] = h
+            with torch.no_grad():
+                slope = (loss(x + e) - loss(x - e)) / (2 * h)
+            assert abs(float(slope) - float(d[i, j])) < 20 * (h * h + 2.0 ** -22 / h)
+
+
+def test_agrees_with_cross_entropy():
+    x, tokens = _logits(6, 300, torch.float32, "cpu", 8)
+    tokens[2] = -100
+    lp = ops.token_logprobs(x, tokens).logprob
+    loss = ops.cross_entropy(x, tokens, reduction="none")
+    assert bool(((lp + loss).abs() <= 2.0 ** -20 * (1 + loss.abs())).all())
+
+
+def test_refusals():
+    x, tokens = _logits(4, 50, torch.float32, "cpu", 1)
+    for bad in (dict(top=-1), dict(top=33), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")),
+                dict(temperature=INF)):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(x, tokens, **bad)
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x[:, :5], tokens, top=6)
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x, tokens[:3])
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x, tokens.int())
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x[:, :0], tokens)
+    with pytest.raises(TypeError):
+        ops.token_logprobs(x.long(), tokens)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    x, tokens = _logits(4, 50, torch.float32, "cuda", 1)
+    with pytest.raises(TypeError):
+        ops.token_logprobs(x.half(), tokens)
+    with pytest.raises(TypeError):
+        ops.token_logprobs(x.double(), tokens)
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x, tokens.cpu())
+
+
+@pytest.mark.gpu
+def test_same_bits_on_streams_and_in_a_captured_graph():
+    for T, V in ((1, 128256), (70, 32003)):
+        x, tokens = _logits(T, V, torch.bfloat16, "cuda", 6)
+        x.requires_grad_(True)
+
+        def step():
+            out = ops.token_logprobs(x, tokens, top=5)
+            (d,) = torch.autograd.grad(out.logprob.sum() + out.entropy.sum(), x)
+            return [t.detach() for t in out] + [d]
+
+        want = step()
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(step())
+        torch.cuda.synchronize()
+        for r in got:
+            assert all(torch.equal(a, b) for a, b in zip(want, r))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = step()
+        other, _ = _logits(T, V, torch.bfloat16, "cuda", 7)
+        with torch.no_grad():
+            x.copy_(other)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in kept]
+        assert all(torch.equal(a, b) for a, b in zip(replayed, step()))
