@@ -47,6 +47,8 @@ def add_common_args(p: argparse.ArgumentParser, default_schedule: str) -> None:
     p.add_argument("--pytorch-profiler-iters", type=int, default=3)
     p.add_argument("--device", default=None, choices=(None, "cuda", "cpu"))
     p.add_argument("--dtype", default="bf16", choices=("bf16", "fp32"))
+    p.add_argument("--optimizer", default="adam", choices=("adam", "adamw", "adamw8"),
+                   help="adamw8: AdamW with moments in 8 bits")
     p.add_argument("--checkpoint-dir", default="", help="save a checkpoint here after the timed iterations")
     p.add_argument("--resume", default="", help="checkpoint directory to resume from")
 
@@ -61,7 +63,9 @@ def run_driver(args, model_class, model_args, cfg, loss_fn, const_attrs) -> dict
     x = torch.randint(0, cfg.vocab_size, (args.batch_size * mbs, args.seq_len), generator=g)
     y = torch.randint(0, cfg.vocab_size, (args.batch_size * mbs, args.seq_len), generator=g)
     dtype = torch.bfloat16 if args.dtype == "bf16" else torch.float32
-    actor = piper_setup(model_class, model_args=model_args, optim_fn=torch.optim.Adam, example_inputs=[x],
+    actor = piper_setup(model_class, model_args=model_args,
+                        optim_fn=torch.optim.Adam if args.optimizer == "adam" else torch.optim.AdamW,
+                        optim_kwargs={"state_bits": 8} if args.optimizer == "adamw8" else None, example_inputs=[x],
                         example_outputs=y, activation_checkpointing=args.activation_checkpointing,
                         num_checkpoints=getattr(args, "num_checkpoints", 1), model_dtype=dtype,
                         nsight=args.nsight, temp_dir=args.temp_dir, visualize_dag=args.viz, const_attrs=const_attrs,

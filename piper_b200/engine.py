@@ -77,7 +77,8 @@ def _adam_config(optim_fn, optim_kwargs: Optional[dict]) -> AdamConfig:
     The reference instantiates ``optim_class(params)`` per bucket (``src/actor.py:573,600``).  Here the update is
     one kernel over flat buffers, so only ``torch.optim.Adam`` (L2 decay added to the gradient) and
     ``torch.optim.AdamW`` (decoupled decay) can be honoured; ``optim_fn`` may be the class, a
-    ``functools.partial`` of it, or ``None`` (Adam).  Anything the kernels cannot reproduce is rejected.
+    ``functools.partial`` of it, or ``None`` (Adam).  ``state_bits=8`` among the arguments keeps the moments of AdamW in
+    8 bits (``ops.AdamWState``).  Anything the kernels cannot reproduce is rejected.
     """
     import functools
 
@@ -106,6 +107,10 @@ def _adam_config(optim_fn, optim_kwargs: Optional[dict]) -> AdamConfig:
             cfg.eps = float(v)
         elif k == "weight_decay":
             cfg.weight_decay = float(v)
+        elif k == "state_bits":
+            cfg.state_bits = int(v)
+            if cfg.state_bits not in (8, 32) or (cfg.state_bits == 8 and not cfg.decoupled):
+                raise ValueError(f"state_bits={v!r}: moments have 32 bits, or 8 with torch.optim.AdamW")
         elif k in ("fused", "foreach", "capturable", "differentiable"):
             continue                                # implementation switches of torch.optim, no effect on the math
         elif k in ("amsgrad", "maximize") and not v:

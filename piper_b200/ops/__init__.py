@@ -15,8 +15,10 @@ from .core import (
     wgrad_store,
 )
 from .logprobs import TokenLogprobs, token_logprobs
+from .optim import AdamWState, adamw_step
 
 __all__ = [
     "native", "linear", "rmsnorm", "add_rmsnorm", "qk_rope", "residual_add", "rope_tables", "attention", "swiglu",
-    "embedding", "cross_entropy", "token_logprobs", "TokenLogprobs", "grad_sinks", "wgrad_store",
+    "embedding", "cross_entropy", "token_logprobs", "TokenLogprobs", "AdamWState",
+    "adamw_step", "grad_sinks", "wgrad_store",
 ]

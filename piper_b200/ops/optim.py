@@ -1,0 +1,227 @@
+"""AdamW over many tensors at once, with moments in 32 or in 8 bits (``csrc/adamw.cu``).
+
+The executor steps flat buckets (``runtime/storage.py``, which uses this state where ``state_bits`` is 8); a program with
+tensors of its own steps them all in one launch::
+
+    state = ops.AdamWState(params, bits=8)
+    ...
+    ops.adamw_step(params, [p.grad for p in params], state, lr=3e-4, betas=(0.9, 0.95), weight_decay=0.1)
+
+8-bit moments take 2.03 bytes an element in place of 8.  A block of 256 elements keeps its largest magnitude as an fp32 scale;
+an element is an 8-bit number relative to it with three bits of mantissa (the first moment 16 binades and a sign, the
+second 32 binades), rounded up or down at random in proportion to the distance.  The random bits depend on the step, the
+tensor's place in the list and the element alone: a step from the same state gives the same bits.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence
+
+import torch
+from torch import Tensor
+
+from . import native
+
+BLOCK = 256
+_M_BASE, _V_BASE = 889, 761        # fp32 bits >> 20 of code 0; those of 1.0 are 1016, codes 127 and 255
+
+
+def _mix32(h: Tensor) -> Tensor:
+    for shift, factor in ((16, 0x7FEB352D), (15, 0x846CA68B)):
+        h = ((h ^ (h >> shift)) * factor) & 0xFFFFFFFF
+    return h ^ (h >> 16)
+
+
+def _random16(step: int, ordinal: int, n: int, device) -> tuple[Tensor, Tensor]:
+    seed = int(_mix32(torch.tensor((step * 0x9E3779B1 + ordinal * 0x85EBCA77) & 0xFFFFFFFF)))
+    h = _mix32((torch.arange(n, device=device) + seed) & 0xFFFFFFFF)
+    return h & 0xFFFF, h >> 16
+
+
+def _decode(codes: Tensor, scale: Tensor, signed: bool) -> Tensor:
+    c = codes.to(torch.int32)
+    low = c & 127 if signed else c
+    x = torch.where(low > 0, (low + (_M_BASE if signed else _V_BASE)) << 20, torch.zeros_like(low)).view(torch.float32)
+    x = (x.view(-1, BLOCK) * scale.unsqueeze(1)).view(-1)
+    return torch.where(c >= 128, -x, x) if signed else x
+
+
+def _encode(x: Tensor, r: Tensor, signed: bool) -> tuple[Tensor, Tensor]:
+    """Codes and scales of whole blocks of fp32 values; r: 16 random bits for each."""
+    a = x.abs().view(-1, BLOCK)
+    scale = torch.where(torch.isfinite(a).all(1), a.amax(1), torch.full((), math.nan, device=x.device))
+    y = (a / torch.where(scale > 0, scale, torch.ones_like(scale)).unsqueeze(1)).view(-1)
+    base = _M_BASE if signed else _V_BASE
+    least = float(torch.tensor((base + 1) << 20, dtype=torch.int32).view(torch.float32))
+    codes = ((y.view(torch.int32) + (r << 4).to(torch.int32)) >> 20) - base
+    small = (r.to(torch.float32) * (least / 65536) < y) if signed else y > 0
+    codes = torch.where(y < least, small.to(torch.int32), codes)
+    if signed:
+        codes = codes + 128 * (x < 0)
+    return (codes & 255).to(torch.uint8), scale
+
+
+class AdamWState:
+    """Moments, master copies and step counts of a list of parameters (bf16 or fp32, contiguous, on one device).
+
+    Everything is flat: parameter ``i`` owns the elements ``[offsets[i], offsets[i] + numel)`` of ``m`` and ``v`` (fp32, or
+    uint8 codes with the scales ``m_scale`` and ``v_scale`` of their blocks of 256) and, where a parameter is bf16, of the
+    fp32 ``master``, from which its update starts.  Tensors begin at whole blocks; what is between them stays zero.
+    """
+
+    def __init__(self, params: Sequence[Tensor], *, bits: int = 32) -> None:
+        params = list(params)
+        if bits not in (8, 32):
+            raise ValueError(f"AdamWState: bits must be 8 or 32, got {bits}")
+        if not params:
+            raise ValueError("AdamWState: no parameters")
+        self.bits, self.device = bits, params[0].device
+        self.shapes = [tuple(p.shape) for p in params]
+        self.dtypes = [p.dtype for p in params]
+        self.offsets, at = [], 0
+        for p in params:
+            if p.dtype not in (torch.bfloat16, torch.float32):
+                raise TypeError(f"AdamWState: parameters are bfloat16 or float32, got {p.dtype}")
+            if p.device != self.device:
+                raise ValueError(f"AdamWState: parameters on {self.device} and {p.device}")
+            if not p.is_contiguous():
+                raise ValueError("AdamWState: parameters must be contiguous")
+            self.offsets.append(at)
+            at += (p.numel() + BLOCK - 1) // BLOCK * BLOCK
+        if len({p.data_ptr() for p in params if p.numel()}) < sum(p.numel() > 0 for p in params):
+            raise ValueError("AdamWState: a parameter is listed twice")
+        self.numel = at
+        self.steps = [0] * len(params)
+        moment = dict(dtype=torch.uint8 if bits == 8 else torch.float32, device=self.device)
+        self.m, self.v = torch.zeros(at, **moment), torch.zeros(at, **moment)
+        self.m_scale = self.v_scale = self.master = None
+        if bits == 8:
+            self.m_scale, self.v_scale = (torch.zeros(at // BLOCK, dtype=torch.float32, device=self.device) for _ in range(2))
+        if torch.bfloat16 in self.dtypes:
+            self.master = torch.zeros(at, dtype=torch.float32, device=self.device)
+            self.read_masters(params)
+
+    def read_masters(self, params: Sequence[Tensor]) -> None:
+        """Master copies from the parameters as they are now (after somebody else wrote them)."""
+        with torch.no_grad():
+            for o, p in zip(self.offsets, params):
+                if p.dtype == torch.bfloat16:
+                    self.master[o:o + p.numel()].copy_(p.detach().reshape(-1))
+
+    def set_step(self, step: int) -> None:
+        """The number of steps taken so far, of all parameters."""
+        self.steps = [int(step)] * len(self.shapes)
+
+    def moments(self) -> tuple[Tensor, Tensor]:
+        """Both moments in fp32, flat as ``m`` and ``v`` are (those themselves if they have 32 bits)."""
+        if self.bits == 32:
+            return self.m, self.v
+        if not self.m.is_cuda:
+            return _decode(self.m, self.m_scale, True), _decode(self.v, self.v_scale, False)
+        out = [torch.empty(self.numel, dtype=torch.float32, device=self.device) for _ in range(2)]
+        native.lib().moments_decode(self.m, self.m_scale, out[0], True)
+        native.lib().moments_decode(self.v, self.v_scale, out[1], False)
+        return out[0], out[1]
+
+    def set_moments(self, m: Tensor, v: Tensor) -> None:
+        """The reverse of ``moments()``; 8-bit codes are the nearest ones, so what came out of it goes back unchanged."""
+        with torch.no_grad():
+            if self.bits == 32:
+                self.m.copy_(m)
+                self.v.copy_(v)
+                return
+            half = torch.full((self.numel,), 1 << 15, dtype=torch.int64, device=self.device)
+            for x, codes, scale, signed in ((m, self.m, self.m_scale, True), (v, self.v, self.v_scale, False)):
+                x = x.to(device=self.device, dtype=torch.float32).contiguous()
+                c, s = _encode(x, half, signed)
+                codes.copy_(c)
+                scale.copy_(s)
+
+    def state_dict(self) -> dict:
+        return {"bits": self.bits, "shapes": list(self.shapes), "steps": list(self.steps), "m": self.m, "v": self.v,
+                "m_scale": self.m_scale, "v_scale": self.v_scale, "master": self.master}
+
+    def load_state_dict(self, state: dict) -> None:
+        """Takes over a state of the same parameters, of either width."""
+        if [tuple(s) for s in state["shapes"]] != self.shapes:
+            raise ValueError("AdamWState: the state is of other parameters")
+        if (state["master"] is None) != (self.master is None):
+            raise ValueError("AdamWState: the state is of parameters of another type")
+        with torch.no_grad():
+            if state["bits"] == self.bits:
+                for name in ("m", "v", "m_scale", "v_scale"):
+                    if getattr(self, name) is not None:
+                        getattr(self, name).copy_(state[name])
+            else:
+                m, v = (state[n].to(self.device) for n in ("m", "v"))
+                if state["bits"] == 8:
+                    m, v = (_decode(c, state[s].to(self.device), sg) for c, s, sg in ((m, "m_scale", True), (v, "v_scale", False)))
+                self.set_moments(m, v)
+            if self.master is not None:
+                self.master.copy_(state["master"])
+        self.steps = [int(s) for s in state["steps"]]
+
+
+def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], state: AdamWState, *, lr: float = 1e-3,
+               betas: tuple = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, grad_scale: float = 1.0) -> None:
+    """One step of AdamW (decoupled weight decay) for all ``params`` with a gradient, in place.
+
+    ``grads`` are bf16 or fp32, shaped like their parameters, and are multiplied by ``grad_scale`` (the mean over
+    microbatches, a clipping factor); a parameter whose gradient is None is left as it is and its step count with it.  The
+    step counts live on the host, so a step cannot be captured into a CUDA graph, which would repeat one bias correction.
+    """
+    params, grads = list(params), list(grads)
+    if len(params) != len(state.shapes) or len(grads) != len(params):
+        raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients, a state of {len(state.shapes)}")
+    for p, g, shape, dtype in zip(params, grads, state.shapes, state.dtypes):
+        if p.shape != shape or p.dtype != dtype or p.device != state.device:
+            raise ValueError(f"adamw_step: the state is of a {dtype} parameter {shape} on {state.device}, got {p.dtype} "
+                             f"{tuple(p.shape)} on {p.device}")
+        if g is not None and (g.shape != shape or g.device != p.device):
+            raise ValueError(f"adamw_step: a gradient is {tuple(g.shape)} on {g.device}, its parameter {shape} on {p.device}")
+    b1, b2 = betas
+    if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1):
+        raise ValueError(f"adamw_step: lr={lr}, betas={betas}, eps={eps}, weight_decay={weight_decay}")
+    if state.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("adamw_step: the step count lives on the host; a captured step would repeat itself")
+    steps = [s + (g is not None) for s, g in zip(state.steps, grads)]
+    with torch.no_grad():
+        if state.device.type == "cuda":
+            grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
+            native.lib().adamw(params, grads, state.m, state.v, state.m_scale, state.v_scale, state.master, state.offsets,
+                               steps, lr, b1, b2, eps, weight_decay, grad_scale)
+        else:
+            for i, (p, g) in enumerate(zip(params, grads)):
+                if g is not None and p.numel():
+                    _step_ref(state, i, p, g, steps[i], lr, b1, b2, eps, weight_decay, grad_scale)
+    torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+    state.steps = steps
+
+
+def _step_ref(state: AdamWState, i: int, p: Tensor, grad: Tensor, step: int, lr: float, b1: float, b2: float, eps: float,
+              wd: float, grad_scale: float) -> None:
+    n, o = p.numel(), state.offsets[i]
+    whole = (n + BLOCK - 1) // BLOCK * BLOCK
+    part, blocks = slice(o, o + whole), slice(o // BLOCK, (o + whole) // BLOCK)
+    g = torch.zeros(whole, dtype=torch.float32, device=p.device)
+    g[:n] = grad.reshape(-1)
+    g *= grad_scale
+    if state.bits == 8:
+        m, v = _decode(state.m[part], state.m_scale[blocks], True), _decode(state.v[part], state.v_scale[blocks], False)
+    else:
+        m, v = state.m[part], state.v[part]
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + g * (1 - b2) * g
+    m[n:] = 0
+    v[n:] = 0
+    w = state.master[o:o + n] if p.dtype == torch.bfloat16 else p.detach().view(-1)
+    update = m[:n] / (torch.sqrt(v[:n]) * (1 / math.sqrt(1 - b2 ** step)) + eps)
+    w.copy_(w * (1 - lr * wd) - update * (lr / (1 - b1 ** step)))
+    if p.dtype == torch.bfloat16:
+        p.detach().view(-1).copy_(w)
+    if state.bits == 8:
+        rm, rv = _random16(step, i, whole, p.device)
+        state.m[part], state.m_scale[blocks] = _encode(m, rm, True)
+        state.v[part], state.v_scale[blocks] = _encode(v, rv, False)
+    else:
+        state.m[part], state.v[part] = m, v

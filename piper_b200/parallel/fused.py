@@ -119,7 +119,7 @@ class FusedCollectives:
         for b in actor.buckets.values():
             st = b.storage
             if st is not None and st.mode in ("allreduce", "zero2", "zero3") and st.numel > 0 \
-                    and st.dtype == torch.bfloat16:
+                    and st.dtype == torch.bfloat16 and st.state8 is None:     # 8-bit moments take the NCCL lowering
                 self._adopt(st, b)
         return self
 

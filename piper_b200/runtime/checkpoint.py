@@ -33,10 +33,11 @@ def _rank_state(actor) -> dict:
         flat = st.full_param_tensor()
         for s in st.slots:
             model[s.fqn] = flat[s.offset:s.offset + s.numel].view(s.shape).detach().cpu().clone()
+        m, v = st.moments()
         for s, a, e, sh in st.owned_pieces():
             key = s.fqn
             sl = slice(sh, sh + e - a)
-            entry = {"step": st.step_count, "exp_avg": st.m[sl].cpu().clone(), "exp_avg_sq": st.v[sl].cpu().clone()}
+            entry = {"step": st.step_count, "exp_avg": m[sl].cpu().clone(), "exp_avg_sq": v[sl].cpu().clone()}
             if getattr(st, "master", None) is not None:
                 entry["master"] = st.master[sl].cpu().clone()
             opt_state[key] = entry
@@ -129,6 +130,7 @@ def load_checkpoint(actor, directory: str) -> int:
         if st is None or st.numel == 0:
             continue
         pieces = {id(s): (a, z, sh) for s, a, z, sh in st.owned_pieces()}
+        m, v = st.moments()
         was_live = st.params_live
         if not was_live:
             st.all_gather_params()
@@ -151,11 +153,13 @@ def load_checkpoint(actor, directory: str) -> int:
                 if st.params_sharded or st.sharded_state or st.row_table is not None:
                     st.shard_params[own].copy_(t.reshape(-1)[src].to(st.dtype))
                 if e is not None:
-                    st.m[own].copy_(e["exp_avg"].reshape(-1)[src])
-                    st.v[own].copy_(e["exp_avg_sq"].reshape(-1)[src])
+                    m[own].copy_(e["exp_avg"].reshape(-1)[src])
+                    v[own].copy_(e["exp_avg_sq"].reshape(-1)[src])
                     if getattr(st, "master", None) is not None:
                         st.master[own].copy_(e["master"].reshape(-1)[src])
                     st.step_count = int(e["step"])
+        if st.state8 is not None:
+            st.set_moments(m, v)
         if not was_live:
             st.free_params()
     actor.iteration = int(full["step"])

@@ -6,7 +6,8 @@ All of them live in one flat buffer each for
 
 * ``flat_params``  model dtype (bf16 in production), parameters are views into it;
 * ``flat_grads``   fp32, the sink that weight-gradient kernels accumulate into;
-* ``master / m / v`` fp32 optimizer state over the range this rank *owns*.
+* ``master / m / v`` fp32 optimizer state over the range this rank *owns* (``state_bits`` 8: the moments are an
+  ``ops.AdamWState`` in their place, a quarter of the bytes).
 
 The owned range is the whole bucket for ``local`` (no data parallelism) and
 ``allreduce`` (replicated update) buckets, and the rank's 1/dp slice for
@@ -35,6 +36,7 @@ import torch.distributed as dist
 
 from ..ops import core as ops_core
 from ..ops import native
+from ..ops.optim import AdamWState, adamw_step
 
 # PIPER_DEBUG_POISON=1: fill gathered ZeRO-3 parameters with NaN right before their storage is released
 _POISON_FREED = os.environ.get("PIPER_DEBUG_POISON", "0") == "1"
@@ -84,6 +86,7 @@ class AdamConfig:
     eps: float = 1e-8
     weight_decay: float = 0.0
     decoupled: bool = False     # True: AdamW (decay shrinks the weight); False: torch.optim.Adam's L2 term in the gradient
+    state_bits: int = 32        # 8: moments of AdamW in 8 bits (ops/optim.py)
 
 
 def _forget_sinks(sinks: dict) -> None:
@@ -130,6 +133,7 @@ class ParamStorage:
         self.row_table: Optional[list] = None
         self.persistent_grads = False      # the full gradient buffer is never freed (it lives in symmetric memory)
         self.fused_stepped = False
+        self.state8: Optional[AdamWState] = None      # in place of m and v where moments have 8 bits
         # what this bucket has registered as gradient sinks and not taken back: the allocator may hand a dead bucket's
         # addresses to another tensor, which must not find the old buffer there
         self._sinks: dict[int, torch.Tensor] = {}
@@ -140,9 +144,14 @@ class ParamStorage:
         for s in self.slots:
             full[s.offset:s.offset + s.numel].copy_(self._init_slot(s, seed).reshape(-1))
         lo, hi = self.owned_range()
-        self.master = full[lo:hi].to(torch.float32) if dtype != torch.float32 else None
-        self.m = torch.zeros(hi - lo, dtype=torch.float32, device=device)
-        self.v = torch.zeros(hi - lo, dtype=torch.float32, device=device)
+        if adam.state_bits == 8:
+            self.state8 = AdamWState([full[lo:hi]], bits=8)
+            self.master = self.state8.master[:hi - lo] if dtype != torch.float32 else None
+            self.m = self.v = None
+        else:
+            self.master = full[lo:hi].to(torch.float32) if dtype != torch.float32 else None
+            self.m = torch.zeros(hi - lo, dtype=torch.float32, device=device)
+            self.v = torch.zeros(hi - lo, dtype=torch.float32, device=device)
         self.flat_params = full
         self.params_live = True
         self._bind(full)
@@ -212,6 +221,8 @@ class ParamStorage:
         paths pass symmetric memory).  Must run before training or right after a checkpoint was loaded into the
         full parameters: master weights are re-derived from the current parameters, moments restart at zero.
         """
+        if self.state8 is not None:
+            raise RuntimeError(f"bucket {self.key}: 8-bit moments are not sharded by rows")
         full = self.full_param_tensor()
         table, shard = self.row_layout(self.slots, self.dp_degree)
         self.row_table = table
@@ -372,7 +383,11 @@ class ParamStorage:
         grads = self.shard_grads if self.sharded_state else self.flat_grads[lo:hi]
         target = self.shard_params if (self.sharded_state or self.params_sharded) else self.flat_params[lo:hi]
         a = self.adam
-        if grads.is_cuda and self.dtype == torch.bfloat16:
+        if self.state8 is not None:
+            self.state8.set_step(self.step_count - 1)
+            adamw_step([target], [grads], self.state8, lr=a.lr, betas=a.betas, eps=a.eps, weight_decay=a.weight_decay,
+                       grad_scale=grad_scale)
+        elif grads.is_cuda and self.dtype == torch.bfloat16:
             native.lib().adam_flat(self.master, self.m, self.v, grads, target, a.lr, a.betas[0], a.betas[1], a.eps,
                                    a.weight_decay, self.step_count, grad_scale, a.decoupled)
         else:
@@ -386,6 +401,22 @@ class ParamStorage:
             self.shard_grads.zero_()
         if self.flat_grads is not None:
             self.flat_grads.zero_()
+
+    def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """Both moments of the owned range in fp32."""
+        if self.state8 is None:
+            return self.m, self.v
+        lo, hi = self.owned_range()
+        m, v = self.state8.moments()
+        return m[:hi - lo], v[:hi - lo]
+
+    def set_moments(self, m: torch.Tensor, v: torch.Tensor) -> None:
+        if self.state8 is None:
+            self.m.copy_(m)
+            self.v.copy_(v)
+            return
+        tail = self.state8.numel - m.numel()
+        self.state8.set_moments(*(torch.nn.functional.pad(t, (0, tail)) for t in (m, v)))
 
     def snapshot_grads(self, scale: float) -> dict:
         """fqn -> scaled copy of the gradient this rank holds (full tensors, or its ZeRO shard as a flat range)."""

@@ -1,0 +1,308 @@
+"""AdamW over many tensors with moments in 32 and in 8 bits, against the formulas in 64 bits.
+
+Tolerances.  A moment is two products and a sum with rounded constants, each within half a step (2^-24): 4 of those relative to
+the sum of the addends' sizes (v has one product more).  A weight is its own product with a rounded constant and the update,
+whose relative error is that of m, half that of v, and six more roundings (root, product, sum, quotient, rate, product).
+An 8-bit moment is one of the two neighbours of the 32-bit one on its grid."""
+import math
+
+import pytest
+import torch
+
+from piper_b200 import ops
+from piper_b200.ops.optim import BLOCK
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+EPS = 2.0 ** -24
+SHAPES = [(1,), (255,), (256,), (257,), (3, 100), (64, 64), (5000,), (7, 11, 13), (0,), (2, 2048)]
+
+
+def _tensors(dtype, grad_dtype, device, seed=0, shapes=SHAPES):
+    g = torch.Generator().manual_seed(seed)
+    params = [(torch.randn(s, generator=g) * 0.1).to(dtype).to(device) for s in shapes]
+    grads = [(torch.randn(s, generator=g) * 10.0 ** -(i % 5)).to(grad_dtype).to(device) for i, s in enumerate(shapes)]
+    return params, grads
+
+
+HYPER = dict(lr=1e-2, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+
+
+def _formula(w, m, v, g, step, lr, betas, eps, weight_decay, grad_scale=1.0):
+    """(w, m, v) after a step and the sizes of what m and v are sums of, all in 64 bits."""
+    b1, b2 = betas
+    g = g.double().cpu() * grad_scale
+    m1, v1 = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    upd = (m1 / (1 - b1 ** step)) / (torch.sqrt(v1 / (1 - b2 ** step)) + eps)
+    return w * (1 - lr * weight_decay) - lr * upd, m1, v1, (b1 * m).abs() + ((1 - b1) * g).abs(), upd
+
+
+def _parts(state, flat):
+    return [flat[o:o + math.prod(s)].double().cpu().view(s) for o, s in zip(state.offsets, state.shapes)]
+
+
+def _weights(params, state):
+    return [w if p.dtype == torch.bfloat16 else p.double().cpu()
+            for p, w in zip(params, _parts(state, state.master) if state.master is not None else params)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("dtype,grad_dtype", [(torch.bfloat16, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                              (torch.float32, torch.float32), (torch.float32, torch.bfloat16)])
+def test_steps_follow_the_formulas(dtype, grad_dtype, bits, device):
+    params, _ = _tensors(dtype, grad_dtype, device)
+    state = ops.AdamWState(params, bits=bits)
+    for step in range(1, 5):
+        _, grads = _tensors(dtype, grad_dtype, device, seed=step)
+        m0, v0 = (_parts(state, t) for t in state.moments())
+        w0 = _weights(params, state)
+        ops.adamw_step(params, grads, state, grad_scale=0.5, **HYPER)
+        m1, v1 = (_parts(state, t) for t in state.moments())
+        w1 = _weights(params, state)
+        assert state.steps == [step] * len(params)
+        for i, g in enumerate(grads):
+            w, m, v, m_size, upd = _formula(w0[i], m0[i], v0[i], g, step, grad_scale=0.5, **HYPER)
+            m_tol, v_tol = 5 * EPS * m_size + 1e-44, 6 * EPS * v + 1e-44
+            if bits == 32:
+                assert bool(((m1[i] - m).abs() <= m_tol).all()) and bool(((v1[i] - v).abs() <= v_tol).all())
+            else:
+                for got, want, tol, least in ((m1[i], m, m_tol, 1.25 * 2.0 ** -16), (v1[i], v, v_tol, 1.25 * 2.0 ** -32)):
+                    if got.numel():
+                        pad = torch.zeros((got.numel() + BLOCK - 1) // BLOCK * BLOCK, dtype=torch.float64)
+                        pad[:got.numel()] = want.reshape(-1).abs()
+                        scale = pad.view(-1, BLOCK).amax(1).repeat_interleave(BLOCK)[:got.numel()].view(got.shape)
+                        apart = torch.maximum(want.abs() / 8, scale * least) * (1 + 8 * EPS) + 2 * tol
+                        assert bool(((got - want).abs() <= apart).all())
+                        assert bool((got[want == 0] == 0).all())
+                assert bool((v1[i][v > 0] > 0).all())
+            ratio = m_tol / (m.abs() + 1e-300) + 12 * EPS
+            w_tol = 4 * EPS * w0[i].abs() + HYPER["lr"] * upd.abs() * ratio + 2 * EPS * w.abs() + 1e-44
+            assert bool(((w1[i] - w).abs() <= w_tol).all()), (i, float(((w1[i] - w).abs() / w_tol).max()))
+            if dtype == torch.bfloat16:
+                assert torch.equal(params[i].cpu(), w1[i].to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.gpu
+def test_kernel_has_the_definitions_bits(bits):
+    """Moments are rounded operation by operation, so the kernel's are those of plain tensor operations."""
+    both = []
+    for device in ("cpu", "cuda"):
+        params, _ = _tensors(torch.bfloat16, torch.float32, device)
+        state = ops.AdamWState(params, bits=bits)
+        for step in range(1, 7):
+            _, grads = _tensors(torch.bfloat16, torch.float32, device, seed=step)
+            ops.adamw_step(params, grads, state, **HYPER)
+        both.append(state)
+    for name in ("m", "v", "m_scale", "v_scale"):
+        a, b = (getattr(s, name) for s in both)
+        assert (a is None and b is None) or torch.equal(a, b.cpu()), name
+    assert all(torch.equal(a, b.cpu()) for a, b in zip(both[0].moments(), both[1].moments()))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_small_changes_arrive_on_average(device):
+    """1,000 steps with a gradient that has dropped: v decays as it should although a step moves it by a hundredth of a code."""
+    n = 1 << 14
+    p = [torch.zeros(n, device=device)]
+    state = ops.AdamWState(p, bits=8)
+    g = torch.ones(n, device=device)
+    g[::BLOCK] = 4.0                       # the block's scale does not fall with the rest
+    state.set_moments(0 * g, g * g)
+    small = torch.full((n,), 0.1, device=device)
+    small[::BLOCK] = 4.0
+    want = 1.0
+    for _ in range(1000):
+        ops.adamw_step(p, [small], state, lr=0.0, betas=(0.9, 0.999), weight_decay=0.0)
+        want = 0.999 * want + 0.001 * 0.01
+    rest = torch.arange(n, device=device) % BLOCK != 0
+    m, v = state.moments()
+    # a step's rounding has at most half a code (v / 16) of deviation, 1,000 of them are independent, 16,320 elements too
+    assert abs(float(v[rest].mean()) - want) < 5 * 1000 ** 0.5 / 16 / 16320 ** 0.5 * want
+    assert abs(float(m[rest].mean()) - 0.1) < 5 * 10 ** 0.5 / 16 / 16320 ** 0.5 * 0.1
+    assert not state.v_scale.isnan().any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_special_gradients(device):
+    n = 3 * BLOCK
+    for bits in (8, 32):
+        p = [torch.ones(n, device=device)]
+        state = ops.AdamWState(p, bits=bits)
+        g = torch.zeros(n, device=device)
+        ops.adamw_step(p, [g], state, lr=0.1, weight_decay=0.0)
+        assert bool((p[0] == 1).all()) and not state.moments()[0].any() and not state.moments()[1].any()
+        g[5], g[BLOCK] = 1e-20, 3e18          # squares below the normal numbers and near the largest
+        ops.adamw_step(p, [g], state, lr=0.1, weight_decay=0.0)
+        m, v = state.moments()
+        assert bool(torch.isfinite(p[0]).all()) and bool((p[0][6:BLOCK] == 1).all()) and m[5] > 0 and v[BLOCK] > 1e33
+        g[2 * BLOCK + 3] = float("nan")
+        ops.adamw_step(p, [g], state, lr=0.1, weight_decay=0.0)
+        m, v = state.moments()
+        assert bool(torch.isnan(m[2 * BLOCK + 3])) and bool(torch.isnan(v[2 * BLOCK + 3]))
+        assert int(torch.isnan(p[0]).sum()) == 1
+        # with 8 bits the whole block has lost its scale; no other block has
+        assert int(torch.isnan(m).sum()) == (BLOCK if bits == 8 else 1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_missing_gradients_and_views(bits, device):
+    base = torch.randn(4096 + 3, generator=torch.Generator().manual_seed(1)).to(device)
+    views = [base[3:1003], base[1003:1004], base[1005:4099].view(2, -1)]       # no alignment but the type's
+    alone = [v.clone() for v in views]
+    grads = [torch.randn(v.shape, generator=torch.Generator().manual_seed(2)).to(device) for v in views]
+    strided = [g.clone() if g.dim() == 1 else g.t().contiguous().t() for g in grads]
+    before = base.clone()
+    a, b = ops.AdamWState(views, bits=bits), ops.AdamWState(alone, bits=bits)
+    for step in range(3):
+        which = [None if step == 1 and i == 0 else g for i, g in enumerate(grads)]
+        ops.adamw_step(views, which, a, **HYPER)
+        ops.adamw_step(alone, [None if w is None else s for w, s in zip(which, strided)], b, **HYPER)
+    assert a.steps == [2, 3, 3]
+    assert all(torch.equal(x, y) for x, y in zip(views, alone)) and torch.equal(a.m, b.m) and torch.equal(a.v, b.v)
+    assert torch.equal(base[:3], before[:3]) and base[1004] == before[1004]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_more_tensors_than_one_launch_takes(device):
+    shapes = [(1 + 37 * i % 700,) for i in range(203)]
+    params, grads = _tensors(torch.float32, torch.float32, device, shapes=shapes)
+    want = [p.clone() for p in params]
+    state = ops.AdamWState(params, bits=32)
+    ops.adamw_step(params, grads, state, **HYPER)
+    for p, w, g in zip(params, want, grads):
+        one = ops.AdamWState([w], bits=32)
+        ops.adamw_step([w], [g], one, **HYPER)
+        assert torch.equal(p, w)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_states_are_saved_and_loaded(device):
+    params, grads = _tensors(torch.bfloat16, torch.float32, device)
+    state = ops.AdamWState(params, bits=8)
+    for _ in range(2):
+        ops.adamw_step(params, grads, state, **HYPER)
+    saved = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in state.state_dict().items()}
+    other = ops.AdamWState(params, bits=8)
+    other.load_state_dict(saved)
+    again = ops.AdamWState(params, bits=8)
+    again.set_moments(*state.moments())                # values on the grid come back unchanged
+    assert torch.equal(again.m, state.m) and torch.equal(again.v, state.v) and torch.equal(again.v_scale, state.v_scale)
+    wide = ops.AdamWState(params, bits=32)
+    wide.load_state_dict(saved)
+    assert torch.equal(wide.m, state.moments()[0]) and wide.steps == state.steps
+    narrow = ops.AdamWState(params, bits=8)
+    narrow.load_state_dict(wide.state_dict())
+    assert torch.equal(narrow.m, state.m) and torch.equal(narrow.master, state.master)
+    twin = [p.clone() for p in params]
+    ops.adamw_step(params, grads, state, **HYPER)
+    ops.adamw_step(twin, grads, other, **HYPER)
+    assert all(torch.equal(a, b) for a, b in zip(params, twin))
+
+
+def test_moments_of_eight_bits_take_two_bytes():
+    p = [torch.zeros(1 << 16)]
+    s = ops.AdamWState(p, bits=8)
+    held = sum(t.numel() * t.element_size() for t in (s.m, s.v, s.m_scale, s.v_scale))
+    assert held == (1 << 16) * 2 + (1 << 16) // BLOCK * 8
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    p = [torch.zeros(10, device=device), torch.zeros(4, 4, device=device)]
+    with pytest.raises(ValueError):
+        ops.AdamWState(p, bits=16)
+    with pytest.raises(ValueError):
+        ops.AdamWState([])
+    with pytest.raises(ValueError):
+        ops.AdamWState([p[0], p[0]])
+    with pytest.raises(TypeError):
+        ops.AdamWState([torch.zeros(4, dtype=torch.float16, device=device)])
+    with pytest.raises(ValueError):
+        ops.AdamWState([torch.zeros(4, 6, device=device).t()])
+    state = ops.AdamWState(p)
+    g = [torch.zeros_like(t) for t in p]
+    for params, grads in ((p[:1], g[:1]), (p, g[:1]), (p, [g[0], g[0]]), (p, [g[1], g[1]]), ([p[1], p[0]], [g[1], g[0]]),
+                          ([p[0].bfloat16(), p[1]], g)):
+        with pytest.raises(ValueError):
+            ops.adamw_step(params, grads, state)
+    for bad in (dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1e-8), dict(weight_decay=-0.1),
+                dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            ops.adamw_step(p, g, state, **bad)
+    assert state.steps == [0, 0]
+    with pytest.raises(ValueError):
+        state.load_state_dict(ops.AdamWState(p[:1]).state_dict())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_saved_tensor_that_was_stepped_is_noticed(device):
+    w = torch.ones(8, device=device, requires_grad=True)
+    state = ops.AdamWState([w])
+    y = (w * w).sum()
+    ops.adamw_step([w], [torch.ones(8, device=device)], state)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+
+
+@pytest.mark.gpu
+def test_a_step_is_not_captured():
+    p = [torch.zeros(256, device="cuda")]
+    state = ops.AdamWState(p)
+    g = [torch.ones(256, device="cuda")]
+    ops.adamw_step(p, g, state)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            ops.adamw_step(p, g, state)
+    torch.cuda.synchronize()
+    ops.adamw_step(p, g, state)
+    assert state.steps == [2]
+
+
+@pytest.mark.gpu
+def test_states_on_two_streams():
+    results = []
+    sets = [_tensors(torch.bfloat16, torch.float32, "cuda", seed=i) for i in range(2)]
+    for streams in ([None, None], [torch.cuda.Stream(), torch.cuda.Stream()]):
+        copies = [[p.clone() for p in s[0]] for s in sets]
+        states = [ops.AdamWState(c, bits=8) for c in copies]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for c, s, st, stream in zip(copies, sets, states, streams):
+                with torch.cuda.stream(stream):
+                    ops.adamw_step(c, s[1], st, **HYPER)
+        torch.cuda.synchronize()
+        results.append([t for c, s in zip(copies, states) for t in (*c, s.m, s.v)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_bucket_with_eight_bit_moments(dtype):
+    from piper_b200.runtime.storage import AdamConfig, ParamSlot, ParamStorage
+    slots = [ParamSlot(0, "a.weight", (40, 30), dtype, True), ParamSlot(1, "b.weight", (70,), dtype, True)]
+    cfg = AdamConfig(lr=1e-2, weight_decay=0.1, decoupled=True, state_bits=8)
+    st = ParamStorage("k", slots, torch.device("cpu"), dtype, "local", 0, 1, None, cfg)
+    want = [st.flat_params.clone()]
+    state = ops.AdamWState(want, bits=8)
+    for step in range(3):
+        g = torch.randn(st.numel, generator=torch.Generator().manual_seed(step))
+        st.flat_grads.copy_(g)
+        st.step(0.25)
+        ops.adamw_step(want, [g], state, lr=1e-2, betas=cfg.betas, eps=cfg.eps, weight_decay=0.1, grad_scale=0.25)
+        assert torch.equal(st.flat_params, want[0]) and not st.flat_grads.any()
+    m, v = st.moments()
+    assert m.shape == (st.numel,) and bool((v >= 0).all())
+    st.set_moments(m, v)
+    assert torch.equal(st.moments()[0], m) and torch.equal(st.moments()[1], v)
+
+
+def test_state_bits_of_a_setup():
+    from piper_b200.engine import _adam_config
+    assert _adam_config(torch.optim.AdamW, {"state_bits": 8}).state_bits == 8
+    assert _adam_config(torch.optim.AdamW, None).state_bits == 32
+    for fn, bits in ((torch.optim.Adam, 8), (torch.optim.AdamW, 4)):
+        with pytest.raises(ValueError):
+            _adam_config(fn, {"state_bits": bits})
