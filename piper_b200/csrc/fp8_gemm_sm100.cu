@@ -1,0 +1,495 @@
+// Products of e4m3 operands with a power-of-two scale for every row and 128 columns: C[M, N] = A[M, K] B[N, K]^T, bf16 or added
+// into fp32.
+//
+//   C[m, n] = sum over blocks k of 2^(ea[m, k] + eb[n, k]) sum over the block of a[m, i] b[n, i]
+//
+// The tensor core multiplies with the scales itself (tcgen05.mma kind::mxf8f6f4 with block_scale, which takes a scale for
+// every 32 of the contraction: four instructions in a row take the same one) and keeps the sum in fp32 in tensor memory, so
+// no partial sum leaves it before the end.  Scaling by powers of two is exact.
+//
+// Persistent CTAs, each by itself or in pairs on two neighbouring SMs (cta_group::2), walk tiles of 128 rows a CTA and 32 to 224 columns.
+// Roles by warp:
+//   warp 0       TMA producer: a ring of shared-memory stages of 128 x 128-byte operand boxes in 128-byte swizzle; hands out tiles.
+//   warp 1       MMA issuer (first CTA of a pair, for both), into one of two accumulators.
+//   warp 2       tensor memory allocation; warp 3 draws the first tile.
+//   warps 4-11   epilogue: accumulator to bf16 or fp32, through shared memory, TMA store or reduce-add.
+//   warps 12-15  scales: words of four blocks from global memory into tensor memory, one warp for each quarter of its lanes, which
+//                all hold the same: row r of A in lane r % 32 of column r / 32, rows of B likewise behind them.
+// Tensor memory: two accumulators of 224 columns, then four slots of 16 columns for the scales of four blocks (4 for 128 rows of A,
+// up to 7 for B).  256 columns would leave no room for the scales beside a second accumulator.
+//
+// What bounds it: a block of 128 of a 256 x 224 tile of a pair takes 448 cycles of MMA and loads 30 KiB into each SM, 472 cycles at
+// the 65 bytes per cycle that an SM takes from L2.
+//
+// All waits are bounded; on expiry the kernel records a status code, drains its copies, frees its tensor memory and returns.
+#include "fp8.h"
+
+#include <algorithm>
+#include <cstddef>
+
+#include "gemm_sm100.h"
+#include "ptx.cuh"
+
+namespace piper {
+namespace {
+
+constexpr int BM = 128;
+constexpr int BK = kFp8Group;                  // elements and bytes
+constexpr int UMMA_K = 32;
+constexpr int A_STAGE_BYTES = BM * BK;
+constexpr int MAX_WIDTH = 224;
+constexpr int MAX_STAGES = 8;
+constexpr int OPERAND_BYTES = 196608;
+constexpr int EPI_WARPS = 8;
+constexpr int SCALE_WARPS = 4;
+constexpr int NUM_THREADS = 128 + 32 * (EPI_WARPS + SCALE_WARPS);
+constexpr int C_STAGE_BYTES = 4096;
+constexpr int BAR_OFF = OPERAND_BYTES + EPI_WARPS * C_STAGE_BYTES;
+constexpr int SMEM_BYTES = BAR_OFF + 768 + 1024;
+constexpr int RING = 16;
+constexpr int SLOTS = 4;
+constexpr uint32_t SLOT_COLUMN = 2 * MAX_WIDTH, SLOT_COLUMNS = 16;
+static_assert(SLOT_COLUMN + SLOTS * SLOT_COLUMNS <= 512, "tensor memory");
+
+struct Bars {
+  uint64_t full[MAX_STAGES];
+  uint64_t empty[MAX_STAGES];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t scale_full[SLOTS];
+  uint64_t scale_empty[SLOTS];
+  uint64_t tile_full[RING];
+  int tile[RING][4];
+  uint32_t tmem_base;
+  int first;
+};
+static_assert(sizeof(Bars) <= 768 && offsetof(Bars, tile) % 16 == 0 && SMEM_BYTES <= 232448, "shared memory");
+
+struct Params {
+  const uint32_t* a_scales;
+  const uint32_t* b_scales;
+  int M, N, K;
+  int a_pad, b_pad;   // rows of a group's words
+  int width;
+  int a_rows;         // rows of an A box: 128, or fewer where a CTA by itself has all rows
+  int stages;
+  int band;
+  int* status;
+  int* sched;
+};
+
+// D[tmem] (+)= (A * scales) * (B * scales), e4m3 inputs.
+template <int CTAS>
+__device__ __forceinline__ void umma_scaled(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scale_a,
+                                            uint32_t scale_b, uint32_t accumulate) {
+  if (CTAS == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(scale_a), "r"(scale_b)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(scale_a), "r"(scale_b)
+        : "memory");
+}
+
+// e4m3 x e4m3, both K-major, scales as exponents; bits 4-5 and 29-30 say which byte of the scales' words belongs to the block.
+__device__ __forceinline__ uint32_t scaled_idesc(int m, int n, uint32_t byte) {
+  return byte << 4 | static_cast<uint32_t>(n >> 3) << 17 | 1u << 23 | static_cast<uint32_t>(m >> 4) << 24 | byte << 29;
+}
+
+__device__ __forceinline__ void tmem_st_32x4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+template <int CTAS, bool F32>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                const __grid_constant__ CUtensorMap tmap_c, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  Bars* bars = reinterpret_cast<Bars*>(smem + BAR_OFF);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
+  const int width = p.width;
+  const int b_rows = width / CTAS;
+  const int stage_bytes = A_STAGE_BYTES + b_rows * BK;
+  const int stages = p.stages;
+  const int tiles_m = (p.M + BM * CTAS - 1) / (BM * CTAS);
+  const int tiles_n = (p.N + width - 1) / width;
+  const int num_tiles = tiles_m * tiles_n;
+  const int k_blocks = (p.K + BK - 1) / BK;
+  const bool n_fast = tiles_n < tiles_m;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < MAX_STAGES; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&bars->acc_full[a], 1);
+      mbar_init(&bars->acc_empty[a], EPI_WARPS * CTAS);
+    }
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&bars->scale_full[s], SCALE_WARPS * CTAS);
+      mbar_init(&bars->scale_empty[s], 1);
+    }
+    for (int i = 0; i < RING; ++i) mbar_init(&bars->tile_full[i], 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+    tma_prefetch_desc(&tmap_c);
+  }
+  if (warp == 2) {
+    tmem_alloc_n<CTAS>(&bars->tmem_base, 512);
+    tmem_relinquish_n<CTAS>();
+  }
+  // As in the bf16 products: tiles come from a counter, but in launches of one round.
+  const int units = static_cast<int>(gridDim.x) / CTAS;
+  const bool draws = p.sched != nullptr && num_tiles > units;
+  grid_wait();
+  if (warp == 3 && rank == 0 && lane == 0)
+    bars->first = draws ? atomicAdd(&p.sched[0], 1) : static_cast<int>(blockIdx.x) / CTAS;
+  tc_fence_before();
+  if (CTAS == 2) cluster_sync(); else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+
+  // The dimension with fewer tiles is walked fastest, in bands where its operand does not stay in L2.
+  auto coords = [&](int tile, int& tm, int& tn) {
+    const int fast = n_fast ? tiles_n : tiles_m, slow = n_fast ? tiles_m : tiles_n;
+    const int b = tile / (p.band * slow), f0 = b * p.band;
+    const int bw = min(p.band, fast - f0), r = tile - f0 * slow;
+    const int f = f0 + r % bw, sl = r / bw;
+    tm = n_fast ? sl : f;
+    tn = n_fast ? f : sl;
+  };
+  auto tile_at = [&](uint32_t n, int& tile) -> bool {
+    if (!__all_sync(0xffffffffu, mbar_wait(&bars->tile_full[n % RING], (n / RING) & 1, p.status))) return false;
+    tile = *reinterpret_cast<volatile int*>(&bars->tile[n % RING]);
+    return true;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------ TMA producer (both CTAs of a pair load their own halves)
+    const int loaded = p.a_rows * BK + b_rows * BK;
+    uint32_t n = 0;
+    int s = 0;
+    uint32_t ph = 0, fills = 0;
+    bool ok = true;
+    for (;; ++n) {
+      if (rank == 0 && elect_one()) {
+        int next = n > 0 && draws ? atomicAdd(&p.sched[0], 1) : bars->first + static_cast<int>(n) * units;
+        if (next >= num_tiles) next = -1;
+        bars->tile[n % RING][0] = next;
+        if (CTAS == 2)
+          st_async_v4(mapa_u32(smem_u32(&bars->tile[n % RING]), 1), mapa_u32(smem_u32(&bars->tile_full[n % RING]), 1),
+                      next, 0, 0, 0);
+        mbar_arrive(&bars->tile_full[n % RING]);
+      } else if (rank == 1 && elect_one()) {
+        mbar_arrive_expect_tx(&bars->tile_full[n % RING], 16);
+      }
+      __syncwarp();
+      int tile;
+      if (!(ok = tile_at(n, tile)) || tile < 0) break;
+      int tm, tn;
+      coords(tile, tm, tn);
+      const int m0 = tm * (BM * CTAS) + static_cast<int>(rank) * BM;
+      const int n0 = tn * width + static_cast<int>(rank) * b_rows;
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[s], ph ^ 1, p.status)))) break;
+        if (elect_one()) {
+          uint8_t* sa = smem + s * stage_bytes;
+          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], CTAS * loaded);
+          tma_load_2d_n<CTAS>(sa, &tmap_a, &bars->full[s], kb * BK, m0);
+          tma_load_2d_n<CTAS>(sa + A_STAGE_BYTES, &tmap_b, &bars->full[s], kb * BK, n0);
+        }
+        __syncwarp();
+        ++fills;
+        if (++s == stages) { s = 0; ph ^= 1; }
+      }
+      if (!ok) break;
+    }
+    grid_launch();
+    if (ok) {
+      for (int i = 0; i < stages && ok; ++i) {   // every stage handed back: no commit is on its way to these barriers
+        ok = mbar_wait(&bars->empty[s], ph ^ 1, p.status);
+        if (++s == stages) { s = 0; ph ^= 1; }
+      }
+    } else if (rank == 0) {
+      for (int i = 0; i < stages; ++i) {         // let the copies already issued land
+        if (fills <= static_cast<uint32_t>(i)) continue;
+        mbar_wait(&bars->full[i], ((fills - 1 - i) / stages) & 1, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- MMA issuer (first CTA of a pair, for both)
+    if (rank == 0) {
+      const uint64_t da0 = umma_desc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t db0 = umma_desc_sw128(smem_u32(smem) + A_STAGE_BYTES, 16, 1024);
+      int s = 0;
+      uint32_t ph = 0, group = 0;
+      bool ok = true;
+      for (uint32_t n = 0; ok; ++n) {
+        int tile;
+        if (!(ok = tile_at(n, tile)) || tile < 0) break;
+        const uint32_t acc = n & 1;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_empty[acc], ((n >> 1) & 1) ^ 1, p.status)))) break;
+        tc_fence_after();
+        const uint32_t tmem_d = tmem_base + acc * MAX_WIDTH;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          const uint32_t slot = group % SLOTS;
+          if ((kb & 3) == 0 &&
+              !(ok = __all_sync(0xffffffffu, mbar_wait(&bars->scale_full[slot], (group / SLOTS) & 1, p.status)))) break;
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[s], ph, p.status)))) break;
+          tc_fence_after();
+          const bool last = (kb & 3) == 3 || kb == k_blocks - 1;        // of its group
+          if (elect_one()) {
+            const uint64_t da = da0 + (static_cast<uint32_t>(s * stage_bytes) >> 4);
+            const uint64_t db = db0 + (static_cast<uint32_t>(s * stage_bytes) >> 4);
+            const uint32_t scales = tmem_base + SLOT_COLUMN + slot * SLOT_COLUMNS;
+            const uint32_t idesc = scaled_idesc(BM * CTAS, width, static_cast<uint32_t>(kb & 3));
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k)
+              umma_scaled<CTAS>(tmem_d, da + k * (UMMA_K >> 4), db + k * (UMMA_K >> 4), idesc, scales, scales + 4,
+                                (kb > 0 || k > 0) ? 1u : 0u);
+            umma_commit_n<CTAS>(&bars->empty[s]);
+            if (last) umma_commit_n<CTAS>(&bars->scale_empty[slot]);
+            if (kb == k_blocks - 1) umma_commit_n<CTAS>(&bars->acc_full[acc]);
+          }
+          __syncwarp();
+          if (last) ++group;
+          if (++s == stages) { s = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else if (warp >= 4 + EPI_WARPS) {
+    // ---------------------------------------------------------- scales
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    uint32_t fills = 0;
+    bool ok = true;
+    for (uint32_t n = 0; ok; ++n) {
+      int tile;
+      if (!tile_at(n, tile) || tile < 0) break;
+      int tm, tn;
+      coords(tile, tm, tn);
+      const int m0 = tm * (BM * CTAS) + static_cast<int>(rank) * BM + lane, n0 = tn * width + lane;
+      for (int kb = 0; kb < k_blocks; kb += 4) {
+        const uint32_t* wa = p.a_scales + static_cast<long long>(kb / 4) * p.a_pad;
+        const uint32_t* wb = p.b_scales + static_cast<long long>(kb / 4) * p.b_pad;
+        uint32_t a[4], b[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = m0 + 32 * i < p.a_pad ? wa[m0 + 32 * i] : 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = 32 * i < width && n0 + 32 * i < p.b_pad ? wb[n0 + 32 * i] : 0u;
+        const uint32_t slot = fills % SLOTS;
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->scale_empty[slot], ((fills / SLOTS) & 1) ^ 1, p.status)))) break;
+        tc_fence_after();
+        const uint32_t at = tmem_base + lanes + SLOT_COLUMN + slot * SLOT_COLUMNS;
+        tmem_st_32x4(at, a);
+        tmem_st_32x8(at + 4, b);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CTAS == 2) mbar_arrive_cluster(mapa_u32(smem_u32(&bars->scale_full[slot]), 0));
+          else mbar_arrive(&bars->scale_full[slot]);
+        }
+        ++fills;
+      }
+    }
+    // every slot handed back: no commit is on its way to these barriers
+    for (int i = 0; i < SLOTS && ok; ++i, ++fills)
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->scale_empty[fills % SLOTS], ((fills / SLOTS) & 1) ^ 1, p.status));
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------- epilogue
+    const int q = warp & 3;                     // TMEM lanes [32q, 32q + 32)
+    const int half = (warp - 4) >> 2;           // odd or even 32-column chunks
+    uint8_t* const stage = smem + BAR_OFF - (warp - 3) * C_STAGE_BYTES;
+    for (uint32_t n = 0;; ++n) {
+      int tile;
+      if (!tile_at(n, tile) || tile < 0) break;
+      const uint32_t acc = n & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->acc_full[acc], (n >> 1) & 1, p.status))) break;
+      int tm, tn;
+      coords(tile, tm, tn);
+      const int row0 = tm * (BM * CTAS) + static_cast<int>(rank) * BM + q * 32;
+      const int n0 = tn * width;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * MAX_WIDTH;
+      constexpr int CHUNKS = F32 ? 1 : 2;       // chunks of 32 columns in flight: 2 KiB staged in bf16, 4 in fp32
+      constexpr int BLOCK = C_STAGE_BYTES / CHUNKS;
+#pragma unroll 1
+      for (int c = half; c < width / 32; c += 2 * CHUNKS) {
+        if (row0 >= p.M || n0 + c * 32 >= p.N) break;
+        uint32_t r[CHUNKS][32];
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j)
+          if (j == 0 || c + 2 * j < width / 32) tmem_ld_32x32(taddr + (c + 2 * j) * 32, r[j]);
+        tmem_ld_wait();
+        if (lane == 0) bulk_wait_group_read<0>();      // the previous blocks have left the buffer
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < CHUNKS; ++j) {
+          uint8_t* blk = stage + j * BLOCK;
+          if (!F32) {
+            // 64-byte rows, 16-byte chunks XOR-swizzled by the row pair
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const uint32_t* x = &r[j][8 * v];
+              uint4 o;
+              o.x = pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+              o.y = pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3]));
+              o.z = pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5]));
+              o.w = pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7]));
+              reinterpret_cast<uint4*>(blk + lane * 64)[v ^ ((lane >> 1) & 3)] = o;
+            }
+          } else {
+            // 128-byte rows, 16-byte chunks XOR-swizzled by row
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              reinterpret_cast<uint4*>(blk + lane * 128)[v ^ (lane & 7)] =
+                  make_uint4(r[j][4 * v], r[j][4 * v + 1], r[j][4 * v + 2], r[j][4 * v + 3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+#pragma unroll
+          for (int j = 0; j < CHUNKS; ++j) {
+            const int col0 = n0 + (c + 2 * j) * 32;
+            if (j > 0 && (c + 2 * j >= width / 32 || col0 >= p.N)) continue;
+            if (F32) tma_reduce_add_2d_bulk(&tmap_c, stage + j * BLOCK, col0, row0);
+            else tma_store_2d_bulk(&tmap_c, stage + j * BLOCK, col0, row0);
+          }
+          bulk_commit_group();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CTAS == 2) mbar_arrive_cluster(mapa_u32(smem_u32(&bars->acc_empty[acc]), 0));
+        else mbar_arrive(&bars->acc_empty[acc]);
+      }
+    }
+    if (lane == 0) bulk_wait_group<0>();         // staged blocks must leave before the CTA does
+  }
+
+  tc_fence_before();
+  if (CTAS == 2) cluster_sync(); else __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc_n<CTAS>(tmem_base, 512);
+  }
+  if (p.sched != nullptr && threadIdx.x == 0) {
+    if (atomicAdd(&p.sched[1], 1) == static_cast<int>(gridDim.x) - 1) {   // last CTA rearms the scheduler slot
+      p.sched[0] = 0;
+      p.sched[1] = 0;
+      __threadfence();
+    }
+  }
+}
+
+template <int CTAS, bool F32>
+int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Params& p, int num_sms, cudaStream_t stream) {
+  auto kern = fp8_gemm_kernel<CTAS, F32>;
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return -2;
+    configured = true;
+  }
+  const int tiles = ((p.M + BM * CTAS - 1) / (BM * CTAS)) * ((p.N + p.width - 1) / p.width);
+  const int units = num_sms / CTAS;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(CTAS * (tiles < units ? tiles : units)));
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = CTAS;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CTAS > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, p) == cudaSuccess ? 0 : -3;
+}
+
+// Cycles of a launch by the model of the bf16 products (gemm_cost): an MMA of twice the elements per cycle on elements of half
+// the size leaves the cycles per block of 128 bytes as they are there.
+double cost(int M, int N, int K, bool f32, int ctas, int width, int num_sms) {
+  const double k_blocks = (K + BK - 1) / BK;
+  const long long tiles = static_cast<long long>((M + BM * ctas - 1) / (BM * ctas)) * ((N + width - 1) / width);
+  const long long units = num_sms / ctas;
+  const double rounds = static_cast<double>((tiles + units - 1) / units);
+  const double block = std::max(2.0 * width, (std::min(M, BM) + width / ctas) * BK / 65.0);
+  const double epilogue = 2000 + (f32 ? 15 : 10) * width;
+  return rounds * std::max(k_blocks * block, epilogue) + epilogue + (ctas == 2 ? 2500 : 2000);
+}
+
+GemmShape shape_of(int M, int N, int K, bool f32, int num_sms) {
+  GemmShape best = {1, MAX_WIDTH, 1};
+  double least = 1e300;
+  for (int ctas = 1; ctas <= 2 && ctas <= num_sms; ++ctas)
+    for (int width = MAX_WIDTH; width >= 32; width -= 32) {
+      const double c = cost(M, N, K, f32, ctas, width, num_sms);
+      if (c < least) {
+        least = c;
+        best = {ctas, width, 1};
+      }
+    }
+  return best;
+}
+
+}  // namespace
+
+int fp8_gemm_launch(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
+  if (g.M <= 0 || g.N <= 0 || g.K <= 0) return 0;
+  const GemmShape shape = shape_of(g.M, g.N, g.K, g.add_f32 != 0, num_sms);
+  Params p;
+  p.a_scales = g.a_scales;
+  p.b_scales = g.b_scales;
+  p.M = g.M;
+  p.N = g.N;
+  p.K = g.K;
+  p.a_pad = static_cast<int>(fp8_scale_rows(g.M));
+  p.b_pad = static_cast<int>(fp8_scale_rows(g.N));
+  p.width = shape.width;
+  // rows of A that do not exist need no room in the copy; what the stage holds there reaches no row that is stored
+  p.a_rows = shape.ctas == 1 && g.M < BM ? (g.M + 7) / 8 * 8 : BM;
+  const int b_rows = shape.width / shape.ctas;
+  const int stage = A_STAGE_BYTES + b_rows * BK;
+  p.stages = std::min(MAX_STAGES, OPERAND_BYTES / stage);
+  const int tiles_m = (g.M + BM * shape.ctas - 1) / (BM * shape.ctas), tiles_n = (g.N + shape.width - 1) / shape.width;
+  const bool n_fast = tiles_n < tiles_m;
+  const long long fast_bytes = static_cast<long long>(n_fast ? g.N : g.M) * g.K;
+  p.band = fast_bytes > (96ll << 20) ? 8 : (n_fast ? tiles_n : tiles_m);
+  p.status = g.status;
+  p.sched = gemm_sched_slot();
+  CUtensorMap ta, tb, tc;
+  int rc = make_tmap_2d_u8(&ta, g.a, g.K, g.M, g.lda, BK, p.a_rows);
+  if (rc == 0) rc = make_tmap_2d_u8(&tb, g.b, g.K, g.N, g.ldb, BK, b_rows);
+  if (rc == 0)
+    rc = g.add_f32 ? make_tmap_c_f32(&tc, g.c, g.N, g.M, static_cast<uint64_t>(g.ldc) * 4)
+                   : make_tmap_c_bf16(&tc, g.c, g.N, g.M, static_cast<uint64_t>(g.ldc) * 2);
+  if (rc != 0) return rc;
+  if (shape.ctas == 2) return g.add_f32 ? launch<2, true>(ta, tb, tc, p, num_sms, stream) : launch<2, false>(ta, tb, tc, p, num_sms, stream);
+  return g.add_f32 ? launch<1, true>(ta, tb, tc, p, num_sms, stream) : launch<1, false>(ta, tb, tc, p, num_sms, stream);
+}
+
+}  // namespace piper

@@ -1,0 +1,201 @@
+// bf16 matrices to e4m3 codes with power-of-two scales, and back.
+//
+// The scale of a group is 2^e with the smallest e at which its largest magnitude is at most 448 * 2^e, 448 being the largest
+// e4m3 number: 448 = 1.75 * 2^8, so e is the exponent of the largest magnitude minus 8, or minus 7 if its mantissa exceeds
+// 1.75; bounded below by -127, the least a scale can say.  Dividing by a power of two is exact, so a code is the group's
+// element rounded once, to the nearest code and ties to even, wherever it is computed.  A group with a NaN or an
+// infinity has the scale NaN.
+//
+// What bounds it: memory.  A CTA takes 128 x 128 elements in one read and writes the codes along the rows, along the
+// columns (which the gradient of the weights contracts over) or both: 2 bytes in, 1 or 2 out.  A thread holds eight rows of eight
+// columns, so the eight codes of a column are one 8-byte word of the turned matrix; the words cross the CTA through shared memory
+// to leave it in rows of 128 bytes.
+#include "fp8.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "ptx.cuh"
+
+namespace piper {
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int TILE = 128;
+
+// |x| as bits of an fp32 number, from the bits of a bf16 one; NaN and infinity compare above all others.
+__device__ __forceinline__ uint32_t most2(uint32_t most, uint32_t pair) {
+  return max(max(most, (pair << 16) & 0x7FFFFFFFu), pair & 0x7FFF0000u);
+}
+
+// The exponent, with its bias, of the scale for a largest magnitude given by its fp32 bits.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
+  const int field = static_cast<int>(most >> 23);
+  if (field == 255) return 255u;
+  return static_cast<uint32_t>(max(0, field - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0)));
+}
+
+// 2^-e: what elements are multiplied by.  e is 120 at most, and -127 at least, whose inverse is a normal number.
+__device__ __forceinline__ float inverse_scale(uint32_t byte) {
+  return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+}
+
+// Four codes of fp32 values, the first in the lowest byte.
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+__device__ __forceinline__ float low_half(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float high_half(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
+
+// Thread t: columns 8 (t % 16) to + 7, rows 8 (t / 16) to + 7.
+template <bool SQUARE>
+__global__ void __launch_bounds__(THREADS)
+fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long long cols, long long ldx, Fp8Out plain, Fp8Out turned) {
+  grid_begin(x);
+  __shared__ __align__(16) uint8_t turn[TILE * TILE];
+  __shared__ uint32_t col_most[THREADS / 32][TILE];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const long long col0 = static_cast<long long>(blockIdx.x) * TILE, row0 = static_cast<long long>(blockIdx.y) * TILE;
+  const long long c0 = col0 + 8 * l, r0 = row0 + 8 * g;
+  uint4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = c0 < cols && r0 + i < rows ? __ldcs(reinterpret_cast<const uint4*>(x + (r0 + i) * ldx + c0)) : make_uint4(0, 0, 0, 0);
+
+  uint32_t row_most[8];                          // of the thread's rows over all columns of the tile
+  uint32_t mine[8];                              // of the thread's columns, then of all rows of the tile
+#pragma unroll
+  for (int i = 0; i < 8; ++i) row_most[i] = most2(most2(most2(most2(0, v[i].x), v[i].y), v[i].z), v[i].w);
+  if (SQUARE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, row_most[i]);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) col_most[0][warp] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) m = max(m, col_most[0][w]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) row_most[i] = mine[i] = m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) row_most[i] = max(row_most[i], __shfl_xor_sync(0xffffffffu, row_most[i], o));
+    if (turned.codes != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mine[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t q[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mine[2 * j] = max(mine[2 * j], (q[j] << 16) & 0x7FFFFFFFu);
+          mine[2 * j + 1] = max(mine[2 * j + 1], q[j] & 0x7FFF0000u);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        mine[j] = max(mine[j], __shfl_xor_sync(0xffffffffu, mine[j], 16));
+        if (lane < 16) col_most[warp][8 * l + j] = mine[j];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        mine[j] = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) mine[j] = max(mine[j], col_most[w][8 * l + j]);
+      }
+    }
+  }
+
+  // The bytes of word (group of four, row); the last tile of a row fills the word.
+  auto put_scale = [&](const Fp8Out& o, long long block, long long blocks, long long row, long long pad, uint32_t byte) {
+    uint8_t* word = reinterpret_cast<uint8_t*>(o.scales + block / 4 * pad + row);
+    word[block & 3] = static_cast<uint8_t>(byte);
+    if (block == blocks - 1)
+      for (int b = static_cast<int>(block & 3) + 1; b < 4; ++b) word[b] = 0;
+  };
+  if (plain.codes != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t byte = scale_byte(row_most[i]);
+      const float inv = inverse_scale(byte);
+      const uint2 o = make_uint2(codes4(low_half(v[i].x) * inv, high_half(v[i].x) * inv, low_half(v[i].y) * inv, high_half(v[i].y) * inv),
+                                 codes4(low_half(v[i].z) * inv, high_half(v[i].z) * inv, low_half(v[i].w) * inv, high_half(v[i].w) * inv));
+      if (r0 + i < rows && c0 < cols) *reinterpret_cast<uint2*>(plain.codes + (r0 + i) * plain.ld + c0) = o;
+      if (l == i)        // rows behind the end have words too, of zeros' scale
+        put_scale(plain, blockIdx.x, gridDim.x, r0 + i, static_cast<long long>(gridDim.y) * TILE, byte);
+    }
+  }
+  if (turned.codes != nullptr) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t byte = scale_byte(mine[j]);
+      const float inv = inverse_scale(byte);
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t q = j < 2 ? v[i].x : j < 4 ? v[i].y : j < 6 ? v[i].z : v[i].w;
+        f[i] = (j & 1 ? high_half(q) : low_half(q)) * inv;
+      }
+      // word g of column 8 l + j, moved by l: the sixteen threads of a half warp meet sixteen pairs of banks
+      *reinterpret_cast<uint2*>(turn + (8 * l + j) * TILE + ((g ^ l) * 8)) =
+          make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
+      if (g == j) put_scale(turned, blockIdx.y, gridDim.y, c0 + j, static_cast<long long>(gridDim.x) * TILE, byte);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TILE * TILE / 16 / THREADS; ++k) {
+      const int c = (threadIdx.x + k * THREADS) / 8, part = threadIdx.x & 7;       // column of x, 16 of its rows
+      const int moved = c / 8;
+      uint4 o = *reinterpret_cast<const uint4*>(turn + c * TILE + ((2 * part ^ moved) & ~1) * 8);
+      if (moved & 1) o = make_uint4(o.z, o.w, o.x, o.y);
+      // ld is rows rounded up to 16: what is behind the rows is zeros
+      if (col0 + c < cols && row0 + 16 * part < turned.ld)
+        *reinterpret_cast<uint4*>(turned.codes + (col0 + c) * turned.ld + row0 + 16 * part) = o;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(THREADS)
+fp8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint32_t* __restrict__ scales, long long ld, float* __restrict__ out,
+                      long long rows, long long cols, long long pad) {
+  grid_begin(codes, scales);
+  const long long n = rows * cols;
+  for (long long i = static_cast<long long>(blockIdx.x) * THREADS + threadIdx.x; i < n; i += static_cast<long long>(gridDim.x) * THREADS) {
+    const long long r = i / cols, c = i - r * cols, block = c / kFp8Group;
+    const uint32_t byte = scales[block / 4 * pad + r] >> (8 * (block & 3)) & 255u;
+    const __half_raw h = __nv_cvt_fp8_to_halfraw(codes[r * ld + c], __NV_E4M3);
+    const float scale = byte == 255u ? __uint_as_float(0x7FC00000u) : byte == 0 ? __uint_as_float(1u << 22) : __uint_as_float(byte << 23);
+    out[i] = __half2float(__half(h)) * scale;
+  }
+}
+
+}  // namespace
+
+int fp8_quantize(const void* x, long long rows, long long cols, long long ldx, int square, const Fp8Out& plain, const Fp8Out& turned,
+                 cudaStream_t st) {
+  if (rows == 0 || cols == 0) return 0;
+  const long long by = (rows + TILE - 1) / TILE, bx = (cols + TILE - 1) / TILE;
+  if (by > 65535 || bx > INT32_MAX || cols % 16 != 0 || ldx % 8 != 0) return -1;
+  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by));
+  const auto kernel = square ? fp8_quantize_kernel<true> : fp8_quantize_kernel<false>;
+  return launch_overlapped(kernel, grid, THREADS, 0, st, static_cast<const __nv_bfloat16*>(x), rows, cols, ldx, plain, turned) ==
+                 cudaSuccess ? 0 : -3;
+}
+
+int fp8_dequantize(const uint8_t* codes, const uint32_t* scales, long long ld, float* out, long long rows, long long cols, cudaStream_t st) {
+  if (rows == 0 || cols == 0) return 0;
+  const long long want = (rows * cols + 8 * THREADS - 1) / (8 * THREADS);
+  const dim3 grid(static_cast<unsigned>(want < 65536 ? want : 65536));
+  return launch_overlapped(fp8_dequantize_kernel, grid, THREADS, 0, st, codes, scales, ld, out, rows, cols, fp8_scale_rows(rows)) ==
+                 cudaSuccess ? 0 : -3;
+}
+
+}  // namespace piper

@@ -428,8 +428,8 @@ int* gemm_sched_slot() {
   return pool == nullptr ? nullptr : pool + 2 * (counter++ % kSchedSlots);
 }
 
-int make_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer,
-                      uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+static int make_tmap_2d(CUtensorMap* out, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
+                        uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer) {
   EncodeFn fn = get_encode_fn();
   if (fn == nullptr) return -1;
   // The driver entry point needs a current context on the calling thread;
@@ -444,10 +444,20 @@ int make_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t inner, uint64
   const cuuint32_t box[2] = {box_inner, box_outer};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r =
-      fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+      fn(out, type, 2, const_cast<void*>(base), dims, strides, box, estr,
          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : static_cast<int>(r);
+}
+
+int make_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer,
+                      uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer) {
+  return make_tmap_2d(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, inner, outer, row_stride_bytes, box_inner, box_outer);
+}
+
+int make_tmap_2d_u8(CUtensorMap* out, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
+                    uint32_t box_inner, uint32_t box_outer) {
+  return make_tmap_2d(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, row_stride_bytes, box_inner, box_outer);
 }
 
 // fp32 tensor map of C with 32x32 boxes and 128-byte swizzle (epilogue staging layout).
@@ -465,7 +475,7 @@ int make_tmap_c_f32(CUtensorMap* out, const void* base, uint64_t cols, uint64_t 
 }
 
 // bf16 tensor map of C with 32x32 boxes and 64-byte swizzle.
-static int make_tmap_c_bf16(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes) {
+int make_tmap_c_bf16(CUtensorMap* out, const void* base, uint64_t cols, uint64_t rows, uint64_t row_stride_bytes) {
   EncodeFn fn = get_encode_fn();
   if (fn == nullptr) return -1;
   const cuuint64_t dims[2] = {cols, rows};

@@ -14,11 +14,12 @@ from .core import (
     swiglu,
     wgrad_store,
 )
+from .fp8 import Fp8Matrix, fp8_linear, fp8_matmul, fp8_quantize
 from .logprobs import TokenLogprobs, token_logprobs
 from .optim import AdamWState, adamw_step
 
 __all__ = [
     "native", "linear", "rmsnorm", "add_rmsnorm", "qk_rope", "residual_add", "rope_tables", "attention", "swiglu",
     "embedding", "cross_entropy", "token_logprobs", "TokenLogprobs", "AdamWState",
-    "adamw_step", "grad_sinks", "wgrad_store",
+    "adamw_step", "Fp8Matrix", "fp8_linear", "fp8_matmul", "fp8_quantize", "grad_sinks", "wgrad_store",
 ]

@@ -1,0 +1,259 @@
+"""Matrix products in 8-bit floating point with a scale for every 128 elements of the contraction.
+
+Operands are rounded to e4m3.  Activations and output gradients have a scale for every 128 neighbouring elements along the
+contraction (``1 x 128``), weights one for every ``128 x 128``, so that a weight and its transpose have the same codes.
+A scale is the smallest power of two that brings the group's largest magnitude to 448, the largest e4m3 number; scaling
+is then exact, and an operand is rounded once.  Sums are kept in fp32 (``csrc/fp8_gemm_sm100.cu``).
+
+``fp8_linear`` is ``linear`` with all three products of a training step in 8 bits: the gradient of the input contracts
+over the weights' rows, the gradient of the weights over the tokens, for which input and output gradient are rounded in
+groups of 128 tokens.  Its backward pass keeps the 8-bit operands, not the bf16 input.  A group with a NaN or an infinity is NaN.
+"""
+from __future__ import annotations
+
+from typing import Union
+
+import torch
+from torch import Tensor
+
+from . import native
+from .core import grad_sinks, wgrad_store
+from .registry import custom_op
+
+GROUP = 128
+_NAN_SCALE = 255
+
+
+class Fp8Matrix:
+    """A matrix ``[rows, cols]`` in e4m3, ready as an operand of a product along ``cols``.
+
+    ``codes`` is uint8 ``[rows, >= cols]``; ``scales`` holds the exponents of the powers of two, with a bias of 127 (255: NaN),
+    of four neighbouring groups of a row in one int32, ``[ceil(cols / 512), rows rounded up to 128]``.
+    """
+
+    def __init__(self, codes: Tensor, scales: Tensor, rows: int, cols: int) -> None:
+        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.cols
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def dequantize(self) -> Tensor:
+        """The values that the codes stand for, in fp32."""
+        if self.codes.is_cuda:
+            out = torch.empty(self.rows, self.cols, dtype=torch.float32, device=self.device)
+            native.lib().fp8_dequantize(self.codes, self.scales, out)
+            return out
+        return _values_ref(self.codes, self.scales, self.rows, self.cols)
+
+    def __repr__(self) -> str:
+        return f"Fp8Matrix({self.rows}, {self.cols}, device={self.device})"
+
+
+# ------------------------------------------------------------------ plain form (CPU)
+def _quantize_ref(x: Tensor, square: bool) -> tuple[Tensor, Tensor]:
+    """Codes and words of scales of x [rows, cols] along its columns."""
+    rows, cols = x.shape
+    if x.numel() == 0:
+        return _operand_buffers(rows, cols, x)
+    R, C = (rows + GROUP - 1) // GROUP, (cols + GROUP - 1) // GROUP
+    pad = torch.zeros(R * GROUP, C * GROUP, dtype=torch.float32)
+    pad[:rows, :cols] = x
+    h = GROUP if square else 1
+    tiles = pad.view(R * GROUP // h, h, C, GROUP)
+    most = tiles.abs().amax((1, 3), keepdim=True)
+    most = torch.where(torch.isfinite(tiles).all(3, keepdim=True).all(1, keepdim=True), most, torch.full_like(most, float("inf")))
+    bits = most.view(torch.int32)
+    byte = torch.where(torch.isinf(most), torch.full_like(bits, _NAN_SCALE),
+                       ((bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000).int()).clamp(min=0))
+    inverse = torch.where(byte == _NAN_SCALE, torch.zeros_like(byte), (254 - byte) << 23).view(torch.float32)
+    codes = torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.uint8)
+    codes[:, :cols] = (tiles * inverse).view(pad.shape)[:rows, :cols].contiguous().to(torch.float8_e4m3fn).view(torch.uint8)
+    words = torch.zeros((C + 3) // 4 * 4, R * GROUP, dtype=torch.uint8)
+    words[:C] = byte.view(R * GROUP // h, 1, C).expand(-1, h, C).reshape(R * GROUP, C).t().to(torch.uint8)
+    return codes, words.view(-1, 4, R * GROUP).transpose(1, 2).contiguous().view(torch.int32).squeeze(2)
+
+
+def _values_ref(codes: Tensor, scales: Tensor, rows: int, cols: int) -> Tensor:
+    groups, pad = scales.shape
+    byte = scales.unsqueeze(2).contiguous().view(torch.uint8).view(groups, pad, 4).transpose(1, 2).reshape(groups * 4, pad)
+    byte = byte[:(cols + GROUP - 1) // GROUP, :rows].t().to(torch.int32)
+    scale = torch.where(byte > 0, byte << 23, torch.full_like(byte, 1 << 22)).view(torch.float32)
+    scale = torch.where(byte == _NAN_SCALE, torch.full_like(scale, float("nan")), scale)
+    values = codes[:, :cols].contiguous().view(torch.float8_e4m3fn).to(torch.float32)
+    return values * scale.repeat_interleave(GROUP, 1)[:, :cols]
+
+
+# ------------------------------------------------------------------ rounding
+def _operand_buffers(rows: int, cols: int, like: Tensor) -> tuple[Tensor, Tensor]:
+    return (torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.uint8, device=like.device),
+            torch.empty((cols + 4 * GROUP - 1) // (4 * GROUP), (rows + GROUP - 1) // GROUP * GROUP, dtype=torch.int32,
+                        device=like.device))
+
+
+def _nothing(like: Tensor) -> tuple[Tensor, Tensor]:
+    return like.new_empty((0, 0), dtype=torch.uint8), like.new_empty((0, 0), dtype=torch.int32)
+
+
+def _quantize(x: Tensor, square: bool, plain: bool, turned: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(codes, scales) of x along its columns and of x^T along the rows of x; what is not wanted is empty."""
+    rows, cols = x.shape
+    p, t = _nothing(x), _nothing(x)
+    if x.is_cuda:
+        if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+        if plain:
+            p = _operand_buffers(rows, cols, x)
+        if turned:
+            t = _operand_buffers(cols, rows, x)
+        native.lib().fp8_quantize(x, square, *(p if plain else (None, None)), *(t if turned else (None, None)))
+    else:
+        if plain:
+            p = _quantize_ref(x, square)
+        if turned:
+            t = _quantize_ref(x.t(), square)
+    return (*p, *t)
+
+
+def _product(a: tuple[Tensor, Tensor], b: tuple[Tensor, Tensor], M: int, N: int, K: int, out: Tensor) -> Tensor:
+    """a [M, K] b [N, K]^T into ``out``; on a GPU into bf16, or added to fp32."""
+    if out.is_cuda:
+        if M and N:
+            native.lib().fp8_gemm(*a, *b, out, K, native.status_tensor(out.device))
+        return out
+    return out.copy_(_values_ref(*a, M, K) @ _values_ref(*b, N, K).t())
+
+
+def _check_matrix(x: Tensor, what: str) -> None:
+    if x.dim() != 2 or x.shape[0] == 0 or x.shape[1] == 0 or x.shape[1] % 16:
+        raise ValueError(f"{what}: expected [rows, cols] with a multiple of 16 columns, got {tuple(x.shape)}")
+    _check_type(x, what)
+
+
+def _check_type(x: Tensor, what: str) -> None:
+    if x.dtype != torch.bfloat16 and (x.is_cuda or x.dtype != torch.float32):
+        raise TypeError(f"{what}: the sm_100a kernels take bfloat16 tensors, got {x.dtype}")
+
+
+def fp8_quantize(x: Tensor, *, square: bool = False, transpose: bool = False) -> Fp8Matrix:
+    """``x`` [rows, cols] (or, with ``transpose``, its transpose) in e4m3, with a scale for every 128 elements along the columns
+    of the result, or with ``square`` for every 128 x 128, as weights have it.  No gradient passes."""
+    _check_matrix(x, "fp8_quantize")
+    with torch.no_grad():
+        codes, scales, turned, turned_scales = _quantize(x.detach(), square, not transpose, transpose)
+    return Fp8Matrix(turned, turned_scales, x.shape[1], x.shape[0]) if transpose else Fp8Matrix(codes, scales, *x.shape)
+
+
+def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix) -> Tensor:
+    """a [M, K] b [N, K]^T in bf16 (fp32 on the CPU); N must be a multiple of 8."""
+    if a.cols != b.cols:
+        raise ValueError(f"fp8_matmul: contraction mismatch: {a.shape} and {b.shape}")
+    if a.device != b.device:
+        raise ValueError(f"fp8_matmul: operands on {a.device} and {b.device}")
+    if b.rows % 8:
+        raise ValueError(f"fp8_matmul: the product must have a multiple of 8 columns, got {b.rows}")
+    out = torch.empty(a.rows, b.rows, dtype=torch.bfloat16 if a.codes.is_cuda else torch.float32, device=a.device)
+    return _product((a.codes, a.scales), (b.codes, b.scales), a.rows, b.rows, a.cols, out)
+
+
+# ------------------------------------------------------------------ linear layer
+@custom_op("piper::fp8_linear_fwd")
+def fp8_linear_fwd(x: Tensor, w: Tensor, keep_x: bool, keep_w: bool) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """y [T, N] = x [T, K] w [N, K]^T, and the transposed operands that the backward pass wants: x^T [K, T] for the gradient of
+    w (keep_x), w^T [K, N] for the gradient of x (keep_w)."""
+    xc, xs, xt, xts = _quantize(x, False, True, keep_x)
+    wc, ws, wt, wts = _quantize(w, True, True, keep_w)
+    y = torch.empty(x.shape[0], w.shape[0], dtype=x.dtype, device=x.device)
+    _product((xc, xs), (wc, ws), x.shape[0], w.shape[0], x.shape[1], y)
+    return y, xt, xts, wt, wts
+
+
+@fp8_linear_fwd.register_fake
+def _(x, w, keep_x, keep_w):
+    T, (N, K) = x.shape[0], w.shape
+
+    def operand(rows, cols, wanted):
+        if not wanted:
+            return x.new_empty((0, 0), dtype=torch.uint8), x.new_empty((0, 0), dtype=torch.int32)
+        return (x.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8),
+                x.new_empty(((cols + 4 * GROUP - 1) // (4 * GROUP), (rows + GROUP - 1) // GROUP * GROUP), dtype=torch.int32))
+
+    return (x.new_empty((T, N)), *operand(K, T, keep_x), *operand(K, N, keep_w))
+
+
+def _linear_setup(ctx, inputs, output):
+    x, w, keep_x, keep_w = inputs
+    ctx.x_shape = tuple(x.shape)
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.save_for_backward(w, *output[1:])
+
+
+def _fp8_wgrad(dyt: Tensor, dyts: Tensor, xt: Tensor, xts: Tensor, w: Tensor, T: int):
+    """dW [N, K] = dY^T X, into the weight's fp32 bucket if it has one (returns None then)."""
+    N, K = w.shape
+    sink = grad_sinks.get(w)
+    if T == 0:
+        return None if sink is not None else torch.zeros_like(w)
+    if sink is not None:
+        if w.is_cuda:
+            _product((dyt, dyts), (xt, xts), N, K, T, sink)
+        else:
+            sink.add_(_values_ref(dyt, dyts, N, T) @ _values_ref(xt, xts, K, T).t())
+        return None
+    return _product((dyt, dyts), (xt, xts), N, K, T, torch.empty_like(w, memory_format=torch.contiguous_format))
+
+
+def _linear_backward(ctx, dy, *_unused):
+    w, xt, xts, wt, wts = ctx.saved_tensors
+    need_x, need_w = ctx.needs_input_grad[:2]
+    T, K = ctx.x_shape
+    N = w.shape[0]
+    if dy is None:
+        return (w.new_zeros((T, K)) if need_x else None, torch.zeros_like(w) if need_w else None, None, None)
+    dyc, dys, dyt, dyts = _quantize(dy, False, need_x, need_w)
+    dx = dw = None
+    if need_x:
+        dx = _product((dyc, dys), (wt, wts), T, K, N, torch.empty((T, K), dtype=dy.dtype, device=dy.device))
+    if need_w:
+        if wgrad_store.active is not None:
+            wgrad_store.active.append((lambda: _fp8_wgrad(dyt, dyts, xt, xts, w, T), w))
+        else:
+            dw = _fp8_wgrad(dyt, dyts, xt, xts, w, T)
+    return dx, dw, None, None
+
+
+fp8_linear_fwd.register_autograd(_linear_backward, setup_context=_linear_setup)
+fp8_linear_fwd = fp8_linear_fwd.overload
+
+
+def fp8_linear(x: Tensor, w: Union[Tensor, Fp8Matrix]) -> Tensor:
+    """y[..., N] = x[..., K] @ w[N, K]^T with both operands rounded to e4m3; so are those of its gradients' products.
+
+    ``w`` may be a weight that was rounded before (``fp8_quantize(w, square=True)``), for calls without gradients.  K and N are
+    multiples of 16; there may be any number of rows.
+    """
+    kept = isinstance(w, Fp8Matrix)
+    N, K = w.shape
+    _check_type(x, "fp8_linear")
+    if x.dim() < 1 or x.shape[-1] != K or K == 0 or N == 0 or K % 16 or N % 16:
+        raise ValueError(f"fp8_linear: x {tuple(x.shape)} and w {(N, K)}: features must agree and be multiples of 16")
+    if x.device != w.device:
+        raise ValueError(f"fp8_linear: x is on {x.device}, w on {w.device}")
+    lead = x.shape[:-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if kept:
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise ValueError("fp8_linear: a weight that was rounded before has no backward pass; give the bf16 weight")
+        codes, scales, _, _ = _quantize(x2.detach(), False, True, False)
+        y = torch.empty(x2.shape[0], N, dtype=x.dtype, device=x.device)
+        _product((codes, scales), (w.codes, w.scales), x2.shape[0], N, K, y)
+    else:
+        if w.dtype != x.dtype:
+            raise TypeError(f"fp8_linear: x is {x.dtype}, w {w.dtype}")
+        grad = torch.is_grad_enabled()
+        y = fp8_linear_fwd(x2, w, grad and w.requires_grad, grad and x.requires_grad)[0]
+    return y if x.dim() == 2 else y.view(*lead, N)
