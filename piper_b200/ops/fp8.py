@@ -17,8 +17,8 @@ import torch
 from torch import Tensor
 
 from . import native
-from .core import grad_sinks, wgrad_store
-from .registry import custom_op
+from .core import HostContext, grad_sinks, wgrad_store
+from .registry import custom_op, host_op
 
 GROUP = 128
 _NAN_SCALE = 255
@@ -227,7 +227,34 @@ def _linear_backward(ctx, dy, *_unused):
 
 
 fp8_linear_fwd.register_autograd(_linear_backward, setup_context=_linear_setup)
+
+
+def _linear_backward_host(dy: Tensor, saved: list[Tensor], T: int, need_x: bool, need_w: bool) -> tuple[Tensor, Tensor]:
+    ctx = HostContext(saved, (need_x, need_w))
+    ctx.x_shape = (T, saved[0].shape[1])
+    dx, dw, _, _ = _linear_backward(ctx, dy)
+    none = torch.empty(0)
+    return none if dx is None else dx, none if dw is None else dw
+
+
+host_op("fp8_linear_backward_host", _linear_backward_host)
+
+
+@custom_op("piper::fp8_linear_kept")
+def fp8_linear_kept(x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
+    """y [T, N] = x [T, K] w^T of a weight [N, K] that was rounded before."""
+    (T, K), N = x.shape, codes.shape[0]
+    xc, xs, _, _ = _quantize(x, False, True, False)
+    return _product((xc, xs), (codes, scales), T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device))
+
+
+@fp8_linear_kept.register_fake
+def _(x, codes, scales):
+    return x.new_empty((x.shape[0], codes.shape[0]))
+
+
 fp8_linear_fwd = fp8_linear_fwd.overload
+fp8_linear_kept = fp8_linear_kept.overload
 
 
 def fp8_linear(x: Tensor, w: Union[Tensor, Fp8Matrix]) -> Tensor:
@@ -248,9 +275,7 @@ def fp8_linear(x: Tensor, w: Union[Tensor, Fp8Matrix]) -> Tensor:
     if kept:
         if torch.is_grad_enabled() and x.requires_grad:
             raise ValueError("fp8_linear: a weight that was rounded before has no backward pass; give the bf16 weight")
-        codes, scales, _, _ = _quantize(x2.detach(), False, True, False)
-        y = torch.empty(x2.shape[0], N, dtype=x.dtype, device=x.device)
-        _product((codes, scales), (w.codes, w.scales), x2.shape[0], N, K, y)
+        y = fp8_linear_kept(x2, w.codes, w.scales)
     else:
         if w.dtype != x.dtype:
             raise TypeError(f"fp8_linear: x is {x.dtype}, w {w.dtype}")
