@@ -46,8 +46,7 @@ __device__ __forceinline__ float decode_v(uint32_t c, float scale) {
 }
 __device__ __forceinline__ float decode_m(uint32_t c, float scale) {
   const uint32_t low = c & 127u;
-  const float x = __fmul_rn(low != 0 ? __uint_as_float((low + M_BASE) << 20) : 0.f, scale);
-  return c >= 128u ? -x : x;
+  return __fmul_rn(__uint_as_float((low != 0 ? (low + M_BASE) << 20 : 0u) | (c & 128u) << 24), scale);
 }
 
 // y in [0, 1] to its code; r: 16 random bits.
@@ -72,8 +71,45 @@ __device__ __forceinline__ float block_scale(const float (&x)[PER]) {
   return most >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(most);
 }
 
+// x / scale, correctly rounded, for 0 <= x <= scale.  With the correctly rounded reciprocal, a product, its exact remainder and a
+// correction give the quotient (Markstein, IBM J. Res. Dev. 34, 1990) where nothing underflows: a quotient that is not small enough for
+// code 0 or 1 anyway comes from x above 2^-101, whose remainder is a normal number, if the scale is above 2^-60.  Other blocks
+// divide.
+struct Quotient {
+  float scale, inverse;
+  bool quick;
+
+  __device__ __forceinline__ explicit Quotient(float s) : scale(s > 0.f ? s : 1.f) {
+    inverse = __frcp_rn(scale);
+    quick = scale >= 8.67361738e-19f && scale <= 1.f;
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    if (!quick) return __fdiv_rn(x, scale);
+    const float q = __fmul_rn(x, inverse);
+    return __fmaf_rn(__fmaf_rn(-q, scale, x), inverse, q);
+  }
+};
+
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ void load4(const float* p, float (&x)[PER], int h) {
+  const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
+  x[4 * h] = v.x;
+  x[4 * h + 1] = v.y;
+  x[4 * h + 2] = v.z;
+  x[4 * h + 3] = v.w;
+}
+__device__ __forceinline__ void store4(float* p, const float (&x)[PER], int h) {
+  __stcs(reinterpret_cast<float4*>(p), make_float4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]));
+}
+
+// A warp takes a block: lane l has elements 4 l to 4 l + 3 of either half, so that its vectors are neighbours of the next lane's.
 template <int BITS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, BITS == 8 ? 4 : 3)
 adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
   grid_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -88,127 +124,150 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
     const AdamwTensor& t = table.t[lo];
     const long long n = t.n;
     const float rate = t.rate, root = t.root;
-    const uintptr_t low = reinterpret_cast<uintptr_t>(t.weight) | reinterpret_cast<uintptr_t>(t.grad) |
-                          reinterpret_cast<uintptr_t>(t.param);
+    const bool aligned = ((reinterpret_cast<uintptr_t>(t.weight) | reinterpret_cast<uintptr_t>(t.grad) |
+                           reinterpret_cast<uintptr_t>(t.param)) & 15u) == 0;
     for (int b = warp; b < CHUNK_BLOCKS; b += WARPS) {
       const long long i0 = (static_cast<long long>(chunk - table.first[lo]) * CHUNK_BLOCKS + b) * kMomentBlock;
       if (i0 >= n) break;
-      const long long i = i0 + lane * PER;
-      const int left = static_cast<int>(min(static_cast<long long>(PER), n - i));      // of this lane; may be negative
-      const bool vec = left == PER && (low & 15u) == 0;
-      const long long block = (t.at + i0) / kMomentBlock, s = t.at + i;
+      const bool whole = i0 + kMomentBlock <= n, vec = whole && aligned;
+      const long long i = i0 + lane * 4, s = t.at + i, block = (t.at + i0) / kMomentBlock;
+      // element of register j, and whether it exists
+      auto at = [&](int j) { return i + (j / 4) * 128 + (j & 3); };
+      auto is = [&](int j) { return whole || at(j) < n; };
       float w[PER], g[PER], m[PER], v[PER];
-      // gradient and weight; what is behind the end is 0
-      if (vec) {
-        const float4 w0 = *reinterpret_cast<const float4*>(t.weight + i), w1 = *reinterpret_cast<const float4*>(t.weight + i + 4);
-        w[0] = w0.x; w[1] = w0.y; w[2] = w0.z; w[3] = w0.w; w[4] = w1.x; w[5] = w1.y; w[6] = w1.z; w[7] = w1.w;
-        if (t.grad_bf16) {
-          const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(t.grad) + i);
-          const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+      uint32_t mc[2], vc[2];
+      float ms = 0.f, vs = 0.f;
+      if (BITS == 8) {
+        // the moments' buffers are aligned and hold whole blocks, zeros behind the end
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            g[2 * j] = __uint_as_float(q[j] << 16);
-            g[2 * j + 1] = __uint_as_float(q[j] & 0xFFFF0000u);
-          }
-        } else {
-          const float* gp = static_cast<const float*>(t.grad) + i;
-          const float4 g0 = *reinterpret_cast<const float4*>(gp), g1 = *reinterpret_cast<const float4*>(gp + 4);
-          g[0] = g0.x; g[1] = g0.y; g[2] = g0.z; g[3] = g0.w; g[4] = g1.x; g[5] = g1.y; g[6] = g1.z; g[7] = g1.w;
+        for (int h = 0; h < 2; ++h) {
+          mc[h] = __ldcs(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + s + 128 * h));
+          vc[h] = __ldcs(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + s + 128 * h));
         }
+        ms = a.m_scale[block];
+        vs = a.v_scale[block];
       } else {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          w[j] = j < left ? t.weight[i + j] : 0.f;
-          g[j] = j >= left ? 0.f
-                 : t.grad_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(t.grad)[i + j])
-                               : static_cast<const float*>(t.grad)[i + j];
+        for (int h = 0; h < 2; ++h) {
+          load4(static_cast<const float*>(a.m) + s + 128 * h, m, h);
+          load4(static_cast<const float*>(a.v) + s + 128 * h, v, h);
         }
       }
-      // the moments' buffers are aligned and hold whole blocks, zeros behind the end
-      if (BITS == 8) {
-        const uint2 mc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + s);
-        const uint2 vc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + s);
-        const float ms = a.m_scale[block], vs = a.v_scale[block];
+      if (vec) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          m[j] = decode_m(((j < 4 ? mc.x : mc.y) >> (8 * (j & 3))) & 255u, ms);
-          v[j] = decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 255u, vs);
+        for (int h = 0; h < 2; ++h) load4(t.weight + i + 128 * h, w, h);
+        if (t.grad_bf16) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint2 u = __ldcs(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(t.grad) + i + 128 * h));
+            g[4 * h] = __uint_as_float(u.x << 16);
+            g[4 * h + 1] = __uint_as_float(u.x & 0xFFFF0000u);
+            g[4 * h + 2] = __uint_as_float(u.y << 16);
+            g[4 * h + 3] = __uint_as_float(u.y & 0xFFFF0000u);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) load4(static_cast<const float*>(t.grad) + i + 128 * h, g, h);
         }
       } else {
-        const float4* mp = reinterpret_cast<const float4*>(static_cast<const float*>(a.m) + s);
-        const float4* vp = reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + s);
-        const float4 m0 = mp[0], m1 = mp[1], v0 = vp[0], v1 = vp[1];
-        m[0] = m0.x; m[1] = m0.y; m[2] = m0.z; m[3] = m0.w; m[4] = m1.x; m[5] = m1.y; m[6] = m1.z; m[7] = m1.w;
-        v[0] = v0.x; v[1] = v0.y; v[2] = v0.z; v[3] = v0.w; v[4] = v1.x; v[5] = v1.y; v[6] = v1.z; v[7] = v1.w;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          w[j] = is(j) ? t.weight[at(j)] : 0.f;
+          g[j] = !is(j) ? 0.f
+                 : t.grad_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(t.grad)[at(j)])
+                               : static_cast<const float*>(t.grad)[at(j)];
+        }
       }
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
+        if (BITS == 8) {
+          m[j] = decode_m(mc[j / 4] >> (8 * (j & 3)) & 255u, ms);
+          v[j] = decode_v(vc[j / 4] >> (8 * (j & 3)) & 255u, vs);
+        }
         const float gj = __fmul_rn(g[j], a.grad_scale);
         m[j] = __fadd_rn(__fmul_rn(m[j], a.b1), __fmul_rn(gj, a.c1));
         v[j] = __fadd_rn(__fmul_rn(v[j], a.b2), __fmul_rn(__fmul_rn(gj, a.c2), gj));
-        if (j >= left) m[j] = v[j] = 0.f;
-        w[j] = w[j] * a.keep - rate * (m[j] / fmaf(sqrtf(v[j]), root, a.eps));
+        if (!is(j)) m[j] = v[j] = 0.f;
+        // the update's root and quotient are within two units of the last place each
+        w[j] = fmaf(-rate, __fdividef(m[j], fmaf(sqrt_approx(v[j]), root, a.eps)), w[j] * a.keep);
       }
       if (vec) {
-        *reinterpret_cast<float4*>(t.weight + i) = make_float4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<float4*>(t.weight + i + 4) = make_float4(w[4], w[5], w[6], w[7]);
-        if (t.param != nullptr)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(t.param) + i) =
-              make_uint4(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]), pack_bf16x2(w[4], w[5]), pack_bf16x2(w[6], w[7]));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          store4(t.weight + i + 128 * h, w, h);
+          if (t.param != nullptr)
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(t.param) + i + 128 * h) =
+                make_uint2(pack_bf16x2(w[4 * h], w[4 * h + 1]), pack_bf16x2(w[4 * h + 2], w[4 * h + 3]));
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          if (j < left) {
-            t.weight[i + j] = w[j];
-            if (t.param != nullptr) static_cast<__nv_bfloat16*>(t.param)[i + j] = __float2bfloat16(w[j]);
+          if (is(j)) {
+            t.weight[at(j)] = w[j];
+            if (t.param != nullptr) static_cast<__nv_bfloat16*>(t.param)[at(j)] = __float2bfloat16(w[j]);
           }
         }
       }
       if (BITS == 8) {
-        const float ms = block_scale(m), vs = block_scale(v);
-        const float dm = ms > 0.f ? ms : 1.f, dv = vs > 0.f ? vs : 1.f;
-        uint32_t mc[2] = {0, 0}, vc[2] = {0, 0};
+        ms = block_scale(m);
+        vs = block_scale(v);
+        const Quotient over_m(ms), over_v(vs);
+        mc[0] = mc[1] = vc[0] = vc[1] = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          const uint32_t r = mix32(static_cast<uint32_t>(i + j) + t.seed);
-          const uint32_t cm = encode_m(__fdiv_rn(fabsf(m[j]), dm), r & 0xFFFFu) | (m[j] < 0.f ? 128u : 0u);
-          const uint32_t cv = encode_v(__fdiv_rn(v[j], dv), r >> 16);
+          const uint32_t r = mix32(static_cast<uint32_t>(at(j)) + t.seed);
+          const uint32_t cm = encode_m(over_m(fabsf(m[j])), r & 0xFFFFu) | (m[j] < 0.f ? 128u : 0u);
+          const uint32_t cv = encode_v(over_v(v[j]), r >> 16);
           mc[j / 4] |= (cm & 255u) << (8 * (j & 3));
           vc[j / 4] |= (cv & 255u) << (8 * (j & 3));
         }
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s) = make_uint2(mc[0], mc[1]);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s) = make_uint2(vc[0], vc[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          __stcs(reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + s + 128 * h), mc[h]);
+          __stcs(reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + s + 128 * h), vc[h]);
+        }
         if (lane == 0) {
           a.m_scale[block] = ms;
           a.v_scale[block] = vs;
         }
       } else {
-        float4* mp = reinterpret_cast<float4*>(static_cast<float*>(a.m) + s);
-        float4* vp = reinterpret_cast<float4*>(static_cast<float*>(a.v) + s);
-        mp[0] = make_float4(m[0], m[1], m[2], m[3]);
-        mp[1] = make_float4(m[4], m[5], m[6], m[7]);
-        vp[0] = make_float4(v[0], v[1], v[2], v[3]);
-        vp[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          store4(static_cast<float*>(a.m) + s + 128 * h, m, h);
+          store4(static_cast<float*>(a.v) + s + 128 * h, v, h);
+        }
       }
     }
   }
 }
 
-template <bool SIGNED>
+// Both moments: a thread has four codes of each in `AHEAD` places, all loaded before the first is written.
 __global__ void __launch_bounds__(256)
-moments_decode_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, float* __restrict__ out, long long n) {
-  grid_begin(codes, scales);
-  for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += 2048ll * gridDim.x) {
-    const uint2 c = *reinterpret_cast<const uint2*>(codes + i);
-    const float s = scales[i / kMomentBlock];
-    float x[8];
+moments_decode_kernel(const uint32_t* __restrict__ m, const float* __restrict__ m_scale, const uint32_t* __restrict__ v,
+                      const float* __restrict__ v_scale, float4* __restrict__ out_m, float4* __restrict__ out_v, long long words) {
+  grid_begin(m, m_scale, v, v_scale);
+  constexpr int AHEAD = 4;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 * AHEAD + threadIdx.x; i < words; i += 256ll * AHEAD * gridDim.x) {
+    uint32_t cm[AHEAD], cv[AHEAD];
+    float sm[AHEAD], sv[AHEAD];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t k = ((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 255u;
-      x[j] = SIGNED ? decode_m(k, s) : decode_v(k, s);
+    for (int k = 0; k < AHEAD; ++k) {
+      const long long at = i + 256 * k;
+      if (at >= words) break;
+      cm[k] = __ldcs(m + at);
+      cv[k] = __ldcs(v + at);
+      sm[k] = m_scale[at / (kMomentBlock / 4)];
+      sv[k] = v_scale[at / (kMomentBlock / 4)];
     }
-    __stcs(reinterpret_cast<float4*>(out + i), make_float4(x[0], x[1], x[2], x[3]));
-    __stcs(reinterpret_cast<float4*>(out + i + 4), make_float4(x[4], x[5], x[6], x[7]));
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const long long at = i + 256 * k;
+      if (at >= words) break;
+      __stcs(out_m + at, make_float4(decode_m(cm[k] & 255u, sm[k]), decode_m(cm[k] >> 8 & 255u, sm[k]),
+                                     decode_m(cm[k] >> 16 & 255u, sm[k]), decode_m(cm[k] >> 24, sm[k])));
+      __stcs(out_v + at, make_float4(decode_v(cv[k] & 255u, sv[k]), decode_v(cv[k] >> 8 & 255u, sv[k]),
+                                     decode_v(cv[k] >> 16 & 255u, sv[k]), decode_v(cv[k] >> 24, sv[k])));
+    }
   }
 }
 
@@ -230,12 +289,14 @@ int adamw_launch(AdamwTable& table, const AdamwArgs& a, int num_sms, cudaStream_
   return e == cudaSuccess ? 0 : -3;
 }
 
-int moments_decode(const void* codes, const float* scales, float* out, long long n, int is_signed, int num_sms, cudaStream_t st) {
+int moments_decode(const void* m, const float* m_scale, const void* v, const float* v_scale, float* out_m, float* out_v, long long n,
+                   int num_sms, cudaStream_t st) {
   if (n == 0) return 0;
-  const long long want = (n + 2047) / 2048, most = 16ll * num_sms;
+  const long long want = (n + 4095) / 4096, most = 8ll * num_sms;
   const dim3 grid(static_cast<unsigned>(want < most ? want : most));
-  const auto kernel = is_signed ? moments_decode_kernel<true> : moments_decode_kernel<false>;
-  return launch_overlapped(kernel, grid, 256, 0, st, static_cast<const uint8_t*>(codes), scales, out, n) == cudaSuccess ? 0 : -3;
+  return launch_overlapped(moments_decode_kernel, grid, 256, 0, st, static_cast<const uint32_t*>(m), m_scale,
+                           static_cast<const uint32_t*>(v), v_scale, reinterpret_cast<float4*>(out_m),
+                           reinterpret_cast<float4*>(out_v), n / 4) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace piper

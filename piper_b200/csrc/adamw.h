@@ -39,7 +39,8 @@ struct AdamwArgs {
 // table.first, in chunks of adamw_chunk() elements, is filled in here.
 int adamw_launch(AdamwTable& table, const AdamwArgs& a, int num_sms, cudaStream_t st);
 
-// fp32 values of n 8-bit codes (a multiple of kMomentBlock) with their scales.
-int moments_decode(const void* codes, const float* scales, float* out, long long n, int is_signed, int num_sms, cudaStream_t st);
+// fp32 values of n codes of either moment (a multiple of kMomentBlock) with their scales.
+int moments_decode(const void* m, const float* m_scale, const void* v, const float* v_scale, float* out_m, float* out_v, long long n,
+                   int num_sms, cudaStream_t st);
 
 }  // namespace piper

@@ -23,16 +23,15 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int TILE = 128;
 
-// |x| as bits of an fp32 number, from the bits of a bf16 one; NaN and infinity compare above all others.
-__device__ __forceinline__ uint32_t most2(uint32_t most, uint32_t pair) {
-  return max(max(most, (pair << 16) & 0x7FFFFFFFu), pair & 0x7FFF0000u);
-}
+// Magnitudes are compared as the bits of bf16 numbers without their sign, two in a word; NaN and infinity are above all others.
+__device__ __forceinline__ uint32_t magnitudes(uint32_t pair) { return pair & 0x7FFF7FFFu; }
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
 
-// The exponent, with its bias, of the scale for a largest magnitude given by its fp32 bits.
+// The exponent, with its bias, of the scale for a largest magnitude given by its bf16 bits (7 of mantissa).
 __device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
-  const int field = static_cast<int>(most >> 23);
+  const int field = static_cast<int>(most >> 7);
   if (field == 255) return 255u;
-  return static_cast<uint32_t>(max(0, field - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0)));
+  return static_cast<uint32_t>(max(0, field - 8 + ((most & 0x7Fu) > 0x60u ? 1 : 0)));
 }
 
 // 2^-e: what elements are multiplied by.  e is 120 at most, and -127 at least, whose inverse is a normal number.
@@ -52,11 +51,11 @@ __device__ __forceinline__ float high_half(uint32_t pair) { return __uint_as_flo
 
 // Thread t: columns 8 (t % 16) to + 7, rows 8 (t / 16) to + 7.
 template <bool SQUARE>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 3)
 fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long long cols, long long ldx, Fp8Out plain, Fp8Out turned) {
   grid_begin(x);
   __shared__ __align__(16) uint8_t turn[TILE * TILE];
-  __shared__ uint32_t col_most[THREADS / 32][TILE];
+  __shared__ __align__(16) uint32_t col_most[THREADS / 32][TILE / 2];      // two columns in a word
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
   const long long col0 = static_cast<long long>(blockIdx.x) * TILE, row0 = static_cast<long long>(blockIdx.y) * TILE;
@@ -66,50 +65,52 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
   for (int i = 0; i < 8; ++i)
     v[i] = c0 < cols && r0 + i < rows ? __ldcs(reinterpret_cast<const uint4*>(x + (r0 + i) * ldx + c0)) : make_uint4(0, 0, 0, 0);
 
-  uint32_t row_most[8];                          // of the thread's rows over all columns of the tile
-  uint32_t mine[8];                              // of the thread's columns, then of all rows of the tile
+  uint32_t row_most[4];                          // of the thread's rows over all columns of the tile, two in a word
+  uint32_t col_of[4] = {0, 0, 0, 0};             // of the thread's columns over all rows of the tile, likewise
 #pragma unroll
-  for (int i = 0; i < 8; ++i) row_most[i] = most2(most2(most2(most2(0, v[i].x), v[i].y), v[i].z), v[i].w);
+  for (int i = 0; i < 4; ++i) {
+    uint32_t m[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4& q = v[2 * i + h];
+      m[h] = max2(max2(magnitudes(q.x), magnitudes(q.y)), max2(magnitudes(q.z), magnitudes(q.w)));
+    }
+    // even columns of both rows against odd ones of both
+    row_most[i] = max2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+  }
   if (SQUARE) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, row_most[i]);
-    m = __reduce_max_sync(0xffffffffu, m);
+    uint32_t m = max2(max2(row_most[0], row_most[1]), max2(row_most[2], row_most[3]));
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
     if (lane == 0) col_most[0][warp] = m;
     __syncthreads();
     m = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) m = max(m, col_most[0][w]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row_most[i] = mine[i] = m;
+    for (int i = 0; i < 4; ++i) row_most[i] = col_of[i] = m | m << 16;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) row_most[i] = max(row_most[i], __shfl_xor_sync(0xffffffffu, row_most[i], o));
+      for (int o = 8; o > 0; o >>= 1) row_most[i] = max2(row_most[i], __shfl_xor_sync(0xffffffffu, row_most[i], o));
     if (turned.codes != nullptr) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mine[j] = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t q[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          mine[2 * j] = max(mine[2 * j], (q[j] << 16) & 0x7FFFFFFFu);
-          mine[2 * j + 1] = max(mine[2 * j + 1], q[j] & 0x7FFF0000u);
-        }
+        for (int j = 0; j < 4; ++j) col_of[j] = max2(col_of[j], magnitudes(q[j]));
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        mine[j] = max(mine[j], __shfl_xor_sync(0xffffffffu, mine[j], 16));
-        if (lane < 16) col_most[warp][8 * l + j] = mine[j];
-      }
+      for (int j = 0; j < 4; ++j) col_of[j] = max2(col_of[j], __shfl_xor_sync(0xffffffffu, col_of[j], 16));
+      if (lane < 16) *reinterpret_cast<uint4*>(&col_most[warp][4 * l]) = make_uint4(col_of[0], col_of[1], col_of[2], col_of[3]);
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        mine[j] = 0;
-#pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) mine[j] = max(mine[j], col_most[w][8 * l + j]);
+      for (int w = 0; w < THREADS / 32; ++w) {
+        const uint4 o = *reinterpret_cast<const uint4*>(&col_most[w][4 * l]);
+        col_of[0] = max2(col_of[0], o.x);
+        col_of[1] = max2(col_of[1], o.y);
+        col_of[2] = max2(col_of[2], o.z);
+        col_of[3] = max2(col_of[3], o.w);
       }
     }
   }
@@ -124,7 +125,7 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
   if (plain.codes != nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t byte = scale_byte(row_most[i]);
+      const uint32_t byte = scale_byte(i & 1 ? row_most[i / 2] >> 16 : row_most[i / 2] & 0xFFFFu);
       const float inv = inverse_scale(byte);
       const uint2 o = make_uint2(codes4(low_half(v[i].x) * inv, high_half(v[i].x) * inv, low_half(v[i].y) * inv, high_half(v[i].y) * inv),
                                  codes4(low_half(v[i].z) * inv, high_half(v[i].z) * inv, low_half(v[i].w) * inv, high_half(v[i].w) * inv));
@@ -136,7 +137,7 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
   if (turned.codes != nullptr) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t byte = scale_byte(mine[j]);
+      const uint32_t byte = scale_byte(j & 1 ? col_of[j / 2] >> 16 : col_of[j / 2] & 0xFFFFu);
       const float inv = inverse_scale(byte);
       float f[8];
 #pragma unroll

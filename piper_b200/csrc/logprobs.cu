@@ -69,34 +69,30 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], __nv_bfloat16) {
   return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
 }
 
-// ------------------------------------------------------------------ running maximum and sums
-// s = sum exp((x - m) / temperature), t = sum exp((x - m) / temperature) (x - m); every term of t has one sign, so the entropy
-// is a sum without cancellation.  m is -inf until something finite has come; `from` is what is subtracted.
+// ------------------------------------------------------------------ maximum and sums
+// m = max x, s = sum exp((x - from) / temperature), t = sum exp((x - from) / temperature) (x - from).
 struct Sums {
   float m, from, s, t;
 
   __device__ __forceinline__ static Sums none() { return {-INFINITY, -FLT_MAX, 0.f, 0.f}; }
 
-  __device__ __forceinline__ void raise(float to, float c2) {
-    const float base = fmaxf(to, -FLT_MAX);
-    const float d = max_nan(from - base, FAR_BELOW), f = ex2(d * c2);
+  // The same sums from another, larger `from`.  With the row's maximum every term of t has one sign, so the entropy is a sum
+  // without cancellation.
+  __device__ __forceinline__ void rebase(float to, float c2) {
+    const float d = max_nan(from - to, FAR_BELOW), f = ex2(d * c2);
     t = f * fmaf(s, d, t);
     s *= f;
-    m = to;
-    from = base;
-  }
-  __device__ __forceinline__ void add(float x, float c2) {
-    const float d = max_nan(x - from, FAR_BELOW), w = ex2(d * c2);
-    s += w;
-    t = fmaf(w, d, t);
-  }
-  __device__ __forceinline__ void merge(const Sums& o, float c2) {
-    if (o.m > m) raise(o.m, c2);
-    const float d = max_nan(o.from - from, FAR_BELOW), f = ex2(d * c2);
-    s = fmaf(f, o.s, s);
-    t = fmaf(f, fmaf(o.s, d, o.t), t);
+    from = to;
   }
 };
+
+// Logits this far down and lower are taken for this number by the quick pass, so that differences are finite; a row whose
+// maximum is not well inside (-BIG, BIG), or whose alternatives reach down here, is read again by the exact pass.
+constexpr float CLAMP = -2.9907629905160607e38f;       // a bf16 number, 0xFF61
+constexpr float BIG = 1e36f;
+// A thread's `from` stays behind its maximum by up to so many nats: exp() and its sums stay finite, and the common case has no
+// branch and no rescaling.
+constexpr float STALE = 20.f;
 
 // ------------------------------------------------------------------ the largest of many keys
 // Value and index of an element as one integer that grows with the value and, among equal values, with a falling index, so no two
@@ -161,22 +157,21 @@ __device__ __forceinline__ void merge_lists(uint64_t own, uint64_t (*lists)[32],
 }
 
 struct Shared {
-  Sums sums[WARPS];
-  Sums parts[MAX_PARTS];
+  float m[WARPS], s[WARPS], t[WARPS];
+  float part_m[MAX_PARTS], part_s[MAX_PARTS], part_t[MAX_PARTS];
   uint64_t lists[WARPS][32];
   uint64_t part_lists[MAX_PARTS][32];
 };
 
-__device__ __forceinline__ void merge_lanes(Sums& v, float c2) {
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums w;
-    w.m = __shfl_xor_sync(0xffffffffu, v.m, o);
-    w.from = __shfl_xor_sync(0xffffffffu, v.from, o);
-    w.s = __shfl_xor_sync(0xffffffffu, v.s, o);
-    w.t = __shfl_xor_sync(0xffffffffu, v.t, o);
-    v.merge(w, c2);
-  }
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
 // Where a part of a row begins, how many single elements stand in front of its first 16-byte boundary, how many vectors and
@@ -200,13 +195,156 @@ struct Span {
   }
 };
 
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// A vector's elements, none below CLAMP, in pairs, and the largest number among them.
+__device__ __forceinline__ float clamped(uint4 u, float2 (&x)[4], __nv_bfloat16) {
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = max_nan_bf16x2(w[i], 0xFF61FF61u);
+    x[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+  }
+  const uint32_t m = max_bf16x2(max_bf16x2(w[0], w[1]), max_bf16x2(w[2], w[3]));
+  return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+}
+__device__ __forceinline__ float clamped(uint4 u, float2 (&x)[2], float) {
+  x[0] = make_float2(max_nan(__uint_as_float(u.x), CLAMP), max_nan(__uint_as_float(u.y), CLAMP));
+  x[1] = make_float2(max_nan(__uint_as_float(u.z), CLAMP), max_nan(__uint_as_float(u.w), CLAMP));
+  return fmaxf(fmaxf(x[0].x, x[0].y), fmaxf(x[1].x, x[1].y));
+}
+
+// A thread's sums over its elements of a span, and (TOP) the first place of its largest.
+template <class T>
+struct Pass {
+  const T* row;
+  const T* head;
+  const T* body;
+  const T* tail;
+  Span sp;
+  float c2;
+
+  // Elements in front of and behind the vectors; `take` gets the element and its place in the row.
+  template <class F>
+  __device__ __forceinline__ void singles(int n, const T* from, F take) const {
+    if (static_cast<int>(threadIdx.x) < n) take(to_float(from[threadIdx.x]), static_cast<uint32_t>(from - row) + threadIdx.x);
+  }
+
+  template <bool TOP>
+  __device__ __forceinline__ Sums quick(float stale, uint32_t& place, bool& any) const {
+    Sums v = {-INFINITY, CLAMP, 0.f, 0.f};
+    float limit = CLAMP;
+    float2 s2 = make_float2(0.f, 0.f), t2 = s2;
+    const float2 cc = make_float2(c2, c2);
+    auto raise = [&](float to) {
+      const float d = v.from - to, f = ex2(d * c2);
+      const float2 f2 = make_float2(f, f);
+      t2 = mul2(f2, fma2(s2, make_float2(d, d), t2));
+      s2 = mul2(s2, f2);
+      v.from = to;
+      limit = to + stale;
+    };
+    auto add = [&](float2 x) {
+      const float2 d = add2(x, make_float2(-v.from, -v.from)), e = mul2(d, cc), w = make_float2(ex2(e.x), ex2(e.y));
+      s2 = add2(s2, w);
+      t2 = fma2(w, d, t2);
+    };
+    auto single = [&](float f, uint32_t at) {
+      const float x = max_nan(f, CLAMP);
+      if (x > v.m) {
+        v.m = x;
+        place = at;
+      }
+      if (!any) place = at;
+      any = true;
+      if (x > limit) raise(x);
+      const float d = x - v.from, w = ex2(d * c2);
+      s2.x += w;
+      t2.x = fmaf(w, d, t2.x);
+    };
+    singles(sp.head, head, single);
+    int best = -1;                                         // vector with the largest element, if that is in one
+    constexpr int AHEAD = 4;
+    const uint4* vecs = reinterpret_cast<const uint4*>(body);
+    for (int i = threadIdx.x; i < sp.vecs; i += AHEAD * THREADS) {
+      uint4 u[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (i + j * THREADS < sp.vecs) u[j] = __ldcs(vecs + i + j * THREADS);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i + j * THREADS >= sp.vecs) break;
+        float2 x[VEC<T> / 2];
+        const float lm = clamped(u[j], x, T());
+        if (TOP && (lm > v.m || !any)) best = i + j * THREADS;
+        any = true;
+        v.m = fmaxf(v.m, lm);
+        if (lm > limit) raise(lm);
+#pragma unroll
+        for (int q = 0; q < VEC<T> / 2; ++q) add(x[q]);
+      }
+    }
+    if (TOP && best >= 0) {
+      float2 x[VEC<T> / 2];
+      clamped(vecs[best], x, T());
+      int first = 0;
+#pragma unroll
+      for (int q = VEC<T> / 2 - 1; q >= 0; --q) {
+        if (x[q].y == v.m) first = 2 * q + 1;
+        if (x[q].x == v.m) first = 2 * q;
+      }
+      place = static_cast<uint32_t>(body - row) + static_cast<uint32_t>(best) * VEC<T> + first;
+    }
+    singles(sp.tail, tail, single);
+    v.s = s2.x + s2.y;
+    v.t = t2.x + t2.y;
+    if (v.m <= CLAMP) v.m = -INFINITY;
+    return v;
+  }
+
+  // Any numbers: element by element, from the running maximum.
+  __device__ __noinline__ Sums exact(uint32_t& place, bool& any) const {
+    Sums v = Sums::none();
+    any = false;
+    auto take = [&](float f, uint32_t at) {
+      if (f > v.m || !any) place = at;
+      any = true;
+      if (f > v.m) {
+        const float to = fmaxf(f, -FLT_MAX);
+        v.rebase(to, c2);
+        v.m = f;
+      }
+      const float d = max_nan(f - v.from, FAR_BELOW), w = ex2(d * c2);
+      v.s += w;
+      v.t = fmaf(w, d, v.t);
+    };
+    singles(sp.head, head, take);
+    for (int i = threadIdx.x; i < sp.vecs; i += THREADS)
+      for (int q = 0; q < VEC<T>; ++q) {
+        const T* p = body + static_cast<long long>(i) * VEC<T> + q;
+        take(to_float(*p), static_cast<uint32_t>(p - row));
+      }
+    singles(sp.tail, tail, take);
+    return v;
+  }
+};
+
 // One CTA per row, or a cluster of `parts` CTAs where there are few rows, whose sums and lists meet in the shared memory of the
-// first.  One pass over the row: every thread keeps the running sums of its elements and the place of its largest.  For
+// first.  One pass over the row: every thread keeps the sums of its elements and the place of its largest.  For
 // the alternatives, the top-th largest of the threads' largest keys is a bound that at least so many elements reach; the elements
-// that reach it belong to the `top` threads whose largest does, so only those threads' elements, a 512th of the row each, are looked
-// at again.
+// that reach it belong to the `top` threads whose largest does, so only those threads' elements, a small part of the row each, are
+// looked at again.
 template <class T, bool TOP>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(THREADS, TOP ? 2 : 3)
 logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
                     float* __restrict__ entropy, float* __restrict__ top_logprob, long long* __restrict__ top_id,
                     float* __restrict__ stats, int V, long long ld, long long ignore_index, int top, int parts, float inv_t) {
@@ -222,68 +360,41 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   const T* body = head + sp.head;
   const T* tail = body + static_cast<long long>(sp.vecs) * VEC<T>;
   const float c2 = inv_t * LOG2E;
+  const Pass<T> pass = {x, head, body, tail, sp, c2};
 
-  Sums v = Sums::none();
-  uint32_t place = 0;                  // of the thread's largest; behind an -inf, of its first element
+  Sums v;
+  uint64_t largest = 0, bound = 0;         // lane l: the l-th largest of the threads' largest keys
+  uint32_t place = 0;
   bool any = false;
-  auto single = [&](const T* p) {
-    const float f = to_float(*p);
-    if (f > v.m) {
-      v.raise(f, c2);
-      place = static_cast<uint32_t>(p - x);
-    } else if (!any) {
-      place = static_cast<uint32_t>(p - x);
+  for (int exact = 0; exact < 2; ++exact) {
+    v = exact ? pass.exact(place, any) : pass.template quick<TOP>(STALE / inv_t, place, any);
+    const float wm = warp_max(v.m);
+    if (lane == 0) sh.m[warp] = wm;
+    if (TOP) {
+      merge_lists(sort_falling(any ? make_key(v.m, place) : 0, lane), sh.lists, WARPS, warp, lane);
+      largest = sh.lists[0][lane];
+      bound = __shfl_sync(0xffffffffu, largest, top - 1);
+    } else {
+      __syncthreads();
     }
-    any = true;
-    v.add(f, c2);
-  };
-  if (static_cast<int>(threadIdx.x) < sp.head) single(head + threadIdx.x);
-  constexpr int AHEAD = 4;
-  for (int i = threadIdx.x; i < sp.vecs; i += AHEAD * THREADS) {
-    uint4 u[AHEAD];
+    v.m = sh.m[0];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-      if (i + j * THREADS < sp.vecs) u[j] = __ldcs(reinterpret_cast<const uint4*>(body) + i + j * THREADS);
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (i + j * THREADS >= sp.vecs) break;
-      float f[VEC<T>];
-      unpack(u[j], f, T());
-      float lm = f[0];
-#pragma unroll
-      for (int q = 1; q < VEC<T>; ++q) lm = fmaxf(lm, f[q]);
-      if (lm > v.m || (TOP && !any)) {
-        if (TOP) {
-          const uint32_t at = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(i + j * THREADS) * VEC<T>;
-          int q0 = 0;
-          if (lm > v.m)
-#pragma unroll
-            for (int q = VEC<T> - 1; q >= 0; --q)
-              if (f[q] == lm) q0 = q;
-          place = at + q0;
-          any = true;
-        }
-        if (lm > v.m) v.raise(lm, c2);
-      }
-#pragma unroll
-      for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
-    }
+    for (int w = 1; w < WARPS; ++w) v.m = fmaxf(v.m, sh.m[w]);
+    __syncthreads();                       // read before it is written again
+    if (fabsf(v.m) < BIG && (!TOP || bound == 0 || key_value(bound) > CLAMP)) break;
   }
-  if (static_cast<int>(threadIdx.x) < sp.tail) single(tail + threadIdx.x);
-  const uint64_t mine = TOP && any ? make_key(v.m, place) : 0;
-
-  merge_lanes(v, c2);
-  if (lane == 0) sh.sums[warp] = v;
+  v.rebase(fmaxf(v.m, -FLT_MAX), c2);
+  const float ws = warp_sum(v.s), wt = warp_sum(v.t);
+  if (lane == 0) {
+    sh.s[warp] = ws;
+    sh.t[warp] = wt;
+  }
 
   uint64_t list = 0;
   if (TOP) {
-    merge_lists(sort_falling(mine, lane), sh.lists, WARPS, warp, lane);
-    const uint64_t largest = sh.lists[0][lane];
-    const uint64_t bound = __shfl_sync(0xffffffffu, largest, top - 1);
-    __syncthreads();                   // the lists are read before they are written again
     for (int o = warp; o < top; o += WARPS) {
       const uint64_t k = __shfl_sync(0xffffffffu, largest, o);
-      if (k == 0) break;               // fewer threads than that have elements
+      if (k == 0) break;                   // fewer threads than that have elements
       const int rel = static_cast<int>(static_cast<long long>(key_index(k)) - sp.first);
       const int owner = rel < sp.head ? rel
                         : rel < sp.head + sp.vecs * VEC<T> ? (rel - sp.head) / VEC<T> % THREADS
@@ -316,31 +427,44 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
     __syncthreads();
   }
   if (warp == 0) {
-    v = lane < WARPS ? sh.sums[lane] : Sums::none();
-    merge_lanes(v, c2);
+    v.s = warp_sum(lane < WARPS ? sh.s[lane] : 0.f);
+    v.t = warp_sum(lane < WARPS ? sh.t[lane] : 0.f);
   }
   if (parts > 1) {
     // the sums and the list of every part into the first CTA of the cluster, which has started by now
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (warp == 0) {
-      const uint32_t sums = mapa_u32(smem_u32(&sh.parts[part]), 0);
-      if (lane == 0)
-        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(sums), "f"(v.m), "f"(v.from), "f"(v.s), "f"(v.t)
-                     : "memory");
+      auto put = [](float* at, float f) {
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(smem_u32(at), 0)), "f"(f) : "memory");
+      };
+      if (lane == 0) {
+        put(&sh.part_m[part], v.m);
+        put(&sh.part_s[part], v.s);
+        put(&sh.part_t[part], v.t);
+      }
       if (TOP)
         asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(mapa_u32(smem_u32(&sh.part_lists[part][lane]), 0)), "l"(list)
                      : "memory");
     }
     cluster_sync();
     if (part != 0 || warp != 0) return;
-    v = lane < parts ? sh.parts[lane] : Sums::none();
-    merge_lanes(v, c2);
+    v = Sums::none();
+    if (lane < parts) {
+      v.m = sh.part_m[lane];
+      v.from = fmaxf(v.m, -FLT_MAX);
+      v.s = sh.part_s[lane];
+      v.t = sh.part_t[lane];
+    }
+    v.m = warp_max(v.m);
+    v.rebase(fmaxf(v.m, -FLT_MAX), c2);
+    v.s = warp_sum(v.s);
+    v.t = warp_sum(v.t);
     if (TOP)
       for (int p = 1; p < parts; ++p) list = merge_falling(list, sh.part_lists[p][lane], lane);
   } else if (warp != 0) {
     return;
   }
-  const bool empty = v.s == 0.f;       // nothing left: every probability is 0
+  const bool empty = v.s == 0.f;           // nothing left: every probability is 0
   const float log_s = empty ? -INFINITY : logf(v.s);
   auto log_p = [&](float f) { return empty ? -INFINITY : fmaf(f - v.from, inv_t, -log_s); };
   if (lane == 0) {

@@ -119,8 +119,7 @@ class AdamWState:
         if not self.m.is_cuda:
             return _decode(self.m, self.m_scale, True), _decode(self.v, self.v_scale, False)
         out = [torch.empty(self.numel, dtype=torch.float32, device=self.device) for _ in range(2)]
-        native.lib().moments_decode(self.m, self.m_scale, out[0], True)
-        native.lib().moments_decode(self.v, self.v_scale, out[1], False)
+        native.lib().moments_decode(self.m, self.m_scale, self.v, self.v_scale, out[0], out[1])
         return out[0], out[1]
 
     def set_moments(self, m: Tensor, v: Tensor) -> None:
