@@ -49,18 +49,14 @@ __device__ __forceinline__ float decode_m(uint32_t c, float scale) {
   return __fmul_rn(__uint_as_float((low != 0 ? (low + M_BASE) << 20 : 0u) | (c & 128u) << 24), scale);
 }
 
-// y in [0, 1] to its code; r: 16 random bits.
-__device__ __forceinline__ uint32_t encode_m(float y, uint32_t r) {
-  constexpr uint32_t least = static_cast<uint32_t>(M_BASE + 1) << 20;
-  if (__float_as_uint(y) < least)
-    return __fmul_rn(static_cast<float>(r), __uint_as_float(least) * (1.f / 65536)) < y ? 1u : 0u;
-  return ((__float_as_uint(y) + (r << 4)) >> 20) - M_BASE;
+// Codes of y in [0, 1], r being 16 random bits: the upper bits of y plus what the random bits carry into them; below code 1,
+// 0 or 1 (v: 1 for all that is above 0).
+constexpr uint32_t M_LEAST = static_cast<uint32_t>(M_BASE + 1) << 20, V_LEAST = static_cast<uint32_t>(V_BASE + 1) << 20;
+__device__ __forceinline__ uint32_t encode(float y, uint32_t r, int base) { return ((__float_as_uint(y) + (r << 4)) >> 20) - base; }
+__device__ __forceinline__ uint32_t encode_small_m(float y, uint32_t r) {
+  return __fmul_rn(static_cast<float>(r), __uint_as_float(M_LEAST) * (1.f / 65536)) < y ? 1u : 0u;
 }
-__device__ __forceinline__ uint32_t encode_v(float y, uint32_t r) {
-  constexpr uint32_t least = static_cast<uint32_t>(V_BASE + 1) << 20;
-  if (__float_as_uint(y) < least) return y > 0.f ? 1u : 0u;
-  return ((__float_as_uint(y) + (r << 4)) >> 20) - V_BASE;
-}
+__device__ __forceinline__ uint32_t encode_small_v(float y) { return y > 0.f ? 1u : 0u; }
 
 // The block's largest magnitude, NaN where a value is infinite or NaN.
 __device__ __forceinline__ float block_scale(const float (&x)[PER]) {
@@ -71,24 +67,24 @@ __device__ __forceinline__ float block_scale(const float (&x)[PER]) {
   return most >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(most);
 }
 
-// x / scale, correctly rounded, for 0 <= x <= scale.  With the correctly rounded reciprocal, a product, its exact remainder and a
+// y = |x| / scale of a block, correctly rounded.  With the correctly rounded reciprocal, a product, its exact remainder and a
 // correction give the quotient (Markstein, IBM J. Res. Dev. 34, 1990) where nothing underflows: a quotient that is not small enough for
 // code 0 or 1 anyway comes from x above 2^-101, whose remainder is a normal number, if the scale is above 2^-60.  Other blocks
 // divide.
-struct Quotient {
-  float scale, inverse;
-  bool quick;
-
-  __device__ __forceinline__ explicit Quotient(float s) : scale(s > 0.f ? s : 1.f) {
-    inverse = __frcp_rn(scale);
-    quick = scale >= 8.67361738e-19f && scale <= 1.f;
+__device__ __forceinline__ void quotients(const float* x, float scale, float (&y)[4]) {
+  const float s = scale > 0.f ? scale : 1.f;
+  if (s >= 8.67361738e-19f && s <= 1.f) {
+    const float inverse = __frcp_rn(s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = fabsf(x[j]), q = __fmul_rn(a, inverse);
+      y[j] = __fmaf_rn(__fmaf_rn(-q, s, a), inverse, q);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = __fdiv_rn(fabsf(x[j]), s);
   }
-  __device__ __forceinline__ float operator()(float x) const {
-    if (!quick) return __fdiv_rn(x, scale);
-    const float q = __fmul_rn(x, inverse);
-    return __fmaf_rn(__fmaf_rn(-q, scale, x), inverse, q);
-  }
-};
+}
 
 __device__ __forceinline__ float sqrt_approx(float x) {
   float r;
@@ -187,9 +183,13 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
         const float gj = __fmul_rn(g[j], a.grad_scale);
         m[j] = __fadd_rn(__fmul_rn(m[j], a.b1), __fmul_rn(gj, a.c1));
         v[j] = __fadd_rn(__fmul_rn(v[j], a.b2), __fmul_rn(__fmul_rn(gj, a.c2), gj));
-        if (!is(j)) m[j] = v[j] = 0.f;
         // the update's root and quotient are within two units of the last place each
         w[j] = fmaf(-rate, __fdividef(m[j], fmaf(sqrt_approx(v[j]), root, a.eps)), w[j] * a.keep);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (!is(j)) m[j] = v[j] = 0.f;
       }
       if (vec) {
 #pragma unroll
@@ -211,15 +211,34 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
       if (BITS == 8) {
         ms = block_scale(m);
         vs = block_scale(v);
-        const Quotient over_m(ms), over_v(vs);
-        mc[0] = mc[1] = vc[0] = vc[1] = 0;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const uint32_t r = mix32(static_cast<uint32_t>(at(j)) + t.seed);
-          const uint32_t cm = encode_m(over_m(fabsf(m[j])), r & 0xFFFFu) | (m[j] < 0.f ? 128u : 0u);
-          const uint32_t cv = encode_v(over_v(v[j]), r >> 16);
-          mc[j / 4] |= (cm & 255u) << (8 * (j & 3));
-          vc[j / 4] |= (cv & 255u) << (8 * (j & 3));
+        for (int h = 0; h < 2; ++h) {
+          float ym[4], yv[4];
+          quotients(m + 4 * h, ms, ym);
+          quotients(v + 4 * h, vs, yv);
+          uint32_t cm[4], cv[4], least_m = 0xFFFFFFFFu, least_v = 0xFFFFFFFFu;
+          const uint32_t first = static_cast<uint32_t>(at(4 * h)) + t.seed;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t r = mix32(first + j);
+            cm[j] = encode(ym[j], r & 0xFFFFu, M_BASE);
+            cv[j] = encode(yv[j], r >> 16, V_BASE);
+            least_m = min(least_m, __float_as_uint(ym[j]));
+            least_v = min(least_v, __float_as_uint(yv[j]));
+          }
+          if (__builtin_expect(least_m < M_LEAST || least_v < V_LEAST, 0)) {      // few have such small elements, or zeros
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (__float_as_uint(ym[j]) < M_LEAST) cm[j] = encode_small_m(ym[j], mix32(first + j) & 0xFFFFu);
+              if (__float_as_uint(yv[j]) < V_LEAST) cv[j] = encode_small_v(yv[j]);
+            }
+          }
+          mc[h] = vc[h] = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mc[h] |= (cm[j] & 127u) << (8 * j) | (__float_as_uint(m[4 * h + j]) >> 31) << (8 * j + 7);
+            vc[h] |= (cv[j] & 255u) << (8 * j);
+          }
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -241,13 +260,16 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
   }
 }
 
+constexpr int DECODE_AHEAD = 4;
+
 // Both moments: a thread has four codes of each in `AHEAD` places, all loaded before the first is written.
 __global__ void __launch_bounds__(256)
 moments_decode_kernel(const uint32_t* __restrict__ m, const float* __restrict__ m_scale, const uint32_t* __restrict__ v,
                       const float* __restrict__ v_scale, float4* __restrict__ out_m, float4* __restrict__ out_v, long long words) {
   grid_begin(m, m_scale, v, v_scale);
-  constexpr int AHEAD = 4;
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 * AHEAD + threadIdx.x; i < words; i += 256ll * AHEAD * gridDim.x) {
+  constexpr int AHEAD = DECODE_AHEAD;
+  {
+    const long long i = static_cast<long long>(blockIdx.x) * 256 * AHEAD + threadIdx.x;
     uint32_t cm[AHEAD], cv[AHEAD];
     float sm[AHEAD], sv[AHEAD];
 #pragma unroll
@@ -290,10 +312,11 @@ int adamw_launch(AdamwTable& table, const AdamwArgs& a, int num_sms, cudaStream_
 }
 
 int moments_decode(const void* m, const float* m_scale, const void* v, const float* v_scale, float* out_m, float* out_v, long long n,
-                   int num_sms, cudaStream_t st) {
+                   cudaStream_t st) {
   if (n == 0) return 0;
-  const long long want = (n + 4095) / 4096, most = 8ll * num_sms;
-  const dim3 grid(static_cast<unsigned>(want < most ? want : most));
+  const long long ctas = (n / 4 + 256 * DECODE_AHEAD - 1) / (256 * DECODE_AHEAD);
+  if (ctas > INT32_MAX) return -1;
+  const dim3 grid(static_cast<unsigned>(ctas));
   return launch_overlapped(moments_decode_kernel, grid, 256, 0, st, static_cast<const uint32_t*>(m), m_scale,
                            static_cast<const uint32_t*>(v), v_scale, reinterpret_cast<float4*>(out_m),
                            reinterpret_cast<float4*>(out_v), n / 4) == cudaSuccess ? 0 : -3;

@@ -41,6 +41,6 @@ int adamw_launch(AdamwTable& table, const AdamwArgs& a, int num_sms, cudaStream_
 
 // fp32 values of n codes of either moment (a multiple of kMomentBlock) with their scales.
 int moments_decode(const void* m, const float* m_scale, const void* v, const float* v_scale, float* out_m, float* out_v, long long n,
-                   int num_sms, cudaStream_t st);
+                   cudaStream_t st);
 
 }  // namespace piper

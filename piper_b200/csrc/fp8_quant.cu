@@ -61,9 +61,18 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
   const long long col0 = static_cast<long long>(blockIdx.x) * TILE, row0 = static_cast<long long>(blockIdx.y) * TILE;
   const long long c0 = col0 + 8 * l, r0 = row0 + 8 * g;
   uint4 v[8];
+  const bool whole = col0 + TILE <= cols && row0 + TILE <= rows;
+  {
+    const __nv_bfloat16* p = x + r0 * ldx + c0;
+    if (whole) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    v[i] = c0 < cols && r0 + i < rows ? __ldcs(reinterpret_cast<const uint4*>(x + (r0 + i) * ldx + c0)) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 8; ++i, p += ldx) v[i] = __ldcs(reinterpret_cast<const uint4*>(p));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i, p += ldx)
+        v[i] = c0 < cols && r0 + i < rows ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+    }
+  }
 
   uint32_t row_most[4];                          // of the thread's rows over all columns of the tile, two in a word
   uint32_t col_of[4] = {0, 0, 0, 0};             // of the thread's columns over all rows of the tile, likewise
@@ -123,18 +132,21 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
       for (int b = static_cast<int>(block & 3) + 1; b < 4; ++b) word[b] = 0;
   };
   if (plain.codes != nullptr) {
+    uint8_t* p = plain.codes + r0 * plain.ld + c0;
+    uint32_t own = 0;                            // of row l: rows behind the end have words too, of zeros' scale
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i, p += plain.ld) {
       const uint32_t byte = scale_byte(i & 1 ? row_most[i / 2] >> 16 : row_most[i / 2] & 0xFFFFu);
       const float inv = inverse_scale(byte);
+      if (l == i) own = byte;
       const uint2 o = make_uint2(codes4(low_half(v[i].x) * inv, high_half(v[i].x) * inv, low_half(v[i].y) * inv, high_half(v[i].y) * inv),
                                  codes4(low_half(v[i].z) * inv, high_half(v[i].z) * inv, low_half(v[i].w) * inv, high_half(v[i].w) * inv));
-      if (r0 + i < rows && c0 < cols) *reinterpret_cast<uint2*>(plain.codes + (r0 + i) * plain.ld + c0) = o;
-      if (l == i)        // rows behind the end have words too, of zeros' scale
-        put_scale(plain, blockIdx.x, gridDim.x, r0 + i, static_cast<long long>(gridDim.y) * TILE, byte);
+      if (whole || (r0 + i < rows && c0 < cols)) *reinterpret_cast<uint2*>(p) = o;
     }
+    if (l < 8) put_scale(plain, blockIdx.x, gridDim.x, r0 + l, static_cast<long long>(gridDim.y) * TILE, own);
   }
   if (turned.codes != nullptr) {
+    uint32_t own = 0;                            // of column 8 l + g
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t byte = scale_byte(j & 1 ? col_of[j / 2] >> 16 : col_of[j / 2] & 0xFFFFu);
@@ -148,8 +160,9 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
       // word g of column 8 l + j, moved by l: the sixteen threads of a half warp meet sixteen pairs of banks
       *reinterpret_cast<uint2*>(turn + (8 * l + j) * TILE + ((g ^ l) * 8)) =
           make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
-      if (g == j) put_scale(turned, blockIdx.y, gridDim.y, c0 + j, static_cast<long long>(gridDim.x) * TILE, byte);
+      if (g == j) own = byte;
     }
+    if (g < 8) put_scale(turned, blockIdx.y, gridDim.y, c0 + g, static_cast<long long>(gridDim.x) * TILE, own);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < TILE * TILE / 16 / THREADS; ++k) {

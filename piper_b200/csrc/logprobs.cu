@@ -23,7 +23,8 @@ namespace {
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_PARTS = 8;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr int AHEAD = 4;                 // vectors in flight per thread
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float FAR_BELOW = -1e30f;      // in place of -inf behind a subtraction: exp() of it is 0, and so is 0 times it
 
 template <class T>
@@ -70,29 +71,34 @@ __device__ __forceinline__ uint4 pack(const float (&f)[8], __nv_bfloat16) {
 }
 
 // ------------------------------------------------------------------ maximum and sums
-// m = max x, s = sum exp((x - from) / temperature), t = sum exp((x - from) / temperature) (x - from).
+// m = max x, s = sum 2^a, t = sum 2^a a, where a = (x - from) c2 and c2 = log2(e) / temperature.
 struct Sums {
   float m, from, s, t;
 
   __device__ __forceinline__ static Sums none() { return {-INFINITY, -FLT_MAX, 0.f, 0.f}; }
 
+  // All exponents `d` more.
+  __device__ __forceinline__ void shift(float d) {
+    const float f = ex2(d);
+    t = f * fmaf(s, d, t);
+    s *= f;
+  }
   // The same sums from another, larger `from`.  With the row's maximum every term of t has one sign, so the entropy is a sum
   // without cancellation.
   __device__ __forceinline__ void rebase(float to, float c2) {
-    const float d = max_nan(from - to, FAR_BELOW), f = ex2(d * c2);
-    t = f * fmaf(s, d, t);
-    s *= f;
+    shift(max_nan((from - to) * c2, FAR_BELOW));
     from = to;
   }
 };
 
-// Logits this far down and lower are taken for this number by the quick pass, so that differences are finite; a row whose
-// maximum is not well inside (-BIG, BIG), or whose alternatives reach down here, is read again by the exact pass.
-constexpr float CLAMP = -2.9907629905160607e38f;       // a bf16 number, 0xFF61
-constexpr float BIG = 1e36f;
-// A thread's `from` stays behind its maximum by up to so many nats: exp() and its sums stay finite, and the common case has no
-// branch and no rescaling.
-constexpr float STALE = 20.f;
+// The quick pass takes logits for at least CLAMP, so that nothing is infinite; a row whose maximum is not well inside
+// (-BIG, BIG), whose alternatives reach down there, or whose temperature is far from 1, is read by the exact pass.
+constexpr float CLAMP = -1.0002555517425873e30f;      // a bf16 number, 0xF14A
+constexpr uint32_t CLAMP_PAIR = 0xF14AF14Au;
+constexpr float BIG = 1e28f;
+// Its exponents are relative to a base that stays behind the thread's maximum by up to so many powers of two: sums stay
+// finite, and the common case has no branch and no rescaling.
+constexpr float STALE = 30.f;
 
 // ------------------------------------------------------------------ the largest of many keys
 // Value and index of an element as one integer that grows with the value and, among equal values, with a falling index, so no two
@@ -206,22 +212,58 @@ __device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// A vector's elements, none below CLAMP, in pairs, and the largest number among them.
-__device__ __forceinline__ float clamped(uint4 u, float2 (&x)[4], __nv_bfloat16) {
-  uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = max_nan_bf16x2(w[i], 0xFF61FF61u);
-    x[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+// A vector, no element below CLAMP, and the largest numbers of two halves of its elements, in the vector's own form.
+template <class T>
+struct Vec;
+template <>
+struct Vec<__nv_bfloat16> {
+  uint4 u;
+  uint32_t most;
+  __device__ __forceinline__ explicit Vec(const uint4& v) {
+    u = make_uint4(max_nan_bf16x2(v.x, CLAMP_PAIR), max_nan_bf16x2(v.y, CLAMP_PAIR), max_nan_bf16x2(v.z, CLAMP_PAIR),
+                   max_nan_bf16x2(v.w, CLAMP_PAIR));
+    most = max_bf16x2(max_bf16x2(u.x, u.y), max_bf16x2(u.z, u.w));
   }
-  const uint32_t m = max_bf16x2(max_bf16x2(w[0], w[1]), max_bf16x2(w[2], w[3]));
-  return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
-}
-__device__ __forceinline__ float clamped(uint4 u, float2 (&x)[2], float) {
-  x[0] = make_float2(max_nan(__uint_as_float(u.x), CLAMP), max_nan(__uint_as_float(u.y), CLAMP));
-  x[1] = make_float2(max_nan(__uint_as_float(u.z), CLAMP), max_nan(__uint_as_float(u.w), CLAMP));
-  return fmaxf(fmaxf(x[0].x, x[0].y), fmaxf(x[1].x, x[1].y));
-}
+  __device__ __forceinline__ void also(const Vec& o) { most = max_bf16x2(most, o.most); }
+  __device__ __forceinline__ float largest() const { return fmaxf(__uint_as_float(most << 16), __uint_as_float(most & 0xFFFF0000u)); }
+  __device__ __forceinline__ void elements(float (&f)[8]) const { unpack(u, f, __nv_bfloat16()); }
+};
+template <>
+struct Vec<float> {
+  float4 u;
+  float most;
+  __device__ __forceinline__ explicit Vec(const uint4& v) {
+    u = make_float4(max_nan(__uint_as_float(v.x), CLAMP), max_nan(__uint_as_float(v.y), CLAMP), max_nan(__uint_as_float(v.z), CLAMP),
+                    max_nan(__uint_as_float(v.w), CLAMP));
+    most = fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w));
+  }
+  __device__ __forceinline__ void also(const Vec& o) { most = fmaxf(most, o.most); }
+  __device__ __forceinline__ float largest() const { return most; }
+  __device__ __forceinline__ void elements(float (&f)[4]) const {
+    f[0] = u.x;
+    f[1] = u.y;
+    f[2] = u.z;
+    f[3] = u.w;
+  }
+};
+
+// Sums of the quick pass: exponents are x c2 - base, one rounded operation.
+struct QuickSums {
+  float base, limit, s, t;               // base, limit: in powers of two
+
+  __device__ __forceinline__ void raise(float x, float c2) {
+    const float to = x * c2, d = max_nan(base - to, FAR_BELOW), f = ex2(d);
+    t = f * fmaf(s, d, t);
+    s *= f;
+    base = to;
+    limit = x + STALE / c2;
+  }
+  __device__ __forceinline__ void add(float x, float c2) {
+    const float a = fmaf(x, c2, -base), w = ex2(a);
+    s += w;
+    t = fmaf(w, a, t);
+  }
+};
 
 // A thread's sums over its elements of a span, and (TOP) the first place of its largest.
 template <class T>
@@ -240,75 +282,80 @@ struct Pass {
   }
 
   template <bool TOP>
-  __device__ __forceinline__ Sums quick(float stale, uint32_t& place, bool& any) const {
-    Sums v = {-INFINITY, CLAMP, 0.f, 0.f};
-    float limit = CLAMP;
-    float2 s2 = make_float2(0.f, 0.f), t2 = s2;
-    const float2 cc = make_float2(c2, c2);
-    auto raise = [&](float to) {
-      const float d = v.from - to, f = ex2(d * c2);
-      const float2 f2 = make_float2(f, f);
-      t2 = mul2(f2, fma2(s2, make_float2(d, d), t2));
-      s2 = mul2(s2, f2);
-      v.from = to;
-      limit = to + stale;
-    };
-    auto add = [&](float2 x) {
-      const float2 d = add2(x, make_float2(-v.from, -v.from)), e = mul2(d, cc), w = make_float2(ex2(e.x), ex2(e.y));
-      s2 = add2(s2, w);
-      t2 = fma2(w, d, t2);
-    };
+  __device__ __forceinline__ Sums quick(uint32_t& place, bool& any) const {
+    QuickSums v = {0.5f * CLAMP * c2, CLAMP, 0.f, 0.f};      // far above what is clamped, far below the first raise
+    float m = -INFINITY;
     auto single = [&](float f, uint32_t at) {
       const float x = max_nan(f, CLAMP);
-      if (x > v.m) {
-        v.m = x;
-        place = at;
-      }
-      if (!any) place = at;
+      if (x > m || !any) place = at;
+      m = fmaxf(m, x);
       any = true;
-      if (x > limit) raise(x);
-      const float d = x - v.from, w = ex2(d * c2);
-      s2.x += w;
-      t2.x = fmaf(w, d, t2.x);
+      if (x > v.limit) v.raise(x, c2);
+      v.add(x, c2);
     };
     singles(sp.head, head, single);
-    int best = -1;                                         // vector with the largest element, if that is in one
-    constexpr int AHEAD = 4;
+    int best = -1;                                         // first vector of the batch with the largest element, if that is in one
     const uint4* vecs = reinterpret_cast<const uint4*>(body);
-    for (int i = threadIdx.x; i < sp.vecs; i += AHEAD * THREADS) {
+    int i = threadIdx.x;
+    for (; i + (AHEAD - 1) * THREADS < sp.vecs; i += AHEAD * THREADS) {
       uint4 u[AHEAD];
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j)
-        if (i + j * THREADS < sp.vecs) u[j] = __ldcs(vecs + i + j * THREADS);
+      for (int j = 0; j < AHEAD; ++j) u[j] = __ldcs(vecs + i + j * THREADS);
+      Vec<T> first(u[0]), rest[AHEAD - 1] = {Vec<T>(u[1]), Vec<T>(u[2]), Vec<T>(u[3])};
+      Vec<T> all = first;
 #pragma unroll
-      for (int j = 0; j < AHEAD; ++j) {
-        if (i + j * THREADS >= sp.vecs) break;
-        float2 x[VEC<T> / 2];
-        const float lm = clamped(u[j], x, T());
-        if (TOP && (lm > v.m || !any)) best = i + j * THREADS;
+      for (int j = 0; j < AHEAD - 1; ++j) all.also(rest[j]);
+      const float lm = all.largest();
+      if (TOP) {
+        if (lm > m || !any) best = i;
         any = true;
-        v.m = fmaxf(v.m, lm);
-        if (lm > limit) raise(lm);
-#pragma unroll
-        for (int q = 0; q < VEC<T> / 2; ++q) add(x[q]);
       }
+      m = fmaxf(m, lm);
+      if (__builtin_expect(lm > v.limit, 0)) v.raise(lm, c2);
+      float f[VEC<T>];
+      first.elements(f);
+#pragma unroll
+      for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
+#pragma unroll
+      for (int j = 0; j < AHEAD - 1; ++j) {
+        rest[j].elements(f);
+#pragma unroll
+        for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
+      }
+    }
+#pragma unroll 1
+    for (; i < sp.vecs; i += THREADS) {
+      const Vec<T> x(__ldcs(vecs + i));
+      const float lm = x.largest();
+      if (TOP) {
+        if (lm > m || !any) best = i;
+        any = true;
+      }
+      m = fmaxf(m, lm);
+      if (lm > v.limit) v.raise(lm, c2);
+      float f[VEC<T>];
+      x.elements(f);
+#pragma unroll
+      for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
     }
     if (TOP && best >= 0) {
-      float2 x[VEC<T> / 2];
-      clamped(vecs[best], x, T());
-      int first = 0;
+      // the batch again, from its end: the first place is what remains
+#pragma unroll 1
+      for (int j = AHEAD - 1; j >= 0; --j) {
+        const int at = best + j * THREADS;
+        if (at >= sp.vecs) continue;
+        float f[VEC<T>];
+        Vec<T>(vecs[at]).elements(f);
 #pragma unroll
-      for (int q = VEC<T> / 2 - 1; q >= 0; --q) {
-        if (x[q].y == v.m) first = 2 * q + 1;
-        if (x[q].x == v.m) first = 2 * q;
+        for (int q = VEC<T> - 1; q >= 0; --q)
+          if (f[q] == m) place = static_cast<uint32_t>(body - row) + static_cast<uint32_t>(at) * VEC<T> + q;
       }
-      place = static_cast<uint32_t>(body - row) + static_cast<uint32_t>(best) * VEC<T> + first;
     }
     singles(sp.tail, tail, single);
-    v.s = s2.x + s2.y;
-    v.t = t2.x + t2.y;
-    if (v.m <= CLAMP) v.m = -INFINITY;
-    return v;
+    if (!(m > CLAMP)) return Sums::none();
+    Sums r = {m, m, v.s, v.t};
+    r.shift(max_nan(fmaf(-r.from, c2, v.base), FAR_BELOW));
+    return r;
   }
 
   // Any numbers: element by element, from the running maximum.
@@ -319,13 +366,12 @@ struct Pass {
       if (f > v.m || !any) place = at;
       any = true;
       if (f > v.m) {
-        const float to = fmaxf(f, -FLT_MAX);
-        v.rebase(to, c2);
+        v.rebase(fmaxf(f, -FLT_MAX), c2);
         v.m = f;
       }
-      const float d = max_nan(f - v.from, FAR_BELOW), w = ex2(d * c2);
+      const float a = max_nan((f - v.from) * c2, FAR_BELOW), w = ex2(a);
       v.s += w;
-      v.t = fmaf(w, d, v.t);
+      v.t = fmaf(w, a, v.t);
     };
     singles(sp.head, head, take);
     for (int i = threadIdx.x; i < sp.vecs; i += THREADS)
@@ -366,8 +412,8 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   uint64_t largest = 0, bound = 0;         // lane l: the l-th largest of the threads' largest keys
   uint32_t place = 0;
   bool any = false;
-  for (int exact = 0; exact < 2; ++exact) {
-    v = exact ? pass.exact(place, any) : pass.template quick<TOP>(STALE / inv_t, place, any);
+  for (int exact = c2 > 1e-6f && c2 < 1e6f ? 0 : 1; exact < 2; ++exact) {
+    v = exact ? pass.exact(place, any) : pass.template quick<TOP>(place, any);
     const float wm = warp_max(v.m);
     if (lane == 0) sh.m[warp] = wm;
     if (TOP) {
@@ -465,13 +511,13 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
     return;
   }
   const bool empty = v.s == 0.f;           // nothing left: every probability is 0
-  const float log_s = empty ? -INFINITY : logf(v.s);
-  auto log_p = [&](float f) { return empty ? -INFINITY : fmaf(f - v.from, inv_t, -log_s); };
+  const float log_s = empty ? -INFINITY : log2f(v.s);
+  auto log_p = [&](float f) { return empty ? -INFINITY : fmaf(f - v.from, inv_t, -log_s * LN2); };
   if (lane == 0) {
     const long long y = tokens[row];
     const bool counted = y != ignore_index && y >= 0 && y < V;
     logprob[row] = counted ? log_p(to_float(x[y])) : 0.f;
-    entropy[row] = empty ? 0.f : fmaf(-v.t / v.s, inv_t, log_s);
+    entropy[row] = empty ? 0.f : (log_s - v.t / v.s) * LN2;
     stats[2 * row] = v.from;
     stats[2 * row + 1] = log_s;
   }
@@ -503,11 +549,12 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   if (d_top != nullptr)
     for (int i = 0; i < top; ++i) g += d_top[row * top + i];
   const bool empty = log_s == -INFINITY;
-  // dx = -exp(u) (a + b u) with u = log p
-  const float a = (g + gh * h) * inv_t, b = gh * inv_t;
+  // dx = 2^u (a + b u) with u = log2 p; a row with nothing left has a = b = 0 and any finite log_s
+  const float c2 = inv_t * LOG2E;
+  const float a = empty ? 0.f : -(g + gh * h) * inv_t, b = empty ? 0.f : -gh * LN2 * inv_t, minus = empty ? 0.f : -log_s;
   auto grad = [&](float f) {
-    const float u = fmaf(max_nan(f - from, FAR_BELOW), inv_t, -log_s);
-    return empty ? 0.f : -ex2(u * LOG2E) * fmaf(b, u, a);
+    const float u = fmaf(max_nan(f - from, FAR_BELOW), c2, minus);
+    return ex2(u) * fmaf(b, u, a);
   };
   const long long begin = sp.first, end = begin + sp.head + static_cast<long long>(sp.vecs) * VEC<T> + sp.tail;
   if (ALIGNED) {                       // x and o have the same offset to a 16-byte boundary
@@ -515,7 +562,6 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
     const int t = threadIdx.x;
     if (t < sp.head) from_float(grad(to_float(x[begin + t])), o[begin + t]);
     if (t < sp.tail) from_float(grad(to_float(x[tail + t])), o[tail + t]);
-    constexpr int AHEAD = 4;
     for (int i = t; i < sp.vecs; i += AHEAD * THREADS) {
       uint4 u[AHEAD];
 #pragma unroll

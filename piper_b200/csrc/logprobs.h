@@ -17,7 +17,7 @@ struct LogprobArgs {
 };
 
 // logprob, entropy [T]; top_logprob, top_id [T, top], by falling logits, equal ones by rising id; stats [T, 2] for the
-// backward pass (largest logit, log of the sum of exp(z - largest z)).
+// backward pass (largest logit, log2 of the sum of exp(z - largest z)).
 int logprobs_fwd(const LogprobArgs& a, float* logprob, float* entropy, float* top_logprob, long long* top_id, float* stats,
                  int num_sms, cudaStream_t st);
 

@@ -64,7 +64,7 @@ def token_logprobs_fwd(logits: Tensor, tokens: Tensor, top: int, temperature: fl
     logprob = torch.where(_counted(tokens, V, ignore_index), logp.gather(1, at).squeeze(1), torch.zeros((), dtype=logp.dtype))
     ranked = torch.where(logits == logits, logits, torch.full_like(logits, -math.inf))
     top_id = torch.sort(ranked, dim=1, descending=True, stable=True).indices[:, :top].contiguous()
-    stats = torch.stack((largest, log_s), 1)
+    stats = torch.stack((largest, log_s / math.log(2.0)), 1)
     return logprob.float(), entropy.float(), logp.gather(1, top_id).float(), top_id, stats.float()
 
 
