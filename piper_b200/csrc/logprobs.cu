@@ -167,6 +167,10 @@ struct Shared {
   float part_m[MAX_PARTS], part_s[MAX_PARTS], part_t[MAX_PARTS];
   uint64_t lists[WARPS][32];
   uint64_t part_lists[MAX_PARTS][32];
+  uint64_t halves[2][32];
+  uint64_t bound;
+  int owners[THREADS];
+  int num_owners, num_found;
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -265,7 +269,13 @@ struct QuickSums {
   }
 };
 
-// A thread's sums over its elements of a span, and (TOP) the first place of its largest.
+// Where a thread's largest element is: not in front of `first`, and not behind `last`.
+struct Place {
+  uint32_t first, last;
+  bool any;              // the thread has elements
+};
+
+// A thread's sums over its elements of a span, and (TOP) where its largest is.
 template <class T>
 struct Pass {
   const T* row;
@@ -282,19 +292,18 @@ struct Pass {
   }
 
   template <bool TOP>
-  __device__ __forceinline__ Sums quick(uint32_t& place, bool& any) const {
+  __device__ __forceinline__ Sums quick(Place& place) const {
     QuickSums v = {0.5f * CLAMP * c2, CLAMP, 0.f, 0.f};      // far above what is clamped, far below the first raise
     float m = -INFINITY;
     auto single = [&](float f, uint32_t at) {
       const float x = max_nan(f, CLAMP);
-      if (x > m || !any) place = at;
+      if (x > m || !place.any) place = {at, at, true};
       m = fmaxf(m, x);
-      any = true;
       if (x > v.limit) v.raise(x, c2);
       v.add(x, c2);
     };
     singles(sp.head, head, single);
-    int best = -1;                                         // first vector of the batch with the largest element, if that is in one
+    int best = -1, span = 0;               // the vectors from `best`, `span` apart at most, among which the largest element is
     const uint4* vecs = reinterpret_cast<const uint4*>(body);
     int i = threadIdx.x;
     for (; i + (AHEAD - 1) * THREADS < sp.vecs; i += AHEAD * THREADS) {
@@ -306,9 +315,10 @@ struct Pass {
 #pragma unroll
       for (int j = 0; j < AHEAD - 1; ++j) all.also(rest[j]);
       const float lm = all.largest();
-      if (TOP) {
-        if (lm > m || !any) best = i;
-        any = true;
+      if (TOP && (lm > m || !place.any)) {
+        best = i;
+        span = (AHEAD - 1) * THREADS;
+        place.any = true;
       }
       m = fmaxf(m, lm);
       if (__builtin_expect(lm > v.limit, 0)) v.raise(lm, c2);
@@ -327,9 +337,10 @@ struct Pass {
     for (; i < sp.vecs; i += THREADS) {
       const Vec<T> x(__ldcs(vecs + i));
       const float lm = x.largest();
-      if (TOP) {
-        if (lm > m || !any) best = i;
-        any = true;
+      if (TOP && (lm > m || !place.any)) {
+        best = i;
+        span = 0;
+        place.any = true;
       }
       m = fmaxf(m, lm);
       if (lm > v.limit) v.raise(lm, c2);
@@ -339,17 +350,8 @@ struct Pass {
       for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
     }
     if (TOP && best >= 0) {
-      // the batch again, from its end: the first place is what remains
-#pragma unroll 1
-      for (int j = AHEAD - 1; j >= 0; --j) {
-        const int at = best + j * THREADS;
-        if (at >= sp.vecs) continue;
-        float f[VEC<T>];
-        Vec<T>(vecs[at]).elements(f);
-#pragma unroll
-        for (int q = VEC<T> - 1; q >= 0; --q)
-          if (f[q] == m) place = static_cast<uint32_t>(body - row) + static_cast<uint32_t>(at) * VEC<T> + q;
-      }
+      place.first = static_cast<uint32_t>(body - row) + static_cast<uint32_t>(best) * VEC<T>;
+      place.last = place.first + static_cast<uint32_t>(span + 1) * VEC<T> - 1;
     }
     singles(sp.tail, tail, single);
     if (!(m > CLAMP)) return Sums::none();
@@ -359,12 +361,11 @@ struct Pass {
   }
 
   // Any numbers: element by element, from the running maximum.
-  __device__ __noinline__ Sums exact(uint32_t& place, bool& any) const {
+  __device__ __noinline__ Sums exact(Place& place) const {
     Sums v = Sums::none();
-    any = false;
+    place.any = false;
     auto take = [&](float f, uint32_t at) {
-      if (f > v.m || !any) place = at;
-      any = true;
+      if (f > v.m || !place.any) place = {at, at, true};
       if (f > v.m) {
         v.rebase(fmaxf(f, -FLT_MAX), c2);
         v.m = f;
@@ -386,9 +387,10 @@ struct Pass {
 
 // One CTA per row, or a cluster of `parts` CTAs where there are few rows, whose sums and lists meet in the shared memory of the
 // first.  One pass over the row: every thread keeps the sums of its elements and the place of its largest.  For
-// the alternatives, the top-th largest of the threads' largest keys is a bound that at least so many elements reach; the elements
-// that reach it belong to the `top` threads whose largest does, so only those threads' elements, a small part of the row each, are
-// looked at again.
+// the alternatives, the threads' largest keys (taken for as small as their places allow) are reduced to 64, the largest of a lane
+// number's in every other warp; the top-th largest of those is a bound that at least so many elements reach.  The elements that reach it
+// belong to the few threads whose largest does, and only those threads' elements, a small part of the row each, are looked at
+// again, by all threads; what they find is sorted.  20 alternatives of 1024 x 128256: FIGURE
 template <class T, bool TOP>
 __global__ void __launch_bounds__(THREADS, TOP ? 2 : 3)
 logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
@@ -409,25 +411,40 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   const Pass<T> pass = {x, head, body, tail, sp, c2};
 
   Sums v;
-  uint64_t largest = 0, bound = 0;         // lane l: the l-th largest of the threads' largest keys
-  uint32_t place = 0;
-  bool any = false;
+  uint64_t bound = 0;
+  Place place = {0, 0, false};
   for (int exact = c2 > 1e-6f && c2 < 1e6f ? 0 : 1; exact < 2; ++exact) {
-    v = exact ? pass.exact(place, any) : pass.template quick<TOP>(place, any);
+    v = exact ? pass.exact(place) : pass.template quick<TOP>(place);
     const float wm = warp_max(v.m);
     if (lane == 0) sh.m[warp] = wm;
-    if (TOP) {
-      merge_lists(sort_falling(any ? make_key(v.m, place) : 0, lane), sh.lists, WARPS, warp, lane);
-      largest = sh.lists[0][lane];
-      bound = __shfl_sync(0xffffffffu, largest, top - 1);
-    } else {
-      __syncthreads();
+    if (TOP) sh.lists[warp][lane] = place.any ? make_key(v.m, place.last) : 0;
+    __syncthreads();
+    if (TOP && warp < 2) {
+      uint64_t k = sh.lists[warp][lane];
+#pragma unroll
+      for (int w = 2; w < WARPS; w += 2) k = max(k, sh.lists[warp + w][lane]);
+      k = sort_falling(k, lane);
+      sh.halves[warp][lane] = k;
+      asm volatile("bar.sync 1, 64;" ::: "memory");
+      if (warp == 0) {
+        k = merge_falling(k, sh.halves[1][lane], lane);
+        if (lane == top - 1) sh.bound = k;
+        if (lane == 0) sh.num_owners = sh.num_found = 0;
+      }
     }
+    const uint64_t most = TOP && place.any ? make_key(v.m, place.first) : 0;
     v.m = sh.m[0];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) v.m = fmaxf(v.m, sh.m[w]);
+    __syncthreads();
+    bool good = fabsf(v.m) < BIG;
+    if (TOP) {
+      bound = sh.bound;
+      good = good && (bound == 0 || key_value(bound) > CLAMP);
+      if ((good || exact) && most != 0 && most >= bound) sh.owners[atomicAdd(&sh.num_owners, 1)] = threadIdx.x;
+    }
+    if (good || exact) break;
     __syncthreads();                       // read before it is written again
-    if (fabsf(v.m) < BIG && (!TOP || bound == 0 || key_value(bound) > CLAMP)) break;
   }
   v.rebase(fmaxf(v.m, -FLT_MAX), c2);
   const float ws = warp_sum(v.s), wt = warp_sum(v.t);
@@ -435,42 +452,75 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
     sh.s[warp] = ws;
     sh.t[warp] = wt;
   }
+  __syncthreads();
 
   uint64_t list = 0;
   if (TOP) {
-    for (int o = warp; o < top; o += WARPS) {
-      const uint64_t k = __shfl_sync(0xffffffffu, largest, o);
-      if (k == 0) break;                   // fewer threads than that have elements
-      const int rel = static_cast<int>(static_cast<long long>(key_index(k)) - sp.first);
-      const int owner = rel < sp.head ? rel
-                        : rel < sp.head + sp.vecs * VEC<T> ? (rel - sp.head) / VEC<T> % THREADS
-                                                           : rel - sp.head - sp.vecs * VEC<T>;
-      auto offer = [&](bool has, float f, uint32_t index) {
+    // A found key into the buffer that the lists were in; there is room for THREADS.
+    uint64_t* const found = &sh.lists[0][0];
+    auto offer = [&](float f, uint32_t index) {
+      const uint64_t key = make_key(f, index);
+      if (key >= bound) {
+        const int at = atomicAdd(&sh.num_found, 1);
+        if (at < THREADS) found[at] = key;
+      }
+    };
+    const int owners = sh.num_owners, rounds = (sp.vecs + THREADS - 1) / THREADS;
+    for (int e = threadIdx.x; e < owners * rounds; e += THREADS) {
+      const int owner = sh.owners[e / rounds], i = owner + e % rounds * THREADS;
+      if (i >= sp.vecs) continue;
+      float f[VEC<T>];
+      unpack(reinterpret_cast<const uint4*>(body)[i], f, T());
+      const uint32_t at = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(i) * VEC<T>;
+#pragma unroll
+      for (int q = 0; q < VEC<T>; ++q) offer(f[q], at + q);
+    }
+    for (int e = threadIdx.x; e < owners; e += THREADS) {
+      const int owner = sh.owners[e];
+      if (owner < sp.head) offer(to_float(head[owner]), static_cast<uint32_t>(head + owner - x));
+      if (owner < sp.tail) offer(to_float(tail[owner]), static_cast<uint32_t>(tail + owner - x));
+    }
+    __syncthreads();
+    const int n = sh.num_found;
+    if (n <= THREADS) {
+      list = sort_falling(static_cast<int>(threadIdx.x) < n ? found[threadIdx.x] : 0, lane);
+      if (n > 32) {
+        __syncthreads();
+        merge_lists(list, sh.lists, WARPS, warp, lane);
+        list = sh.lists[0][lane];
+      }
+    } else {
+      // rows of many equal logits: every warp puts what it finds into a list of its own
+      __syncthreads();
+      auto insert = [&](bool has, float f, uint32_t index) {
         const uint64_t key = has ? make_key(f, index) : 0;
-        unsigned waiting = __ballot_sync(0xffffffffu, key >= bound && key != 0);
+        const uint64_t least = __shfl_sync(0xffffffffu, list, 31);       // by all lanes, in front of any condition
+        unsigned waiting = __ballot_sync(0xffffffffu, key >= bound && key > least);
         while (waiting != 0) {
           const int from = __ffs(waiting) - 1;
           waiting &= waiting - 1;
           list = insert_falling(list, __shfl_sync(0xffffffffu, key, from), lane);
         }
       };
-      const bool at_head = lane == 0 && owner < sp.head, at_tail = lane == 1 && owner < sp.tail;
-      const T* s = at_head ? head + owner : tail + owner;
-      offer(at_head || at_tail, at_head || at_tail ? to_float(*s) : 0.f, static_cast<uint32_t>(s - x));
-      for (int i0 = owner; i0 < sp.vecs; i0 += 32 * THREADS) {
-        const int i = i0 + lane * THREADS;
-        const bool has = i < sp.vecs;
-        float f[VEC<T>];
-        unpack(has ? reinterpret_cast<const uint4*>(body)[i] : make_uint4(0, 0, 0, 0), f, T());
-        const uint32_t at = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(i) * VEC<T>;
+      list = 0;
+      for (int e = warp; e < owners; e += WARPS) {
+        const int owner = sh.owners[e];
+        const bool at_head = lane == 0 && owner < sp.head, at_tail = lane == 1 && owner < sp.tail;
+        const T* s = at_head ? head + owner : tail + owner;
+        insert(at_head || at_tail, at_head || at_tail ? to_float(*s) : 0.f, static_cast<uint32_t>(s - x));
+        for (int i0 = owner; i0 < sp.vecs; i0 += 32 * THREADS) {
+          const int i = i0 + lane * THREADS;
+          const bool has = i < sp.vecs;
+          float f[VEC<T>];
+          unpack(has ? reinterpret_cast<const uint4*>(body)[i] : make_uint4(0, 0, 0, 0), f, T());
+          const uint32_t at = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(i) * VEC<T>;
 #pragma unroll
-        for (int q = 0; q < VEC<T>; ++q) offer(has, f[q], at + q);
+          for (int q = 0; q < VEC<T>; ++q) insert(has, f[q], at + q);
+        }
       }
+      merge_lists(list, sh.lists, WARPS, warp, lane);
+      list = sh.lists[0][lane];
     }
-    merge_lists(list, sh.lists, WARPS, warp, lane);
-    list = sh.lists[0][lane];
-  } else {
-    __syncthreads();
   }
   if (warp == 0) {
     v.s = warp_sum(lane < WARPS ? sh.s[lane] : 0.f);
