@@ -3,7 +3,7 @@
 // An operand is a matrix of e4m3 codes [rows, cols], cols along the contraction, rows `ld` bytes apart (a multiple of 16), with
 // one power-of-two scale for every row and 128 columns.  Scales are exponents with a bias of 127 (255: NaN), four neighbouring ones
 // of a row in one word: words [scale_groups(cols)][scale_rows(rows)], the row fastest.  A scale that a whole block of
-// 128 x 128 shares stands in each of its rows.
+// 128 x 128 shares stands in each of its rows.  Codes and, behind them, words are one piece of memory.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -15,28 +15,45 @@ constexpr int kFp8Group = 128;
 inline long long fp8_scale_rows(long long rows) { return (rows + 127) / 128 * 128; }
 inline long long fp8_scale_groups(long long cols) { return (cols + 4 * kFp8Group - 1) / (4 * kFp8Group); }
 
-struct Fp8Out {
-  uint8_t* codes;      // null: not wanted
+inline long long fp8_row_bytes(long long cols) { return (cols + 15) / 16 * 16; }
+inline long long fp8_bytes(long long rows, long long cols) {
+  return rows * fp8_row_bytes(cols) + 4 * fp8_scale_groups(cols) * fp8_scale_rows(rows);
+}
+
+struct Fp8Operand {
+  uint8_t* codes;      // null: none
   uint32_t* scales;
   long long ld;
+
+  // An operand [rows, cols] in fp8_bytes(rows, cols) of 16-byte aligned memory.
+  static Fp8Operand at(void* memory, long long rows, long long cols) {
+    if (memory == nullptr) return {nullptr, nullptr, 0};
+    uint8_t* codes = static_cast<uint8_t*>(memory);
+    const long long ld = fp8_row_bytes(cols);
+    return {codes, reinterpret_cast<uint32_t*>(codes + rows * ld), ld};
+  }
 };
 
 // bf16 x [rows, cols], rows ldx elements apart (16-byte aligned vectors, cols % 16 == 0), as operand with the contraction along
 // its columns (`plain`) and with the contraction along its rows (`turned`: codes [cols, rows]).  square: one scale
 // for 128 x 128, the same in both.
-int fp8_quantize(const void* x, long long rows, long long cols, long long ldx, int square, const Fp8Out& plain, const Fp8Out& turned,
-                 cudaStream_t st);
+struct Fp8Rounding {
+  const void* x;
+  long long rows, cols, ldx;
+  int square;
+  Fp8Operand plain, turned;
+};
+
+// One or two matrices in one launch.
+int fp8_quantize(const Fp8Rounding* what, int count, cudaStream_t st);
 
 // fp32 [rows, cols] of an operand.
-int fp8_dequantize(const uint8_t* codes, const uint32_t* scales, long long ld, float* out, long long rows, long long cols, cudaStream_t st);
+int fp8_dequantize(const Fp8Operand& a, float* out, long long rows, long long cols, cudaStream_t st);
 
 struct Fp8GemmArgs {
-  const uint8_t* a;            // [M, K]
-  const uint8_t* b;            // [N, K]
-  const uint32_t* a_scales;
-  const uint32_t* b_scales;
+  Fp8Operand a, b;             // [M, K], [N, K]
   void* c;                     // [M, N] bf16, or fp32 that is added to
-  long long lda, ldb, ldc;
+  long long ldc;
   int M, N, K;
   int add_f32;
   int* status;

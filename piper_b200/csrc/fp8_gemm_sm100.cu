@@ -462,8 +462,8 @@ int fp8_gemm_launch(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   if (g.M <= 0 || g.N <= 0 || g.K <= 0) return 0;
   const GemmShape shape = shape_of(g.M, g.N, g.K, g.add_f32 != 0, num_sms);
   Params p;
-  p.a_scales = g.a_scales;
-  p.b_scales = g.b_scales;
+  p.a_scales = g.a.scales;
+  p.b_scales = g.b.scales;
   p.M = g.M;
   p.N = g.N;
   p.K = g.K;
@@ -482,8 +482,8 @@ int fp8_gemm_launch(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   p.status = g.status;
   p.sched = gemm_sched_slot();
   CUtensorMap ta, tb, tc;
-  int rc = make_tmap_2d_u8(&ta, g.a, g.K, g.M, g.lda, BK, p.a_rows);
-  if (rc == 0) rc = make_tmap_2d_u8(&tb, g.b, g.K, g.N, g.ldb, BK, b_rows);
+  int rc = make_tmap_2d_u8(&ta, g.a.codes, g.K, g.M, g.a.ld, BK, p.a_rows);
+  if (rc == 0) rc = make_tmap_2d_u8(&tb, g.b.codes, g.K, g.N, g.b.ld, BK, b_rows);
   if (rc == 0)
     rc = g.add_f32 ? make_tmap_c_f32(&tc, g.c, g.N, g.M, static_cast<uint64_t>(g.ldc) * 4)
                    : make_tmap_c_bf16(&tc, g.c, g.N, g.M, static_cast<uint64_t>(g.ldc) * 2);

@@ -49,16 +49,29 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
 __device__ __forceinline__ float low_half(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_half(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
 
-// Thread t: columns 8 (t % 16) to + 7, rows 8 (t / 16) to + 7.
-template <bool SQUARE>
+struct Roundings {
+  Fp8Rounding what[2];
+  int tiles_x[2], tiles_y[2];
+};
+
+// Thread t: columns 8 (t % 16) to + 7, rows 8 (t / 16) to + 7 of a tile.  The tiles of the second matrix follow those of the first.
 __global__ void __launch_bounds__(THREADS, 3)
-fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long long cols, long long ldx, Fp8Out plain, Fp8Out turned) {
-  grid_begin(x);
+fp8_quantize_kernel(const __grid_constant__ Roundings both) {
+  grid_begin();
+  const int first = both.tiles_x[0] * both.tiles_y[0];
+  const int which = static_cast<int>(blockIdx.x) < first ? 0 : 1;
+  const Fp8Rounding& r = both.what[which];
+  const int tile = static_cast<int>(blockIdx.x) - which * first, tiles_x = both.tiles_x[which], tiles_y = both.tiles_y[which];
+  const int tile_y = tile / tiles_x, tile_x = tile - tile_y * tiles_x;
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(r.x);
+  const long long rows = r.rows, cols = r.cols, ldx = r.ldx;
+  const bool square = r.square != 0;
+  const Fp8Operand &plain = r.plain, &turned = r.turned;
   __shared__ __align__(16) uint8_t turn[TILE * TILE];
   __shared__ __align__(16) uint32_t col_most[THREADS / 32][TILE / 2];      // two columns in a word
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const long long col0 = static_cast<long long>(blockIdx.x) * TILE, row0 = static_cast<long long>(blockIdx.y) * TILE;
+  const long long col0 = static_cast<long long>(tile_x) * TILE, row0 = static_cast<long long>(tile_y) * TILE;
   const long long c0 = col0 + 8 * l, r0 = row0 + 8 * g;
   uint4 v[8];
   const bool whole = col0 + TILE <= cols && row0 + TILE <= rows;
@@ -87,7 +100,7 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
     // even columns of both rows against odd ones of both
     row_most[i] = max2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
   }
-  if (SQUARE) {
+  if (square) {
     uint32_t m = max2(max2(row_most[0], row_most[1]), max2(row_most[2], row_most[3]));
     m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
     if (lane == 0) col_most[0][warp] = m;
@@ -125,7 +138,7 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
   }
 
   // The bytes of word (group of four, row); the last tile of a row fills the word.
-  auto put_scale = [&](const Fp8Out& o, long long block, long long blocks, long long row, long long pad, uint32_t byte) {
+  auto put_scale = [&](const Fp8Operand& o, long long block, long long blocks, long long row, long long pad, uint32_t byte) {
     uint8_t* word = reinterpret_cast<uint8_t*>(o.scales + block / 4 * pad + row);
     word[block & 3] = static_cast<uint8_t>(byte);
     if (block == blocks - 1)
@@ -143,7 +156,7 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
                                  codes4(low_half(v[i].z) * inv, high_half(v[i].z) * inv, low_half(v[i].w) * inv, high_half(v[i].w) * inv));
       if (whole || (r0 + i < rows && c0 < cols)) *reinterpret_cast<uint2*>(p) = o;
     }
-    if (l < 8) put_scale(plain, blockIdx.x, gridDim.x, r0 + l, static_cast<long long>(gridDim.y) * TILE, own);
+    if (l < 8) put_scale(plain, tile_x, tiles_x, r0 + l, static_cast<long long>(tiles_y) * TILE, own);
   }
   if (turned.codes != nullptr) {
     uint32_t own = 0;                            // of column 8 l + g
@@ -162,7 +175,7 @@ fp8_quantize_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
           make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
       if (g == j) own = byte;
     }
-    if (g < 8) put_scale(turned, blockIdx.y, gridDim.y, c0 + g, static_cast<long long>(gridDim.x) * TILE, own);
+    if (g < 8) put_scale(turned, tile_y, tiles_y, c0 + g, static_cast<long long>(tiles_x) * TILE, own);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < TILE * TILE / 16 / THREADS; ++k) {
@@ -193,23 +206,27 @@ fp8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint32_t* __restr
 
 }  // namespace
 
-int fp8_quantize(const void* x, long long rows, long long cols, long long ldx, int square, const Fp8Out& plain, const Fp8Out& turned,
-                 cudaStream_t st) {
-  if (rows == 0 || cols == 0) return 0;
-  const long long by = (rows + TILE - 1) / TILE, bx = (cols + TILE - 1) / TILE;
-  if (by > 65535 || bx > INT32_MAX || cols % 16 != 0 || ldx % 8 != 0) return -1;
-  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by));
-  const auto kernel = square ? fp8_quantize_kernel<true> : fp8_quantize_kernel<false>;
-  return launch_overlapped(kernel, grid, THREADS, 0, st, static_cast<const __nv_bfloat16*>(x), rows, cols, ldx, plain, turned) ==
-                 cudaSuccess ? 0 : -3;
+int fp8_quantize(const Fp8Rounding* what, int count, cudaStream_t st) {
+  Roundings both = {};
+  long long tiles = 0;
+  for (int i = 0; i < count && i < 2; ++i) {
+    const Fp8Rounding& r = what[i];
+    const long long x = (r.cols + TILE - 1) / TILE, y = (r.rows + TILE - 1) / TILE;
+    if (r.cols % 16 != 0 || r.ldx % 8 != 0 || x > INT32_MAX / 2 || y > INT32_MAX / 2 || (tiles += x * y) > INT32_MAX / 2) return -1;
+    both.what[i] = r;
+    both.tiles_x[i] = static_cast<int>(x);
+    both.tiles_y[i] = static_cast<int>(y);
+  }
+  if (tiles == 0) return 0;
+  return launch_overlapped(fp8_quantize_kernel, static_cast<unsigned>(tiles), THREADS, 0, st, both) == cudaSuccess ? 0 : -3;
 }
 
-int fp8_dequantize(const uint8_t* codes, const uint32_t* scales, long long ld, float* out, long long rows, long long cols, cudaStream_t st) {
+int fp8_dequantize(const Fp8Operand& a, float* out, long long rows, long long cols, cudaStream_t st) {
   if (rows == 0 || cols == 0) return 0;
   const long long want = (rows * cols + 8 * THREADS - 1) / (8 * THREADS);
   const dim3 grid(static_cast<unsigned>(want < 65536 ? want : 65536));
-  return launch_overlapped(fp8_dequantize_kernel, grid, THREADS, 0, st, codes, scales, ld, out, rows, cols, fp8_scale_rows(rows)) ==
-                 cudaSuccess ? 0 : -3;
+  return launch_overlapped(fp8_dequantize_kernel, grid, THREADS, 0, st, a.codes, a.scales, a.ld, out, rows, cols,
+                           fp8_scale_rows(rows)) == cudaSuccess ? 0 : -3;
 }
 
 }  // namespace piper

@@ -24,15 +24,36 @@ GROUP = 128
 _NAN_SCALE = 255
 
 
+def _sizes(rows: int, cols: int) -> tuple[int, int, int]:
+    """Bytes of a row of codes, words of scales for a group of four, groups of four."""
+    return (cols + 15) // 16 * 16, (rows + GROUP - 1) // GROUP * GROUP, (cols + 4 * GROUP - 1) // (4 * GROUP)
+
+
+def _bytes(rows: int, cols: int) -> int:
+    ld, pad, groups = _sizes(rows, cols)
+    return rows * ld + 4 * groups * pad
+
+
 class Fp8Matrix:
     """A matrix ``[rows, cols]`` in e4m3, ready as an operand of a product along ``cols``.
 
-    ``codes`` is uint8 ``[rows, >= cols]``; ``scales`` holds the exponents of the powers of two, with a bias of 127 (255: NaN),
-    of four neighbouring groups of a row in one int32, ``[ceil(cols / 512), rows rounded up to 128]``.
+    ``data`` is one piece of memory, uint8: the ``codes`` ``[rows, cols rounded up to 16]`` and, behind them, the ``scales``, the
+    exponents of the powers of two, with a bias of 127 (255: NaN), of four neighbouring groups of a row in one int32,
+    ``[ceil(cols / 512), rows rounded up to 128]``.
     """
 
-    def __init__(self, codes: Tensor, scales: Tensor, rows: int, cols: int) -> None:
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+    def __init__(self, data: Tensor, rows: int, cols: int) -> None:
+        self.data, self.rows, self.cols = data, rows, cols
+
+    @property
+    def codes(self) -> Tensor:
+        ld = _sizes(self.rows, self.cols)[0]
+        return self.data[:self.rows * ld].view(self.rows, ld)
+
+    @property
+    def scales(self) -> Tensor:
+        ld, pad, groups = _sizes(self.rows, self.cols)
+        return self.data[self.rows * ld:].view(torch.int32).view(groups, pad)
 
     @property
     def shape(self) -> tuple[int, int]:
@@ -40,26 +61,26 @@ class Fp8Matrix:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.data.device
 
     def dequantize(self) -> Tensor:
         """The values that the codes stand for, in fp32."""
-        if self.codes.is_cuda:
+        if self.data.is_cuda:
             out = torch.empty(self.rows, self.cols, dtype=torch.float32, device=self.device)
-            native.lib().fp8_dequantize(self.codes, self.scales, out)
+            native.lib().fp8_dequantize(self.data, out)
             return out
-        return _values_ref(self.codes, self.scales, self.rows, self.cols)
+        return _values_ref(self.data, self.rows, self.cols)
 
     def __repr__(self) -> str:
         return f"Fp8Matrix({self.rows}, {self.cols}, device={self.device})"
 
 
 # ------------------------------------------------------------------ plain form (CPU)
-def _quantize_ref(x: Tensor, square: bool) -> tuple[Tensor, Tensor]:
-    """Codes and words of scales of x [rows, cols] along its columns."""
+def _quantize_ref(x: Tensor, square: bool) -> Tensor:
+    """x [rows, cols] as an operand along its columns."""
     rows, cols = x.shape
     if x.numel() == 0:
-        return _operand_buffers(rows, cols, x)
+        return torch.zeros(_bytes(rows, cols), dtype=torch.uint8)
     R, C = (rows + GROUP - 1) // GROUP, (cols + GROUP - 1) // GROUP
     pad = torch.zeros(R * GROUP, C * GROUP, dtype=torch.float32)
     pad[:rows, :cols] = x
@@ -71,16 +92,17 @@ def _quantize_ref(x: Tensor, square: bool) -> tuple[Tensor, Tensor]:
     byte = torch.where(torch.isinf(most), torch.full_like(bits, _NAN_SCALE),
                        ((bits >> 23) - 8 + ((bits & 0x7FFFFF) > 0x600000).int()).clamp(min=0))
     inverse = torch.where(byte == _NAN_SCALE, torch.zeros_like(byte), (254 - byte) << 23).view(torch.float32)
-    codes = torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.uint8)
+    codes = torch.zeros(rows, _sizes(rows, cols)[0], dtype=torch.uint8)
     codes[:, :cols] = (tiles * inverse).view(pad.shape)[:rows, :cols].contiguous().to(torch.float8_e4m3fn).view(torch.uint8)
     words = torch.zeros((C + 3) // 4 * 4, R * GROUP, dtype=torch.uint8)
     words[:C] = byte.view(R * GROUP // h, 1, C).expand(-1, h, C).reshape(R * GROUP, C).t().to(torch.uint8)
-    return codes, words.view(-1, 4, R * GROUP).transpose(1, 2).contiguous().view(torch.int32).squeeze(2)
+    return torch.cat((codes.view(-1), words.view(-1, 4, R * GROUP).transpose(1, 2).reshape(-1)))
 
 
-def _values_ref(codes: Tensor, scales: Tensor, rows: int, cols: int) -> Tensor:
-    groups, pad = scales.shape
-    byte = scales.unsqueeze(2).contiguous().view(torch.uint8).view(groups, pad, 4).transpose(1, 2).reshape(groups * 4, pad)
+def _values_ref(data: Tensor, rows: int, cols: int) -> Tensor:
+    ld, pad, groups = _sizes(rows, cols)
+    codes = data[:rows * ld].view(rows, ld)
+    byte = data[rows * ld:].view(groups, pad, 4).transpose(1, 2).reshape(groups * 4, pad)
     byte = byte[:(cols + GROUP - 1) // GROUP, :rows].t().to(torch.int32)
     scale = torch.where(byte > 0, byte << 23, torch.full_like(byte, 1 << 22)).view(torch.float32)
     scale = torch.where(byte == _NAN_SCALE, torch.full_like(scale, float("nan")), scale)
@@ -89,43 +111,27 @@ def _values_ref(codes: Tensor, scales: Tensor, rows: int, cols: int) -> Tensor:
 
 
 # ------------------------------------------------------------------ rounding
-def _operand_buffers(rows: int, cols: int, like: Tensor) -> tuple[Tensor, Tensor]:
-    return (torch.empty(rows, (cols + 15) // 16 * 16, dtype=torch.uint8, device=like.device),
-            torch.empty((cols + 4 * GROUP - 1) // (4 * GROUP), (rows + GROUP - 1) // GROUP * GROUP, dtype=torch.int32,
-                        device=like.device))
-
-
-def _nothing(like: Tensor) -> tuple[Tensor, Tensor]:
-    return like.new_empty((0, 0), dtype=torch.uint8), like.new_empty((0, 0), dtype=torch.int32)
-
-
-def _quantize(x: Tensor, square: bool, plain: bool, turned: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-    """(codes, scales) of x along its columns and of x^T along the rows of x; what is not wanted is empty."""
+def _quantize(x: Tensor, square: bool, plain: bool, turned: bool) -> tuple[Tensor, Tensor]:
+    """x as an operand along its columns, and x^T along the rows of x; what is not wanted is empty."""
     rows, cols = x.shape
-    p, t = _nothing(x), _nothing(x)
-    if x.is_cuda:
-        if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.contiguous_format)
-        if plain:
-            p = _operand_buffers(rows, cols, x)
-        if turned:
-            t = _operand_buffers(cols, rows, x)
-        native.lib().fp8_quantize(x, square, *(p if plain else (None, None)), *(t if turned else (None, None)))
-    else:
-        if plain:
-            p = _quantize_ref(x, square)
-        if turned:
-            t = _quantize_ref(x.t(), square)
-    return (*p, *t)
+    if not x.is_cuda:
+        none = torch.empty(0, dtype=torch.uint8)
+        return _quantize_ref(x, square) if plain else none, _quantize_ref(x.t(), square) if turned else none
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    p = torch.empty(_bytes(rows, cols) if plain else 0, dtype=torch.uint8, device=x.device)
+    t = torch.empty(_bytes(cols, rows) if turned else 0, dtype=torch.uint8, device=x.device)
+    native.lib().fp8_quantize(x, square, p if plain else None, t if turned else None, None, None, None)
+    return p, t
 
 
-def _product(a: tuple[Tensor, Tensor], b: tuple[Tensor, Tensor], M: int, N: int, K: int, out: Tensor) -> Tensor:
+def _product(a: Tensor, b: Tensor, M: int, N: int, K: int, out: Tensor) -> Tensor:
     """a [M, K] b [N, K]^T into ``out``; on a GPU into bf16, or added to fp32."""
     if out.is_cuda:
         if M and N:
-            native.lib().fp8_gemm(*a, *b, out, K, native.status_tensor(out.device))
+            native.lib().fp8_gemm(a, b, out, K, native.status_tensor(out.device))
         return out
-    return out.copy_(_values_ref(*a, M, K) @ _values_ref(*b, N, K).t())
+    return out.copy_(_values_ref(a, M, K) @ _values_ref(b, N, K).t())
 
 
 def _check_matrix(x: Tensor, what: str) -> None:
@@ -144,8 +150,8 @@ def fp8_quantize(x: Tensor, *, square: bool = False, transpose: bool = False) ->
     of the result, or with ``square`` for every 128 x 128, as weights have it.  No gradient passes."""
     _check_matrix(x, "fp8_quantize")
     with torch.no_grad():
-        codes, scales, turned, turned_scales = _quantize(x.detach(), square, not transpose, transpose)
-    return Fp8Matrix(turned, turned_scales, x.shape[1], x.shape[0]) if transpose else Fp8Matrix(codes, scales, *x.shape)
+        plain, turned = _quantize(x.detach(), square, not transpose, transpose)
+    return Fp8Matrix(turned, x.shape[1], x.shape[0]) if transpose else Fp8Matrix(plain, *x.shape)
 
 
 def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix) -> Tensor:
@@ -156,82 +162,75 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix) -> Tensor:
         raise ValueError(f"fp8_matmul: operands on {a.device} and {b.device}")
     if b.rows % 8:
         raise ValueError(f"fp8_matmul: the product must have a multiple of 8 columns, got {b.rows}")
-    out = torch.empty(a.rows, b.rows, dtype=torch.bfloat16 if a.codes.is_cuda else torch.float32, device=a.device)
-    return _product((a.codes, a.scales), (b.codes, b.scales), a.rows, b.rows, a.cols, out)
+    out = torch.empty(a.rows, b.rows, dtype=torch.bfloat16 if a.data.is_cuda else torch.float32, device=a.device)
+    return _product(a.data, b.data, a.rows, b.rows, a.cols, out)
 
 
 # ------------------------------------------------------------------ linear layer
 @custom_op("piper::fp8_linear_fwd")
-def fp8_linear_fwd(x: Tensor, w: Tensor, keep_x: bool, keep_w: bool) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+def fp8_linear_fwd(x: Tensor, w: Tensor, keep_x: bool, keep_w: bool) -> tuple[Tensor, Tensor, Tensor]:
     """y [T, N] = x [T, K] w [N, K]^T, and the transposed operands that the backward pass wants: x^T [K, T] for the gradient of
     w (keep_x), w^T [K, N] for the gradient of x (keep_w)."""
-    xc, xs, xt, xts = _quantize(x, False, True, keep_x)
-    wc, ws, wt, wts = _quantize(w, True, True, keep_w)
-    y = torch.empty(x.shape[0], w.shape[0], dtype=x.dtype, device=x.device)
-    _product((xc, xs), (wc, ws), x.shape[0], w.shape[0], x.shape[1], y)
-    return y, xt, xts, wt, wts
+    (T, K), N = x.shape, w.shape[0]
+    xp, xt = _quantize(x, False, True, keep_x)
+    wp, wt = _quantize(w, True, True, keep_w)
+    return _product(xp, wp, T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device)), xt, wt
 
 
 @fp8_linear_fwd.register_fake
 def _(x, w, keep_x, keep_w):
     T, (N, K) = x.shape[0], w.shape
-
-    def operand(rows, cols, wanted):
-        if not wanted:
-            return x.new_empty((0, 0), dtype=torch.uint8), x.new_empty((0, 0), dtype=torch.int32)
-        return (x.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.uint8),
-                x.new_empty(((cols + 4 * GROUP - 1) // (4 * GROUP), (rows + GROUP - 1) // GROUP * GROUP), dtype=torch.int32))
-
-    return (x.new_empty((T, N)), *operand(K, T, keep_x), *operand(K, N, keep_w))
+    return (x.new_empty((T, N)), x.new_empty((_bytes(K, T) if keep_x else 0,), dtype=torch.uint8),
+            x.new_empty((_bytes(K, N) if keep_w else 0,), dtype=torch.uint8))
 
 
 def _linear_setup(ctx, inputs, output):
     x, w, keep_x, keep_w = inputs
-    ctx.x_shape = tuple(x.shape)
-    ctx.mark_non_differentiable(*output[1:])
-    ctx.save_for_backward(w, *output[1:])
+    _y, xt, wt = output
+    ctx.rows = x.shape[0]
+    ctx.mark_non_differentiable(xt, wt)
+    ctx.save_for_backward(w, xt, wt)
 
 
-def _fp8_wgrad(dyt: Tensor, dyts: Tensor, xt: Tensor, xts: Tensor, w: Tensor, T: int):
+def _fp8_wgrad(dyt: Tensor, xt: Tensor, w: Tensor, T: int):
     """dW [N, K] = dY^T X, into the weight's fp32 bucket if it has one (returns None then)."""
     N, K = w.shape
     sink = grad_sinks.get(w)
     if T == 0:
         return None if sink is not None else torch.zeros_like(w)
-    if sink is not None:
-        if w.is_cuda:
-            _product((dyt, dyts), (xt, xts), N, K, T, sink)
-        else:
-            sink.add_(_values_ref(dyt, dyts, N, T) @ _values_ref(xt, xts, K, T).t())
-        return None
-    return _product((dyt, dyts), (xt, xts), N, K, T, torch.empty_like(w, memory_format=torch.contiguous_format))
+    if sink is None:
+        return _product(dyt, xt, N, K, T, torch.empty_like(w, memory_format=torch.contiguous_format))
+    if w.is_cuda:
+        _product(dyt, xt, N, K, T, sink)
+    else:
+        sink.add_(_values_ref(dyt, N, T) @ _values_ref(xt, K, T).t())
+    return None
 
 
 def _linear_backward(ctx, dy, *_unused):
-    w, xt, xts, wt, wts = ctx.saved_tensors
+    w, xt, wt = ctx.saved_tensors
     need_x, need_w = ctx.needs_input_grad[:2]
-    T, K = ctx.x_shape
-    N = w.shape[0]
+    T, (N, K) = ctx.rows, w.shape
     if dy is None:
         return (w.new_zeros((T, K)) if need_x else None, torch.zeros_like(w) if need_w else None, None, None)
-    dyc, dys, dyt, dyts = _quantize(dy, False, need_x, need_w)
+    dyp, dyt = _quantize(dy, False, need_x, need_w)
     dx = dw = None
     if need_x:
-        dx = _product((dyc, dys), (wt, wts), T, K, N, torch.empty((T, K), dtype=dy.dtype, device=dy.device))
+        dx = _product(dyp, wt, T, K, N, torch.empty((T, K), dtype=dy.dtype, device=dy.device))
     if need_w:
         if wgrad_store.active is not None:
-            wgrad_store.active.append((lambda: _fp8_wgrad(dyt, dyts, xt, xts, w, T), w))
+            wgrad_store.active.append((lambda: _fp8_wgrad(dyt, xt, w, T), w))
         else:
-            dw = _fp8_wgrad(dyt, dyts, xt, xts, w, T)
+            dw = _fp8_wgrad(dyt, xt, w, T)
     return dx, dw, None, None
 
 
 fp8_linear_fwd.register_autograd(_linear_backward, setup_context=_linear_setup)
 
 
-def _linear_backward_host(dy: Tensor, saved: list[Tensor], T: int, need_x: bool, need_w: bool) -> tuple[Tensor, Tensor]:
-    ctx = HostContext(saved, (need_x, need_w))
-    ctx.x_shape = (T, saved[0].shape[1])
+def _linear_backward_host(dy: Tensor, w: Tensor, xt: Tensor, wt: Tensor, T: int, need_x: bool, need_w: bool) -> tuple[Tensor, Tensor]:
+    ctx = HostContext((w, xt, wt), (need_x, need_w))
+    ctx.rows = T
     dx, dw, _, _ = _linear_backward(ctx, dy)
     none = torch.empty(0)
     return none if dx is None else dx, none if dw is None else dw
@@ -241,16 +240,15 @@ host_op("fp8_linear_backward_host", _linear_backward_host)
 
 
 @custom_op("piper::fp8_linear_kept")
-def fp8_linear_kept(x: Tensor, codes: Tensor, scales: Tensor) -> Tensor:
+def fp8_linear_kept(x: Tensor, w: Tensor, N: int) -> Tensor:
     """y [T, N] = x [T, K] w^T of a weight [N, K] that was rounded before."""
-    (T, K), N = x.shape, codes.shape[0]
-    xc, xs, _, _ = _quantize(x, False, True, False)
-    return _product((xc, xs), (codes, scales), T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device))
+    T, K = x.shape
+    return _product(_quantize(x, False, True, False)[0], w, T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device))
 
 
 @fp8_linear_kept.register_fake
-def _(x, codes, scales):
-    return x.new_empty((x.shape[0], codes.shape[0]))
+def _(x, w, N):
+    return x.new_empty((x.shape[0], N))
 
 
 fp8_linear_fwd = fp8_linear_fwd.overload
@@ -275,7 +273,7 @@ def fp8_linear(x: Tensor, w: Union[Tensor, Fp8Matrix]) -> Tensor:
     if kept:
         if torch.is_grad_enabled() and x.requires_grad:
             raise ValueError("fp8_linear: a weight that was rounded before has no backward pass; give the bf16 weight")
-        y = fp8_linear_kept(x2, w.codes, w.scales)
+        y = fp8_linear_kept(x2, w.data, N)
     else:
         if w.dtype != x.dtype:
             raise TypeError(f"fp8_linear: x is {x.dtype}, w {w.dtype}")

@@ -78,6 +78,7 @@ class AdamWState:
         self.bits, self.device = bits, params[0].device
         self.shapes = [tuple(p.shape) for p in params]
         self.dtypes = [p.dtype for p in params]
+        self.sizes = [2 * p.numel() + (p.dtype == torch.bfloat16) for p in params]
         self.offsets, at = [], 0
         for p in params:
             if p.dtype not in (torch.bfloat16, torch.float32):
@@ -170,31 +171,32 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], stat
     step counts live on the host, so a step cannot be captured into a CUDA graph, which would repeat one bias correction.
     """
     params, grads = list(params), list(grads)
-    if len(params) != len(state.shapes) or len(grads) != len(params):
-        raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients, a state of {len(state.shapes)}")
-    for p, g, shape, dtype in zip(params, grads, state.shapes, state.dtypes):
-        if p.shape != shape or p.dtype != dtype or p.device != state.device:
-            raise ValueError(f"adamw_step: the state is of a {dtype} parameter {shape} on {state.device}, got {p.dtype} "
-                             f"{tuple(p.shape)} on {p.device}")
-        if g is not None and (g.shape != shape or g.device != p.device):
-            raise ValueError(f"adamw_step: a gradient is {tuple(g.shape)} on {g.device}, its parameter {shape} on {p.device}")
     b1, b2 = betas
     if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1):
         raise ValueError(f"adamw_step: lr={lr}, betas={betas}, eps={eps}, weight_decay={weight_decay}")
-    if state.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("adamw_step: the step count lives on the host; a captured step would repeat itself")
-    steps = [s + (g is not None) for s, g in zip(state.steps, grads)]
-    with torch.no_grad():
-        if state.device.type == "cuda":
-            grads = [g if g is None or g.is_contiguous() else g.contiguous() for g in grads]
-            native.lib().adamw(params, grads, state.m, state.v, state.m_scale, state.v_scale, state.master, state.offsets,
-                               steps, lr, b1, b2, eps, weight_decay, grad_scale)
-        else:
+    if state.device.type == "cuda":
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("adamw_step: the step count lives on the host; a captured step would repeat itself")
+        if params and params[0].device != state.device:
+            raise ValueError(f"adamw_step: the state is on {state.device}, a parameter on {params[0].device}")
+        # the library checks every tensor before it launches anything
+        native.lib().adamw.default(params, grads, state.m, state.v, state.m_scale, state.v_scale, state.master, state.offsets,
+                                   state.sizes, state.steps, lr, b1, b2, eps, weight_decay, grad_scale)
+    else:
+        if len(params) != len(state.shapes) or len(grads) != len(params):
+            raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients, a state of {len(state.shapes)}")
+        for p, g, size in zip(params, grads, state.sizes):
+            if 2 * p.numel() + (p.dtype == torch.bfloat16) != size or p.device != state.device:
+                raise ValueError(f"adamw_step: the state is of a parameter of {size // 2} elements on {state.device}, got "
+                                 f"{p.dtype} {tuple(p.shape)} on {p.device}")
+            if g is not None and (g.shape != p.shape or g.device != p.device):
+                raise ValueError(f"adamw_step: a gradient is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)}")
+        with torch.no_grad():
             for i, (p, g) in enumerate(zip(params, grads)):
                 if g is not None and p.numel():
-                    _step_ref(state, i, p, g, steps[i], lr, b1, b2, eps, weight_decay, grad_scale)
-    torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
-    state.steps = steps
+                    _step_ref(state, i, p, g, state.steps[i] + 1, lr, b1, b2, eps, weight_decay, grad_scale)
+        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+    state.steps = [s + (g is not None) for s, g in zip(state.steps, grads)]
 
 
 def _step_ref(state: AdamWState, i: int, p: Tensor, grad: Tensor, step: int, lr: float, b1: float, b2: float, eps: float,
