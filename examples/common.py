@@ -49,6 +49,7 @@ def add_common_args(p: argparse.ArgumentParser, default_schedule: str) -> None:
     p.add_argument("--dtype", default="bf16", choices=("bf16", "fp32"))
     p.add_argument("--optimizer", default="adam", choices=("adam", "adamw", "adamw8"),
                    help="adamw8: AdamW with moments in 8 bits")
+    p.add_argument("--fp8", action="store_true", default=False, help="projections of the layers in 8-bit floating point")
     p.add_argument("--checkpoint-dir", default="", help="save a checkpoint here after the timed iterations")
     p.add_argument("--resume", default="", help="checkpoint directory to resume from")
 

@@ -1,5 +1,6 @@
 """End-to-end Qwen3 MoE driver for the JSON-driven training-DAG runtime (run through ``examples/test_harness.py``)."""
 import argparse
+import dataclasses
 import os
 import sys
 
@@ -11,7 +12,7 @@ from piper_b200.nn import cross_entropy_loss  # noqa: E402
 
 
 def main(args, pg=None):
-    cfg = QWEN3_CONFIGS[args.model]
+    cfg = dataclasses.replace(QWEN3_CONFIGS[args.model], fp8=args.fp8)
     num_stages = int(getattr(args, "num_stages", 0) or derive_num_stages(args.schedule_directives_file))
     return run_driver(args, PiperQwen3Model, (cfg, num_stages, args.seq_len), cfg, cross_entropy_loss,
                       PiperQwen3Model.const_attrs(cfg, args.seq_len))

@@ -34,6 +34,7 @@ class LlamaConfig:
     norm_eps: float = 1e-5
     rope_theta: float = 500000.0
     max_seq_len: int = 4096
+    fp8: bool = False               # projections of the layers (not the head) in 8 bits, see nn.Linear
 
     @property
     def head_dim(self) -> int:
@@ -58,9 +59,9 @@ class TransformerBlock(nn.Module):
         super().__init__()
         self.attention_norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.attention = Attention(cfg.dim, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, qk_norm=False,
-                                   rope_interleaved=True, norm_eps=cfg.norm_eps)
+                                   rope_interleaved=True, norm_eps=cfg.norm_eps, fp8=cfg.fp8)
         self.ffn_norm = RMSNorm(cfg.dim, cfg.norm_eps)
-        self.feed_forward = FeedForward(cfg.dim, cfg.ffn_hidden)
+        self.feed_forward = FeedForward(cfg.dim, cfg.ffn_hidden, cfg.fp8)
 
     def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor], cos, sin, batch: int, seq: int):
         """``h`` is the residual stream and ``delta`` a branch output not yet added to it.

@@ -46,6 +46,7 @@ class Qwen3Config:
     # different positions are strongly correlated before any training); benchmark runs set a std that dominates
     # the initial logits so that the load over experts is near-uniform from the first step.  0 disables it.
     router_jitter_std: float = 0.0
+    fp8: bool = False               # projections of attention and of dense MLPs in 8 bits, see nn.Linear
 
 
 QWEN3_CONFIGS = {
@@ -105,10 +106,10 @@ class Qwen3Block(nn.Module):
         super().__init__()
         self.attention_norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.attention = Attention(cfg.dim, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, qk_norm=True,
-                                   rope_interleaved=False, norm_eps=cfg.norm_eps)
+                                   rope_interleaved=False, norm_eps=cfg.norm_eps, fp8=cfg.fp8)
         self.ffn_norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.moe = MoE(cfg) if cfg.moe_enabled else None
-        self.feed_forward = None if cfg.moe_enabled else FeedForward(cfg.dim, cfg.ffn_hidden)
+        self.feed_forward = None if cfg.moe_enabled else FeedForward(cfg.dim, cfg.ffn_hidden, cfg.fp8)
 
     def forward(self, h, delta, cos, sin, batch: int, seq: int, jitter=None):
         if delta is None:

@@ -16,15 +16,16 @@ from .. import ops
 
 
 class Linear(nn.Module):
-    """y = x W^T with W stored ``[out_features, in_features]`` (no bias)."""
+    """y = x W^T with W stored ``[out_features, in_features]`` (no bias); ``fp8``: products of e4m3 operands with a scale for
+    every 128 of the contraction, features in multiples of 16."""
 
-    def __init__(self, in_features: int, out_features: int) -> None:
+    def __init__(self, in_features: int, out_features: int, fp8: bool = False) -> None:
         super().__init__()
-        self.in_features, self.out_features = in_features, out_features
+        self.in_features, self.out_features, self.fp8 = in_features, out_features, fp8
         self.weight = nn.Parameter(torch.empty(out_features, in_features))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return ops.linear(x, self.weight)
+        return ops.fp8_linear(x, self.weight) if self.fp8 else ops.linear(x, self.weight)
 
 
 class RMSNorm(nn.Module):
@@ -53,12 +54,12 @@ class Attention(nn.Module):
     """Causal grouped-query self-attention with a fused QKV projection, optional QK-RMSNorm, and RoPE."""
 
     def __init__(self, dim: int, n_heads: int, n_kv_heads: int, head_dim: int, qk_norm: bool = False,
-                 rope_interleaved: bool = True, norm_eps: float = 1e-6) -> None:
+                 rope_interleaved: bool = True, norm_eps: float = 1e-6, fp8: bool = False) -> None:
         super().__init__()
         self.n_heads, self.n_kv_heads, self.head_dim = n_heads, n_kv_heads, head_dim
         self.rope_interleaved, self.norm_eps = rope_interleaved, norm_eps
-        self.wqkv = Linear(dim, (n_heads + 2 * n_kv_heads) * head_dim)
-        self.wo = Linear(n_heads * head_dim, dim)
+        self.wqkv = Linear(dim, (n_heads + 2 * n_kv_heads) * head_dim, fp8)
+        self.wo = Linear(n_heads * head_dim, dim, fp8)
         self.q_norm = RMSNorm(head_dim, norm_eps) if qk_norm else None
         self.k_norm = RMSNorm(head_dim, norm_eps) if qk_norm else None
 
@@ -76,10 +77,10 @@ class Attention(nn.Module):
 class FeedForward(nn.Module):
     """SwiGLU MLP with the gate and up projections fused into one weight ``w13 = [w1; w3]``."""
 
-    def __init__(self, dim: int, hidden: int) -> None:
+    def __init__(self, dim: int, hidden: int, fp8: bool = False) -> None:
         super().__init__()
-        self.w13 = Linear(dim, 2 * hidden)
-        self.w2 = Linear(hidden, dim)
+        self.w13 = Linear(dim, 2 * hidden, fp8)
+        self.w2 = Linear(hidden, dim, fp8)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return self.w2(ops.swiglu(self.w13(x)))
@@ -97,3 +98,16 @@ class CrossEntropyLoss(nn.Module):
 
     def forward(self, output: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         return cross_entropy_loss(output, labels, self.ignore_index)
+
+
+def policy_gradient_loss(output: torch.Tensor, tokens: torch.Tensor, advantages: Optional[torch.Tensor] = None, *,
+                         entropy_coef: float = 0.0, temperature: float = 1.0, ignore_index: int = -100) -> torch.Tensor:
+    """Minus the mean over the counted tokens of advantage (1 without) x log probability + ``entropy_coef`` x entropy, of
+    ``[.., V]`` logits at ``temperature``."""
+    flat = tokens.reshape(-1)
+    r = ops.token_logprobs(output.reshape(-1, output.shape[-1]), flat, temperature=temperature, ignore_index=ignore_index)
+    counted = (flat != ignore_index).to(r.logprob.dtype)
+    gain = r.logprob if advantages is None else r.logprob * advantages.reshape(-1)
+    if entropy_coef:
+        gain = gain + entropy_coef * r.entropy * counted
+    return -gain.sum() / counted.sum().clamp(min=1)

@@ -167,8 +167,8 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix) -> Tensor:
 
 
 # ------------------------------------------------------------------ linear layer
-@custom_op("piper::fp8_linear_fwd")
-def fp8_linear_fwd(x: Tensor, w: Tensor, keep_x: bool, keep_w: bool) -> tuple[Tensor, Tensor, Tensor]:
+@custom_op("piper::fp8_linear_keep")
+def fp8_linear_keep(x: Tensor, w: Tensor, keep_x: bool, keep_w: bool) -> tuple[Tensor, Tensor, Tensor]:
     """y [T, N] = x [T, K] w [N, K]^T, and the transposed operands that the backward pass wants: x^T [K, T] for the gradient of
     w (keep_x), w^T [K, N] for the gradient of x (keep_w)."""
     (T, K), N = x.shape, w.shape[0]
@@ -177,19 +177,30 @@ def fp8_linear_fwd(x: Tensor, w: Tensor, keep_x: bool, keep_w: bool) -> tuple[Te
     return _product(xp, wp, T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device)), xt, wt
 
 
-@fp8_linear_fwd.register_fake
+@fp8_linear_keep.register_fake
 def _(x, w, keep_x, keep_w):
     T, (N, K) = x.shape[0], w.shape
     return (x.new_empty((T, N)), x.new_empty((_bytes(K, T) if keep_x else 0,), dtype=torch.uint8),
             x.new_empty((_bytes(K, N) if keep_w else 0,), dtype=torch.uint8))
 
 
-def _linear_setup(ctx, inputs, output):
-    x, w, keep_x, keep_w = inputs
-    _y, xt, wt = output
+@custom_op("piper::fp8_linear")
+def fp8_linear_op(x: Tensor, w: Tensor) -> Tensor:
+    """y [T, N] = x [T, K] w [N, K]^T.  Which operands the backward pass needs is decided where it is known, when the op runs, and
+    not by the caller, whose program may be traced without gradients."""
+    return fp8_linear_keep(x, w, False, False)[0]
+
+
+@fp8_linear_op.register_fake
+def _(x, w):
+    return x.new_empty((x.shape[0], w.shape[0]))
+
+
+def _linear_forward(ctx, x, w):
+    y, xt, wt = fp8_linear_keep(x, w, w.requires_grad, x.requires_grad)
     ctx.rows = x.shape[0]
-    ctx.mark_non_differentiable(xt, wt)
     ctx.save_for_backward(w, xt, wt)
+    return y
 
 
 def _fp8_wgrad(dyt: Tensor, xt: Tensor, w: Tensor, T: int):
@@ -207,12 +218,10 @@ def _fp8_wgrad(dyt: Tensor, xt: Tensor, w: Tensor, T: int):
     return None
 
 
-def _linear_backward(ctx, dy, *_unused):
+def _linear_backward(ctx, dy):
     w, xt, wt = ctx.saved_tensors
     need_x, need_w = ctx.needs_input_grad[:2]
     T, (N, K) = ctx.rows, w.shape
-    if dy is None:
-        return (w.new_zeros((T, K)) if need_x else None, torch.zeros_like(w) if need_w else None, None, None)
     dyp, dyt = _quantize(dy, False, need_x, need_w)
     dx = dw = None
     if need_x:
@@ -222,16 +231,16 @@ def _linear_backward(ctx, dy, *_unused):
             wgrad_store.active.append((lambda: _fp8_wgrad(dyt, xt, w, T), w))
         else:
             dw = _fp8_wgrad(dyt, xt, w, T)
-    return dx, dw, None, None
+    return dx, dw
 
 
-fp8_linear_fwd.register_autograd(_linear_backward, setup_context=_linear_setup)
+fp8_linear_op.register_autograd(_linear_backward, forward=_linear_forward)
 
 
 def _linear_backward_host(dy: Tensor, w: Tensor, xt: Tensor, wt: Tensor, T: int, need_x: bool, need_w: bool) -> tuple[Tensor, Tensor]:
     ctx = HostContext((w, xt, wt), (need_x, need_w))
     ctx.rows = T
-    dx, dw, _, _ = _linear_backward(ctx, dy)
+    dx, dw = _linear_backward(ctx, dy)
     none = torch.empty(0)
     return none if dx is None else dx, none if dw is None else dw
 
@@ -251,7 +260,8 @@ def _(x, w, N):
     return x.new_empty((x.shape[0], N))
 
 
-fp8_linear_fwd = fp8_linear_fwd.overload
+fp8_linear_keep = fp8_linear_keep.overload
+fp8_linear_op = fp8_linear_op.overload
 fp8_linear_kept = fp8_linear_kept.overload
 
 
@@ -277,6 +287,5 @@ def fp8_linear(x: Tensor, w: Union[Tensor, Fp8Matrix]) -> Tensor:
     else:
         if w.dtype != x.dtype:
             raise TypeError(f"fp8_linear: x is {x.dtype}, w {w.dtype}")
-        grad = torch.is_grad_enabled()
-        y = fp8_linear_fwd(x2, w, grad and w.requires_grad, grad and x.requires_grad)[0]
+        y = fp8_linear_op(x2, w)
     return y if x.dim() == 2 else y.view(*lead, N)

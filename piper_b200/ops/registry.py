@@ -87,14 +87,20 @@ class Op:
         torch.library.register_fake(self.qualname, fn, lib=self._lib, allow_override=True)
         return fn
 
-    def register_autograd(self, backward: Callable, *, setup_context: Optional[Callable] = None) -> None:
-        """``backward(ctx, *grads)`` returns a gradient per input; see above for gradients that did not arrive."""
+    def register_autograd(self, backward: Callable, *, setup_context: Optional[Callable] = None,
+                          forward: Optional[Callable] = None) -> None:
+        """``backward(ctx, *grads)`` returns a gradient per input; see above for gradients that did not arrive.  ``forward(ctx,
+        *args)``, run below autograd, takes the place of the op and of ``setup_context`` where the formula keeps what the op
+        does not return."""
         overload = self.overload
         one_output = len(overload._schema.returns) == 1
 
         class Formula(torch.autograd.Function):
             @staticmethod
             def forward(ctx, *args):
+                if forward is not None:
+                    with _below_autograd():
+                        return forward(ctx, *args)
                 with _below_autograd():
                     out = overload(*args)
                 if not one_output:

@@ -1,0 +1,131 @@
+"""A fine-tuning step through the engine: projections in 8 bits, a policy-gradient loss on token log probabilities with an
+entropy term, AdamW with 8-bit moments; against the same model and ops stepped by hand.
+
+Both sides run the same ops on the same microbatches.  They may differ where fp32 sums are added in another order: weight gradients
+of two microbatches (in the bucket, or by autograd in the parameters' type)."""
+import pytest
+import torch
+
+from piper_b200 import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _schedule(stages):
+    return [{"op": "place", "filter": {"PP": i}, "devices": [0]} for i in range(stages)] + \
+        [{"op": "split", "filter": {}, "dim_name": "MB", "num_microbatches": 2}]
+
+
+def _loss(output, tokens):
+    from piper_b200.nn import policy_gradient_loss
+    return policy_gradient_loss(output, tokens, entropy_coef=0.01, temperature=0.9)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_step_through_the_engine(device, tmp_path):
+    from piper_b200 import piper_exec_dag, piper_setup
+    from piper_b200.models.llama3 import LlamaConfig, Transformer
+    from piper_b200.runtime.checkpoint import load_checkpoint, save_checkpoint
+    from piper_b200.runtime.storage import init_tensor
+
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    cfg = LlamaConfig(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=1024, ffn_hidden=688, norm_eps=1e-6,
+                      rope_theta=10000.0, max_seq_len=128, fp8=True)
+    g = torch.Generator().manual_seed(0)
+    x = torch.randint(0, cfg.vocab_size, (4, 128), generator=g)
+    y = torch.randint(0, cfg.vocab_size, (4, 128), generator=g)
+    y[:, :9] = -100                                   # the prompt
+    hyper = {"lr": 1e-3, "weight_decay": 0.1, "betas": (0.9, 0.95)}
+
+    def setup():
+        actor = piper_setup(Transformer, (cfg, 128, 2), optim_fn=torch.optim.AdamW, optim_kwargs={**hyper, "state_bits": 8},
+                            example_inputs=[x], example_outputs=y, model_dtype=dtype,
+                            const_attrs=Transformer.const_attrs(cfg, 128), schedule_directives=_schedule(2), device=device)
+        actor.debug_keep_grads = True
+        return actor
+
+    actor = setup()
+    model = Transformer(cfg, 128, 2).to(device).to(dtype)         # the add at the stage boundary included
+    consts = Transformer.const_attrs(cfg, 128, device)
+    model.rope_cos, model.rope_sin = consts["rope_cos"], consts["rope_sin"]
+    names = [n for n, _ in model.named_parameters()]
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            p.copy_(init_tensor(n, p.shape, dtype, torch.device(device)))
+    state = ops.AdamWState(list(model.parameters()), bits=8)
+    for step in range(2):
+        losses = [float(v) for v in piper_exec_dag(_loss)]
+        got = {k: v.float() for k, v in actor.last_grads.items()}
+        want = []
+        for p in model.parameters():
+            p.grad = None
+        for a, b in zip(x.to(device).split(2), y.to(device).split(2)):
+            loss = _loss(model(a), b)
+            want.append(float(loss.detach()))
+            loss.backward()
+        half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -20
+        for a, b in zip(losses, want):
+            # the first step starts from the same weights; the second from weights whose gradients differ in their last digits
+            assert abs(a - b) <= (2.0 ** -20 if step == 0 else 2.0 ** -6) * abs(b), (losses, want)
+        if step == 0:
+            for n, p in model.named_parameters():
+                # the engine keeps the mean over the microbatches; two roundings of autograd's sum, and sums in another order
+                a, b = got[n], p.grad.float() / 2
+                assert float((a - b).norm()) <= 3 * half * float(b.norm()) + 1e-8, n
+        ops.adamw_step(list(model.parameters()), [p.grad for p in model.parameters()], state, grad_scale=0.5, **hyper)
+    assert names and all(b.storage.state8 is not None for b in actor.buckets.values() if b.storage is not None and b.storage.numel)
+    if device == "cuda":
+        ops.native.check_status()
+    # a checkpoint holds decoded moments, and a resumed run continues with the same values
+    save_checkpoint(actor, str(tmp_path), step=2, schedule=_schedule(2))
+    before = {k: tuple(t.clone() for t in (*b.storage.moments(), b.storage.flat_params))
+              for k, b in actor.buckets.items() if b.storage is not None and b.storage.numel}
+    again = setup()
+    assert load_checkpoint(again, str(tmp_path)) == 2
+    for k, b in again.buckets.items():
+        if k in before:
+            st = b.storage
+            assert all(torch.equal(a, c) for a, c in zip(before[k], (*st.moments(), st.flat_params)))
+            assert st.step_count == 2
+    assert [float(v) for v in piper_exec_dag(_loss)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_gradient_loss(device):
+    from piper_b200.nn import cross_entropy_loss, policy_gradient_loss
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn(2, 5, 64, generator=g).to(device).requires_grad_(True)
+    tokens = torch.randint(0, 64, (2, 5), generator=g).to(device)
+    tokens[0, :2] = -100
+    a, b = policy_gradient_loss(logits, tokens), torch.nn.functional.cross_entropy(logits.reshape(-1, 64), tokens.reshape(-1))
+    da, db = (torch.autograd.grad(v, logits)[0] for v in (a, b))
+    assert abs(float(a - b)) < 2.0 ** -20 * 10 and float((da - db).abs().max()) < 2.0 ** -20
+    adv = torch.randn(2, 5, generator=g).to(device)
+    z = logits.detach().double() / 0.7
+    logp = torch.log_softmax(z, -1)
+    on = tokens != -100
+    lp = logp.gather(-1, tokens.clamp(min=0).unsqueeze(-1)).squeeze(-1)
+    h = -(logp.exp() * logp).sum(-1)
+    want = -((adv * lp + 0.2 * h) * on).sum() / on.sum()
+    got = policy_gradient_loss(logits, tokens, adv, entropy_coef=0.2, temperature=0.7)
+    assert abs(float(got) - float(want)) < 2.0 ** -20 * 20
+    none = torch.full_like(tokens, -100)
+    assert float(policy_gradient_loss(logits, none, entropy_coef=0.5)) == 0.0
+
+
+def test_eight_bit_models_of_both_families():
+    import dataclasses
+
+    from piper_b200.models.llama3 import LLAMA_CONFIGS, Transformer
+    from piper_b200.models.qwen3 import QWEN3_CONFIGS, PiperQwen3Model
+    from piper_b200.nn import Linear
+    llama = Transformer(dataclasses.replace(LLAMA_CONFIGS["tiny"], fp8=True), 128, 1)
+    qwen = PiperQwen3Model(dataclasses.replace(QWEN3_CONFIGS["9M"], fp8=True, n_layers=2), 1, 128)
+    for model in (llama, qwen):
+        wide = [n for n, m in model.named_modules() if isinstance(m, Linear) and not m.fp8]
+        assert all(n.endswith(("output", "gate")) for n in wide), wide
+        assert any(isinstance(m, Linear) and m.fp8 for m in model.modules())
+    x = Linear(32, 48, fp8=True)
+    torch.nn.init.normal_(x.weight)
+    a = torch.randn(3, 32)
+    assert torch.equal(x(a), ops.fp8_linear(a, x.weight))
