@@ -41,30 +41,46 @@ __device__ __forceinline__ uint32_t mix32(uint32_t h) {
   return h ^ (h >> 16);
 }
 
-__device__ __forceinline__ float decode_v(uint32_t c, float scale) {
-  return __fmul_rn(c != 0 ? __uint_as_float((c + V_BASE) << 20) : 0.f, scale);
+// Code in byte `Byte` of a word to its value.  A byte moved to bits 16-23 is a multiplication away from the upper bits of the number.
+template <int BYTE>
+__device__ __forceinline__ float decode_v(uint32_t word, float scale) {
+  const uint32_t c = __byte_perm(word, 0, 0x4044u | BYTE << 8);
+  return __fmul_rn(__uint_as_float(c != 0 ? c * 16 + (static_cast<uint32_t>(V_BASE) << 20) : 0u), scale);
 }
-__device__ __forceinline__ float decode_m(uint32_t c, float scale) {
-  const uint32_t low = c & 127u;
-  return __fmul_rn(__uint_as_float((low != 0 ? (low + M_BASE) << 20 : 0u) | (c & 128u) << 24), scale);
+template <int BYTE>
+__device__ __forceinline__ float decode_m(uint32_t word, float scale) {
+  const uint32_t c = __byte_perm(word, 0, 0x4044u | BYTE << 8), low = c & 0x7F0000u;
+  const uint32_t bits = low != 0 ? low * 16 + (static_cast<uint32_t>(M_BASE) << 20) : 0u;
+  return __fmul_rn(__uint_as_float(bits | (c << 8 & 0x80000000u)), scale);
 }
 
-// Codes of y in [0, 1], r being 16 random bits: the upper bits of y plus what the random bits carry into them; below code 1,
-// 0 or 1 (v: 1 for all that is above 0).
+// Codes of y in [0, 1], in the top byte of the result: the upper bits of y plus what 16 random bits (the lower or the upper ones of r)
+// carry into them; below code 1, 0 or 1 (v: 1 for all that is above 0).  Bits 20-27 of y and the base are brought to the top
+// byte by a shift, whose overflow is what the base takes away.
 constexpr uint32_t M_LEAST = static_cast<uint32_t>(M_BASE + 1) << 20, V_LEAST = static_cast<uint32_t>(V_BASE + 1) << 20;
-__device__ __forceinline__ uint32_t encode(float y, uint32_t r, int base) { return ((__float_as_uint(y) + (r << 4)) >> 20) - base; }
-__device__ __forceinline__ uint32_t encode_small_m(float y, uint32_t r) {
-  return __fmul_rn(static_cast<float>(r), __uint_as_float(M_LEAST) * (1.f / 65536)) < y ? 1u : 0u;
+__device__ __forceinline__ uint32_t encode_m(float y, uint32_t r) {
+  return (__float_as_uint(y) << 4) + __byte_perm(r, (256u - M_BASE % 256) << 24, 0x7104u);
 }
-__device__ __forceinline__ uint32_t encode_small_v(float y) { return y > 0.f ? 1u : 0u; }
+__device__ __forceinline__ uint32_t encode_v(float y, uint32_t r) {
+  return (__float_as_uint(y) << 4) + __byte_perm(r, (256u - V_BASE % 256) << 24, 0x7324u);
+}
+__device__ __forceinline__ uint32_t encode_small_m(float y, uint32_t r) {
+  return __fmul_rn(static_cast<float>(r & 0xFFFFu), __uint_as_float(M_LEAST) * (1.f / 65536)) < y ? 1u << 24 : 0u;
+}
+__device__ __forceinline__ uint32_t encode_small_v(float y) { return y > 0.f ? 1u << 24 : 0u; }
+
+// The top bytes of four words, the first lowest.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&t)[4]) {
+  return __byte_perm(__byte_perm(t[0], t[1], 0x0073u), __byte_perm(t[2], t[3], 0x0073u), 0x5410u);
+}
 
 // The block's largest magnitude, NaN where a value is infinite or NaN.
 __device__ __forceinline__ float block_scale(const float (&x)[PER]) {
-  uint32_t most = 0;
+  float most = 0.f;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) most = max(most, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-  most = __reduce_max_sync(0xffffffffu, most);
-  return most >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(most);
+  for (int i = 0; i < PER; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(fabsf(x[i])));
+  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7FFFFFFFu);
+  return bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(bits);
 }
 
 // y = |x| / scale of a block, correctly rounded.  With the correctly rounded reciprocal, a product, its exact remainder and a
@@ -86,10 +102,14 @@ __device__ __forceinline__ void quotients(const float* x, float scale, float (&y
   }
 }
 
-__device__ __forceinline__ float sqrt_approx(float x) {
-  float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
+// m / (sqrt(v) root + eps), within two units of the last place for the root and for the quotient; numbers below the normal ones
+// count as 0, so a vanishing eps, beside which they would matter, takes the exact operations.
+__device__ __forceinline__ float update(float m, float v, float root, float eps) {
+  if (eps < 1e-30f) return m / fmaf(sqrtf(v), root, eps);
+  float r, q;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(fmaf(r, root, eps)));
+  return q;
 }
 
 __device__ __forceinline__ void load4(const float* p, float (&x)[PER], int h) {
@@ -174,17 +194,25 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
                                : static_cast<const float*>(t.grad)[at(j)];
         }
       }
+      if (BITS == 8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          m[4 * h] = decode_m<0>(mc[h], ms);
+          m[4 * h + 1] = decode_m<1>(mc[h], ms);
+          m[4 * h + 2] = decode_m<2>(mc[h], ms);
+          m[4 * h + 3] = decode_m<3>(mc[h], ms);
+          v[4 * h] = decode_v<0>(vc[h], vs);
+          v[4 * h + 1] = decode_v<1>(vc[h], vs);
+          v[4 * h + 2] = decode_v<2>(vc[h], vs);
+          v[4 * h + 3] = decode_v<3>(vc[h], vs);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        if (BITS == 8) {
-          m[j] = decode_m(mc[j / 4] >> (8 * (j & 3)) & 255u, ms);
-          v[j] = decode_v(vc[j / 4] >> (8 * (j & 3)) & 255u, vs);
-        }
         const float gj = __fmul_rn(g[j], a.grad_scale);
         m[j] = __fadd_rn(__fmul_rn(m[j], a.b1), __fmul_rn(gj, a.c1));
         v[j] = __fadd_rn(__fmul_rn(v[j], a.b2), __fmul_rn(__fmul_rn(gj, a.c2), gj));
-        // the update's root and quotient are within two units of the last place each
-        w[j] = fmaf(-rate, __fdividef(m[j], fmaf(sqrt_approx(v[j]), root, a.eps)), w[j] * a.keep);
+        w[j] = fmaf(-rate, update(m[j], v[j], root, a.eps), w[j] * a.keep);
       }
       if (!whole) {
 #pragma unroll
@@ -221,24 +249,22 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const uint32_t r = mix32(first + j);
-            cm[j] = encode(ym[j], r & 0xFFFFu, M_BASE);
-            cv[j] = encode(yv[j], r >> 16, V_BASE);
+            cm[j] = encode_m(ym[j], r);
+            cv[j] = encode_v(yv[j], r);
             least_m = min(least_m, __float_as_uint(ym[j]));
             least_v = min(least_v, __float_as_uint(yv[j]));
           }
           if (__builtin_expect(least_m < M_LEAST || least_v < V_LEAST, 0)) {      // few have such small elements, or zeros
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              if (__float_as_uint(ym[j]) < M_LEAST) cm[j] = encode_small_m(ym[j], mix32(first + j) & 0xFFFFu);
+              if (__float_as_uint(ym[j]) < M_LEAST) cm[j] = encode_small_m(ym[j], mix32(first + j));
               if (__float_as_uint(yv[j]) < V_LEAST) cv[j] = encode_small_v(yv[j]);
             }
           }
-          mc[h] = vc[h] = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            mc[h] |= (cm[j] & 127u) << (8 * j) | (__float_as_uint(m[4 * h + j]) >> 31) << (8 * j + 7);
-            vc[h] |= (cv[j] & 255u) << (8 * j);
-          }
+          for (int j = 0; j < 4; ++j) cm[j] = (cm[j] & 0x7FFFFFFFu) | (__float_as_uint(m[4 * h + j]) & 0x80000000u);
+          mc[h] = top_bytes(cm);
+          vc[h] = top_bytes(cv);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -285,10 +311,10 @@ moments_decode_kernel(const uint32_t* __restrict__ m, const float* __restrict__ 
     for (int k = 0; k < AHEAD; ++k) {
       const long long at = i + 256 * k;
       if (at >= words) break;
-      __stcs(out_m + at, make_float4(decode_m(cm[k] & 255u, sm[k]), decode_m(cm[k] >> 8 & 255u, sm[k]),
-                                     decode_m(cm[k] >> 16 & 255u, sm[k]), decode_m(cm[k] >> 24, sm[k])));
-      __stcs(out_v + at, make_float4(decode_v(cv[k] & 255u, sv[k]), decode_v(cv[k] >> 8 & 255u, sv[k]),
-                                     decode_v(cv[k] >> 16 & 255u, sv[k]), decode_v(cv[k] >> 24, sv[k])));
+      __stcs(out_m + at, make_float4(decode_m<0>(cm[k], sm[k]), decode_m<1>(cm[k], sm[k]), decode_m<2>(cm[k], sm[k]),
+                                     decode_m<3>(cm[k], sm[k])));
+      __stcs(out_v + at, make_float4(decode_v<0>(cv[k], sv[k]), decode_v<1>(cv[k], sv[k]), decode_v<2>(cv[k], sv[k]),
+                                     decode_v<3>(cv[k], sv[k])));
     }
   }
 }

@@ -27,16 +27,18 @@ constexpr int TILE = 128;
 __device__ __forceinline__ uint32_t magnitudes(uint32_t pair) { return pair & 0x7FFF7FFFu; }
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
 
-// The exponent, with its bias, of the scale for a largest magnitude given by its bf16 bits (7 of mantissa).
-__device__ __forceinline__ uint32_t scale_byte(uint32_t most) {
-  const int field = static_cast<int>(most >> 7);
-  if (field == 255) return 255u;
-  return static_cast<uint32_t>(max(0, field - 8 + ((most & 0x7Fu) > 0x60u ? 1 : 0)));
-}
+// For a largest magnitude given by its bf16 bits (7 of mantissa): 8 more than the exponent, with its bias, of the scale.  31 carries
+// into the exponent what is above 1.75.
+__device__ __forceinline__ uint32_t scale_of(uint32_t most) { return max((most + 31u) >> 7, 8u); }
+__device__ __forceinline__ uint32_t scale_byte(uint32_t most) { return most >= 0x7F80u ? 255u : scale_of(most) - 8u; }
+// 2^-e as a bf16 number, what elements are multiplied by.  e is 120 at most, and -127 at least, whose inverse is a normal number.
+__device__ __forceinline__ uint32_t inverse_scale(uint32_t most) { return (262u - scale_of(most)) << 7; }
 
-// 2^-e: what elements are multiplied by.  e is 120 at most, and -127 at least, whose inverse is a normal number.
-__device__ __forceinline__ float inverse_scale(uint32_t byte) {
-  return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23);
+// Two bf16 products by powers of two, exact but for what is far below the smallest code.
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // Four codes of fp32 values, the first in the lowest byte.
@@ -149,11 +151,12 @@ fp8_quantize_kernel(const __grid_constant__ Roundings both) {
     uint32_t own = 0;                            // of row l: rows behind the end have words too, of zeros' scale
 #pragma unroll
     for (int i = 0; i < 8; ++i, p += plain.ld) {
-      const uint32_t byte = scale_byte(i & 1 ? row_most[i / 2] >> 16 : row_most[i / 2] & 0xFFFFu);
-      const float inv = inverse_scale(byte);
-      if (l == i) own = byte;
-      const uint2 o = make_uint2(codes4(low_half(v[i].x) * inv, high_half(v[i].x) * inv, low_half(v[i].y) * inv, high_half(v[i].y) * inv),
-                                 codes4(low_half(v[i].z) * inv, high_half(v[i].z) * inv, low_half(v[i].w) * inv, high_half(v[i].w) * inv));
+      const uint32_t most = i & 1 ? row_most[i / 2] >> 16 : row_most[i / 2] & 0xFFFFu;
+      const uint32_t inv = inverse_scale(most) * 0x10001u;
+      if (l == i) own = scale_byte(most);
+      const uint32_t q[4] = {mul_bf16x2(v[i].x, inv), mul_bf16x2(v[i].y, inv), mul_bf16x2(v[i].z, inv), mul_bf16x2(v[i].w, inv)};
+      const uint2 o = make_uint2(codes4(low_half(q[0]), high_half(q[0]), low_half(q[1]), high_half(q[1])),
+                                 codes4(low_half(q[2]), high_half(q[2]), low_half(q[3]), high_half(q[3])));
       if (whole || (r0 + i < rows && c0 < cols)) *reinterpret_cast<uint2*>(p) = o;
     }
     if (l < 8) put_scale(plain, tile_x, tiles_x, r0 + l, static_cast<long long>(tiles_y) * TILE, own);
@@ -161,19 +164,20 @@ fp8_quantize_kernel(const __grid_constant__ Roundings both) {
   if (turned.codes != nullptr) {
     uint32_t own = 0;                            // of column 8 l + g
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t byte = scale_byte(j & 1 ? col_of[j / 2] >> 16 : col_of[j / 2] & 0xFFFFu);
-      const float inv = inverse_scale(byte);
-      float f[8];
+    for (int j = 0; j < 4; ++j) {                // two columns
+      const uint32_t even = col_of[j] & 0xFFFFu, odd = col_of[j] >> 16;
+      const uint32_t inv = inverse_scale(even) | inverse_scale(odd) << 16;
+      if (g == 2 * j) own = scale_byte(even);
+      if (g == 2 * j + 1) own = scale_byte(odd);
+      uint32_t q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t q = j < 2 ? v[i].x : j < 4 ? v[i].y : j < 6 ? v[i].z : v[i].w;
-        f[i] = (j & 1 ? high_half(q) : low_half(q)) * inv;
-      }
-      // word g of column 8 l + j, moved by l: the sixteen threads of a half warp meet sixteen pairs of banks
-      *reinterpret_cast<uint2*>(turn + (8 * l + j) * TILE + ((g ^ l) * 8)) =
-          make_uint2(codes4(f[0], f[1], f[2], f[3]), codes4(f[4], f[5], f[6], f[7]));
-      if (g == j) own = byte;
+      for (int i = 0; i < 8; ++i) q[i] = mul_bf16x2(j == 0 ? v[i].x : j == 1 ? v[i].y : j == 2 ? v[i].z : v[i].w, inv);
+      // word g of column 8 l + 2 j, moved by l: the sixteen threads of a half warp meet sixteen pairs of banks
+      uint8_t* const word = turn + (8 * l + 2 * j) * TILE + ((g ^ l) * 8);
+      *reinterpret_cast<uint2*>(word) = make_uint2(codes4(low_half(q[0]), low_half(q[1]), low_half(q[2]), low_half(q[3])),
+                                                   codes4(low_half(q[4]), low_half(q[5]), low_half(q[6]), low_half(q[7])));
+      *reinterpret_cast<uint2*>(word + TILE) = make_uint2(codes4(high_half(q[0]), high_half(q[1]), high_half(q[2]), high_half(q[3])),
+                                                          codes4(high_half(q[4]), high_half(q[5]), high_half(q[6]), high_half(q[7])));
     }
     if (g < 8) put_scale(turned, tile_y, tiles_y, c0 + g, static_cast<long long>(tiles_x) * TILE, own);
     __syncthreads();
