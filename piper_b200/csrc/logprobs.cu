@@ -624,7 +624,7 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
         unpack(u[j], f, T());
 #pragma unroll
         for (int q = 0; q < VEC<T>; ++q) f[q] = grad(f[q]);
-        __stcs(reinterpret_cast<uint4*>(o + body) + i + j * THREADS, pack(f, T()));
+        reinterpret_cast<uint4*>(o + body)[i + j * THREADS] = pack(f, T());
       }
     }
   } else {
