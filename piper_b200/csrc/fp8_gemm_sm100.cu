@@ -18,6 +18,8 @@
 // Tensor memory: two accumulators of 224 columns, then four slots of 16 columns for the scales of four blocks (4 for 128 rows of A,
 // up to 7 for B).  256 columns would leave no room for the scales beside a second accumulator.
 //
+// A stage holds one block of the contraction, or two.
+//
 // What bounds it: a block of 128 of a 256 x 224 tile of a pair takes 448 cycles of MMA and loads 30 KiB into each SM, 472 cycles at
 // the 65 bytes per cycle that an SM takes from L2.
 //
@@ -103,6 +105,8 @@ __device__ __forceinline__ uint32_t scaled_idesc(int m, int n, uint32_t byte) {
   return byte << 4 | static_cast<uint32_t>(n >> 3) << 17 | 1u << 23 | static_cast<uint32_t>(m >> 4) << 24 | byte << 29;
 }
 
+constexpr uint32_t NEXT_BYTE = 1u << 4 | 1u << 29;
+
 __device__ __forceinline__ void tmem_st_32x4(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
                ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
@@ -114,7 +118,7 @@ __device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)
                : "memory");
 }
 
-template <int CTAS, bool F32>
+template <int CTAS, bool F32, int BLOCKS>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                 const __grid_constant__ CUtensorMap tmap_c, const Params p) {
@@ -126,7 +130,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
   const int width = p.width;
   const int b_rows = width / CTAS;
-  const int stage_bytes = A_STAGE_BYTES + b_rows * BK;
+  const int block_bytes = A_STAGE_BYTES + b_rows * BK, stage_bytes = block_bytes * BLOCKS;
   const int stages = p.stages;
   const int tiles_m = (p.M + BM * CTAS - 1) / (BM * CTAS);
   const int tiles_n = (p.N + width - 1) / width;
@@ -209,13 +213,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       coords(tile, tm, tn);
       const int m0 = tm * (BM * CTAS) + static_cast<int>(rank) * BM;
       const int n0 = tn * width + static_cast<int>(rank) * b_rows;
-      for (int kb = 0; kb < k_blocks; ++kb) {
+      for (int kb = 0; kb < k_blocks; kb += BLOCKS) {
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[s], ph ^ 1, p.status)))) break;
         if (elect_one()) {
           uint8_t* sa = smem + s * stage_bytes;
-          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], CTAS * loaded);
-          tma_load_2d_n<CTAS>(sa, &tmap_a, &bars->full[s], kb * BK, m0);
-          tma_load_2d_n<CTAS>(sa + A_STAGE_BYTES, &tmap_b, &bars->full[s], kb * BK, n0);
+          const int have = min(BLOCKS, k_blocks - kb);
+          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], CTAS * loaded * have);
+#pragma unroll
+          for (int i = 0; i < BLOCKS; ++i, sa += block_bytes) {
+            if (i >= have) break;
+            tma_load_2d_n<CTAS>(sa, &tmap_a, &bars->full[s], (kb + i) * BK, m0);
+            tma_load_2d_n<CTAS>(sa + A_STAGE_BYTES, &tmap_b, &bars->full[s], (kb + i) * BK, n0);
+          }
         }
         __syncwarp();
         ++fills;
@@ -250,25 +259,30 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_empty[acc], ((n >> 1) & 1) ^ 1, p.status)))) break;
         tc_fence_after();
         const uint32_t tmem_d = tmem_base + acc * MAX_WIDTH;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        for (int kb = 0; kb < k_blocks; kb += BLOCKS) {
           const uint32_t slot = group % SLOTS;
           if ((kb & 3) == 0 &&
               !(ok = __all_sync(0xffffffffu, mbar_wait(&bars->scale_full[slot], (group / SLOTS) & 1, p.status)))) break;
           if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[s], ph, p.status)))) break;
           tc_fence_after();
-          const bool last = (kb & 3) == 3 || kb == k_blocks - 1;        // of its group
+          const int end = min(kb + BLOCKS, k_blocks);
+          const bool last = (end & 3) == 0 || end == k_blocks;          // of its group
           if (elect_one()) {
-            const uint64_t da = da0 + (static_cast<uint32_t>(s * stage_bytes) >> 4);
-            const uint64_t db = db0 + (static_cast<uint32_t>(s * stage_bytes) >> 4);
             const uint32_t scales = tmem_base + SLOT_COLUMN + slot * SLOT_COLUMNS;
+            const uint32_t at = static_cast<uint32_t>(s * stage_bytes) >> 4;
             const uint32_t idesc = scaled_idesc(BM * CTAS, width, static_cast<uint32_t>(kb & 3));
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k)
-              umma_scaled<CTAS>(tmem_d, da + k * (UMMA_K >> 4), db + k * (UMMA_K >> 4), idesc, scales, scales + 4,
-                                (kb > 0 || k > 0) ? 1u : 0u);
+            for (int i = 0; i < BLOCKS; ++i) {
+              if (kb + i >= k_blocks) break;
+              const uint32_t block = at + i * (static_cast<uint32_t>(block_bytes) >> 4);
+#pragma unroll
+              for (int k = 0; k < BK / UMMA_K; ++k)
+                umma_scaled<CTAS>(tmem_d, da0 + block + k * (UMMA_K >> 4), db0 + block + k * (UMMA_K >> 4),
+                                  idesc + i * NEXT_BYTE, scales, scales + 4, (kb > 0 || i > 0 || k > 0) ? 1u : 0u);
+            }
             umma_commit_n<CTAS>(&bars->empty[s]);
             if (last) umma_commit_n<CTAS>(&bars->scale_empty[slot]);
-            if (kb == k_blocks - 1) umma_commit_n<CTAS>(&bars->acc_full[acc]);
+            if (end == k_blocks) umma_commit_n<CTAS>(&bars->acc_full[acc]);
           }
           __syncwarp();
           if (last) ++group;
@@ -403,9 +417,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
   }
 }
 
-template <int CTAS, bool F32>
+template <int CTAS, bool F32, int BLOCKS>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Params& p, int num_sms, cudaStream_t stream) {
-  auto kern = fp8_gemm_kernel<CTAS, F32>;
+  auto kern = fp8_gemm_kernel<CTAS, F32, BLOCKS>;
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return -2;
@@ -430,22 +444,32 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
   return cudaLaunchKernelEx(&cfg, kern, ta, tb, tc, p) == cudaSuccess ? 0 : -3;
 }
 
+// Two k-blocks to a stage, and to a round of waiting and committing, where they leave room for four such stages (three for a
+// CTA by itself).  A block costs the issuing warp as long as a narrow tile's MMAs take: 24 x 4096 x 14336 in 64 tiles of 64 columns
+// 31.2 us by single blocks, 24.8 by two (453 and 344 cycles a block), by pairs 25.8 and 19.9; 1000 x 2048 x 8192 in pairs of 128
+// columns 18.2 and 15.8.
+bool two_blocks(int ctas, int width) { return ctas == 2 ? width <= 128 : width <= 96; }
+
 // Cycles of a launch by the model of the bf16 products (gemm_cost): an MMA of twice the elements per cycle on elements of half
-// the size leaves the cycles per block of 128 bytes as they are there.
+// the size leaves the cycles per block of 128 bytes as they are there.  What the issue of a block takes is fitted to 14 shapes in
+// all widths (M 16-4096, N 256-8192, K 256-14336), where the choice is 4 % behind the fastest on average; a pair, half of
+// whose rows would be empty, is not considered.
 double cost(int M, int N, int K, bool f32, int ctas, int width, int num_sms) {
   const double k_blocks = (K + BK - 1) / BK;
   const long long tiles = static_cast<long long>((M + BM * ctas - 1) / (BM * ctas)) * ((N + width - 1) / width);
   const long long units = num_sms / ctas;
   const double rounds = static_cast<double>((tiles + units - 1) / units);
-  const double block = std::max(2.0 * width, (std::min(M, BM) + width / ctas) * BK / 65.0);
+  const double fill = (std::min(M, BM) + width / ctas) * BK / 65.0;
+  const double issue = ctas == 2 ? 250 : two_blocks(1, width) ? 295 + 0.8 * width : 430 + 0.4 * width;
+  const double block = std::max({2.0 * width, fill, issue});
   const double epilogue = 2000 + (f32 ? 15 : 10) * width;
-  return rounds * std::max(k_blocks * block, epilogue) + epilogue + (ctas == 2 ? 2500 : 2000);
+  return rounds * std::max(k_blocks * block, epilogue) + epilogue + (ctas == 2 ? 3600 : 2000);
 }
 
 GemmShape shape_of(int M, int N, int K, bool f32, int num_sms) {
   GemmShape best = {1, MAX_WIDTH, 1};
   double least = 1e300;
-  for (int ctas = 1; ctas <= 2 && ctas <= num_sms; ++ctas)
+  for (int ctas = 1; ctas <= (M > BM ? 2 : 1) && ctas <= num_sms; ++ctas)
     for (int width = MAX_WIDTH; width >= 32; width -= 32) {
       const double c = cost(M, N, K, f32, ctas, width, num_sms);
       if (c < least) {
@@ -474,7 +498,8 @@ int fp8_gemm_launch(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   p.a_rows = shape.ctas == 1 && g.M < BM ? (g.M + 7) / 8 * 8 : BM;
   const int b_rows = shape.width / shape.ctas;
   const int stage = A_STAGE_BYTES + b_rows * BK;
-  p.stages = std::min(MAX_STAGES, OPERAND_BYTES / stage);
+  const bool two = two_blocks(shape.ctas, shape.width);
+  p.stages = std::min(MAX_STAGES, OPERAND_BYTES / (two ? 2 * stage : stage));
   const int tiles_m = (g.M + BM * shape.ctas - 1) / (BM * shape.ctas), tiles_n = (g.N + shape.width - 1) / shape.width;
   const bool n_fast = tiles_n < tiles_m;
   const long long fast_bytes = static_cast<long long>(n_fast ? g.N : g.M) * g.K;
@@ -488,8 +513,17 @@ int fp8_gemm_launch(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
     rc = g.add_f32 ? make_tmap_c_f32(&tc, g.c, g.N, g.M, static_cast<uint64_t>(g.ldc) * 4)
                    : make_tmap_c_bf16(&tc, g.c, g.N, g.M, static_cast<uint64_t>(g.ldc) * 2);
   if (rc != 0) return rc;
-  if (shape.ctas == 2) return g.add_f32 ? launch<2, true>(ta, tb, tc, p, num_sms, stream) : launch<2, false>(ta, tb, tc, p, num_sms, stream);
-  return g.add_f32 ? launch<1, true>(ta, tb, tc, p, num_sms, stream) : launch<1, false>(ta, tb, tc, p, num_sms, stream);
+  const int key = (shape.ctas == 2 ? 4 : 0) | (g.add_f32 ? 2 : 0) | (two ? 1 : 0);
+  switch (key) {
+    case 0: return launch<1, false, 1>(ta, tb, tc, p, num_sms, stream);
+    case 1: return launch<1, false, 2>(ta, tb, tc, p, num_sms, stream);
+    case 2: return launch<1, true, 1>(ta, tb, tc, p, num_sms, stream);
+    case 3: return launch<1, true, 2>(ta, tb, tc, p, num_sms, stream);
+    case 4: return launch<2, false, 1>(ta, tb, tc, p, num_sms, stream);
+    case 5: return launch<2, false, 2>(ta, tb, tc, p, num_sms, stream);
+    case 6: return launch<2, true, 1>(ta, tb, tc, p, num_sms, stream);
+    default: return launch<2, true, 2>(ta, tb, tc, p, num_sms, stream);
+  }
 }
 
 }  // namespace piper
