@@ -92,14 +92,10 @@ struct Sums {
 };
 
 // The quick pass takes logits for at least CLAMP, so that nothing is infinite; a row whose maximum is not well inside
-// (-BIG, BIG), whose alternatives reach down there, or whose temperature is far from 1, is read by the exact pass.
+// (-BIG, BIG), or whose alternatives reach down there, is read again by the exact pass.
 constexpr float CLAMP = -1.0002555517425873e30f;      // a bf16 number, 0xF14A
 constexpr uint32_t CLAMP_PAIR = 0xF14AF14Au;
 constexpr float BIG = 1e28f;
-// Its exponents are relative to a base that stays behind the thread's maximum by up to so many powers of two: sums stay
-// finite, and the common case has no branch and no rescaling.
-constexpr float STALE = 30.f;
-
 // ------------------------------------------------------------------ the largest of many keys
 // Value and index of an element as one integer that grows with the value and, among equal values, with a falling index, so no two
 // elements of a row have the same key and the order of ties is the order of ids.  0 is below every key.  A NaN counts as
@@ -251,16 +247,18 @@ struct Vec<float> {
   }
 };
 
-// Sums of the quick pass: exponents are x c2 - base, one rounded operation.
+// Sums of the quick pass: exponents are x c2 - base, one rounded operation, with the base of the largest element so far, `top`.  A
+// base that stays behind it by up to 2^30, which would leave out most of the raising, costs a peaked row's entropy its last digits: terms
+// of t then have both signs (error 2e-6 against 2e-7).
 struct QuickSums {
-  float base, limit, s, t;               // base, limit: in powers of two
+  float base, top, s, t;
 
   __device__ __forceinline__ void raise(float x, float c2) {
     const float to = x * c2, d = max_nan(base - to, FAR_BELOW), f = ex2(d);
     t = f * fmaf(s, d, t);
     s *= f;
     base = to;
-    limit = x + STALE / c2;
+    top = x;
   }
   __device__ __forceinline__ void add(float x, float c2) {
     const float a = fmaf(x, c2, -base), w = ex2(a);
@@ -299,7 +297,7 @@ struct Pass {
       const float x = max_nan(f, CLAMP);
       if (x > m || !place.any) place = {at, at, true};
       m = fmaxf(m, x);
-      if (x > v.limit) v.raise(x, c2);
+      if (x > v.top) v.raise(x, c2);
       v.add(x, c2);
     };
     singles(sp.head, head, single);
@@ -321,7 +319,7 @@ struct Pass {
         place.any = true;
       }
       m = fmaxf(m, lm);
-      if (__builtin_expect(lm > v.limit, 0)) v.raise(lm, c2);
+      if (lm > v.top) v.raise(lm, c2);
       float f[VEC<T>];
       first.elements(f);
 #pragma unroll
@@ -343,7 +341,7 @@ struct Pass {
         place.any = true;
       }
       m = fmaxf(m, lm);
-      if (lm > v.limit) v.raise(lm, c2);
+      if (lm > v.top) v.raise(lm, c2);
       float f[VEC<T>];
       x.elements(f);
 #pragma unroll
@@ -413,7 +411,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   Sums v;
   uint64_t bound = 0;
   Place place = {0, 0, false};
-  for (int exact = c2 > 1e-6f && c2 < 1e6f ? 0 : 1; exact < 2; ++exact) {
+  for (int exact = 0; exact < 2; ++exact) {
     v = exact ? pass.exact(place) : pass.template quick<TOP>(place);
     const float wm = warp_max(v.m);
     if (lane == 0) sh.m[warp] = wm;
@@ -603,7 +601,7 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   const float c2 = inv_t * LOG2E;
   const float a = empty ? 0.f : -(g + gh * h) * inv_t, b = empty ? 0.f : -gh * LN2 * inv_t, minus = empty ? 0.f : -log_s;
   auto grad = [&](float f) {
-    const float u = fmaf(max_nan(f - from, FAR_BELOW), c2, minus);
+    const float u = max_nan(fmaf(f - from, c2, minus), -200.f);       // 2^-200 is 0 here, and so is 0 (a - 200 b)
     return ex2(u) * fmaf(b, u, a);
   };
   const long long begin = sp.first, end = begin + sp.head + static_cast<long long>(sp.vecs) * VEC<T> + sp.tail;

@@ -141,8 +141,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top: int = 0, temperature:
     V = logits.shape[-1]
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"token_logprobs: top must be 0 to {min(MAX_TOP, V)}, got {top}")
-    if not (temperature > 0 and math.isfinite(temperature) and 1e-30 < temperature < 1e30):
-        raise ValueError(f"token_logprobs: temperature must be a positive number, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"token_logprobs: temperature must be 1e-6 to 1e6, got {temperature}")
     lg = logits if logits.dim() == 2 else logits.reshape(-1, V)
     lead = tokens.shape
     logprob, entropy, top_logprob, top_id, _ = token_logprobs_fwd(lg, tokens.reshape(-1), top, float(temperature), ignore_index)

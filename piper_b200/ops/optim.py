@@ -62,7 +62,8 @@ def _encode(x: Tensor, r: Tensor, signed: bool) -> tuple[Tensor, Tensor]:
 
 
 class AdamWState:
-    """Moments, master copies and step counts of a list of parameters (bf16 or fp32, contiguous, on one device).
+    """Moments, master copies and step counts of a list of parameters (bf16 or fp32, contiguous, on one device, no two of which
+    share memory).
 
     Everything is flat: parameter ``i`` owns the elements ``[offsets[i], offsets[i] + numel)`` of ``m`` and ``v`` (fp32, or
     uint8 codes with the scales ``m_scale`` and ``v_scale`` of their blocks of 256) and, where a parameter is bf16, of the
@@ -195,7 +196,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], stat
             for i, (p, g) in enumerate(zip(params, grads)):
                 if g is not None and p.numel():
                     _step_ref(state, i, p, g, state.steps[i] + 1, lr, b1, b2, eps, weight_decay, grad_scale)
-        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None and not p.is_inference()])
     state.steps = [s + (g is not None) for s, g in zip(state.steps, grads)]
 
 

@@ -146,6 +146,30 @@ def test_special_gradients(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("eps", [0.0, 1e-35, 1.0])
+def test_eps_of_any_size(eps, device):
+    p, state = [torch.ones(300, device=device)], None
+    g = torch.full((300,), 1e-20, device=device)          # a square below the normal numbers
+    g[100:200], g[200:] = 1.0, -1e10
+    state = ops.AdamWState(p, bits=32)
+    ops.adamw_step(p, [g], state, lr=0.1, eps=eps, weight_decay=0.0)
+    w, _m, v, _size, upd = _formula(torch.ones(300).double(), torch.zeros(300).double(), torch.zeros(300).double(), g, 1, 0.1, (0.9, 0.999), eps, 0.0)
+    # v of the first hundred is 1e-43, 71 of the smallest numbers: a 142nd of itself, half that in its root
+    tol = torch.full((300,), 40 * EPS)
+    tol[:100] = 1 / 142 + 1 / 70 if eps < 1.0 else 40 * EPS
+    assert bool(((p[0].double().cpu() - w).abs() <= 0.1 * upd.abs() * tol + 2 * EPS).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_inference_tensors(device):
+    with torch.inference_mode():
+        p = [torch.ones(300, device=device)]
+        state = ops.AdamWState(p, bits=8)
+        ops.adamw_step(p, [torch.ones(300, device=device)], state, lr=0.1)
+        assert bool((p[0] < 1).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("bits", [8, 32])
 def test_missing_gradients_and_views(bits, device):
     base = torch.randn(4096 + 3, generator=torch.Generator().manual_seed(1)).to(device)

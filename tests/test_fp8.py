@@ -274,3 +274,49 @@ def test_same_bits_on_streams_and_in_a_captured_graph():
     after = step()
     assert all(torch.equal(a, b) for r in kept for a, b in zip(after, r))
     ops.native.check_status()
+
+
+def test_traced_programs_record_one_op():
+    x, w = _matrix(6, 64, "cpu", 1, dtype=torch.float32).requires_grad_(True), _matrix(32, 64, "cpu", 2, dtype=torch.float32)
+    (want,) = torch.autograd.grad(ops.fp8_linear(x, w).sum(), x)
+    for backend in ("eager", "aot_eager"):
+        f = torch.compile(lambda a: ops.fp8_linear(a, w).sum(), backend=backend, fullgraph=True)
+        assert torch.allclose(torch.autograd.grad(f(x), x)[0], want)
+    torch.library.opcheck(torch.ops.piper.fp8_linear.default, (x, w))
+    with torch.no_grad():
+        kept = ops.fp8_quantize(w, square=True)
+        torch.library.opcheck(torch.ops.piper.fp8_linear_kept.default, (x.detach(), kept.data, 32))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_checkpointed_layers_recompute_what_they_keep(device):
+    from torch.utils.checkpoint import checkpoint
+    x, w = _matrix(40, 64, device, 1).requires_grad_(True), _matrix(32, 64, device, 2, std=0.1).requires_grad_(True)
+    dy = _matrix(40, 32, device, 3)
+    want = torch.autograd.grad(ops.fp8_linear(x, w), [x, w], dy)
+    for reentrant in (False, True):
+        y = checkpoint(lambda a, b: ops.fp8_linear(a, b), x, w, use_reentrant=reentrant)
+        if reentrant:                     # this form wants backward()
+            x.grad = w.grad = None
+            y.backward(dy)
+            got = (x.grad, w.grad)
+        else:
+            got = torch.autograd.grad(y, [x, w], dy)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_one_weight_in_two_calls_of_a_pass_and_two_buckets():
+    """The same weight twice: both gradients in its bucket; and calls on two streams at once with buckets of their own."""
+    w = _matrix(96, 256, "cuda", 2, std=0.1).requires_grad_(True)
+    a, b = (_matrix(n, 256, "cuda", n).requires_grad_(True) for n in (130, 70))
+    da, db = _matrix(130, 96, "cuda", 5), _matrix(70, 96, "cuda", 6)
+    sink = torch.zeros(96, 256, device="cuda")
+    ops.grad_sinks.register(w, sink)
+    try:
+        torch.autograd.grad([ops.fp8_linear(a, w), ops.fp8_linear(b, w)], [a, b, w], [da, db], allow_unused=True)
+    finally:
+        ops.grad_sinks.unregister(w)
+    parts = [_rounded(d.t()) @ _rounded(x.t()).t() for d, x in ((da, a), (db, b))]
+    size = sum(_rounded(d.t()).abs() @ _rounded(x.t()).t().abs() for d, x in ((da, a), (db, b)))
+    assert bool(((sink.double().cpu() - sum(parts)).abs() <= 10 * 2.0 ** -22 * size).all())

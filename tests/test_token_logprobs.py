@@ -153,6 +153,41 @@ def test_largest_values_in_one_threads_elements(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_peaked_rows_keep_their_last_digits(dtype, device):
+    """Nearly all of the probability in one token, far above what a thread has seen before it: log S is close to 0, so an absolute
+    error of a few steps of 1 is what S itself has, and every other term keeps its own relative one."""
+    V = 32003
+    x, tokens = _logits(6, V, dtype, device, 12, std=1.0)
+    for i, (at, height) in enumerate([(0, 12.0), (V - 1, 15.0), (20000, 18.0), (4097, 24.0), (31000, 30.0), (9, 60.0)]):
+        x[i, at] = height
+        tokens[i] = at
+    for temperature in (0.7, 1.0):
+        out = ops.token_logprobs(x, tokens, top=2, temperature=temperature)
+        _logp, _p, H, _on, lp, _ids, _left = _definition(x, tokens, 2, temperature)
+        depth = (V if device == "cpu" else V / 512 + 20) + 40
+        for got, want in ((out.entropy, H), (out.logprob, lp)):
+            err = (got.double().cpu() - want).abs()
+            assert bool((err <= 2.0 ** -24 * (8 + depth * want.abs())).all()), (err, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_extreme_temperatures(device):
+    x, tokens = _logits(5, 3000, torch.float32, device, 3)
+    x[2, 100:] = -INF
+    x.requires_grad_(True)
+    for temperature in (1e-6, 1e-3, 1e3, 1e6):
+        out = ops.token_logprobs(x, tokens, top=3, temperature=temperature)
+        gradients = [torch.ones(5), torch.ones(5), torch.ones(5, 3)]
+        (d,) = torch.autograd.grad([out.logprob, out.entropy, out.top_logprob], x, [g.to(device) for g in gradients])
+        logp, _p, H, on, lp, ids, _left = _definition(x, tokens, 3, temperature)
+        # the temperature's inverse and log2(e) are rounded: a log probability is off by so many steps of itself
+        err = (out.logprob.double().cpu() - lp).abs()
+        assert bool(((err <= 2.0 ** -24 * (3100 + 8 * lp.abs())) | (out.logprob.double().cpu() == lp)).all())
+        assert torch.equal(out.top_id.cpu(), ids) and bool(torch.isfinite(d).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_strides_offsets_and_shapes(device):
     base = torch.randn(6, 1003, generator=torch.Generator().manual_seed(2)).to(device)
     for dtype in (torch.bfloat16, torch.float32):
@@ -220,7 +255,7 @@ def test_agrees_with_cross_entropy():
 def test_refusals():
     x, tokens = _logits(4, 50, torch.float32, "cpu", 1)
     for bad in (dict(top=-1), dict(top=33), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")),
-                dict(temperature=INF)):
+                dict(temperature=INF), dict(temperature=1e-7), dict(temperature=1e7)):
         with pytest.raises(ValueError):
             ops.token_logprobs(x, tokens, **bad)
     with pytest.raises(ValueError):
@@ -278,3 +313,19 @@ def test_same_bits_on_streams_and_in_a_captured_graph():
         torch.cuda.synchronize()
         replayed = [t.clone() for t in kept]
         assert all(torch.equal(a, b) for a, b in zip(replayed, step()))
+
+
+def test_traced_programs_record_one_op():
+    x, tokens = _logits(4, 60, torch.float32, "cpu", 2)
+    x.requires_grad_(True)
+
+    def f(v):
+        r = ops.token_logprobs(v, tokens, top=2)
+        return (r.logprob + 0.1 * r.entropy).sum() + r.top_logprob.sum()
+
+    (want,) = torch.autograd.grad(f(x), x)
+    for backend in ("eager", "aot_eager"):
+        compiled = torch.compile(f, backend=backend, fullgraph=True)
+        (d,) = torch.autograd.grad(compiled(x), x)
+        assert torch.allclose(d, want)
+    torch.library.opcheck(torch.ops.piper.token_logprobs_fwd.default, (x, tokens, 2, 1.0, -100))
