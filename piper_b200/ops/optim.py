@@ -79,7 +79,6 @@ class AdamWState:
         self.bits, self.device = bits, params[0].device
         self.shapes = [tuple(p.shape) for p in params]
         self.dtypes = [p.dtype for p in params]
-        self.sizes = [2 * p.numel() + (p.dtype == torch.bfloat16) for p in params]
         self.offsets, at = [], 0
         for p in params:
             if p.dtype not in (torch.bfloat16, torch.float32):
@@ -93,7 +92,9 @@ class AdamWState:
         if len({p.data_ptr() for p in params if p.numel()}) < sum(p.numel() > 0 for p in params):
             raise ValueError("AdamWState: a parameter is listed twice")
         self.numel = at
-        self.steps = [0] * len(params)
+        # what the library reads and counts on: offsets, twice the elements and one for bf16, steps
+        self._table = torch.tensor([self.offsets, [2 * p.numel() + (p.dtype == torch.bfloat16) for p in params],
+                                    [0] * len(params)], dtype=torch.int64)
         moment = dict(dtype=torch.uint8 if bits == 8 else torch.float32, device=self.device)
         self.m, self.v = torch.zeros(at, **moment), torch.zeros(at, **moment)
         self.m_scale = self.v_scale = self.master = None
@@ -110,9 +111,14 @@ class AdamWState:
                 if p.dtype == torch.bfloat16:
                     self.master[o:o + p.numel()].copy_(p.detach().reshape(-1))
 
+    @property
+    def steps(self) -> list:
+        """The number of steps taken so far, of each parameter."""
+        return self._table[2].tolist()
+
     def set_step(self, step: int) -> None:
         """The number of steps taken so far, of all parameters."""
-        self.steps = [int(step)] * len(self.shapes)
+        self._table[2] = int(step)
 
     def moments(self) -> tuple[Tensor, Tensor]:
         """Both moments in fp32, flat as ``m`` and ``v`` are (those themselves if they have 32 bits)."""
@@ -160,7 +166,7 @@ class AdamWState:
                 self.set_moments(m, v)
             if self.master is not None:
                 self.master.copy_(state["master"])
-        self.steps = [int(s) for s in state["steps"]]
+        self._table[2] = torch.tensor([int(s) for s in state["steps"]], dtype=torch.int64)
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], state: AdamWState, *, lr: float = 1e-3,
@@ -181,23 +187,23 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], stat
         if params and params[0].device != state.device:
             raise ValueError(f"adamw_step: the state is on {state.device}, a parameter on {params[0].device}")
         # the library checks every tensor before it launches anything
-        native.lib().adamw.default(params, grads, state.m, state.v, state.m_scale, state.v_scale, state.master, state.offsets,
-                                   state.sizes, state.steps, lr, b1, b2, eps, weight_decay, grad_scale)
+        native.lib().adamw.default(params, grads, state.m, state.v, state.m_scale, state.v_scale, state.master, state._table,
+                                   lr, b1, b2, eps, weight_decay, grad_scale)
     else:
         if len(params) != len(state.shapes) or len(grads) != len(params):
             raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients, a state of {len(state.shapes)}")
-        for p, g, size in zip(params, grads, state.sizes):
+        for p, g, size in zip(params, grads, state._table[1].tolist()):
             if 2 * p.numel() + (p.dtype == torch.bfloat16) != size or p.device != state.device:
                 raise ValueError(f"adamw_step: the state is of a parameter of {size // 2} elements on {state.device}, got "
                                  f"{p.dtype} {tuple(p.shape)} on {p.device}")
             if g is not None and (g.shape != p.shape or g.device != p.device):
                 raise ValueError(f"adamw_step: a gradient is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)}")
         with torch.no_grad():
-            for i, (p, g) in enumerate(zip(params, grads)):
+            for i, (p, g, done) in enumerate(zip(params, grads, state.steps)):
                 if g is not None and p.numel():
-                    _step_ref(state, i, p, g, state.steps[i] + 1, lr, b1, b2, eps, weight_decay, grad_scale)
+                    _step_ref(state, i, p, g, done + 1, lr, b1, b2, eps, weight_decay, grad_scale)
         torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None and not p.is_inference()])
-    state.steps = [s + (g is not None) for s, g in zip(state.steps, grads)]
+        state._table[2] += torch.tensor([g is not None for g in grads], dtype=torch.int64)
 
 
 def _step_ref(state: AdamWState, i: int, p: Tensor, grad: Tensor, step: int, lr: float, b1: float, b2: float, eps: float,
