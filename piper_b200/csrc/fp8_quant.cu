@@ -81,11 +81,11 @@ fp8_quantize_kernel(const __grid_constant__ Roundings both) {
     const __nv_bfloat16* p = x + r0 * ldx + c0;
     if (whole) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i, p += ldx) v[i] = __ldcs(reinterpret_cast<const uint4*>(p));
+      for (int i = 0; i < 8; ++i, p += ldx) v[i] = *reinterpret_cast<const uint4*>(p);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i, p += ldx)
-        v[i] = c0 < cols && r0 + i < rows ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+        v[i] = c0 < cols && r0 + i < rows ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
     }
   }
 

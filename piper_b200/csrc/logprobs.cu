@@ -388,7 +388,8 @@ struct Pass {
 // the alternatives, the threads' largest keys (taken for as small as their places allow) are reduced to 64, the largest of a lane
 // number's in every other warp; the top-th largest of those is a bound that at least so many elements reach.  The elements that reach it
 // belong to the few threads whose largest does, and only those threads' elements, a small part of the row each, are looked at
-// again, by all threads; what they find is sorted.  20 alternatives of 1024 x 128256: FIGURE
+// again, by all threads; what they find is sorted.  1024 rows of 128256: 55.7 us without alternatives, 65.4 with 5, 72.3 with 20 (floor
+// 40): a CTA that looks for them reads nothing meanwhile, and an SM has two.
 template <class T, bool TOP>
 __global__ void __launch_bounds__(THREADS, TOP ? 2 : 3)
 logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
@@ -463,15 +464,26 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
         if (at < THREADS) found[at] = key;
       }
     };
-    const int owners = sh.num_owners, rounds = (sp.vecs + THREADS - 1) / THREADS;
-    for (int e = threadIdx.x; e < owners * rounds; e += THREADS) {
-      const int owner = sh.owners[e / rounds], i = owner + e % rounds * THREADS;
-      if (i >= sp.vecs) continue;
-      float f[VEC<T>];
-      unpack(reinterpret_cast<const uint4*>(body)[i], f, T());
-      const uint32_t at = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(i) * VEC<T>;
+    // A warp takes two owners at a time, their vectors lane by lane, both loads in front of the first comparison.
+    const int owners = sh.num_owners;
+    for (int o = warp; o < owners; o += 2 * WARPS) {
+      const int one = sh.owners[o], two = o + WARPS < owners ? sh.owners[o + WARPS] : sp.vecs;
+      for (int k = lane * THREADS; k < sp.vecs; k += 32 * THREADS) {
+        const int at[2] = {one + k, two + k};
+        uint4 u[2];
 #pragma unroll
-      for (int q = 0; q < VEC<T>; ++q) offer(f[q], at + q);
+        for (int h = 0; h < 2; ++h)
+          if (at[h] < sp.vecs) u[h] = reinterpret_cast<const uint4*>(body)[at[h]];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (at[h] >= sp.vecs) continue;
+          float f[VEC<T>];
+          unpack(u[h], f, T());
+          const uint32_t first = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(at[h]) * VEC<T>;
+#pragma unroll
+          for (int q = 0; q < VEC<T>; ++q) offer(f[q], first + q);
+        }
+      }
     }
     for (int e = threadIdx.x; e < owners; e += THREADS) {
       const int owner = sh.owners[e];
@@ -642,7 +654,9 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   from_float(fmaf(sum, inv_t, grad(to_float(x[at]))), o[at]);
 }
 
-// CTAs per row: with fewer rows than SMs have room for, a row is cut into up to eight pieces of at least 4,096 elements.
+// CTAs per row: with fewer rows than SMs have room for, a row is cut into up to eight pieces of at least 4,096 elements.  Not with
+// more rows, where a cluster waits for SMs together: 444 rows of 128256 with 5 alternatives 32.7 us, in two pieces each, which would fill
+// the SMs better, 43.4; 1024 rows without 55.7 and 64.6.
 int row_parts(long long T, int V, int num_sms) {
   int parts = 1;
   while (parts < MAX_PARTS && T * parts * 2 <= 2ll * num_sms && V / (parts * 2) >= 4096) parts *= 2;
