@@ -83,6 +83,10 @@ __device__ __forceinline__ float block_scale(const float (&x)[PER]) {
   return bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(bits);
 }
 
+// The rare operations, out of the way of the common ones in the instruction cache.
+__device__ __noinline__ float divide(float a, float b) { return __fdiv_rn(a, b); }
+__device__ __noinline__ float exact_update(float m, float v, float root, float eps) { return m / fmaf(sqrtf(v), root, eps); }
+
 // y = |x| / scale of a block, correctly rounded.  With the correctly rounded reciprocal, a product, its exact remainder and a
 // correction give the quotient (Markstein, IBM J. Res. Dev. 34, 1990) where nothing underflows: a quotient that is not small enough for
 // code 0 or 1 anyway comes from x above 2^-101, whose remainder is a normal number, if the scale is above 2^-60.  Other blocks
@@ -98,14 +102,14 @@ __device__ __forceinline__ void quotients(const float* x, float scale, float (&y
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = __fdiv_rn(fabsf(x[j]), s);
+    for (int j = 0; j < 4; ++j) y[j] = divide(fabsf(x[j]), s);
   }
 }
 
 // m / (sqrt(v) root + eps), within two units of the last place for the root and for the quotient; numbers below the normal ones
 // count as 0, so a vanishing eps, beside which they would matter, takes the exact operations.
 __device__ __forceinline__ float update(float m, float v, float root, float eps) {
-  if (eps < 1e-30f) return m / fmaf(sqrtf(v), root, eps);
+  if (eps < 1e-30f) return exact_update(m, v, root, eps);
   float r, q;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(fmaf(r, root, eps)));
@@ -125,11 +129,11 @@ __device__ __forceinline__ void store4(float* p, const float (&x)[PER], int h) {
 
 // A warp takes a block: lane l has elements 4 l to 4 l + 3 of either half, so that its vectors are neighbours of the next lane's.
 // The CTAs that are resident walk the chunks together, a block per warp at a time: 64 Mi elements with 8-bit moments and bf16
-// parameters 221 us (floor 184), with 16 blocks per chunk 249 us, with twice the CTAs 267; 32-bit moments and bf16
-// gradients 311 us (287).  Without the arithmetic the same accesses take 212 us.  Blocks fetched two ahead through shared
+// parameters 222 us (floor 184), with 16 blocks per chunk 249 us, with twice the CTAs 267; 32-bit moments and bf16
+// gradients 294 us (287), with three CTAs per SM 330 us.  Without the 8-bit arithmetic the same accesses take 212 us.  Blocks fetched two ahead through shared
 // memory bring nothing (268 us in either form, with chunks of 16).
 template <int BITS>
-constexpr int CTAS = BITS == 8 ? 4 : 3;
+constexpr int CTAS = BITS == 8 ? 4 : 2;
 template <int BITS>
 __global__ void __launch_bounds__(THREADS, CTAS<BITS>)
 adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
