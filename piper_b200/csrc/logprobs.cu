@@ -388,10 +388,13 @@ struct Pass {
 // the alternatives, the threads' largest keys (taken for as small as their places allow) are reduced to 64, the largest of a lane
 // number's in every other warp; the top-th largest of those is a bound that at least so many elements reach.  The elements that reach it
 // belong to the few threads whose largest does, and only those threads' elements, a small part of the row each, are looked at
-// again, by all threads; what they find is sorted.  1024 rows of 128256: 55.7 us without alternatives, 65.4 with 5, 72.3 with 20 (floor
-// 40): a CTA that looks for them reads nothing meanwhile, and an SM has two.
-template <class T, bool TOP>
-__global__ void __launch_bounds__(THREADS, TOP ? 2 : 3)
+// again, by all threads; what they find is sorted.  1024 rows of 128256: 55.7 us without alternatives, 58.4 with 5, 67.2 with 20 (floor
+// 40): a CTA that looks for them reads nothing meanwhile.
+// CTAS of them share an SM, with the registers that leaves: three where there are rows for them, so that others read while one
+// looks for its alternatives (2048 x 128256 with 20: 136 us by two, 123 by three); two, each of them faster, where there are not (296 rows
+// 22 and 28 us).  Without alternatives three are as fast with few rows.
+template <class T, bool TOP, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
 logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
                     float* __restrict__ entropy, float* __restrict__ top_logprob, long long* __restrict__ top_id,
                     float* __restrict__ stats, int V, long long ld, long long ignore_index, int top, int parts, float inv_t) {
@@ -685,7 +688,9 @@ template <class T>
 int fwd(const LogprobArgs& a, float* logprob, float* entropy, float* top_logprob, long long* top_id, float* stats, int num_sms,
         cudaStream_t st) {
   const int parts = row_parts(a.T, a.V, num_sms);
-  auto kernel = a.top > 0 ? logprobs_fwd_kernel<T, true> : logprobs_fwd_kernel<T, false>;
+  auto kernel = a.top == 0                    ? logprobs_fwd_kernel<T, false, 3>
+                : a.T * parts > 2ll * num_sms ? logprobs_fwd_kernel<T, true, 3>
+                                              : logprobs_fwd_kernel<T, true, 2>;
   return launch_clusters(kernel, a.T * parts, parts, st, static_cast<const T*>(a.logits), a.tokens, logprob, entropy, top_logprob,
                          top_id, stats, a.V, a.ld, a.ignore_index, a.top, parts, a.inv_temperature);
 }
