@@ -7,7 +7,9 @@ is then exact, and an operand is rounded once.  Sums are kept in fp32 (``csrc/fp
 
 ``fp8_linear`` is ``linear`` with all three products of a training step in 8 bits: the gradient of the input contracts
 over the weights' rows, the gradient of the weights over the tokens, for which input and output gradient are rounded in
-groups of 128 tokens.  Its backward pass keeps the 8-bit operands, not the bf16 input.  A group with a NaN or an infinity is NaN.
+groups of 128 tokens.  Between the passes it keeps the input as that 8-bit operand, half the bytes of the bf16 input, and of the
+weight nothing but the weight, which is rounded again: every microbatch in flight would have a copy of its own, and a sharded
+parameter would stay gathered.  A group with a NaN or an infinity is NaN.
 """
 from __future__ import annotations
 
@@ -168,27 +170,26 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix) -> Tensor:
 
 # ------------------------------------------------------------------ linear layer
 @custom_op("piper::fp8_linear_keep")
-def fp8_linear_keep(x: Tensor, w: Tensor, keep_x: bool, keep_w: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """y [T, N] = x [T, K] w [N, K]^T, and the transposed operands that the backward pass wants: x^T [K, T] for the gradient of
-    w (keep_x), w^T [K, N] for the gradient of x (keep_w)."""
+def fp8_linear_keep(x: Tensor, w: Tensor) -> tuple[Tensor, Tensor]:
+    """y [T, N] = x [T, K] w [N, K]^T, and x^T [K, T] as the operand that the gradient of w wants."""
     (T, K), N = x.shape, w.shape[0]
-    xp, xt = _quantize(x, False, True, keep_x)
-    wp, wt = _quantize(w, True, True, keep_w)
-    return _product(xp, wp, T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device)), xt, wt
+    xp, xt = _quantize(x, False, True, True)
+    return _product(xp, _quantize(w, True, True, False)[0], T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device)), xt
 
 
 @fp8_linear_keep.register_fake
-def _(x, w, keep_x, keep_w):
+def _(x, w):
     T, (N, K) = x.shape[0], w.shape
-    return (x.new_empty((T, N)), x.new_empty((_bytes(K, T) if keep_x else 0,), dtype=torch.uint8),
-            x.new_empty((_bytes(K, N) if keep_w else 0,), dtype=torch.uint8))
+    return x.new_empty((T, N)), x.new_empty((_bytes(K, T),), dtype=torch.uint8)
 
 
 @custom_op("piper::fp8_linear")
 def fp8_linear_op(x: Tensor, w: Tensor) -> Tensor:
-    """y [T, N] = x [T, K] w [N, K]^T.  Which operands the backward pass needs is decided where it is known, when the op runs, and
+    """y [T, N] = x [T, K] w [N, K]^T.  Whether the backward pass needs x is decided where it is known, when the op runs, and
     not by the caller, whose program may be traced without gradients."""
-    return fp8_linear_keep(x, w, False, False)[0]
+    (T, K), N = x.shape, w.shape[0]
+    xp, wp = _quantize(x, False, True, False)[0], _quantize(w, True, True, False)[0]
+    return _product(xp, wp, T, N, K, torch.empty(T, N, dtype=x.dtype, device=x.device))
 
 
 @fp8_linear_op.register_fake
@@ -197,9 +198,9 @@ def _(x, w):
 
 
 def _linear_forward(ctx, x, w):
-    y, xt, wt = fp8_linear_keep(x, w, w.requires_grad, x.requires_grad)
+    y, xt = fp8_linear_keep(x, w) if w.requires_grad else (fp8_linear_op(x, w), None)
     ctx.rows = x.shape[0]
-    ctx.save_for_backward(w, xt, wt)
+    ctx.save_for_backward(w, xt)
     return y
 
 
@@ -219,12 +220,13 @@ def _fp8_wgrad(dyt: Tensor, xt: Tensor, w: Tensor, T: int):
 
 
 def _linear_backward(ctx, dy):
-    w, xt, wt = ctx.saved_tensors
+    w, xt = ctx.saved_tensors
     need_x, need_w = ctx.needs_input_grad[:2]
     T, (N, K) = ctx.rows, w.shape
     dyp, dyt = _quantize(dy, False, need_x, need_w)
     dx = dw = None
     if need_x:
+        wt = _quantize(w, True, False, True)[1]
         dx = _product(dyp, wt, T, K, N, torch.empty((T, K), dtype=dy.dtype, device=dy.device))
     if need_w:
         if wgrad_store.active is not None:
@@ -237,8 +239,8 @@ def _linear_backward(ctx, dy):
 fp8_linear_op.register_autograd(_linear_backward, forward=_linear_forward)
 
 
-def _linear_backward_host(dy: Tensor, w: Tensor, xt: Tensor, wt: Tensor, T: int, need_x: bool, need_w: bool) -> tuple[Tensor, Tensor]:
-    ctx = HostContext((w, xt, wt), (need_x, need_w))
+def _linear_backward_host(dy: Tensor, w: Tensor, xt: Tensor, T: int, need_x: bool, need_w: bool) -> tuple[Tensor, Tensor]:
+    ctx = HostContext((w, xt), (need_x, need_w))
     ctx.rows = T
     dx, dw = _linear_backward(ctx, dy)
     none = torch.empty(0)
