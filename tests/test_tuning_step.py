@@ -129,3 +129,70 @@ def test_eight_bit_models_of_both_families():
     torch.nn.init.normal_(x.weight)
     a = torch.randn(3, 32)
     assert torch.equal(x(a), ops.fp8_linear(a, x.weight))
+
+
+def _pipeline_worker(rank, world, schedule, stages, checkpointing):
+    import dataclasses
+
+    from piper_b200 import piper_exec_dag, piper_setup
+    from piper_b200.models.llama3 import LLAMA_CONFIGS, Transformer
+
+    cfg = dataclasses.replace(LLAMA_CONFIGS["tiny"], fp8=True)
+    x, y = _tokens(cfg)
+    actor = piper_setup(Transformer, (cfg, 64, stages), optim_fn=torch.optim.AdamW, optim_kwargs={"state_bits": 8, "lr": 1e-3},
+                        example_inputs=[x], example_outputs=y, model_dtype=torch.float32,
+                        const_attrs=Transformer.const_attrs(cfg, 64), schedule_directives=schedule, device="cpu",
+                        activation_checkpointing=checkpointing)
+    actor.debug_keep_grads = True
+    losses = [float(v) for v in piper_exec_dag(_loss)]
+    grads = dict(actor.last_grads)
+    again = [float(v) for v in piper_exec_dag(_loss)]
+    return {"losses": losses, "again": again, "grads": grads}
+
+
+def _tokens(cfg):
+    g = torch.Generator().manual_seed(3)
+    tok = torch.randint(0, cfg.vocab_size, (4, 65), generator=g)
+    return tok[:, :-1].contiguous(), tok[:, 1:].contiguous()
+
+
+@pytest.mark.parametrize("kind,checkpointing", [("zerobubble", False), ("zerobubble", True), ("1f1b", False)])
+def test_pipelines_of_two_ranks(kind, checkpointing, tmp_path):
+    """The split backward pass defers the 8-bit weight gradients, recomputation keeps operands of its own; both sides round each
+    microbatch by itself.  One sum in another order would take an element over a border between two codes, a sixteenth of it, and
+    the next layer's rounding then more of them, up to the roundings' own size after a few layers: no small tolerance follows.  So
+    the plain run adds in the ranks' order (one thread, the same stages); the loss's quarter is a power of two, which the scales
+    pass on exactly, and gradients are the same but for the order in which four microbatches are added: 3 roundings, 2^-24 each,
+    of sums that do not cancel to less than a hundredth of their terms' norm."""
+    import dataclasses
+
+    from piper_b200.compiler.builders import build_1f1b_schedule, build_zerobubble_schedule
+    from piper_b200.models.llama3 import LLAMA_CONFIGS, Transformer
+    from piper_b200.runtime.storage import materialize_module
+    from tests.dist_utils import run_ranks
+
+    order = build_zerobubble_schedule(2, 4) if kind == "zerobubble" else build_1f1b_schedule(2, 4)
+    schedule = [{"op": "place", "filter": {"PP": i}, "devices": [i], "stream": "pp_stream"} for i in range(2)] + \
+        [{"op": "split", "filter": {}, "dim_name": "MB", "num_microbatches": 4}] + list(order)
+    results = run_ranks(2, _pipeline_worker, (schedule, 2, checkpointing), tmp_path)
+    cfg = dataclasses.replace(LLAMA_CONFIGS["tiny"], fp8=True)
+    model = Transformer(cfg, 64, 2)
+    model.load_const_attrs()
+    materialize_module(model)
+    x, y = _tokens(cfg)
+    want = []
+    threads = torch.get_num_threads()
+    torch.set_num_threads(1)
+    try:
+        for a, b in zip(x.split(1), y.split(1)):
+            loss = _loss(model(a), b)
+            (loss / 4).backward()
+            want.append(float(loss.detach()))
+    finally:
+        torch.set_num_threads(threads)
+    losses = [v for r in results for v in r["losses"]]
+    assert len(losses) == 4 and all(abs(a - b) < 1e-6 * abs(b) for a, b in zip(losses, want)), (losses, want)
+    grads = {k: v for r in results for k, v in r["grads"].items()}
+    for n, p in model.named_parameters():
+        assert float((grads[n] - p.grad).norm()) <= 2e-5 * float(p.grad.norm()), n
+    assert sum(v for r in results for v in r["again"]) != sum(losses)          # the step was taken
