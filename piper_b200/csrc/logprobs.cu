@@ -609,14 +609,27 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   const float gy = counted && d_logprob != nullptr ? d_logprob[row] : 0.f;
   const float gh = d_entropy != nullptr ? d_entropy[row] : 0.f;
   float g = gy;
+  bool live = gy != 0.f || gh != 0.f;
   if (d_top != nullptr)
-    for (int i = 0; i < top; ++i) g += d_top[row * top + i];
-  const bool empty = log_s == -INFINITY;
-  // dx = 2^u (a + b u) with u = log2 p; a row with nothing left has a = b = 0 and any finite log_s
+    for (int i = 0; i < top; ++i) {
+      g += d_top[row * top + i];
+      live = live || d_top[row * top + i] != 0.f;
+    }
+  if (!live || log_s == -INFINITY) {
+    // nothing asks for this row (padding, whatever its logits are), or nothing is left in it: its logits are not read
+    const Span out = Span::of(o, V, part, parts);
+    T* const first = o + out.first;
+    const int t = threadIdx.x;
+    if (t < out.head) from_float(0.f, first[t]);
+    if (t < out.tail) from_float(0.f, first[out.head + static_cast<long long>(out.vecs) * VEC<T> + t]);
+    for (int i = t; i < out.vecs; i += THREADS) reinterpret_cast<uint4*>(first + out.head)[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  // dx = 2^u (a + b u) with u = log2 p
   const float c2 = inv_t * LOG2E;
-  const float a = empty ? 0.f : -(g + gh * h) * inv_t, b = empty ? 0.f : -gh * LN2 * inv_t, minus = empty ? 0.f : -log_s;
+  const float a = -(g + gh * h) * inv_t, b = -gh * LN2 * inv_t;
   auto grad = [&](float f) {
-    const float u = max_nan(fmaf(f - from, c2, minus), -200.f);       // 2^-200 is 0 here, and so is 0 (a - 200 b)
+    const float u = max_nan(fmaf(f - from, c2, -log_s), -200.f);      // 2^-200 is 0 here, and so is 0 (a - 200 b)
     return ex2(u) * fmaf(b, u, a);
   };
   const long long begin = sp.first, end = begin + sp.head + static_cast<long long>(sp.vecs) * VEC<T> + sp.tail;
@@ -647,7 +660,7 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   // the token may be one of the alternatives: whoever writes a place has all that belongs to it
   const int who = static_cast<int>(threadIdx.x);
   const int listed = d_top != nullptr ? top : 0;
-  if (who > listed || (who == listed && !counted) || empty) return;
+  if (who > listed || (who == listed && !counted)) return;
   auto id = [&](int i) { return i < listed ? top_id[row * top + i] : y; };
   const long long at = id(who);
   if (at < begin || at >= end) return;

@@ -104,13 +104,21 @@ def _backward(ctx, d_logprob, d_entropy, d_top, _d_id, _d_stats):
     up = torch.zeros_like(p)                         # gradient with respect to log p
     if d_logprob is not None:
         on = _counted(tokens, V, ignore_index)
-        up.scatter_add_(1, tokens.clamp(0, V - 1).unsqueeze(1), (d_logprob.to(p.dtype) * on).unsqueeze(1))
+        up.scatter_add_(1, tokens.clamp(0, V - 1).unsqueeze(1), torch.where(on, d_logprob, 0).to(p.dtype).unsqueeze(1))
     if d_top is not None:
         up.scatter_add_(1, top_id, d_top.to(p.dtype))
     d = up - p * up.sum(1, keepdim=True)
     if d_entropy is not None:
         d = d - d_entropy.to(p.dtype).unsqueeze(1) * torch.where(p == 0, torch.zeros_like(p), p * (logp + h.unsqueeze(1)))
-    d = torch.where(torch.isinf(log_s).unsqueeze(1), torch.zeros_like(d), d / temperature)
+    # nothing asks for a row (padding, whatever its logits are), or nothing is left in it
+    live = torch.zeros(T, dtype=torch.bool)
+    if d_logprob is not None:
+        live |= (d_logprob != 0) & on
+    if d_entropy is not None:
+        live |= d_entropy != 0
+    if d_top is not None:
+        live |= (d_top != 0).any(1)
+    d = torch.where((live & ~torch.isinf(log_s)).unsqueeze(1), d / temperature, torch.zeros_like(d))
     return d.to(logits.dtype), None, None, None, None
 
 
@@ -127,7 +135,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top: int = 0, temperature:
     differentiable with respect to the logits (the ids are taken as given).  A token that is ``ignore_index`` or no id
     of the vocabulary has log probability 0 and no gradient through it.  Masked ids (-inf) have probability 0; a row that
     has nothing else has entropy 0, log probabilities of -inf and no gradient.  A row with a NaN or +inf is NaN; its ids
-    are some of the vocabulary's.
+    are some of the vocabulary's.  A row whose outputs get no gradient but zeros gives none, whatever its logits are.
     """
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits have no vocabulary: {tuple(logits.shape)}")

@@ -140,6 +140,40 @@ def test_rows_without_numbers_are_nan(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,offset", [(6, 9, 0), (6, 10007, 1), (600, 1031, 3)])
+def test_rows_that_nothing_asks_for_have_no_gradient(T, V, offset, dtype, device):
+    """Padding, whatever its logits are (0 x NaN is NaN in the formula): by an ignored token, by gradients of zero; and what the
+    gradient's memory held shows nowhere, other rows are as without padding."""
+    g = torch.Generator().manual_seed(5)
+    x = (torch.randn(T, V, generator=g) * 3).to(dtype)
+    tokens = torch.randint(0, V, (T,), generator=g)
+    tokens[1::3] = -100
+    tokens[2::3] = V + 7
+    dlp, dH, dtop = torch.randn(T, generator=g), torch.randn(T, generator=g), torch.randn(T, 3, generator=g)
+    padded = torch.arange(T) % 3 != 0
+    dlp[padded] = float("nan")             # behind a token that does not count
+    dH[padded] = 0
+    dtop[padded] = 0
+    bad = x.clone()
+    bad[1::3, V // 2] = float("nan")
+    bad[2::3, :] = INF
+    grads = []
+    for values in (x, bad):
+        room = torch.zeros(T, V + 8, dtype=dtype, device=device)
+        leaf = room[:, offset:offset + V]
+        leaf.copy_(values)
+        leaf.requires_grad_(True)
+        r = ops.token_logprobs(leaf, tokens.to(device), top=3)
+        dirty = torch.full((T, V), float("nan"), dtype=dtype, device=device)
+        del dirty
+        (d,) = torch.autograd.grad((r.logprob, r.entropy, r.top_logprob), leaf, (dlp.to(device), dH.to(device), dtop.to(device)))
+        grads.append(d.cpu())
+    assert all(bool((d[padded] == 0).all()) for d in grads)
+    assert bool((grads[0][~padded] == grads[1][~padded]).all()) and bool((grads[0][~padded] != 0).any())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_largest_values_in_one_threads_elements(device):
     """The alternatives all at one place of the pattern in which threads take vectors, and in an order that keeps replacing them."""
     V = 65536
