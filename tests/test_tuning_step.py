@@ -113,6 +113,31 @@ def test_policy_gradient_loss(device):
     assert float(policy_gradient_loss(logits, none, entropy_coef=0.5)) == 0.0
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_gradient_loss_of_padding(device):
+    """What stands at places that do not count changes nothing: neither logits nor advantages, for either kind of such tokens."""
+    from piper_b200.nn import policy_gradient_loss
+    g = torch.Generator().manual_seed(2)
+    clean = torch.randn(3, 6, 72, generator=g)
+    tokens = torch.randint(0, 72, (3, 6), generator=g)
+    adv = torch.randn(3, 6, generator=g)
+    tokens[0, 4:] = -100
+    tokens[2, 3:] = 72
+    pad = (tokens < 0) | (tokens >= 72)
+    dirty = clean.clone()
+    dirty[pad] = float("nan")
+    results = []
+    for logits, a in ((clean, adv), (dirty, torch.where(pad, float("nan"), adv))):
+        x = logits.to(device).requires_grad_(True)
+        loss = policy_gradient_loss(x, tokens.to(device), a.to(device), entropy_coef=0.3)
+        results.append((loss.detach().cpu(), torch.autograd.grad(loss, x)[0].cpu()))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    only = clean[~pad].double()
+    logp = torch.log_softmax(only, -1)
+    want = -(adv[~pad] * logp.gather(-1, tokens[~pad].unsqueeze(-1)).squeeze(-1) - 0.3 * (logp.exp() * logp).sum(-1)).mean()
+    assert abs(float(results[0][0]) - float(want)) < 2.0 ** -20 * 20
+
+
 def test_eight_bit_models_of_both_families():
     import dataclasses
 
