@@ -720,7 +720,7 @@ int bwd(const LogprobArgs& a, const float* stats, const float* entropy, const lo
 }
 
 bool sound(const LogprobArgs& a) {
-  return a.T >= 0 && a.T <= (1ll << 27) && a.V > 0 && a.top >= 0 && a.top <= kMaxTopTokens && a.top <= a.V;
+  return a.T >= 0 && a.T <= (1ll << 27) && a.V > 0 && a.V <= kMaxVocabulary && a.top >= 0 && a.top <= kMaxTopTokens && a.top <= a.V;
 }
 
 }  // namespace

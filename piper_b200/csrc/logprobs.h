@@ -6,6 +6,7 @@
 namespace piper {
 
 constexpr int kMaxTopTokens = 32;
+constexpr int kMaxVocabulary = 1 << 30;     // places in a row, and what is added to them, stay in 32 bits
 
 // Logits [T, V] in bf16 or fp32 (f32 != 0), rows ld elements apart, any alignment of the type; z = logits / temperature.
 struct LogprobArgs {

@@ -16,6 +16,7 @@ from . import native
 from .registry import custom_op
 
 MAX_TOP = 32
+MAX_VOCAB = 1 << 30
 
 
 class TokenLogprobs(NamedTuple):
@@ -139,6 +140,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top: int = 0, temperature:
     """
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits have no vocabulary: {tuple(logits.shape)}")
+    if logits.shape[-1] > MAX_VOCAB:
+        raise ValueError(f"token_logprobs: at most {MAX_VOCAB} ids, got {logits.shape[-1]}")
     if not logits.is_floating_point():
         raise TypeError(f"token_logprobs: logits must be floating point, got {logits.dtype}")
     if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1]:

@@ -304,6 +304,12 @@ def test_refusals():
         ops.token_logprobs(x.long(), tokens)
 
 
+def test_a_vocabulary_that_is_too_large_is_refused():
+    x = torch.zeros(1, 1, dtype=torch.bfloat16).expand(2, (1 << 30) + 1)        # no memory behind it
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x, torch.zeros(2, dtype=torch.int64))
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_device():
     x, tokens = _logits(4, 50, torch.float32, "cuda", 1)
