@@ -1,4 +1,5 @@
-// Host-side launchers of adamw.cu.  They enqueue on `st`, allocate nothing, and return 0 on success and -3 for a launch error.
+// Host-side launchers of adamw.cu.  They enqueue on `st`, allocate nothing, and return 0 on success, -1 for
+// more elements than a launch has chunks for and -3 for a launch error.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -36,7 +37,7 @@ struct AdamwArgs {
   float grad_scale;
 };
 
-// table.first, in chunks of adamw_chunk() elements, is filled in here.
+// table.first is filled in here.
 int adamw_launch(AdamwTable& table, const AdamwArgs& a, int num_sms, cudaStream_t st);
 
 // fp32 values of n codes of either moment (a multiple of kMomentBlock) with their scales.

@@ -61,13 +61,20 @@ def _encode(x: Tensor, r: Tensor, signed: bool) -> tuple[Tensor, Tensor]:
     return (codes & 255).to(torch.uint8), scale
 
 
+def _check_apart(params: Sequence[Tensor], what: str) -> None:
+    at = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+    if any(a[1] > b[0] for a, b in zip(at, at[1:])):
+        raise ValueError(f"{what}: two parameters share memory, or one is listed twice")
+
+
 class AdamWState:
     """Moments, master copies and step counts of a list of parameters (bf16 or fp32, contiguous, on one device, no two of which
     share memory).
 
     Everything is flat: parameter ``i`` owns the elements ``[offsets[i], offsets[i] + numel)`` of ``m`` and ``v`` (fp32, or
     uint8 codes with the scales ``m_scale`` and ``v_scale`` of their blocks of 256) and, where a parameter is bf16, of the
-    fp32 ``master``, from which its update starts.  Tensors begin at whole blocks; what is between them stays zero.
+    fp32 ``master``, from which its update starts.  Tensors begin at whole blocks; what is between them stays zero.  With 8 bits, a
+    moment that is infinite or NaN makes its block NaN.
     """
 
     def __init__(self, params: Sequence[Tensor], *, bits: int = 32) -> None:
@@ -89,8 +96,7 @@ class AdamWState:
                 raise ValueError("AdamWState: parameters must be contiguous")
             self.offsets.append(at)
             at += (p.numel() + BLOCK - 1) // BLOCK * BLOCK
-        if len({p.data_ptr() for p in params if p.numel()}) < sum(p.numel() > 0 for p in params):
-            raise ValueError("AdamWState: a parameter is listed twice")
+        _check_apart(params, "AdamWState")
         self.numel = at
         # what the library reads and counts on: offsets, twice the elements and one for bf16, steps
         self._table = torch.tensor([self.offsets, [2 * p.numel() + (p.dtype == torch.bfloat16) for p in params],
@@ -118,6 +124,8 @@ class AdamWState:
 
     def set_step(self, step: int) -> None:
         """The number of steps taken so far, of all parameters."""
+        if step < 0:
+            raise ValueError(f"AdamWState: steps are counted from 0, got {step}")
         self._table[2] = int(step)
 
     def moments(self) -> tuple[Tensor, Tensor]:
@@ -196,8 +204,11 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], stat
             if 2 * p.numel() + (p.dtype == torch.bfloat16) != size or p.device != state.device:
                 raise ValueError(f"adamw_step: the state is of a parameter of {size // 2} elements on {state.device}, got "
                                  f"{p.dtype} {tuple(p.shape)} on {p.device}")
+            if not p.is_contiguous():
+                raise ValueError("adamw_step: parameters must be contiguous")
             if g is not None and (g.shape != p.shape or g.device != p.device):
                 raise ValueError(f"adamw_step: a gradient is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)}")
+        _check_apart(params, "adamw_step")
         with torch.no_grad():
             for i, (p, g, done) in enumerate(zip(params, grads, state.steps)):
                 if g is not None and p.numel():

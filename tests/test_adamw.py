@@ -261,6 +261,31 @@ def test_refusals(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bits", [8, 32])
+def test_parameters_that_share_memory_are_refused(bits, device):
+    """Two of them would be stepped by one launch in no order; neighbours, and parameters without elements, are none of those."""
+    room = torch.zeros(600, device=device)
+    with pytest.raises(ValueError):
+        ops.AdamWState([room[:300], room[299:]], bits=bits)
+    with pytest.raises(ValueError):
+        ops.AdamWState([room, room[5:9]], bits=bits)
+    apart = [room[300:], room[:300], room[10:10]]
+    state = ops.AdamWState(apart, bits=bits)
+    g = [torch.ones_like(t) for t in apart]
+    with pytest.raises(ValueError):
+        ops.adamw_step([room[300:], room[1:301], room[10:10]], g, state)
+    with pytest.raises(ValueError):
+        ops.adamw_step([room[:300], room[:300], room[10:10]], g, state)
+    with pytest.raises(ValueError):
+        ops.adamw_step([torch.zeros(300, 2, device=device)[:, 0], room[:300], room[10:10]], g, state)
+    assert state.steps == [0, 0, 0] and not room.any()
+    ops.adamw_step(apart, g, state)
+    assert state.steps == [1, 1, 1] and bool((room != 0).all())
+    with pytest.raises(ValueError):
+        state.set_step(-1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_a_saved_tensor_that_was_stepped_is_noticed(device):
     w = torch.ones(8, device=device, requires_grad=True)
     state = ops.AdamWState([w])
