@@ -11,7 +11,7 @@
 // Roles by warp:
 //   warp 0       TMA producer: a ring of shared-memory stages of 128 x 128-byte operand boxes in 128-byte swizzle; hands out tiles.
 //   warp 1       MMA issuer (first CTA of a pair, for both), into one of two accumulators.
-//   warp 2       tensor memory allocation; warp 3 draws the first tile.
+//   warp 2       tensor memory allocation.
 //   warps 4-11   epilogue: accumulator to bf16 or fp32, through shared memory, TMA store or reduce-add.
 //   warps 12-15  scales: words of four blocks from global memory into tensor memory, one warp for each quarter of its lanes, which
 //                all hold the same: row r of A in lane r % 32 of column r / 32, rows of B likewise behind them.
@@ -27,7 +27,9 @@
 #include "fp8.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstddef>
+#include <cstdlib>
 
 #include "gemm_sm100.h"
 #include "ptx.cuh"
@@ -63,7 +65,6 @@ struct Bars {
   uint64_t tile_full[RING];
   int tile[RING][4];
   uint32_t tmem_base;
-  int first;
 };
 static_assert(sizeof(Bars) <= 768 && offsetof(Bars, tile) % 16 == 0 && SMEM_BYTES <= 232448, "shared memory");
 
@@ -77,8 +78,13 @@ struct Params {
   int stages;
   int band;
   int* status;
-  int* sched;
+  int slot;           // counter of the launch, or -1: tiles in a fixed order
 };
+
+// Counters of tiles, one per launch in rotation; the launch 4,096 before, whose last draw rearms the counter, has to have ended on its
+// stream by then.  They are the module's own, so every device has its zeros without an allocation.
+constexpr unsigned SCHED_SLOTS = 4096;
+__device__ int sched_slots[SCHED_SLOTS];
 
 // D[tmem] (+)= (A * scales) * (B * scales), e4m3 inputs.
 template <int CTAS>
@@ -161,12 +167,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     tmem_alloc_n<CTAS>(&bars->tmem_base, 512);
     tmem_relinquish_n<CTAS>();
   }
-  // As in the bf16 products: tiles come from a counter, but in launches of one round.
+  // The first tile is the unit's own, later ones come from a counter, drawn while the last stage of the tile before is waited for: 4096 x
+  // 4096 x 28672 354-377 us, 351-388 in a fixed order; 1000 x 8192 x 2048 21 and 23, with all tiles drawn when they are needed 25.
   const int units = static_cast<int>(gridDim.x) / CTAS;
-  const bool draws = p.sched != nullptr && num_tiles > units;
+  const bool draws = p.slot >= 0 && num_tiles > units;
+  int* const counter = sched_slots + (draws ? p.slot : 0);
   grid_wait();
-  if (warp == 3 && rank == 0 && lane == 0)
-    bars->first = draws ? atomicAdd(&p.sched[0], 1) : static_cast<int>(blockIdx.x) / CTAS;
   tc_fence_before();
   if (CTAS == 2) cluster_sync(); else __syncthreads();
   tc_fence_after();
@@ -193,17 +199,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     uint32_t n = 0;
     int s = 0;
     uint32_t ph = 0, fills = 0;
+    int drawn = static_cast<int>(blockIdx.x) / CTAS;       // the next tile (lane 0 of the first CTA)
     bool ok = true;
     for (;; ++n) {
-      if (rank == 0 && elect_one()) {
-        int next = n > 0 && draws ? atomicAdd(&p.sched[0], 1) : bars->first + static_cast<int>(n) * units;
-        if (next >= num_tiles) next = -1;
+      if (rank == 0 && lane == 0) {
+        const int next = drawn < num_tiles ? drawn : -1;
         bars->tile[n % RING][0] = next;
         if (CTAS == 2)
           st_async_v4(mapa_u32(smem_u32(&bars->tile[n % RING]), 1), mapa_u32(smem_u32(&bars->tile_full[n % RING]), 1),
                       next, 0, 0, 0);
         mbar_arrive(&bars->tile_full[n % RING]);
-      } else if (rank == 1 && elect_one()) {
+      } else if (rank == 1 && lane == 0) {
         mbar_arrive_expect_tx(&bars->tile_full[n % RING], 16);
       }
       __syncwarp();
@@ -214,6 +220,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       const int m0 = tm * (BM * CTAS) + static_cast<int>(rank) * BM;
       const int n0 = tn * width + static_cast<int>(rank) * b_rows;
       for (int kb = 0; kb < k_blocks; kb += BLOCKS) {
+        // the draw is on its way while the last stage of the tile is waited for
+        if (rank == 0 && lane == 0 && kb + BLOCKS >= k_blocks) drawn = draws ? units + atomicAdd(counter, 1) : drawn + units;
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[s], ph ^ 1, p.status)))) break;
         if (elect_one()) {
           uint8_t* sa = smem + s * stage_bytes;
@@ -233,6 +241,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
       if (!ok) break;
     }
     grid_launch();
+    if (draws && rank == 0 && lane == 0) {
+      // Every unit draws until there is nothing left, so there are as many draws as tiles and the last one can rearm the counter.
+      while (drawn < num_tiles) drawn = units + atomicAdd(counter, 1);        // after a wait that ran out
+      if (drawn == units + num_tiles - 1) *counter = 0;
+    }
+    __syncwarp();
     if (ok) {
       for (int i = 0; i < stages && ok; ++i) {   // every stage handed back: no commit is on its way to these barriers
         ok = mbar_wait(&bars->empty[s], ph ^ 1, p.status);
@@ -408,22 +422,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     tc_fence_after();
     tmem_dealloc_n<CTAS>(tmem_base, 512);
   }
-  if (p.sched != nullptr && threadIdx.x == 0) {
-    if (atomicAdd(&p.sched[1], 1) == static_cast<int>(gridDim.x) - 1) {   // last CTA rearms the scheduler slot
-      p.sched[0] = 0;
-      p.sched[1] = 0;
-      __threadfence();
-    }
-  }
 }
 
 template <int CTAS, bool F32, int BLOCKS>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Params& p, int num_sms, cudaStream_t stream) {
   auto kern = fp8_gemm_kernel<CTAS, F32, BLOCKS>;
-  static bool configured = false;
-  if (!configured) {
+  static std::atomic<uint64_t> configured{0};    // a bit for every device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return -2;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if ((configured.load(std::memory_order_relaxed) & bit) == 0) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return -2;
-    configured = true;
+    configured.fetch_or(bit, std::memory_order_relaxed);
   }
   const int tiles = ((p.M + BM * CTAS - 1) / (BM * CTAS)) * ((p.N + p.width - 1) / p.width);
   const int units = num_sms / CTAS;
@@ -466,6 +476,19 @@ double cost(int M, int N, int K, bool f32, int ctas, int width, int num_sms) {
   return rounds * std::max(k_blocks * block, epilogue) + epilogue + (ctas == 2 ? 3600 : 2000);
 }
 
+// A counter for a launch on `stream`.  None while it is captured: the graph would keep it, and count in it beside another graph's or a
+// later launch's CTAs when it is replayed.
+int sched_slot(cudaStream_t stream) {
+  static const bool fixed = [] {
+    const char* env = getenv("PIPER_GEMM_STATIC_TILES");
+    return env != nullptr && env[0] == '1';
+  }();
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (fixed || cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) return -1;
+  static std::atomic<unsigned> launches{0};
+  return static_cast<int>(launches++ % SCHED_SLOTS);
+}
+
 GemmShape shape_of(int M, int N, int K, bool f32, int num_sms) {
   GemmShape best = {1, MAX_WIDTH, 1};
   double least = 1e300;
@@ -505,7 +528,7 @@ int fp8_gemm_launch(const Fp8GemmArgs& g, int num_sms, cudaStream_t stream) {
   const long long fast_bytes = static_cast<long long>(n_fast ? g.N : g.M) * g.K;
   p.band = fast_bytes > (96ll << 20) ? 8 : (n_fast ? tiles_n : tiles_m);
   p.status = g.status;
-  p.sched = gemm_sched_slot();
+  p.slot = sched_slot(stream);
   CUtensorMap ta, tb, tc;
   int rc = make_tmap_2d_u8(&ta, g.a.codes, g.K, g.M, g.a.ld, BK, p.a_rows);
   if (rc == 0) rc = make_tmap_2d_u8(&tb, g.b.codes, g.K, g.N, g.b.ld, BK, b_rows);

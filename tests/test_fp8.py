@@ -243,6 +243,43 @@ def test_refusals(device):
 
 
 @pytest.mark.gpu
+def test_captured_products_share_no_counters():
+    """Graphs captured 4,096 launches apart, the number of places in which launches count their tiles, and an eager launch on a third
+    stream, all in flight at once: several rounds of tiles each, every one of them written."""
+    g = torch.Generator().manual_seed(7)
+    a, b = (ops.fp8_quantize(torch.randn(n, 128, generator=g).bfloat16().cuda()) for n in (4096, 4096))
+    want = ops.fp8_matmul(a, b)
+    lib, status = ops.native.lib(), ops.native.status_tensor(want.device)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    graphs, outs = [], [torch.empty_like(want) for _ in range(3)]
+    small = ops.fp8_quantize(torch.ones(16, 16, dtype=torch.bfloat16, device="cuda"))
+    few = torch.empty(16, 16, dtype=torch.bfloat16, device="cuda")
+    for out in outs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            for _ in range(3):
+                lib.fp8_gemm(a.data, b.data, out, 128, status)
+        graphs.append(graph)
+        for _ in range(4093):
+            lib.fp8_gemm(small.data, small.data, few, 16, status)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for out in outs:
+            out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            for _ in range(3):
+                lib.fp8_gemm(a.data, b.data, outs[2], 128, status)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out in outs)
+    ops.native.check_status()
+
+
+@pytest.mark.gpu
 def test_same_bits_on_streams_and_in_a_captured_graph():
     x = _matrix(700, 1024, "cuda", 1).requires_grad_(True)
     w = _matrix(1376, 1024, "cuda", 2, std=0.03).requires_grad_(True)
