@@ -274,6 +274,8 @@ def fp8_linear(x: Tensor, w: Union[Tensor, Fp8Matrix]) -> Tensor:
     multiples of 16; there may be any number of rows.
     """
     kept = isinstance(w, Fp8Matrix)
+    if x.is_cuda and x.dim() == 2 and not kept:
+        return fp8_linear_op(x, w)                   # makes the checks below by itself
     N, K = w.shape
     _check_type(x, "fp8_linear")
     if x.dim() < 1 or x.shape[-1] != K or K == 0 or N == 0 or K % 16 or N % 16:

@@ -138,6 +138,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top: int = 0, temperature:
     has nothing else has entropy 0, log probabilities of -inf and no gradient.  A row with a NaN or +inf is NaN; its ids
     are some of the vocabulary's.  A row whose outputs get no gradient but zeros gives none, whatever its logits are.
     """
+    if logits.is_cuda and logits.dim() == 2:         # the op makes the checks below by itself
+        return TokenLogprobs(*token_logprobs_fwd(logits, tokens, top, temperature, ignore_index)[:4])
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"token_logprobs: logits have no vocabulary: {tuple(logits.shape)}")
     if logits.shape[-1] > MAX_VOCAB:

@@ -243,6 +243,25 @@ def test_refusals(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lead", [(6,), (2, 3)])
+def test_the_same_refusals_by_the_library(lead):
+    x, w = (torch.ones(*n, dtype=torch.bfloat16, device="cuda") for n in ((*lead, 64), (32, 64)))
+    for a, b in ((x[..., :48], w), (x[..., :40], w[:, :40]), (x, w[:24]), (x, w[:0]), (x[..., :0], w[:, :0]), (x, w.cpu()), (x.cpu(), w)):
+        with pytest.raises(ValueError):
+            ops.fp8_linear(a, b)
+        with pytest.raises(ValueError):
+            ops.fp8_linear(a, b.clone().requires_grad_(True))
+    for a, b in ((x.float(), w), (x, w.float()), (x.half(), w.half()), (x, w.half())):
+        with pytest.raises(TypeError):
+            ops.fp8_linear(a, b)
+    kept = ops.fp8_quantize(w, square=True)
+    for a in (x[..., :48], x.cpu(), x.clone().requires_grad_(True)):
+        with pytest.raises(ValueError):
+            ops.fp8_linear(a, kept)
+    assert ops.fp8_linear(x, kept).shape == (*lead, 32) and ops.fp8_linear(x[:0], w).shape == (0, *lead[1:], 32)
+
+
+@pytest.mark.gpu
 def test_captured_products_share_no_counters():
     """Graphs captured 4,096 launches apart, the number of places in which launches count their tiles, and an eager launch on a third
     stream, all in flight at once: several rounds of tiles each, every one of them written."""

@@ -322,6 +322,25 @@ def test_refusals_on_the_device():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lead", [(4,), (2, 2)])
+def test_the_same_refusals_by_the_library(lead):
+    x, tokens = _logits(4, 50, torch.float32, "cuda", 1)
+    x, tokens = x.detach().view(*lead, 50), tokens.view(lead)
+    for bad in (dict(top=-1), dict(top=33), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")),
+                dict(temperature=INF), dict(temperature=1e-7), dict(temperature=1e7)):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(x, tokens, **bad)
+    for a, b, top in ((x[..., :5], tokens, 6), (x, tokens[:1], 0), (x, tokens.int(), 0), (x, tokens.unsqueeze(0), 0), (x[..., :0], tokens, 0),
+                      (x, tokens.cpu(), 0), (x[:1, ..., :1].expand(*lead, (1 << 30) + 1), tokens, 0)):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(a, b, top=top)
+    for a in (x.long(), x.half(), x.double()):
+        with pytest.raises(TypeError):
+            ops.token_logprobs(a, tokens)
+    assert ops.token_logprobs(x, tokens, temperature=1).logprob.shape == lead
+
+
+@pytest.mark.gpu
 def test_same_bits_on_streams_and_in_a_captured_graph():
     for T, V in ((1, 128256), (70, 32003)):
         x, tokens = _logits(T, V, torch.bfloat16, "cuda", 6)
