@@ -165,7 +165,7 @@ struct Shared {
   uint64_t part_lists[MAX_PARTS][32];
   uint64_t halves[2][32];
   uint64_t bound;
-  int owners[THREADS];
+  int owners[THREADS], groups[THREADS];
   int num_owners, num_found;
 };
 
@@ -271,6 +271,8 @@ struct QuickSums {
 struct Place {
   uint32_t first, last;
   bool any;              // the thread has elements
+  int group;             // in the vectors group + j THREADS, j < AHEAD, ...
+  float second;          // ... and nothing else of the thread is above this; -1: it may be anywhere
 };
 
 // A thread's sums over its elements of a span, and (TOP) where its largest is.
@@ -293,9 +295,11 @@ struct Pass {
   __device__ __forceinline__ Sums quick(Place& place) const {
     QuickSums v = {0.5f * CLAMP * c2, CLAMP, 0.f, 0.f};      // far above what is clamped, far below the first raise
     float m = -INFINITY;
+    float second = -INFINITY;              // what is above it is there too
     auto single = [&](float f, uint32_t at) {
       const float x = max_nan(f, CLAMP);
-      if (x > m || !place.any) place = {at, at, true};
+      if (x > m || !place.any) place = {at, at, true, -1, 0.f};
+      second = fmaxf(second, fminf(x, m));
       m = fmaxf(m, x);
       if (x > v.top) v.raise(x, c2);
       v.add(x, c2);
@@ -318,6 +322,7 @@ struct Pass {
         span = (AHEAD - 1) * THREADS;
         place.any = true;
       }
+      if (TOP) second = fmaxf(second, fminf(lm, m));
       m = fmaxf(m, lm);
       if (lm > v.top) v.raise(lm, c2);
       float f[VEC<T>];
@@ -340,6 +345,7 @@ struct Pass {
         span = 0;
         place.any = true;
       }
+      if (TOP) second = fmaxf(second, fminf(lm, m));
       m = fmaxf(m, lm);
       if (lm > v.top) v.raise(lm, c2);
       float f[VEC<T>];
@@ -351,7 +357,9 @@ struct Pass {
       place.first = static_cast<uint32_t>(body - row) + static_cast<uint32_t>(best) * VEC<T>;
       place.last = place.first + static_cast<uint32_t>(span + 1) * VEC<T> - 1;
     }
+    place.group = best;
     singles(sp.tail, tail, single);
+    place.second = second;
     if (!(m > CLAMP)) return Sums::none();
     Sums r = {m, m, v.s, v.t};
     r.shift(max_nan(fmaf(-r.from, c2, v.base), FAR_BELOW));
@@ -363,7 +371,7 @@ struct Pass {
     Sums v = Sums::none();
     place.any = false;
     auto take = [&](float f, uint32_t at) {
-      if (f > v.m || !place.any) place = {at, at, true};
+      if (f > v.m || !place.any) place = {at, at, true, -1, 0.f};
       if (f > v.m) {
         v.rebase(fmaxf(f, -FLT_MAX), c2);
         v.m = f;
@@ -383,6 +391,17 @@ struct Pass {
   }
 };
 
+constexpr unsigned long long FETCH = 16384;
+// The beginning of a row into L2.
+template <class T>
+__device__ __forceinline__ void fetch_ahead(const T* row, int V) {
+  const uintptr_t first = (reinterpret_cast<uintptr_t>(row) + 15) & ~static_cast<uintptr_t>(15);
+  const uintptr_t end = reinterpret_cast<uintptr_t>(row + V) & ~static_cast<uintptr_t>(15);
+  if (end <= first) return;
+  const uint32_t bytes = static_cast<uint32_t>(min(static_cast<unsigned long long>(end - first), FETCH));
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(first), "r"(bytes) : "memory");
+}
+
 // One CTA per row, or a cluster of `parts` CTAs where there are few rows, whose sums and lists meet in the shared memory of the
 // first.  One pass over the row: every thread keeps the sums of its elements and the place of its largest.  For
 // the alternatives, the threads' largest keys (taken for as small as their places allow) are reduced to 64, the largest of a lane
@@ -397,7 +416,8 @@ template <class T, bool TOP, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
 logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
                     float* __restrict__ entropy, float* __restrict__ top_logprob, long long* __restrict__ top_id,
-                    float* __restrict__ stats, int V, long long ld, long long ignore_index, int top, int parts, float inv_t) {
+                    float* __restrict__ stats, int V, long long ld, long long ignore_index, int top, int parts, float inv_t,
+                    long long later) {
   if (parts > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   grid_begin(logits, tokens);
   __shared__ Shared sh;
@@ -414,9 +434,10 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
 
   Sums v;
   uint64_t bound = 0;
-  Place place = {0, 0, false};
+  Place place = {0, 0, false, -1, 0.f};
   for (int exact = 0; exact < 2; ++exact) {
     v = exact ? pass.exact(place) : pass.template quick<TOP>(place);
+    if (!TOP && parts == 1 && threadIdx.x == 0 && exact == 0 && row < 2 * later && row + later < gridDim.x) fetch_ahead(x + later * ld, V);
     const float wm = warp_max(v.m);
     if (lane == 0) sh.m[warp] = wm;
     if (TOP) sh.lists[warp][lane] = place.any ? make_key(v.m, place.last) : 0;
@@ -443,7 +464,11 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
     if (TOP) {
       bound = sh.bound;
       good = good && (bound == 0 || key_value(bound) > CLAMP);
-      if ((good || exact) && most != 0 && most >= bound) sh.owners[atomicAdd(&sh.num_owners, 1)] = threadIdx.x;
+      if ((good || exact) && most != 0 && most >= bound) {
+        const int at = atomicAdd(&sh.num_owners, 1);
+        sh.owners[at] = threadIdx.x;
+        sh.groups[at] = bound != 0 && place.second < key_value(bound) ? place.group : -1;
+      }
     }
     if (good || exact) break;
     __syncthreads();                       // read before it is written again
@@ -467,27 +492,27 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
         if (at < THREADS) found[at] = key;
       }
     };
-    // A warp takes two owners at a time, their vectors lane by lane, both loads in front of the first comparison.
+    const float least = bound == 0 ? -INFINITY : key_value(bound);
+    auto offer_vec = [&](int at) {
+      const uint4 u = reinterpret_cast<const uint4*>(body)[at];
+      // most vectors have nothing that reaches the bound; NaN counts as -inf, which reaches it if it is as low
+      if (Vec<T>(u).largest() < least) return;
+      float f[VEC<T>];
+      unpack(u, f, T());
+      const uint32_t first = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(at) * VEC<T>;
+#pragma unroll
+      for (int q = 0; q < VEC<T>; ++q) offer(f[q], first + q);
+    };
+    // Of most owners only the group of vectors that their largest element is in, a vector per thread; of the others all vectors,
+    // lane by lane.
     const int owners = sh.num_owners;
-    for (int o = warp; o < owners; o += 2 * WARPS) {
-      const int one = sh.owners[o], two = o + WARPS < owners ? sh.owners[o + WARPS] : sp.vecs;
-      for (int k = lane * THREADS; k < sp.vecs; k += 32 * THREADS) {
-        const int at[2] = {one + k, two + k};
-        uint4 u[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (at[h] < sp.vecs) u[h] = reinterpret_cast<const uint4*>(body)[at[h]];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (at[h] >= sp.vecs) continue;
-          float f[VEC<T>];
-          unpack(u[h], f, T());
-          const uint32_t first = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(at[h]) * VEC<T>;
-#pragma unroll
-          for (int q = 0; q < VEC<T>; ++q) offer(f[q], first + q);
-        }
-      }
+    for (int i = threadIdx.x; i < owners * AHEAD; i += THREADS) {
+      const int group = sh.groups[i / AHEAD], at = group + i % AHEAD * THREADS;
+      if (group >= 0 && at < sp.vecs) offer_vec(at);
     }
+    for (int o = warp; o < owners; o += WARPS)
+      if (sh.groups[o] < 0)
+        for (int at = sh.owners[o] + lane * THREADS; at < sp.vecs; at += 32 * THREADS) offer_vec(at);
     for (int e = threadIdx.x; e < owners; e += THREADS) {
       const int owner = sh.owners[e];
       if (owner < sp.head) offer(to_float(head[owner]), static_cast<uint32_t>(head + owner - x));
@@ -496,7 +521,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
     __syncthreads();
     const int n = sh.num_found;
     if (n <= THREADS) {
-      list = sort_falling(static_cast<int>(threadIdx.x) < n ? found[threadIdx.x] : 0, lane);
+      if (warp == 0 || n > 32) list = sort_falling(static_cast<int>(threadIdx.x) < n ? found[threadIdx.x] : 0, lane);
       if (n > 32) {
         __syncthreads();
         merge_lists(list, sh.lists, WARPS, warp, lane);
@@ -705,8 +730,10 @@ int fwd(const LogprobArgs& a, float* logprob, float* entropy, float* top_logprob
   auto kernel = a.top == 0                    ? logprobs_fwd_kernel<T, false, 3>
                 : a.T * parts > 2ll * num_sms ? logprobs_fwd_kernel<T, true, 3>
                                               : logprobs_fwd_kernel<T, true, 2>;
+  const bool three = a.top == 0 || a.T * parts > 2ll * num_sms;
+  const long long later = (three ? 3ll : 2ll) * num_sms;
   return launch_clusters(kernel, a.T * parts, parts, st, static_cast<const T*>(a.logits), a.tokens, logprob, entropy, top_logprob,
-                         top_id, stats, a.V, a.ld, a.ignore_index, a.top, parts, a.inv_temperature);
+                         top_id, stats, a.V, a.ld, a.ignore_index, a.top, parts, a.inv_temperature, later);
 }
 
 template <class T>
