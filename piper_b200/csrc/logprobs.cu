@@ -403,15 +403,18 @@ __device__ __forceinline__ void fetch_ahead(const T* row, int V) {
 }
 
 // One CTA per row, or a cluster of `parts` CTAs where there are few rows, whose sums and lists meet in the shared memory of the
-// first.  One pass over the row: every thread keeps the sums of its elements and the place of its largest.  For
-// the alternatives, the threads' largest keys (taken for as small as their places allow) are reduced to 64, the largest of a lane
-// number's in every other warp; the top-th largest of those is a bound that at least so many elements reach.  The elements that reach it
-// belong to the few threads whose largest does, and only those threads' elements, a small part of the row each, are looked at
-// again, by all threads; what they find is sorted.  1024 rows of 128256: 55.7 us without alternatives, 58.4 with 5, 67.2 with 20 (floor
-// 40): a CTA that looks for them reads nothing meanwhile.
+// first.  One pass over the row: every thread keeps the sums of its elements, the place of its largest and the largest outside the
+// group of vectors that this is in.  For the alternatives, the threads' largest keys (taken for as small as their places allow) are
+// reduced to 64, the largest of a lane number's in every other warp; the top-th largest of those is a bound that at least so many
+// elements reach.  The elements that reach it belong to the few threads whose largest does, and of most of those to that one group of
+// vectors, which is looked at again; what is found is sorted.  1024 rows of 128256: 50 us without alternatives, 60 with 5 or 20 (floor 40),
+// of which the bound and the sorting take 2.5, looking again 4 (with all vectors of those threads 12).  Those groups kept in shared
+// memory, and rows that start apart, bring nothing.
 // CTAS of them share an SM, with the registers that leaves: three where there are rows for them, so that others read while one
-// looks for its alternatives (2048 x 128256 with 20: 136 us by two, 123 by three); two, each of them faster, where there are not (296 rows
+// looks for its alternatives (2048 x 128256 with 20: 127 us by two, 110 by three); two, each of them faster, where there are not (296 rows
 // 22 and 28 us).  Without alternatives three are as fast with few rows.
+// The row that a later CTA is likely to take next here, `later` rows on, is fetched in part while the warps wait for one another: 1024
+// rows without alternatives 56 -> 50 us, 4096 rows 171-183 -> 172 (floor 160); with alternatives no gain, and none taken.
 template <class T, bool TOP, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
 logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
@@ -437,7 +440,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   Place place = {0, 0, false, -1, 0.f};
   for (int exact = 0; exact < 2; ++exact) {
     v = exact ? pass.exact(place) : pass.template quick<TOP>(place);
-    if (!TOP && parts == 1 && threadIdx.x == 0 && exact == 0 && row < 2 * later && row + later < gridDim.x) fetch_ahead(x + later * ld, V);
+    if (!TOP && parts == 1 && threadIdx.x == 0 && exact == 0 && row + later < gridDim.x) fetch_ahead(x + later * ld, V);
     const float wm = warp_max(v.m);
     if (lane == 0) sh.m[warp] = wm;
     if (TOP) sh.lists[warp][lane] = place.any ? make_key(v.m, place.last) : 0;
@@ -697,8 +700,8 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
 }
 
 // CTAs per row: with fewer rows than SMs have room for, a row is cut into up to eight pieces of at least 4,096 elements.  Not with
-// more rows, where a cluster waits for SMs together: 444 rows of 128256 with 5 alternatives 32.7 us, in two pieces each, which would fill
-// the SMs better, 43.4; 1024 rows without 55.7 and 64.6.
+// more rows, where a cluster waits for SMs together: 296 rows of 128256 with 20 alternatives 22.5 us, in four pieces 42; 1024 rows 60 us,
+// in two 83, without alternatives 50 and 65.
 int row_parts(long long T, int V, int num_sms) {
   int parts = 1;
   while (parts < MAX_PARTS && T * parts * 2 <= 2ll * num_sms && V / (parts * 2) >= 4096) parts *= 2;

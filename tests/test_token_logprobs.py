@@ -188,6 +188,44 @@ def test_largest_values_in_one_threads_elements(device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,offset", [(32003, 0), (32003, 1), (5003, 3), (70001, 7)])
+def test_where_the_largest_values_are(V, offset, dtype, device):
+    """The alternatives, one after the other: in one vector; in one thread's vectors near each other, and far apart; in front of the first
+    whole vector and behind the last; the largest alone in its thread and the next ones together in another."""
+    vec = 128 // torch.finfo(dtype).bits
+    step = 512 * vec
+    head = (-offset) % vec
+    starts = [[head + 5 * vec + q for q in range(vec)], [head + 9 * vec + j * step for j in range(4)],
+              [head + 9 * vec + j * step + j % vec for j in range(0, (V - 100) // step, 3)], [0, 1, V - 1, V - 2, V - 3],
+              [head + 40 * vec, head + 77 * vec, head + 77 * vec + step, head + 77 * vec + 1],
+              [head, V // 2, V - 1] + [head + 200 * vec + j * step for j in range(2, 14, 4)]]
+    g = torch.Generator().manual_seed(11)
+    room = torch.zeros(2 * len(starts), V + 8, dtype=dtype)
+    x = room[:, offset:offset + V]
+    x.copy_(torch.rand(2 * len(starts), V, generator=g))
+    for r, places in enumerate(starts):
+        at = torch.tensor([p for p in places if p < V])
+        x[2 * r, at] = torch.arange(2, 2 + len(at)).to(dtype)                # rising, and equal
+        x[2 * r + 1, at] = torch.full((len(at),), 3.0, dtype=dtype)
+    room = room.to(device)
+    x = room[:, offset:offset + V]
+    tokens = torch.zeros(len(x), dtype=torch.int64, device=device)
+    for top in (1, 5, 20, 32):
+        _check(x, tokens, top, 1.0, ops.token_logprobs(x, tokens, top=top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,top", [(1000, 4099, 0), (1000, 4099, 20), (700, 7, 0), (900, 1, 0), (460, 33000, 0)])
+def test_more_rows_than_are_read_at_a_time(T, V, top, dtype):
+    room = torch.randn(T, V + 5, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    x = room[:, 3:3 + V]
+    tokens = torch.randint(0, V, (T,), generator=torch.Generator().manual_seed(4)).cuda()
+    _check(x, tokens, top, 0.7, ops.token_logprobs(x, tokens, top=top, temperature=0.7))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_peaked_rows_keep_their_last_digits(dtype, device):
     """Nearly all of the probability in one token, far above what a thread has seen before it: log S is close to 0, so an absolute
     error of a few steps of 1 is what S itself has, and every other term keeps its own relative one."""
