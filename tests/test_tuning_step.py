@@ -221,3 +221,63 @@ def test_pipelines_of_two_ranks(kind, checkpointing, tmp_path):
     for n, p in model.named_parameters():
         assert float((grads[n] - p.grad).norm()) <= 2e-5 * float(p.grad.norm()), n
     assert sum(v for r in results for v in r["again"]) != sum(losses)          # the step was taken
+
+
+def _replica_worker(rank, world, schedule, bits, directory):
+    from piper_b200 import piper_exec_dag, piper_setup
+    from piper_b200.models.llama3 import LLAMA_CONFIGS, Transformer
+    from piper_b200.nn import cross_entropy_loss
+    from piper_b200.runtime.checkpoint import load_checkpoint, save_checkpoint
+
+    cfg = LLAMA_CONFIGS["tiny"]
+    x, y = _tokens(cfg)
+    mine = slice(2 * rank, 2 * rank + 2)
+    actor = piper_setup(Transformer, (cfg, 64, 1), optim_fn=torch.optim.AdamW, optim_kwargs={"state_bits": bits, "lr": 1e-3},
+                        example_inputs=[x[mine]], example_outputs=y[mine], model_dtype=torch.float32,
+                        const_attrs=Transformer.const_attrs(cfg, 64), schedule_directives=schedule, device="cpu")
+
+    def params():
+        return {k: v.detach().clone() for k, v in actor.named_parameters().items()}
+
+    before = params()
+    piper_exec_dag(cross_entropy_loss)
+    once = params()
+    save_checkpoint(actor, directory, 1)
+    piper_exec_dag(cross_entropy_loss)
+    twice = params()
+    load_checkpoint(actor, directory)
+    piper_exec_dag(cross_entropy_loss)
+    return {"before": before, "once": once, "twice": twice, "again": params()}
+
+
+def _replicas(flags, bits, folder):
+    from tests.dist_utils import run_ranks
+
+    schedule = [{"op": "place", "filter": {"PP": 0}, "devices": [0, 1], "stream": "pp_stream"},
+                {"op": "split", "filter": {}, "dim_name": "MB", "num_microbatches": 2},
+                {"op": "replicate", "filter": {"PP": 0}, "devices": [0, 1], "gather_stream": "dp_stream",
+                 "reduce_stream": "dp_stream", **flags}]
+    return run_ranks(2, _replica_worker, (schedule, bits, str(folder / "saved")), folder)
+
+
+@pytest.mark.parametrize("flags", [{}, {"shard_grads": True}, {"shard_params": True, "shard_grads": True}])
+def test_replicas_with_eight_bit_moments(flags, tmp_path):
+    """Every way to shard the optimizer: ranks agree to the bit, and steps from a checkpoint repeat to the bit.  The first step uses the
+    moments as they are before they are rounded, so it is that of 32 bits on the same layout (another would add gradients in another
+    order, and an update has the size of lr whatever its gradient's): the same operations but for a division by a square root's
+    correction in place of a product, half a dozen roundings of an update of at most lr (1 + |w| / 10)."""
+    one, other = _replicas(flags, 8, tmp_path)
+    for when in ("once", "twice", "again"):
+        assert one[when].keys() == other[when].keys()
+        for k in one[when]:
+            assert torch.equal(one[when][k], other[when][k]), (when, k)
+    for k, w in one["before"].items():
+        assert torch.equal(one["twice"][k], one["again"][k]), k
+        assert not torch.equal(one["once"][k], w) and not torch.equal(one["twice"][k], one["once"][k]), k
+    if not flags:
+        folder = tmp_path / "wide"
+        folder.mkdir()
+        wide = _replicas(flags, 32, folder)[0]
+        for k, w in one["before"].items():
+            off = (one["once"][k] - wide["once"][k]).abs()
+            assert bool((off <= 2.0 ** -23 * w.abs() + 8 * 2.0 ** -24 * 1e-3 * 1.1).all()), (k, float(off.max()))
