@@ -243,6 +243,18 @@ def test_refusals(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [(1376, 256), (4096, 1024), (6144, 4096)])
+def test_a_row_has_the_same_bits_in_a_batch_of_any_size(N, K):
+    """Tiles of every width and height add along the contraction in one order."""
+    x, w = _matrix(4096, K, "cuda", 1), _matrix(N, K, "cuda", 2, std=0.05)
+    kept = ops.fp8_quantize(w, square=True)
+    whole = ops.fp8_linear(x, w)
+    for T in (1, 3, 24, 64, 100, 129, 300, 700, 1000, 2048):
+        assert torch.equal(ops.fp8_linear(x[:T], w), whole[:T]), T
+        assert torch.equal(ops.fp8_linear(x[4096 - T:], kept), whole[4096 - T:]), T
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lead", [(6,), (2, 3)])
 def test_the_same_refusals_by_the_library(lead):
     x, w = (torch.ones(*n, dtype=torch.bfloat16, device="cuda") for n in ((*lead, 64), (32, 64)))
