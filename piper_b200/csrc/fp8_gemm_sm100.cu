@@ -456,9 +456,8 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
 }
 
 // Two k-blocks to a stage, and to a round of waiting and committing, where they leave room for four such stages (three for a
-// CTA by itself).  A block costs the issuing warp as long as a narrow tile's MMAs take: 24 x 4096 x 14336 in 64 tiles of 64 columns
-// 31.2 us by single blocks, 24.8 by two (453 and 344 cycles a block), by pairs 25.8 and 19.9; 1000 x 2048 x 8192 in pairs of 128
-// columns 18.2 and 15.8.
+// CTA by itself).  A block costs the issuing warp as long as a narrow tile's MMAs take: 24 x 4096 x 14336 29.4 us by single blocks, 22.5
+// by two (453 and 344 cycles a block of 64 columns); 1000 x 2048 x 8192 in pairs 18.9 and 16.0.
 bool two_blocks(int ctas, int width) { return ctas == 2 ? width <= 128 : width <= 96; }
 
 // Cycles of a launch by the model of the bf16 products (gemm_cost): an MMA of twice the elements per cycle on elements of half
