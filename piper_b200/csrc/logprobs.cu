@@ -14,6 +14,7 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 
 #include "ptx.cuh"
 
@@ -91,11 +92,21 @@ struct Sums {
   }
 };
 
-// The quick pass takes logits for at least CLAMP, so that nothing is infinite; a row whose maximum is not well inside
-// (-BIG, BIG), or whose alternatives reach down there, is read again by the exact pass.
-constexpr float CLAMP = -1.0002555517425873e30f;      // a bf16 number, 0xF14A
-constexpr uint32_t CLAMP_PAIR = 0xF14AF14Au;
-constexpr float BIG = 1e28f;
+// The quick pass takes logits for at least `low`, a bf16 number of which low c2 is -2^30 or little above.  Its exponents fma(x, c2, -base)
+// keep what was lost when base = x c2 was rounded, half a unit of the last place: 64 at most for what is not below low, so a sum
+// of a thread that has seen nothing but masked ids, whatever finite number they are masked by, is at most 2^64 times its length
+// until it is brought to the row's maximum, beside which it is 0.  A row whose maximum is not inside (low / 2, -low / 2), or whose
+// alternatives reach down to low, is read again by the exact pass.
+float lowest_logit(float inv_t) {
+  const float low = -1073741824.f / (inv_t * LOG2E);
+  uint32_t bits;
+  memcpy(&bits, &low, sizeof bits);
+  bits &= 0xFFFF0000u;                     // towards 0
+  float r;
+  memcpy(&r, &bits, sizeof r);
+  return r;
+}
+
 // ------------------------------------------------------------------ the largest of many keys
 // Value and index of an element as one integer that grows with the value and, among equal values, with a falling index, so no two
 // elements of a row have the same key and the order of ties is the order of ids.  0 is below every key.  A NaN counts as
@@ -212,16 +223,16 @@ __device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// A vector, no element below CLAMP, and the largest numbers of two halves of its elements, in the vector's own form.
+// A vector, no element below `low`, and the largest numbers of two halves of its elements, in the vector's own form.
 template <class T>
 struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   uint4 u;
   uint32_t most;
-  __device__ __forceinline__ explicit Vec(const uint4& v) {
-    u = make_uint4(max_nan_bf16x2(v.x, CLAMP_PAIR), max_nan_bf16x2(v.y, CLAMP_PAIR), max_nan_bf16x2(v.z, CLAMP_PAIR),
-                   max_nan_bf16x2(v.w, CLAMP_PAIR));
+  __device__ __forceinline__ Vec(const uint4& v, float low) {
+    const uint32_t pair = __byte_perm(__float_as_uint(low), 0, 0x3232u);
+    u = make_uint4(max_nan_bf16x2(v.x, pair), max_nan_bf16x2(v.y, pair), max_nan_bf16x2(v.z, pair), max_nan_bf16x2(v.w, pair));
     most = max_bf16x2(max_bf16x2(u.x, u.y), max_bf16x2(u.z, u.w));
   }
   __device__ __forceinline__ void also(const Vec& o) { most = max_bf16x2(most, o.most); }
@@ -232,9 +243,9 @@ template <>
 struct Vec<float> {
   float4 u;
   float most;
-  __device__ __forceinline__ explicit Vec(const uint4& v) {
-    u = make_float4(max_nan(__uint_as_float(v.x), CLAMP), max_nan(__uint_as_float(v.y), CLAMP), max_nan(__uint_as_float(v.z), CLAMP),
-                    max_nan(__uint_as_float(v.w), CLAMP));
+  __device__ __forceinline__ Vec(const uint4& v, float low) {
+    u = make_float4(max_nan(__uint_as_float(v.x), low), max_nan(__uint_as_float(v.y), low), max_nan(__uint_as_float(v.z), low),
+                    max_nan(__uint_as_float(v.w), low));
     most = fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w));
   }
   __device__ __forceinline__ void also(const Vec& o) { most = fmaxf(most, o.most); }
@@ -283,7 +294,7 @@ struct Pass {
   const T* body;
   const T* tail;
   Span sp;
-  float c2;
+  float c2, low;
 
   // Elements in front of and behind the vectors; `take` gets the element and its place in the row.
   template <class F>
@@ -293,11 +304,12 @@ struct Pass {
 
   template <bool TOP>
   __device__ __forceinline__ Sums quick(Place& place) const {
-    QuickSums v = {0.5f * CLAMP * c2, CLAMP, 0.f, 0.f};      // far above what is clamped, far below the first raise
+    // a base that belongs to `top` as all later ones do, so that none lies below it, and far above the exponents of low
+    QuickSums v = {0.5f * low * c2, 0.5f * low, 0.f, 0.f};
     float m = -INFINITY;
     float second = -INFINITY;              // what is above it is there too
     auto single = [&](float f, uint32_t at) {
-      const float x = max_nan(f, CLAMP);
+      const float x = max_nan(f, low);
       if (x > m || !place.any) place = {at, at, true, -1, 0.f};
       second = fmaxf(second, fminf(x, m));
       m = fmaxf(m, x);
@@ -312,7 +324,7 @@ struct Pass {
       uint4 u[AHEAD];
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) u[j] = __ldcs(vecs + i + j * THREADS);
-      Vec<T> first(u[0]), rest[AHEAD - 1] = {Vec<T>(u[1]), Vec<T>(u[2]), Vec<T>(u[3])};
+      Vec<T> first(u[0], low), rest[AHEAD - 1] = {Vec<T>(u[1], low), Vec<T>(u[2], low), Vec<T>(u[3], low)};
       Vec<T> all = first;
 #pragma unroll
       for (int j = 0; j < AHEAD - 1; ++j) all.also(rest[j]);
@@ -338,7 +350,7 @@ struct Pass {
     }
 #pragma unroll 1
     for (; i < sp.vecs; i += THREADS) {
-      const Vec<T> x(__ldcs(vecs + i));
+      const Vec<T> x(__ldcs(vecs + i), low);
       const float lm = x.largest();
       if (TOP && (lm > m || !place.any)) {
         best = i;
@@ -360,9 +372,9 @@ struct Pass {
     place.group = best;
     singles(sp.tail, tail, single);
     place.second = second;
-    if (!(m > CLAMP)) return Sums::none();
-    Sums r = {m, m, v.s, v.t};
-    r.shift(max_nan(fmaf(-r.from, c2, v.base), FAR_BELOW));
+    if (!(m > low)) return Sums::none();
+    Sums r = {m, v.top, v.s, v.t};
+    r.shift(fmaf(-r.from, c2, v.base));
     return r;
   }
 
@@ -419,7 +431,7 @@ template <class T, bool TOP, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
 logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ tokens, float* __restrict__ logprob,
                     float* __restrict__ entropy, float* __restrict__ top_logprob, long long* __restrict__ top_id,
-                    float* __restrict__ stats, int V, long long ld, long long ignore_index, int top, int parts, float inv_t,
+                    float* __restrict__ stats, int V, long long ld, long long ignore_index, int top, int parts, float inv_t, float low,
                     long long later) {
   if (parts > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   grid_begin(logits, tokens);
@@ -433,7 +445,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
   const T* body = head + sp.head;
   const T* tail = body + static_cast<long long>(sp.vecs) * VEC<T>;
   const float c2 = inv_t * LOG2E;
-  const Pass<T> pass = {x, head, body, tail, sp, c2};
+  const Pass<T> pass = {x, head, body, tail, sp, c2, low};
 
   Sums v;
   uint64_t bound = 0;
@@ -463,10 +475,10 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) v.m = fmaxf(v.m, sh.m[w]);
     __syncthreads();
-    bool good = fabsf(v.m) < BIG;
+    bool good = fabsf(v.m) < -0.5f * low;
     if (TOP) {
       bound = sh.bound;
-      good = good && (bound == 0 || key_value(bound) > CLAMP);
+      good = good && (bound == 0 || key_value(bound) > low);
       if ((good || exact) && most != 0 && most >= bound) {
         const int at = atomicAdd(&sh.num_owners, 1);
         sh.owners[at] = threadIdx.x;
@@ -499,7 +511,7 @@ logprobs_fwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
     auto offer_vec = [&](int at) {
       const uint4 u = reinterpret_cast<const uint4*>(body)[at];
       // most vectors have nothing that reaches the bound; NaN counts as -inf, which reaches it if it is as low
-      if (Vec<T>(u).largest() < least) return;
+      if (Vec<T>(u, low).largest() < least) return;
       float f[VEC<T>];
       unpack(u, f, T());
       const uint32_t first = static_cast<uint32_t>(body - x) + static_cast<uint32_t>(at) * VEC<T>;
@@ -736,7 +748,8 @@ int fwd(const LogprobArgs& a, float* logprob, float* entropy, float* top_logprob
   const bool three = a.top == 0 || a.T * parts > 2ll * num_sms;
   const long long later = (three ? 3ll : 2ll) * num_sms;
   return launch_clusters(kernel, a.T * parts, parts, st, static_cast<const T*>(a.logits), a.tokens, logprob, entropy, top_logprob,
-                         top_id, stats, a.V, a.ld, a.ignore_index, a.top, parts, a.inv_temperature, later);
+                         top_id, stats, a.V, a.ld, a.ignore_index, a.top, parts, a.inv_temperature, lowest_logit(a.inv_temperature),
+                         later);
 }
 
 template <class T>

@@ -127,6 +127,64 @@ def test_rows_that_are_special(V, dtype, device):
     assert out.top_id[0].tolist() == list(range(top))
 
 
+MASKS = [-1e4, -7e8, -1e9, -1e10, -1e20, -7e29, -3e38]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,offset", [(1, 9, 0), (1, 32003, 1), (6, 4099, 0), (6, 17003, 0), (600, 515, 3)])
+def test_rows_that_are_masked_by_large_numbers(T, V, offset, dtype, device):
+    """Masks that are finite, over most of a row, all of it, its first half and around single ids: a masked id has probability 0 beside
+    one that is not, and a row of nothing else is uniform.  Log probabilities below the smallest fp32 number are -inf."""
+    few = 4
+    for mask in MASKS:
+        for temperature in (0.1, 0.3, 0.6, 0.8, 1.0) if T * V < 50000 else (0.3, 0.6, 1.0):
+            x, tokens = _logits(T, V, dtype, "cpu", V)
+            real = x.clone()
+            for r in range(T):
+                if r % 6 == 0:
+                    x[r, :V - few - 1] = mask                 # all but a few at the end, one more behind them
+                    x[r, V - 1] = mask
+                    tokens[r] = V - 2
+                elif r % 6 == 1:
+                    x[r] = mask
+                elif r % 6 == 2:
+                    x[r, :V // 2] = mask
+                elif r % 6 == 3:
+                    x[r, few:] = mask                         # all but a few in front
+                elif r % 6 == 4:
+                    x[r] = mask
+                    x[r, V // 3] = real[r, V // 3]            # a single one left
+                else:
+                    x[r, :V // 2] = mask
+                    x[r, V // 2:V // 2 + few] = 2 * mask if mask > -1e38 else -INF
+            store = torch.zeros(T * V + 8, dtype=dtype, device=device)
+            x = store[offset:offset + T * V].copy_(x.reshape(-1)).view(T, V).requires_grad_(True)
+            tokens = tokens.to(device)
+            out = ops.token_logprobs(x, tokens, top=few, temperature=temperature)
+            g = torch.Generator().manual_seed(6)
+            gradients = [torch.randn(s, generator=g).to(device) for s in ((T,), (T,), (T, few))]
+            (d,) = torch.autograd.grad([out.logprob, out.entropy, out.top_logprob], x, gradients)
+            logp, _p, H, _on, lp, ids, _left = _definition(x, tokens, few, temperature)
+            assert torch.equal(out.top_id.cpu(), ids)
+            eps, row = 2.0 ** -24, 2.0 ** -24 * ((V if device == "cpu" else V / 512 + 20) + 40)
+            for got, want, extra in ((out.logprob, lp, 0), (out.top_logprob, logp.gather(-1, ids), 0), (out.entropy, H, row * H + 8 * eps * math.log(V + 1))):
+                got, want = got.double().cpu(), want.float().double()
+                assert bool(((got == want) | ((got - want).abs() <= row + extra + 6 * eps * want.abs().nan_to_num(posinf=0))).all()), \
+                    (mask, temperature, got[got != want][:4], want[got != want][:4])
+            want, size = _gradient(x, tokens, few, temperature, *gradients)
+            # p = 2^u with u = (x - M) c2 - log S: four roundings (the difference, 1 / temperature, c2, the sum) and log2(e)'s own of
+            # numbers up to |u| are 5 2^-24 |log p| of p.  A p below the normal numbers is 0, which loses less than the
+            # smallest of them times what p is multiplied by.
+            u = torch.where(logp.isfinite(), logp, 0.0).abs()
+            d_logprob, d_entropy, d_top = (t.double().cpu().abs().view(T, -1) for t in gradients)
+            times = (d_logprob + d_top.sum(1, keepdim=True) + d_entropy * (u + H.unsqueeze(1))) / temperature
+            bound = (torch.finfo(dtype).eps / 2 * want.abs() + (2.0 ** -20 + 2 * row + 5 * eps * u) * size
+                     + torch.finfo(dtype).tiny * (1 + times))
+            far = (d.double().cpu() - want).abs() > bound
+            assert not bool(far.any()), (mask, temperature, d.cpu()[far][:4], want[far][:4])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_rows_without_numbers_are_nan(device):
     for bad in (float("nan"), INF):
