@@ -372,7 +372,7 @@ struct Pass {
     place.group = best;
     singles(sp.tail, tail, single);
     place.second = second;
-    if (!(m > low)) return Sums::none();
+    // of a thread with nothing above low the sums are 0, or NaN
     Sums r = {m, v.top, v.s, v.t};
     r.shift(fmaf(-r.from, c2, v.base));
     return r;

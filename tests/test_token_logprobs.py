@@ -199,6 +199,26 @@ def test_rows_without_numbers_are_nan(device):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,masked,where", [(3, 7, None, [3]), (3, 7, None, [0]), (3, 7, 1, [6]), (2, 1000, 256, [300]), (3, 1000, None, range(16, 24)),
+                                              (3, 1000, 0, range(1000)), (2, 4000, 100, [3999]), (600, 4000, 256, [1300]),
+                                              (1, 128256, None, range(64, 72)), (1, 128256, 4096, [100000])])
+def test_a_nan_wherever_it_is(T, V, masked, where, dtype, device):
+    """Alone in a thread's elements, among masked ids, a whole vector of them, in a piece of a row that is cut: the row is NaN."""
+    for mask in (-INF, -1e9):
+        x, tokens = _logits(T, V, dtype, "cpu", 2)
+        if masked is not None:
+            x[0, masked:] = mask
+        x[0, list(where)] = float("nan")
+        for top in (0, 3):
+            out = ops.token_logprobs(x.to(device), tokens.to(device), top=top)
+            for t in (out.logprob, out.entropy, out.top_logprob):
+                assert bool(torch.isnan(t[0]).all()) and not bool(torch.isnan(t[1:]).any())
+            assert bool((out.top_id >= 0).all()) and bool((out.top_id < V).all())
+            assert len(set(out.top_id[0].tolist())) == top
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("T,V,offset", [(6, 9, 0), (6, 10007, 1), (600, 1031, 3)])
 def test_rows_that_nothing_asks_for_have_no_gradient(T, V, offset, dtype, device):
     """Padding, whatever its logits are (0 x NaN is NaN in the formula): by an ignored token, by gradients of zero; and what the
