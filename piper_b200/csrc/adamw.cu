@@ -85,7 +85,13 @@ __device__ __forceinline__ float block_scale(const float (&x)[PER]) {
 
 // The rare operations, out of the way of the common ones in the instruction cache.
 __device__ __noinline__ float divide(float a, float b) { return __fdiv_rn(a, b); }
-__device__ __noinline__ float exact_update(float m, float v, float root, float eps) { return m / fmaf(sqrtf(v), root, eps); }
+__device__ __noinline__ float small_eps_update(float m, float v, float root, float eps) {
+  if (eps < 1e-30f) return m / fmaf(sqrtf(v), root, eps);
+  float r, q;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("div.approx.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(fmaf(r, root, eps)));
+  return q;
+}
 
 // y = |x| / scale of a block, correctly rounded.  With the correctly rounded reciprocal, a product, its exact remainder and a
 // correction give the quotient (Markstein, IBM J. Res. Dev. 34, 1990) where nothing underflows: a quotient that is not small enough for
@@ -106,10 +112,12 @@ __device__ __forceinline__ void quotients(const float* x, float scale, float (&y
   }
 }
 
-// m / (sqrt(v) root + eps), within two units of the last place for the root and for the quotient; numbers below the normal ones
-// count as 0, so a vanishing eps, beside which they would matter, takes the exact operations.
-__device__ __forceinline__ float update(float m, float v, float root, float eps) {
-  if (eps < 1e-30f) return exact_update(m, v, root, eps);
+// m / (sqrt(v) root + eps), within two units of the last place for the root and for the quotient.  Where eps is small enough for the
+// root of a v below the normal numbers to matter beside it (`small_eps`), that is not taken for 0: 64 Mi elements with 8-bit
+// moments 257 us in place of 222; within the common path that is 241, but 224 for all others.  A vanishing eps, beside which a denominator
+// may be below them, takes the exact operations.
+__device__ __forceinline__ float update(float m, float v, float root, float eps, int small_eps) {
+  if (small_eps) return small_eps_update(m, v, root, eps);
   float r, q;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(q) : "f"(m), "f"(fmaf(r, root, eps)));
@@ -222,7 +230,7 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
         const float gj = __fmul_rn(g[j], a.grad_scale);
         m[j] = __fadd_rn(__fmul_rn(m[j], a.b1), __fmul_rn(gj, a.c1));
         v[j] = __fadd_rn(__fmul_rn(v[j], a.b2), __fmul_rn(__fmul_rn(gj, a.c2), gj));
-        w[j] = fmaf(-rate, update(m[j], v[j], root, a.eps), w[j] * a.keep);
+        w[j] = fmaf(-rate, update(m[j], v[j], root, a.eps, a.small_eps), w[j] * a.keep);
       }
       if (!whole) {
 #pragma unroll
@@ -332,9 +340,12 @@ moments_decode_kernel(const uint32_t* __restrict__ m, const float* __restrict__ 
 
 }  // namespace
 
-int adamw_launch(AdamwTable& table, const AdamwArgs& a, int num_sms, cudaStream_t st) {
+int adamw_launch(AdamwTable& table, AdamwArgs a, int num_sms, cudaStream_t st) {
   long long chunks = 0;
+  a.small_eps = 0;
   for (int i = 0; i < table.count; ++i) {
+    // 2^-63, the root of the smallest normal number, times root: 2^-22 of eps or more
+    if (a.eps < 4.5474735e-13f * table.t[i].root) a.small_eps = 1;
     table.first[i] = static_cast<int>(chunks);
     chunks += (table.t[i].n + CHUNK - 1) / CHUNK;
     if (chunks > INT32_MAX / 2) return -1;

@@ -34,11 +34,12 @@ struct AdamwArgs {
   float* v_scale;
   float b1, b2, c1, c2;      // c1 = 1 - beta1, c2 = 1 - beta2
   float eps, keep;           // keep = 1 - lr * weight_decay
+  int small_eps;             // the roots of numbers below the normal ones count beside eps
   float grad_scale;
 };
 
-// table.first is filled in here.
-int adamw_launch(AdamwTable& table, const AdamwArgs& a, int num_sms, cudaStream_t st);
+// table.first and a.small_eps are filled in here.
+int adamw_launch(AdamwTable& table, AdamwArgs a, int num_sms, cudaStream_t st);
 
 // fp32 values of n codes of either moment (a multiple of kMomentBlock) with their scales.
 int moments_decode(const void* m, const float* m_scale, const void* v, const float* v_scale, float* out_m, float* out_v, long long n,

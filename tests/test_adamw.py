@@ -161,6 +161,23 @@ def test_eps_of_any_size(eps, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("eps", [1e-35, 1e-28, 1e-20, 1e-18, 1e-16, 1e-14, 1e-12, 1e-10, 1e-8])
+def test_vanishing_gradients_beside_any_eps(eps, device):
+    """Squares below the normal numbers count beside an eps that is as small as their roots.  v is off by one of the smallest numbers, 2^-149, at
+    most, and with it the root."""
+    g = torch.tensor([1e-20, -1e-20, 1e-19, 1e-18, 3e-18, -3e-18, 4e-18, 1e-17, 1e-15, 1.0]).repeat_interleave(30)
+    p = [torch.zeros(300, device=device)]
+    state = ops.AdamWState(p, bits=32)
+    w, m, v = (torch.zeros(300).double() for _ in range(3))
+    for step in range(1, 4):
+        before = p[0].double().cpu()
+        ops.adamw_step(p, [g.to(device)], state, lr=1.0, eps=eps, weight_decay=0.0)
+        w, m, v, _size, upd = _formula(w, m, v, g, step, 1.0, (0.9, 0.999), eps, 0.0)
+        tol = 40 * EPS + 1 - torch.sqrt((1 - step * 2.0 ** -149 / v).clamp(min=0))
+        assert bool(((before - p[0].double().cpu() - upd).abs() <= upd.abs() * tol + 2 * EPS * before.abs()).all()), step
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_inference_tensors(device):
     with torch.inference_mode():
         p = [torch.ones(300, device=device)]
