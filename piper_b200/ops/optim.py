@@ -153,15 +153,21 @@ class AdamWState:
                 scale.copy_(s)
 
     def state_dict(self) -> dict:
-        return {"bits": self.bits, "shapes": list(self.shapes), "steps": list(self.steps), "m": self.m, "v": self.v,
-                "m_scale": self.m_scale, "v_scale": self.v_scale, "master": self.master}
+        return {"bits": self.bits, "shapes": list(self.shapes), "dtypes": list(self.dtypes), "steps": list(self.steps),
+                "m": self.m, "v": self.v, "m_scale": self.m_scale, "v_scale": self.v_scale, "master": self.master}
 
     def load_state_dict(self, state: dict) -> None:
-        """Takes over a state of the same parameters, of either width."""
+        """Takes over a state of the same parameters, of either width.  Nothing is written if it is of others."""
         if [tuple(s) for s in state["shapes"]] != self.shapes:
             raise ValueError("AdamWState: the state is of other parameters")
-        if (state["master"] is None) != (self.master is None):
+        # which of its parameters have a master copy; a state that does not say had better be of one type
+        dtypes = state.get("dtypes")
+        if (state["master"] is None) != (self.master is None) or (
+                list(dtypes) != self.dtypes if dtypes is not None else len(set(self.dtypes)) > 1):
             raise ValueError("AdamWState: the state is of parameters of another type")
+        if len(state["steps"]) != len(self.shapes) or any(
+                state[n].numel() != self.numel for n in ("m", "v", "master") if state[n] is not None):
+            raise ValueError("AdamWState: the state is of another layout")
         with torch.no_grad():
             if state["bits"] == self.bits:
                 for name in ("m", "v", "m_scale", "v_scale"):

@@ -242,6 +242,38 @@ def test_states_are_saved_and_loaded(device):
     assert all(torch.equal(a, b) for a, b in zip(params, twin))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_state_of_other_types_is_refused(device):
+    """Same shapes, types in another order: the master copies would be those of other parameters.  A refused state changes nothing."""
+    def tensors(*dtypes):
+        return [torch.ones(300, dtype=t, device=device) for t in dtypes]
+
+    f32, b16 = torch.float32, torch.bfloat16
+    for bits in (8, 32):
+        for source, target in (((f32, b16), (b16, f32)), ((f32, b16), (b16, b16)), ((b16, b16), (b16, f32)), ((b16, b16), (f32, f32)),
+                               ((f32, f32), (b16, f32))):
+            params = tensors(*target)
+            other = ops.AdamWState(tensors(*source), bits=bits)
+            state = ops.AdamWState(params, bits=40 - bits)
+            ops.adamw_step(params, [torch.ones_like(p) for p in params], state)
+            before = [t.clone() for t in (*state.moments(), *([] if state.master is None else [state.master]))]
+            with pytest.raises(ValueError):
+                state.load_state_dict(other.state_dict())
+            after = [*state.moments(), *([] if state.master is None else [state.master])]
+            assert all(torch.equal(x, y) for x, y in zip(before, after)) and state.steps == [1, 1]
+            # a state without its types, as once saved
+            old = {k: v for k, v in state.state_dict().items() if k != "dtypes"}
+            if len(set(target)) == 1:
+                state.load_state_dict(old)
+            else:
+                with pytest.raises(ValueError):
+                    state.load_state_dict(old)
+                state.load_state_dict(state.state_dict())
+            cut = dict(state.state_dict(), m=state.m[:BLOCK], v=state.v[:BLOCK])
+            with pytest.raises(ValueError):
+                state.load_state_dict(cut)
+
+
 def test_moments_of_eight_bits_take_two_bytes():
     p = [torch.zeros(1 << 16)]
     s = ops.AdamWState(p, bits=8)
