@@ -103,11 +103,15 @@ class CrossEntropyLoss(nn.Module):
 def policy_gradient_loss(output: torch.Tensor, tokens: torch.Tensor, advantages: Optional[torch.Tensor] = None, *,
                          entropy_coef: float = 0.0, temperature: float = 1.0, ignore_index: int = -100) -> torch.Tensor:
     """Minus the mean over the counted tokens of advantage (1 without) x log probability + ``entropy_coef`` x entropy, of
-    ``[.., V]`` logits at ``temperature``.  Tokens that are ``ignore_index`` or no ids do not count, whatever stands beside them."""
+    ``[.., V]`` logits at ``temperature``.  Tokens that are ``ignore_index`` or no ids do not count, whatever stands beside them.  A
+    masked token (log probability -inf) whose advantage is 0 adds nothing."""
     flat, V = tokens.reshape(-1), output.shape[-1]
     r = ops.token_logprobs(output.reshape(-1, V), flat, temperature=temperature, ignore_index=ignore_index)
     counted = (flat != ignore_index) & (flat >= 0) & (flat < V)
-    gain = r.logprob if advantages is None else r.logprob * torch.where(counted, advantages.reshape(-1), 0)
+    gain = r.logprob
+    if advantages is not None:
+        factor = torch.where(counted, advantages.reshape(-1), 0)
+        gain = torch.where((factor == 0) & (gain == -math.inf), 0, gain) * factor
     if entropy_coef:
         gain = gain + entropy_coef * torch.where(counted, r.entropy, 0)
     return -gain.sum() / counted.sum().clamp(min=1)

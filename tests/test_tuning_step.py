@@ -3,6 +3,8 @@ entropy term, AdamW with 8-bit moments; against the same model and ops stepped b
 
 Both sides run the same ops on the same microbatches.  They may differ where fp32 sums are added in another order: weight gradients
 of two microbatches (in the bucket, or by autograd in the parameters' type)."""
+import math
+
 import pytest
 import torch
 
@@ -136,6 +138,29 @@ def test_policy_gradient_loss_of_padding(device):
     logp = torch.log_softmax(only, -1)
     want = -(adv[~pad] * logp.gather(-1, tokens[~pad].unsqueeze(-1)).squeeze(-1) - 0.3 * (logp.exp() * logp).sum(-1)).mean()
     assert abs(float(results[0][0]) - float(want)) < 2.0 ** -20 * 20
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_gradient_loss_of_a_masked_token_without_advantage(device):
+    """Its log probability is -inf, but it is asked nothing: no loss and no gradient, as if it were not there (but counted)."""
+    from piper_b200.nn import policy_gradient_loss
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(5, 40, generator=g)
+    x[1, 7] = x[4, 0] = -math.inf
+    x[3] = -math.inf
+    tokens = torch.tensor([2, 7, -100, 5, 1])
+    adv = torch.tensor([0.5, 0.0, 1.0, 0.0, 0.0])
+    x = x.to(device).requires_grad_(True)
+    for coef in (0.0, 0.25):
+        loss = policy_gradient_loss(x, tokens.to(device), adv.to(device), entropy_coef=coef)
+        (d,) = torch.autograd.grad(loss, x)
+        logp = torch.log_softmax(x.detach().double().cpu(), -1)
+        entropy = -torch.where(logp > -math.inf, logp.exp() * logp, 0).sum(-1)[[0, 1, 4]].sum()
+        want = -(0.5 * logp[0, 2] + coef * entropy) / 4
+        assert abs(float(loss.detach()) - float(want)) < 2.0 ** -20 * 20
+        assert bool(torch.isfinite(d).all()) and not bool(d[2:4].any()) and bool(d[1].any()) == (coef > 0)
+    # with an advantage it is what it is
+    assert float(policy_gradient_loss(x, tokens.to(device), torch.ones(5, device=device))) == math.inf
 
 
 def test_eight_bit_models_of_both_families():
