@@ -10,7 +10,7 @@ tensors of its own steps them all in one launch::
 8-bit moments take 2.03 bytes an element in place of 8.  A block of 256 elements keeps its largest magnitude as an fp32 scale;
 an element is an 8-bit number relative to it with three bits of mantissa (the first moment 16 binades and a sign, the
 second 32 binades), rounded up or down at random in proportion to the distance.  The random bits depend on the step, the
-tensor's place in the list and the element alone: a step from the same state gives the same bits.
+tensor's place in the list (counted from the state's ``first``) and the element alone: a step from the same state gives the same bits.
 """
 from __future__ import annotations
 
@@ -74,16 +74,19 @@ class AdamWState:
     Everything is flat: parameter ``i`` owns the elements ``[offsets[i], offsets[i] + numel)`` of ``m`` and ``v`` (fp32, or
     uint8 codes with the scales ``m_scale`` and ``v_scale`` of their blocks of 256) and, where a parameter is bf16, of the
     fp32 ``master``, from which its update starts.  Tensors begin at whole blocks; what is between them stays zero.  With 8 bits, a
-    moment that is infinite or NaN makes its block NaN.
+    moment that is infinite or NaN makes its block NaN.  ``first`` is the place of the first parameter among those of other states of
+    the same model, which would otherwise round with the same random bits.
     """
 
-    def __init__(self, params: Sequence[Tensor], *, bits: int = 32) -> None:
+    def __init__(self, params: Sequence[Tensor], *, bits: int = 32, first: int = 0) -> None:
         params = list(params)
         if bits not in (8, 32):
             raise ValueError(f"AdamWState: bits must be 8 or 32, got {bits}")
         if not params:
             raise ValueError("AdamWState: no parameters")
-        self.bits, self.device = bits, params[0].device
+        if not 0 <= first < 1 << 32:
+            raise ValueError(f"AdamWState: first must be 0 to 2^32 - 1, got {first}")
+        self.bits, self.first, self.device = bits, first, params[0].device
         self.shapes = [tuple(p.shape) for p in params]
         self.dtypes = [p.dtype for p in params]
         self.offsets, at = [], 0
@@ -202,7 +205,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], stat
             raise ValueError(f"adamw_step: the state is on {state.device}, a parameter on {params[0].device}")
         # the library checks every tensor before it launches anything
         native.lib().adamw.default(params, grads, state.m, state.v, state.m_scale, state.v_scale, state.master, state._table,
-                                   lr, b1, b2, eps, weight_decay, grad_scale)
+                                   state.first, lr, b1, b2, eps, weight_decay, grad_scale)
     else:
         if len(params) != len(state.shapes) or len(grads) != len(params):
             raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients, a state of {len(state.shapes)}")
@@ -245,7 +248,7 @@ def _step_ref(state: AdamWState, i: int, p: Tensor, grad: Tensor, step: int, lr:
     if p.dtype == torch.bfloat16:
         p.detach().view(-1).copy_(w)
     if state.bits == 8:
-        rm, rv = _random16(step, i, whole, p.device)
+        rm, rv = _random16(step, state.first + i, whole, p.device)
         state.m[part], state.m_scale[blocks] = _encode(m, rm, True)
         state.v[part], state.v_scale[blocks] = _encode(v, rv, False)
     else:

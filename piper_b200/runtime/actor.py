@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import os
 import time
+import zlib
 from dataclasses import dataclass, field
 from typing import Any, Callable, Optional
 
@@ -218,7 +219,8 @@ class PiperActor:
                 mode = "local"          # experts are partitioned, not replicated: no data-parallel sync
             dtype = slots[0].dtype
             storage = ParamStorage(key, slots, self.device, dtype, mode, self.layout.dp_rank, self.layout.dp_degree,
-                                   self.groups.dp_group if self.groups else None, self.adam, self.seed)
+                                   self.groups.dp_group if self.groups else None, self.adam, self.seed,
+                                   ordinal=zlib.crc32(key.encode()))
             if ep and ep_degree > 1 and ep.get("groups") and len(ep["groups"]) > 1 and self.groups is not None:
                 # the same expert shard lives in every expert-parallel group: sum its gradients over those replicas
                 storage.replica_group = self.groups.expert_replica_group

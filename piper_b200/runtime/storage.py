@@ -96,10 +96,11 @@ def _forget_sinks(sinks: dict) -> None:
 
 
 class ParamStorage:
-    """Flat buffers of one bucket plus its (possibly sharded) Adam state."""
+    """Flat buffers of one bucket plus its (possibly sharded) Adam state.  ``ordinal`` tells the buckets of a model apart where 8-bit
+    moments are rounded."""
 
     def __init__(self, key: str, slots: list[ParamSlot], device: torch.device, dtype: torch.dtype, mode: str,
-                 dp_rank: int, dp_degree: int, dp_group, adam: AdamConfig, seed: int = 0) -> None:
+                 dp_rank: int, dp_degree: int, dp_group, adam: AdamConfig, seed: int = 0, ordinal: int = 0) -> None:
         self.key = key
         self.slots = [s for s in slots if s.requires_grad]
         self.device = device
@@ -145,7 +146,9 @@ class ParamStorage:
             full[s.offset:s.offset + s.numel].copy_(self._init_slot(s, seed).reshape(-1))
         lo, hi = self.owned_range()
         if adam.state_bits == 8:
-            self.state8 = AdamWState([full[lo:hi]], bits=8)
+            # other random bits for other buckets and for other shards of one; the same for replicas, which have to agree
+            shard = self.dp_rank if self.sharded_state else max((s.ep_index for s in self.slots if s.ep_sharded), default=0)
+            self.state8 = AdamWState([full[lo:hi]], bits=8, first=(ordinal + shard) & 0xFFFFFFFF)
             self.master = self.state8.master[:hi - lo] if dtype != torch.float32 else None
             self.m = self.v = None
         else:

@@ -397,6 +397,65 @@ def test_bucket_with_eight_bit_moments(dtype):
     assert torch.equal(st.moments()[0], m) and torch.equal(st.moments()[1], v)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_the_random_bits_of_a_state_that_continues_a_list(device):
+    params, grads = _tensors(torch.float32, torch.float32, device, shapes=[(1000,)] * 4)
+    params, grads = [params[0].clone() for _ in params], [grads[0]] * 4
+    state = ops.AdamWState(params, bits=8)
+    halves = [ops.AdamWState(params[:2], bits=8), ops.AdamWState(params[2:], bits=8, first=2)]
+    for _ in range(2):
+        copies = [p.clone() for p in params]
+        ops.adamw_step(params, grads, state, **HYPER)
+        for part, h in zip((slice(0, 2), slice(2, 4)), halves):
+            ops.adamw_step(copies[part], grads[part], h, **HYPER)
+        assert torch.equal(torch.cat([h.m for h in halves]), state.m) and torch.equal(torch.cat([h.v for h in halves]), state.v)
+    codes = state.v.view(4, -1)
+    assert all(not torch.equal(codes[i], codes[j]) for i in range(4) for j in range(i))
+    last = ops.AdamWState(params[:1], bits=8, first=2 ** 32 - 1)
+    ops.adamw_step(params[:1], grads[:1], last, **HYPER)
+    for bad in (-1, 2 ** 32):
+        with pytest.raises(ValueError):
+            ops.AdamWState(params[:1], bits=8, first=bad)
+
+
+def test_buckets_and_shards_round_by_bits_of_their_own():
+    """Equal gradients of equal weights: buckets of other ordinals and shards of one bucket draw other bits, replicas the same."""
+    from piper_b200.runtime.storage import AdamConfig, ParamSlot, ParamStorage
+    cfg = AdamConfig(lr=1e-2, decoupled=True, state_bits=8)
+
+    def codes(mode, rank, ordinal, ep=None):
+        slot = ParamSlot(0, "a.gain", (4096,), torch.float32, True)
+        if ep is not None:
+            slot.ep_sharded, slot.full_shape, slot.ep_index, slot.ep_degree = True, (8192,), ep, 2
+        st = ParamStorage("k", [slot], torch.device("cpu"), torch.float32, mode, rank, 2, None, cfg, ordinal=ordinal)
+        st.step_count = 1
+        n = st.state8.numel
+        ops.adamw_step([torch.ones(n)], [torch.linspace(0.1, 1.0, 256).repeat(n // 256)], st.state8)
+        return st.state8.m[:2048]
+
+    one = codes("allreduce", 0, 7)
+    assert torch.equal(one, codes("allreduce", 1, 7)) and not torch.equal(one, codes("allreduce", 0, 8))
+    assert not torch.equal(codes("zero2", 0, 7), codes("zero2", 1, 7))
+    assert torch.equal(codes("local", 0, 7, ep=1), codes("local", 1, 7, ep=1))
+    assert not torch.equal(codes("local", 0, 7, ep=0), codes("local", 1, 7, ep=1))
+
+
+def test_buckets_of_a_setup_have_ordinals():
+    from piper_b200 import piper_setup
+    from piper_b200.models.llama3 import LLAMA_CONFIGS, Transformer
+    cfg = LLAMA_CONFIGS["tiny"]
+    tok = torch.zeros(2, 64, dtype=torch.int64)
+    schedule = [{"op": "place", "filter": {"PP": i}, "devices": [0]} for i in range(2)] + \
+        [{"op": "split", "filter": {}, "dim_name": "MB", "num_microbatches": 2}]
+    firsts = []
+    for _ in range(2):
+        actor = piper_setup(Transformer, (cfg, 64, 2), optim_fn=torch.optim.AdamW, optim_kwargs={"state_bits": 8}, example_inputs=[tok],
+                            example_outputs=tok, model_dtype=torch.float32, const_attrs=Transformer.const_attrs(cfg, 64),
+                            schedule_directives=schedule, device="cpu")
+        firsts.append({k: b.storage.state8.first for k, b in actor.buckets.items() if b.storage is not None and b.storage.numel})
+    assert firsts[0] == firsts[1] and len(firsts[0]) == 2 and len(set(firsts[0].values())) == 2
+
+
 def test_state_bits_of_a_setup():
     from piper_b200.engine import _adam_config
     assert _adam_config(torch.optim.AdamW, {"state_bits": 8}).state_bits == 8
