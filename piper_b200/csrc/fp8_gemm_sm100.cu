@@ -31,6 +31,8 @@
 #include <atomic>
 #include <cstddef>
 #include <cstdlib>
+#include <mutex>
+#include <unordered_map>
 
 #include "gemm_sm100.h"
 #include "ptx.cuh"
@@ -79,12 +81,12 @@ struct Params {
   int stages;
   int band;
   int* status;
-  int slot;           // counter of the launch, or -1: tiles in a fixed order
+  int slot;           // counter of the stream, or -1: tiles in a fixed order
 };
 
-// Counters of tiles, one per launch in rotation; the launch 4,096 before, whose last draw rearms the counter, has to have ended on its
-// stream by then.  They are the module's own, so every device has its zeros without an allocation.
-constexpr unsigned SCHED_SLOTS = 4096;
+// Counters of tiles, one per stream: a launch draws behind its wait for the kernel before it, whose last draw has rearmed the counter.
+// They are the module's own, so every device has its zeros without an allocation.
+constexpr unsigned SCHED_SLOTS = 1024;
 __device__ int sched_slots[SCHED_SLOTS];
 
 // D[tmem] (+)= (A * scales) * (B * scales), e4m3 inputs.
@@ -476,17 +478,27 @@ double cost(int M, int N, int K, bool f32, int ctas, int width, int num_sms) {
   return rounds * std::max(k_blocks * block, epilogue) + epilogue + (ctas == 2 ? 3600 : 2000);
 }
 
-// A counter for a launch on `stream`.  None while it is captured: the graph would keep it, and count in it beside another graph's or a
-// later launch's CTAs when it is replayed.
+// The counter of `stream`.  In rotation over the launches, two of them that run at once on two streams could have the same one, however
+// many there are, when one has waited long enough; then tiles would be left out.  None while the stream is captured: the graph
+// would keep it, and count in it beside later launches' CTAs when it is replayed on another stream.  None for the handle behind which
+// every thread has another stream, and none for streams beyond the last counter.
 int sched_slot(cudaStream_t stream) {
   static const bool fixed = [] {
     const char* env = getenv("PIPER_GEMM_STATIC_TILES");
     return env != nullptr && env[0] == '1';
   }();
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (fixed || cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) return -1;
-  static std::atomic<unsigned> launches{0};
-  return static_cast<int>(launches++ % SCHED_SLOTS);
+  unsigned long long id = 0;
+  if (fixed || stream == cudaStreamPerThread || cudaStreamIsCapturing(stream, &capture) != cudaSuccess ||
+      capture != cudaStreamCaptureStatusNone || cudaStreamGetId(stream, &id) != cudaSuccess)
+    return -1;
+  static std::mutex mutex;
+  static std::unordered_map<unsigned long long, int> slots;      // by the stream's id, which no later stream has again
+  const std::lock_guard<std::mutex> lock(mutex);
+  const auto known = slots.find(id);
+  if (known != slots.end()) return known->second;
+  if (slots.size() >= SCHED_SLOTS) return -1;
+  return slots.emplace(id, static_cast<int>(slots.size())).first->second;
 }
 
 GemmShape shape_of(int M, int N, int K, bool f32, int num_sms) {

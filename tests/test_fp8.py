@@ -311,6 +311,31 @@ def test_captured_products_share_no_counters():
 
 
 @pytest.mark.gpu
+def test_a_product_that_waited_while_thousands_ran_on_another_stream():
+    """Streams count their tiles by themselves: a product that was launched long before the others and runs beside them has all its tiles,
+    and so have those on the default stream and on more streams than one."""
+    a, b = (ops.fp8_quantize(_matrix(r, 128, "cuda", r)) for r in (4096, 2048))
+    want = ops.fp8_matmul(a, b)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    held = torch.cuda.Event()
+    with torch.cuda.stream(streams[0]):
+        torch.cuda._sleep(100_000_000)                     # some 50 ms
+        held.record()
+    waiting = []
+    for s in streams[:2]:
+        with torch.cuda.stream(s):
+            s.wait_event(held)
+            waiting.append(ops.fp8_matmul(a, b))
+    with torch.cuda.stream(streams[2]):
+        last = [ops.fp8_matmul(a, b) for _ in range(4200)][-50:]
+    last += [ops.fp8_matmul(a, b) for _ in range(10)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, want) for t in waiting + last)
+    ops.native.check_status()
+
+
+@pytest.mark.gpu
 def test_same_bits_on_streams_and_in_a_captured_graph():
     x = _matrix(700, 1024, "cuda", 1).requires_grad_(True)
     w = _matrix(1376, 1024, "cuda", 2, std=0.03).requires_grad_(True)
