@@ -13,14 +13,14 @@ parameter would stay gathered.  A group with a NaN or an infinity is NaN.
 """
 from __future__ import annotations
 
-from typing import Union
+from typing import Optional, Union
 
 import torch
 from torch import Tensor
 
 from . import native
-from .core import HostContext, grad_sinks, wgrad_store
-from .registry import custom_op, host_op
+from .core import grad_sinks, wgrad_store
+from .registry import custom_op, host_op, once_differentiable
 
 GROUP = 128
 _NAN_SCALE = 255
@@ -200,7 +200,8 @@ def _(x, w):
 def _linear_forward(ctx, x, w):
     y, xt = fp8_linear_keep(x, w) if w.requires_grad else (fp8_linear_op(x, w), None)
     ctx.rows = x.shape[0]
-    ctx.save_for_backward(w, xt)
+    # x only to be found by gradients of the gradients, which raise; on a GPU it would keep what xt is there to save
+    ctx.save_for_backward(w, xt, None if x.is_cuda else x)
     return y
 
 
@@ -219,10 +220,8 @@ def _fp8_wgrad(dyt: Tensor, xt: Tensor, w: Tensor, T: int):
     return None
 
 
-def _linear_backward(ctx, dy):
-    w, xt = ctx.saved_tensors
-    need_x, need_w = ctx.needs_input_grad[:2]
-    T, (N, K) = ctx.rows, w.shape
+def _linear_backward(dy: Tensor, w: Tensor, xt: Optional[Tensor], T: int, need_x: bool, need_w: bool):
+    N, K = w.shape
     dyp, dyt = _quantize(dy, False, need_x, need_w)
     dx = dw = None
     if need_x:
@@ -236,13 +235,17 @@ def _linear_backward(ctx, dy):
     return dx, dw
 
 
-fp8_linear_op.register_autograd(_linear_backward, forward=_linear_forward)
+def _linear_formula(ctx, dy):
+    w, xt, x = ctx.saved_tensors
+    grads = _linear_backward(dy, w, xt, ctx.rows, *ctx.needs_input_grad[:2])
+    return tuple(once_differentiable("fp8_linear", g, dy, w, *([] if x is None else [x])) for g in grads)
+
+
+fp8_linear_op.register_autograd(_linear_formula, forward=_linear_forward)
 
 
 def _linear_backward_host(dy: Tensor, w: Tensor, xt: Tensor, T: int, need_x: bool, need_w: bool) -> tuple[Tensor, Tensor]:
-    ctx = HostContext((w, xt), (need_x, need_w))
-    ctx.rows = T
-    dx, dw = _linear_backward(ctx, dy)
+    dx, dw = _linear_backward(dy, w, xt, T, need_x, need_w)
     none = torch.empty(0)
     return none if dx is None else dx, none if dw is None else dw
 
@@ -271,7 +274,7 @@ def fp8_linear(x: Tensor, w: Union[Tensor, Fp8Matrix]) -> Tensor:
     """y[..., N] = x[..., K] @ w[N, K]^T with both operands rounded to e4m3; so are those of its gradients' products.
 
     ``w`` may be a weight that was rounded before (``fp8_quantize(w, square=True)``), for calls without gradients.  K and N are
-    multiples of 16; there may be any number of rows.
+    multiples of 16; there may be any number of rows.  Gradients of the gradients raise.
     """
     kept = isinstance(w, Fp8Matrix)
     if x.is_cuda and x.dim() == 2 and not kept:

@@ -13,7 +13,7 @@ import torch
 from torch import Tensor
 
 from . import native
-from .registry import custom_op
+from .registry import custom_op, once_differentiable
 
 MAX_TOP = 32
 MAX_VOCAB = 1 << 30
@@ -100,7 +100,7 @@ def _backward(ctx, d_logprob, d_entropy, d_top, _d_id, _d_stats):
         d = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
         native.lib().logprobs_bwd(lg, tokens.contiguous(), stats, entropy, top_id, dense(d_logprob), dense(d_entropy), dense(d_top),
                                   d, temperature, ignore_index)
-        return d, None, None, None, None
+        return once_differentiable("token_logprobs on a GPU", d, logits), None, None, None, None
     logp, p, h, _largest, log_s = _stats_ref(logits, temperature)
     up = torch.zeros_like(p)                         # gradient with respect to log p
     if d_logprob is not None:
@@ -136,7 +136,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top: int = 0, temperature:
     differentiable with respect to the logits (the ids are taken as given).  A token that is ``ignore_index`` or no id
     of the vocabulary has log probability 0 and no gradient through it.  Masked ids (-inf) have probability 0; a row that
     has nothing else has entropy 0, log probabilities of -inf and no gradient.  A row with a NaN or +inf is NaN; its ids
-    are some of the vocabulary's.  A row whose outputs get no gradient but zeros gives none, whatever its logits are.
+    are some of the vocabulary's.  A row whose outputs get no gradient but zeros gives none, whatever its logits are.  Gradients
+    of the gradient exist on the CPU only; on a GPU they raise.
     """
     if logits.is_cuda and logits.dim() == 2:         # the op makes the checks below by itself
         return TokenLogprobs(*token_logprobs_fwd(logits, tokens, top, temperature, ignore_index)[:4])

@@ -54,6 +54,25 @@ def _install_native(lib) -> None:
 native.install["registry"] = _install_native
 
 
+class _NoDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, grad, *inputs):
+        ctx.what = what
+        return grad.detach()
+
+    @staticmethod
+    def backward(ctx, _grad):
+        raise RuntimeError(f"{ctx.what}: its gradient has no derivative")
+
+
+def once_differentiable(what: str, grad: Optional[torch.Tensor], *inputs: torch.Tensor) -> Optional[torch.Tensor]:
+    """A gradient without a graph that raises where a second derivative, on its way to one of the ``inputs``, would silently
+    leave it out (under create_graph)."""
+    if grad is None or not torch.is_grad_enabled():
+        return grad
+    return _NoDerivative.apply(what, grad, *inputs)
+
+
 class Op:
     """What ``custom_op`` returns.  The registration methods of ``torch.library.custom_op`` objects are also attributes of
     ``overload``, the callable that the op modules export."""

@@ -413,3 +413,18 @@ def test_one_weight_in_two_calls_of_a_pass_and_two_buckets():
     parts = [_rounded(d.t()) @ _rounded(x.t()).t() for d, x in ((da, a), (db, b))]
     size = sum(_rounded(d.t()).abs() @ _rounded(x.t()).t().abs() for d, x in ((da, a), (db, b)))
     assert bool(((sink.double().cpu() - sum(parts)).abs() <= 10 * 2.0 ** -22 * size).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_of_the_gradients_raise(device):
+    """Rounded operands have none; left out silently, a penalty on gradients would train nothing."""
+    x, w = _matrix(40, 64, device, 1).requires_grad_(True), _matrix(32, 64, device, 2, std=0.1).requires_grad_(True)
+    dy = _matrix(40, 32, device, 3)
+    want = torch.autograd.grad(ops.fp8_linear(x, w), [x, w], dy)
+    got = torch.autograd.grad(ops.fp8_linear(x, w), [x, w], dy, create_graph=True)
+    assert all(torch.equal(a.detach(), b) and a.requires_grad and not b.requires_grad for a, b in zip(got, want))
+    for g in got:
+        with pytest.raises(RuntimeError, match="no derivative"):
+            torch.autograd.grad(g.float().square().sum() + x.float().sum() + w.float().sum(), [x, w])
+    only = torch.autograd.grad(ops.fp8_linear(x.detach(), w), w, dy, create_graph=True)[0]
+    assert torch.equal(only.detach(), want[1])

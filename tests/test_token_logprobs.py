@@ -504,3 +504,34 @@ def test_traced_programs_record_one_op():
         (d,) = torch.autograd.grad(compiled(x), x)
         assert torch.allclose(d, want)
     torch.library.opcheck(torch.ops.piper.token_logprobs_fwd.default, (x, tokens, 2, 1.0, -100))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_of_the_gradient(device):
+    """On the CPU those of the plain formula; kernels' gradients have none, and say so in place of being left out."""
+    x, tokens = _logits(5, 40, torch.float32, device, 9, std=1.0)
+    x.requires_grad_(True)
+    g = torch.Generator().manual_seed(2)
+    up, v = torch.randn(5, generator=g).to(device), torch.randn(5, 40, generator=g).to(device)
+
+    def first(create):
+        out = ops.token_logprobs(x, tokens, top=3, temperature=0.7)
+        loss = (out.logprob * up).sum() + out.entropy.square().sum() + 0.3 * out.top_logprob.sum()
+        return torch.autograd.grad(loss, x, create_graph=create)[0]
+
+    d = first(True)
+    assert torch.equal(d.detach(), first(False)) and not first(False).requires_grad
+    if device == "cuda":
+        with pytest.raises(RuntimeError, match="no derivative"):
+            torch.autograd.grad((d * v).sum() + x.sum(), x)
+        return
+    (got,) = torch.autograd.grad((d * v).sum(), x)
+    y = x.detach().double().requires_grad_(True)
+    logp = torch.log_softmax(y / 0.7, -1)
+    entropy = -(logp.exp() * logp).sum(-1)
+    ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :3]
+    loss = (logp.gather(1, tokens.unsqueeze(1)).squeeze(1) * up).sum() + entropy.square().sum() + 0.3 * logp.gather(1, ids).sum()
+    (d,) = torch.autograd.grad(loss, y, create_graph=True)
+    (want,) = torch.autograd.grad((d * v.double()).sum(), y)
+    # some 40 operations on numbers of at most 100 times the result's size
+    assert float((got - want).abs().max()) <= 4000 * 2.0 ** -24 * float(want.abs().max())
