@@ -248,7 +248,10 @@ def piper_setup(model_class, model_args=(), model_kwargs: Optional[dict] = None,
 
 def piper_exec_dag(loss_fn: Callable, log_stats: bool = False, step_timeout: Optional[float] = None,
                    inputs: Optional[list] = None, labels=None) -> list:
-    """Run one training step; returns this rank's per-microbatch losses (empty off the loss stage)."""
+    """Run one training step; returns this rank's per-microbatch losses (empty off the loss stage).
+
+    ``loss_fn(output, labels)`` gets each microbatch's rows of ``labels``, a tensor or a tuple, list or dictionary of tensors
+    (``lambda out, y: policy_gradient_loss(out, *y)`` with tokens and advantages)."""
     actors = piper_metadata.actors
     if not actors:
         raise RuntimeError("piper_exec_dag called before piper_setup")

@@ -263,7 +263,8 @@ class PiperActor:
         self.inputs = [t.to(self.device, non_blocking=True) if isinstance(t, torch.Tensor) else t for t in inputs]
 
     def load_labels(self, labels) -> None:
-        self.labels = labels.to(self.device, non_blocking=True) if isinstance(labels, torch.Tensor) else labels
+        """A tensor, or a tuple, list or dictionary of what the loss takes beside the output (tokens and their advantages)."""
+        self.labels = _map_tensors(lambda t: t.to(self.device, non_blocking=True), labels)
 
     def has_first_stage(self) -> bool:
         """True when some forward node takes the model inputs (no upstream segment, receive or exchange)."""
@@ -376,6 +377,18 @@ class PiperActor:
         return out
 
 
+def _map_tensors(f: Callable, x):
+    """``x`` with ``f`` of every tensor in it, down tuples, lists and dictionaries."""
+    if isinstance(x, torch.Tensor):
+        return f(x)
+    if isinstance(x, dict):
+        return {k: _map_tensors(f, v) for k, v in x.items()}
+    if isinstance(x, (tuple, list)):
+        items = [_map_tensors(f, v) for v in x]
+        return type(x)(*items) if hasattr(x, "_fields") else type(x)(items)
+    return x
+
+
 def _node_label(node: TrainingDAGNode) -> str:
     tags = ",".join(f"{k}={v}" for k, v in sorted(node.tag.items(), key=lambda kv: kv[0]) if v is not None)
     return f"{node.node_kind}:{tags}:uid{node.uid}"
@@ -450,6 +463,14 @@ class DagExecutor:
             per = t.shape[0] // n
             return t[mb * per:(mb + 1) * per]
         return t
+
+    def _microbatch_labels(self, labels, mb: int):
+        """Of several tensors those with as many rows as the first one are cut; others (a weight per class) are every microbatch's."""
+        if isinstance(labels, torch.Tensor):
+            return self._microbatch(labels, mb)
+        rows: list = []
+        _map_tensors(lambda t: rows.extend(t.shape[:1]), labels)
+        return _map_tensors(lambda t: self._microbatch(t, mb) if t.dim() and t.shape[0] == rows[0] else t, labels)
 
     def _stream(self, node: TrainingDAGNode):
         """CUDA stream a node runs on.  Pipeline messages get one stream per channel, so a send that waits for
@@ -825,7 +846,7 @@ class DagExecutor:
         join_scope.__enter__()
         try:
             if node.node_meta.get("compute_loss"):
-                labels = self._microbatch(a.labels, self._mb(node))
+                labels = self._microbatch_labels(a.labels, self._mb(node))
                 loss = loss_fn(outs[0], labels)
                 self.losses.append(loss.detach())
                 loss.backward()

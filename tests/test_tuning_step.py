@@ -93,6 +93,60 @@ def test_a_step_through_the_engine(device, tmp_path):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("form", ["tuple", "dict"])
+def test_advantages_through_the_engine(form, device):
+    """What the loss takes beside the output comes in several tensors: each microbatch has its rows of tokens and advantages, and all of a
+    tensor that has another number of rows."""
+    from piper_b200 import piper_exec_dag, piper_setup
+    from piper_b200.models.llama3 import LlamaConfig, Transformer
+    from piper_b200.nn import policy_gradient_loss
+    from piper_b200.runtime.storage import init_tensor
+
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    cfg = LlamaConfig(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=512, ffn_hidden=688, norm_eps=1e-6,
+                      rope_theta=10000.0, max_seq_len=128)
+    g = torch.Generator().manual_seed(4)
+    x, y = (torch.randint(0, cfg.vocab_size, (4, 128), generator=g) for _ in range(2))
+    adv, scale = torch.randn(4, 128, generator=g), torch.tensor([0.5, 2.0, 1.0])
+    y[:, :9] = -100
+
+    def loss_fn(out, labels):
+        tokens, a, s = labels.values() if isinstance(labels, dict) else labels
+        assert tokens.shape == a.shape == (2, 128) and s.shape == (3,) and a.device == s.device == out.device
+        return policy_gradient_loss(out, tokens, a * s[0], entropy_coef=0.01)
+
+    def pack(t, a):
+        return {"tokens": t, "advantages": a, "scale": scale} if form == "dict" else (t, a, scale)
+
+    actor = piper_setup(Transformer, (cfg, 128, 2), optim_fn=torch.optim.AdamW, optim_kwargs={"lr": 0.0, "state_bits": 8},
+                        example_inputs=[x], example_outputs=pack(y, adv), model_dtype=dtype,
+                        const_attrs=Transformer.const_attrs(cfg, 128), schedule_directives=_schedule(2), device=device)
+    actor.debug_keep_grads = True
+    model = Transformer(cfg, 128, 2).to(device).to(dtype)
+    consts = Transformer.const_attrs(cfg, 128, device)
+    model.rope_cos, model.rope_sin = consts["rope_cos"], consts["rope_sin"]
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            p.copy_(init_tensor(n, p.shape, dtype, torch.device(device)))
+    for labels in (None, pack(y.flip(0), -adv)):            # those of the setup, then those of the call
+        losses = [float(v) for v in piper_exec_dag(loss_fn, labels=labels)]
+        want = []
+        for p in model.parameters():
+            p.grad = None
+        t, a = (y, adv) if labels is None else (y.flip(0), -adv)
+        for xs, ts, s in zip(*(v.to(device).split(2) for v in (x, t, a))):
+            loss = policy_gradient_loss(model(xs), ts, s * 0.5, entropy_coef=0.01)
+            want.append(float(loss.detach()))
+            loss.backward()
+        half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -20
+        # the same ops on the same rows; losses are sums of some 250 terms of the size of a log probability, 6
+        assert len(losses) == 2 and all(abs(p - q) <= 2.0 ** -20 * 6 for p, q in zip(losses, want)), (losses, want)
+        for n, p in model.named_parameters():
+            got = actor.last_grads[n].float()
+            assert float((got - p.grad.float() / 2).norm()) <= 3 * half * float(p.grad.float().norm()) + 1e-8, n
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_policy_gradient_loss(device):
     from piper_b200.nn import cross_entropy_loss, policy_gradient_loss
     g = torch.Generator().manual_seed(1)
