@@ -199,11 +199,9 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], stat
     if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1):
         raise ValueError(f"adamw_step: lr={lr}, betas={betas}, eps={eps}, weight_decay={weight_decay}")
     if state.device.type == "cuda":
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("adamw_step: the step count lives on the host; a captured step would repeat itself")
         if params and params[0].device != state.device:
             raise ValueError(f"adamw_step: the state is on {state.device}, a parameter on {params[0].device}")
-        # the library checks every tensor before it launches anything
+        # the library checks every tensor, and that its stream is not captured, before it launches anything
         native.lib().adamw.default(params, grads, state.m, state.v, state.m_scale, state.v_scale, state.master, state._table,
                                    state.first, lr, b1, b2, eps, weight_decay, grad_scale)
     else:

@@ -361,6 +361,30 @@ def test_a_step_is_not_captured():
 
 
 @pytest.mark.gpu
+def test_a_captured_step_is_refused_by_the_library():
+    """It asks the stream of the parameters' device, whichever device is current where the step is called; also beside a capture that is
+    another stream's alone."""
+    p, g = [torch.zeros(256, device="cuda")], [torch.ones(256, device="cuda")]
+    state = ops.AdamWState(p, bits=8)
+    args = (p, g, state.m, state.v, state.m_scale, state.v_scale, state.master, state._table, 0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        graph.capture_begin(capture_error_mode="thread_local")
+        kept = torch.zeros(8, device="cuda")
+        try:
+            with pytest.raises(RuntimeError, match="captured"):
+                ops.native.lib().adamw(*args)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                ops.adamw_step(p, g, state)
+        finally:
+            graph.capture_end()
+    torch.cuda.synchronize()
+    assert state.steps == [1] and bool((p[0] < 0).all()) and kept.numel() == 8
+
+
+@pytest.mark.gpu
 def test_states_on_two_streams():
     results = []
     sets = [_tensors(torch.bfloat16, torch.float32, "cuda", seed=i) for i in range(2)]
