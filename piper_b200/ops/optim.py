@@ -23,6 +23,7 @@ from torch import Tensor
 from . import native
 
 BLOCK = 256
+_PIECE = BLOCK << 14               # elements of a state that are encoded or decoded at a time
 _M_BASE, _V_BASE = 889, 761        # fp32 bits >> 20 of code 0; those of 1.0 are 1016, codes 127 and 255
 
 
@@ -142,18 +143,24 @@ class AdamWState:
         return out[0], out[1]
 
     def set_moments(self, m: Tensor, v: Tensor) -> None:
-        """The reverse of ``moments()``; 8-bit codes are the nearest ones, so what came out of it goes back unchanged."""
+        """The reverse of ``moments()``; 8-bit codes are the nearest ones, so what came out of it goes back unchanged.  What is
+        missing at the end counts as zeros."""
+        if m.dim() != 1 or m.shape != v.shape or m.numel() > self.numel:
+            raise ValueError(f"AdamWState: moments are two tensors of at most {self.numel} elements, got {tuple(m.shape)} and {tuple(v.shape)}")
         with torch.no_grad():
             if self.bits == 32:
-                self.m.copy_(m)
-                self.v.copy_(v)
+                for x, own in ((m, self.m), (v, self.v)):
+                    own[:x.numel()] = x
+                    own[x.numel():] = 0
                 return
-            half = torch.full((self.numel,), 1 << 15, dtype=torch.int64, device=self.device)
+            # in pieces: encoding takes some fifty bytes an element, many times what the state holds
+            half = torch.full((min(self.numel, _PIECE),), 1 << 15, dtype=torch.int64, device=self.device)
             for x, codes, scale, signed in ((m, self.m, self.m_scale, True), (v, self.v, self.v_scale, False)):
-                x = x.to(device=self.device, dtype=torch.float32).contiguous()
-                c, s = _encode(x, half, signed)
-                codes.copy_(c)
-                scale.copy_(s)
+                for a in range(0, self.numel, _PIECE):
+                    z = min(a + _PIECE, self.numel)
+                    part = torch.zeros(z - a, dtype=torch.float32, device=self.device)
+                    part[:max(min(x.numel(), z) - a, 0)] = x[a:z]
+                    codes[a:z], scale[a // BLOCK:z // BLOCK] = _encode(part, half[:z - a], signed)
 
     def state_dict(self) -> dict:
         return {"bits": self.bits, "shapes": list(self.shapes), "dtypes": list(self.dtypes), "steps": list(self.steps),
@@ -177,10 +184,13 @@ class AdamWState:
                     if getattr(self, name) is not None:
                         getattr(self, name).copy_(state[name])
             else:
-                m, v = (state[n].to(self.device) for n in ("m", "v"))
-                if state["bits"] == 8:
-                    m, v = (_decode(c, state[s].to(self.device), sg) for c, s, sg in ((m, "m_scale", True), (v, "v_scale", False)))
-                self.set_moments(m, v)
+                if state["bits"] == 32:
+                    self.set_moments(state["m"], state["v"])
+                for name, signed in (("m", True), ("v", False)) if state["bits"] == 8 else ():
+                    for a in range(0, self.numel, _PIECE):
+                        z = min(a + _PIECE, self.numel)
+                        getattr(self, name)[a:z] = _decode(state[name][a:z].to(self.device),
+                                                           state[name + "_scale"][a // BLOCK:z // BLOCK].to(self.device), signed)
             if self.master is not None:
                 self.master.copy_(state["master"])
         self._table[2] = torch.tensor([int(s) for s in state["steps"]], dtype=torch.int64)

@@ -418,8 +418,7 @@ class ParamStorage:
             self.m.copy_(m)
             self.v.copy_(v)
             return
-        tail = self.state8.numel - m.numel()
-        self.state8.set_moments(*(torch.nn.functional.pad(t, (0, tail)) for t in (m, v)))
+        self.state8.set_moments(m, v)
 
     def snapshot_grads(self, scale: float) -> dict:
         """fqn -> scaled copy of the gradient this rank holds (full tensors, or its ZeRO shard as a flat range)."""

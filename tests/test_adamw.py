@@ -243,6 +243,57 @@ def test_states_are_saved_and_loaded(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_moments_are_set_in_pieces(device, monkeypatch):
+    """Pieces that end anywhere among the blocks give what one piece gives, short moments have zeros behind them."""
+    from piper_b200.ops import optim
+    params = [torch.zeros(n, device=device) for n in (1000, 5000, 3)]
+    g = torch.Generator().manual_seed(1)
+    states = []
+    for piece in (1 << 20, 5 * BLOCK, BLOCK):
+        monkeypatch.setattr(optim, "_PIECE", piece)
+        state = ops.AdamWState(params, bits=8)
+        g.manual_seed(1)
+        m, v = (torch.randn(state.numel, generator=g).to(device) for _ in range(2))
+        m, v = m * (torch.arange(state.numel, device=device) < 700), v.abs()
+        state.set_moments(m, v)
+        wide = ops.AdamWState(params, bits=32)
+        wide.load_state_dict(state.state_dict())
+        assert all(torch.equal(a, b) for a, b in zip(wide.moments(), state.moments()))
+        narrow = ops.AdamWState(params, bits=8)
+        narrow.load_state_dict(wide.state_dict())
+        assert torch.equal(narrow.m, state.m) and torch.equal(narrow.v, state.v) and torch.equal(narrow.v_scale, state.v_scale)
+        for bits in (8, 32):
+            short = ops.AdamWState(params, bits=bits)
+            short.set_moments(torch.ones_like(m), torch.ones_like(v))
+            short.set_moments(m[:700], v[:700])
+            a, b = short.moments()
+            assert not a[700:].any() and not b[700:].any() and bool(a[:700].any())
+        states.append(state)
+    for s in states[1:]:
+        assert torch.equal(s.m, states[0].m) and torch.equal(s.v, states[0].v) and torch.equal(s.m_scale, states[0].m_scale)
+    for bad in ((m, v[:5]), (torch.zeros(state.numel + 1),) * 2, (m.view(2, -1), v.view(2, -1))):
+        with pytest.raises(ValueError):
+            state.set_moments(*bad)
+
+
+@pytest.mark.gpu
+def test_setting_moments_takes_little_memory():
+    p = torch.zeros(64 << 20, device="cuda", dtype=torch.bfloat16)
+    state = ops.AdamWState([p], bits=8)
+    m, v = state.moments()
+    m.normal_(), v.uniform_()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    state.set_moments(m, v)
+    # a piece of 4 Mi elements at a time, a hundred bytes for each
+    assert torch.cuda.max_memory_allocated() - before < (4 << 20) * 100
+    a, b = state.moments()
+    assert bool(((a - m).abs() <= m.abs() / 16 + state.m_scale.repeat_interleave(BLOCK) * 2.0 ** -16).all())
+    assert bool(((b - v).abs() <= v / 16 + state.v_scale.repeat_interleave(BLOCK) * 2.0 ** -31).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_a_state_of_other_types_is_refused(device):
     """Same shapes, types in another order: the master copies would be those of other parameters.  A refused state changes nothing."""
     def tensors(*dtypes):
