@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t encode_v(float y, uint32_t r) {
 __device__ __forceinline__ uint32_t encode_small_m(float y, uint32_t r) {
   return __fmul_rn(static_cast<float>(r & 0xFFFFu), __uint_as_float(M_LEAST) * (1.f / 65536)) < y ? 1u << 24 : 0u;
 }
-__device__ __forceinline__ uint32_t encode_small_v(float y) { return y > 0.f ? 1u << 24 : 0u; }
+__device__ __forceinline__ uint32_t encode_small_v(float v) { return v > 0.f ? 1u << 24 : 0u; }
 
 // The top bytes of four words, the first lowest.
 __device__ __forceinline__ uint32_t top_bytes(const uint32_t (&t)[4]) {
@@ -276,7 +276,7 @@ adamw_kernel(const __grid_constant__ AdamwTable table, const AdamwArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               if (__float_as_uint(ym[j]) < M_LEAST) cm[j] = encode_small_m(ym[j], mix32(first + j));
-              if (__float_as_uint(yv[j]) < V_LEAST) cv[j] = encode_small_v(yv[j]);
+              if (__float_as_uint(yv[j]) < V_LEAST) cv[j] = encode_small_v(v[4 * h + j]);      // y may be below all numbers
             }
           }
 #pragma unroll

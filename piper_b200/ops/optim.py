@@ -55,7 +55,7 @@ def _encode(x: Tensor, r: Tensor, signed: bool) -> tuple[Tensor, Tensor]:
     base = _M_BASE if signed else _V_BASE
     least = float(torch.tensor((base + 1) << 20, dtype=torch.int32).view(torch.float32))
     codes = ((y.view(torch.int32) + (r << 4).to(torch.int32)) >> 20) - base
-    small = (r.to(torch.float32) * (least / 65536) < y) if signed else y > 0
+    small = (r.to(torch.float32) * (least / 65536) < y) if signed else x > 0      # y may be below all numbers
     codes = torch.where(y < least, small.to(torch.int32), codes)
     if signed:
         codes = codes + 128 * (x < 0)

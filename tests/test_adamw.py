@@ -178,6 +178,22 @@ def test_vanishing_gradients_beside_any_eps(eps, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("large", [1e-3, 1.0, 1e5, 1e15])
+def test_a_second_moment_above_0_stays_above_0(large, device):
+    """However small beside the largest of its block: also where their quotient is below all numbers."""
+    g = torch.full((2 * BLOCK,), 1.2e-21, device=device)         # v is 1e-45, the smallest number
+    g[7] = large
+    g[BLOCK + 3:BLOCK + 9] = 0.0
+    p = [torch.zeros(2 * BLOCK, device=device)]
+    state, wide = ops.AdamWState(p, bits=8), ops.AdamWState(p, bits=32)
+    ops.adamw_step(p, [g], state)
+    ops.adamw_step(p, [g], wide)
+    assert torch.equal(state.v > 0, wide.v > 0) and int((state.v == 0).sum()) == 6
+    state.set_moments(*wide.moments())
+    assert torch.equal(state.v > 0, wide.v > 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_inference_tensors(device):
     with torch.inference_mode():
         p = [torch.ones(300, device=device)]
