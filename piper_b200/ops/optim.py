@@ -217,14 +217,16 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Optional[Tensor]], stat
     else:
         if len(params) != len(state.shapes) or len(grads) != len(params):
             raise ValueError(f"adamw_step: {len(params)} parameters, {len(grads)} gradients, a state of {len(state.shapes)}")
-        for p, g, size in zip(params, grads, state._table[1].tolist()):
-            if 2 * p.numel() + (p.dtype == torch.bfloat16) != size or p.device != state.device:
-                raise ValueError(f"adamw_step: the state is of a parameter of {size // 2} elements on {state.device}, got "
+        for p, g, size, dtype in zip(params, grads, state._table[1].tolist(), state.dtypes):
+            if p.dtype != dtype or 2 * p.numel() + (p.dtype == torch.bfloat16) != size or p.device != state.device:
+                raise ValueError(f"adamw_step: the state is of a {dtype} parameter of {size // 2} elements on {state.device}, got "
                                  f"{p.dtype} {tuple(p.shape)} on {p.device}")
             if not p.is_contiguous():
                 raise ValueError("adamw_step: parameters must be contiguous")
             if g is not None and (g.shape != p.shape or g.device != p.device):
                 raise ValueError(f"adamw_step: a gradient is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)}")
+            if g is not None and g.dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError(f"adamw_step: gradients are bfloat16 or float32, got {g.dtype}")
         _check_apart(params, "adamw_step")
         with torch.no_grad():
             for i, (p, g, done) in enumerate(zip(params, grads, state.steps)):

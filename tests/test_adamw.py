@@ -377,6 +377,18 @@ def test_refusals(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_other_types_are_refused_on_either_device(device):
+    p = [torch.ones(10, device=device), torch.ones(10, device=device, dtype=torch.bfloat16)]
+    state = ops.AdamWState(p)
+    g = [torch.ones(10, device=device) for _ in p]
+    for params, grads in (([p[0].double(), p[1]], g), ([p[0].half(), p[1]], g), ([p[1], p[0]], g), (p, [g[0].double(), g[1]]),
+                          (p, [g[0], g[1].half()]), (p, [g[0].long(), None])):
+        with pytest.raises(ValueError):
+            ops.adamw_step(params, grads, state)
+    assert state.steps == [0, 0] and bool((p[0] == 1).all()) and bool((p[1] == 1).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("bits", [8, 32])
 def test_parameters_that_share_memory_are_refused(bits, device):
     """Two of them would be stepped by one launch in no order; neighbours, and parameters without elements, are none of those."""
