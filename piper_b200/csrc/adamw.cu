@@ -33,14 +33,6 @@ constexpr int CHUNK = CHUNK_BLOCKS * kMomentBlock;
 constexpr int PER = kMomentBlock / 32;                   // elements of a lane
 constexpr int M_BASE = 889, V_BASE = 761;                // fp32 bits >> 20 of code 0: those of 1.0 are 1016, codes 127 and 255
 
-__device__ __forceinline__ uint32_t mix32(uint32_t h) {
-  h ^= h >> 16;
-  h *= 0x7FEB352Du;
-  h ^= h >> 15;
-  h *= 0x846CA68Bu;
-  return h ^ (h >> 16);
-}
-
 // Code in byte `Byte` of a word to its value.  A byte moved to bits 16-23 is a multiplication away from the upper bits of the number.
 template <int BYTE>
 __device__ __forceinline__ float decode_v(uint32_t word, float scale) {

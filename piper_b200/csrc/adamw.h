@@ -2,8 +2,19 @@
 // more elements than a launch has chunks for and -3 for a launch error.
 #pragma once
 #include <cuda_runtime.h>
+#include <stdint.h>
 
 namespace piper {
+
+// 32 bits mixed by two multiplications, with the shifts and factors that C. Wellons published in 2018 (from a search for such mixers of
+// little bias).
+__host__ __device__ inline uint32_t mix32(uint32_t h) {
+  h ^= h >> 16;
+  h *= 0x7FEB352Du;
+  h ^= h >> 15;
+  h *= 0x846CA68Bu;
+  return h ^ (h >> 16);
+}
 
 constexpr int kMomentBlock = 256;      // elements that share a scale where moments have 8 bits
 constexpr int kAdamwTensors = 80;      // tensors of one launch: their table travels with its arguments

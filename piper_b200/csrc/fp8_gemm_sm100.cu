@@ -5,7 +5,10 @@
 //
 // The tensor core multiplies with the scales itself (tcgen05.mma kind::mxf8f6f4 with block_scale, which takes a scale for
 // every 32 of the contraction: four instructions in a row take the same one) and keeps the sum in fp32 in tensor memory, so
-// no partial sum leaves it before the end.  Scaling by powers of two is exact.
+// no partial sum leaves it before the end.  Scaling by powers of two is exact; the sum is a little coarser than single additions in fp32:
+// within 2^-22 of the sum of the magnitudes for every 32 of the contraction, which is added at once.  A contraction of 28672
+// differs from an fp32 sum by 1.1e-4 of the result's norm, a last bit of bf16 in one of a thousand elements; both are 1.66e-3 of the norm,
+// bf16's own rounding, from the exact product.
 //
 // Persistent CTAs, each by itself or in pairs on two neighbouring SMs (cta_group::2), walk tiles of 128 rows a CTA and 32 to 224 columns.
 // Roles by warp:
@@ -21,8 +24,9 @@
 // A stage holds one block of the contraction, or two.
 //
 // What bounds it: a block of 128 of a 256 x 224 tile of a pair takes 448 cycles of MMA and loads 30 KiB into each SM, 472 cycles at
-// the 65 bytes per cycle that an SM takes from L2.  4096 x 28672 x 4096: 324 us, 2.97 PFLOP/s, tensor pipe 90 % busy; in a loop of
-// many such products the clock falls under the power limit, to some 390 us.  Few rows: a block's issue, see two_blocks().
+// the 65 bytes per cycle that an SM takes from L2.  4096 x 28672 x 4096: 306-309 us by itself (3.1 PFLOP/s, tensor pipe 88 % busy),
+// 316-327 in a loop of some; in a long loop the clock falls under the power limit, to some 390 us.  Few rows: a block's issue, see
+// two_blocks().
 //
 // All waits are bounded; on expiry the kernel records a status code, drains its copies, frees its tensor memory and returns.
 #include "fp8.h"
@@ -170,8 +174,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     tmem_alloc_n<CTAS>(&bars->tmem_base, 512);
     tmem_relinquish_n<CTAS>();
   }
-  // The first tile is the unit's own, later ones come from a counter, drawn while the last stage of the tile before is waited for: 4096 x
-  // 4096 x 28672 354-377 us, 351-388 in a fixed order; 1000 x 8192 x 2048 21 and 23, with all tiles drawn when they are needed 25.
+  // The first tile is the unit's own, later ones come from a counter, drawn while the last stage of the tile before is waited for.  With
+  // the GPU to itself that changes little (4096 x 4096 x 28672 347 us, 353 in a fixed order; 2048 x 8192 x 992 17.7 and 17.2), but beside
+  // another kernel that keeps 8 SMs: 4096 x 28672 x 4096 316 us and 525, 4096 x 4096 x 4096 66 and 81.
   const int units = static_cast<int>(gridDim.x) / CTAS;
   const bool draws = p.slot >= 0 && num_tiles > units;
   int* const counter = sched_slots + (draws ? p.slot : 0);
@@ -464,8 +469,9 @@ bool two_blocks(int ctas, int width) { return ctas == 2 ? width <= 128 : width <
 
 // Cycles of a launch by the model of the bf16 products (gemm_cost): an MMA of twice the elements per cycle on elements of half
 // the size leaves the cycles per block of 128 bytes as they are there.  What the issue of a block takes is fitted to 14 shapes in
-// all widths (M 16-4096, N 256-8192, K 256-14336), where the choice is 4 % behind the fastest on average; a pair, half of
-// whose rows would be empty, is not considered.
+// all widths (M 16-4096, N 256-8192, K 256-14336), where the choice is 4 % behind the fastest on average.  A pair of which one CTA would
+// have no rows is not considered: with weights from DRAM 24 x 4096 x 14336 takes 23.1 us as chosen and 23.3 in pairs of 64 columns,
+// 128 x 4096 x 4096 9.5 and 10.0, but 100 x 2048 x 8192 14.4 and 13.0.
 double cost(int M, int N, int K, bool f32, int ctas, int width, int num_sms) {
   const double k_blocks = (K + BK - 1) / BK;
   const long long tiles = static_cast<long long>((M + BM * ctas - 1) / (BM * ctas)) * ((N + width - 1) / width);

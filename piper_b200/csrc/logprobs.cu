@@ -713,7 +713,11 @@ logprobs_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ 
 
 // CTAs per row: with fewer rows than SMs have room for, a row is cut into up to eight pieces of at least 4,096 elements.  Not with
 // more rows, where a cluster waits for SMs together: 296 rows of 128256 with 20 alternatives 22.5 us, in four pieces 42; 1024 rows 60 us,
-// in two 83, without alternatives 50 and 65.
+// in two 83, without alternatives 50 and 65.  One row of 128256 5.2 us, in one piece 8.7.  For rows of a quarter of that the forward pass
+// loses by it what waiting for the cluster costs: 37 rows of 32003 6.8 us, in one piece 5.4 (with 20 alternatives 9.4 and 7.9; of fp32
+// without alternatives 7.0 and 8.1), 74 rows 7.9 and 6.4 (14.8 and 8.5), one row 4.6 either way; and where eight pieces fill the
+// SMs, alternatives do: 37 rows of 128256 17.7, in four 12.8, without alternatives 9.5 and 10.5.  The backward pass, whose pieces need no
+// cluster, gains: 37 rows of 32003 3.0 us, in one piece 4.6; 37 of 128256 4.7 and 11.9.
 int row_parts(long long T, int V, int num_sms) {
   int parts = 1;
   while (parts < MAX_PARTS && T * parts * 2 <= 2ll * num_sms && V / (parts * 2) >= 4096) parts *= 2;

@@ -11,6 +11,9 @@ tensors of its own steps them all in one launch::
 an element is an 8-bit number relative to it with three bits of mantissa (the first moment 16 binades and a sign, the
 second 32 binades), rounded up or down at random in proportion to the distance.  The random bits depend on the step, the
 tensor's place in the list (counted from the state's ``first``) and the element alone: a step from the same state gives the same bits.
+
+The kernel's square root and quotient are approximate, each within two units of the last place: an update differs by up to 2^-20 of itself
+from the same formula with rounded operations, which is what the executor's 32-bit buckets use (``adam_flat``).
 """
 from __future__ import annotations
 
@@ -28,6 +31,7 @@ _M_BASE, _V_BASE = 889, 761        # fp32 bits >> 20 of code 0; those of 1.0 are
 
 
 def _mix32(h: Tensor) -> Tensor:
+    """The mixer of ``csrc/adamw.h`` (C. Wellons, 2018)."""
     for shift, factor in ((16, 0x7FEB352D), (15, 0x846CA68B)):
         h = ((h ^ (h >> shift)) * factor) & 0xFFFFFFFF
     return h ^ (h >> 16)
