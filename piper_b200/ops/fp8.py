@@ -200,8 +200,10 @@ def _(x, w):
 def _linear_forward(ctx, x, w):
     y, xt = fp8_linear_keep(x, w) if w.requires_grad else (fp8_linear_op(x, w), None)
     ctx.rows = x.shape[0]
-    # x only to be found by gradients of the gradients, which raise; on a GPU it would keep what xt is there to save
-    ctx.save_for_backward(w, xt, None if x.is_cuda else x)
+    ctx.save_for_backward(w, xt)
+    # only to be found by gradients of the gradients, which raise: its values are not read, and the caller may write over them.  On a
+    # GPU it would keep what xt is there to save.
+    ctx.x = None if x.is_cuda else x
     return y
 
 
@@ -236,9 +238,9 @@ def _linear_backward(dy: Tensor, w: Tensor, xt: Optional[Tensor], T: int, need_x
 
 
 def _linear_formula(ctx, dy):
-    w, xt, x = ctx.saved_tensors
+    w, xt = ctx.saved_tensors
     grads = _linear_backward(dy, w, xt, ctx.rows, *ctx.needs_input_grad[:2])
-    return tuple(once_differentiable("fp8_linear", g, dy, w, *([] if x is None else [x])) for g in grads)
+    return tuple(once_differentiable("fp8_linear", g, dy, w, *([] if ctx.x is None else [ctx.x])) for g in grads)
 
 
 fp8_linear_op.register_autograd(_linear_formula, forward=_linear_forward)

@@ -428,3 +428,17 @@ def test_gradients_of_the_gradients_raise(device):
             torch.autograd.grad(g.float().square().sum() + x.float().sum() + w.float().sum(), [x, w])
     only = torch.autograd.grad(ops.fp8_linear(x.detach(), w), w, dy, create_graph=True)[0]
     assert torch.equal(only.detach(), want[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_input_that_is_written_over_after_the_layer(device):
+    """The backward pass has its own copy of it, in 8 bits."""
+    x, w = _matrix(40, 64, device, 1), _matrix(32, 64, device, 2, std=0.1).requires_grad_(True)
+    dy = _matrix(40, 32, device, 3)
+    a = x.clone().requires_grad_(True)
+    want = torch.autograd.grad(ops.fp8_linear(a * 1, w), [a, w], dy)
+    h = a * 1
+    y = ops.fp8_linear(h, w)
+    h.add_(1)
+    got = torch.autograd.grad([y, h], [a, w], [dy, torch.zeros_like(h)])
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
