@@ -378,14 +378,16 @@ class PiperActor:
 
 
 def _map_tensors(f: Callable, x):
-    """``x`` with ``f`` of every tensor in it, down tuples, lists and dictionaries."""
+    """``x`` with ``f`` of every tensor in it, down tuples (named ones too), lists and dictionaries; objects of other types, a program's
+    own subclasses of these among them, are as they are."""
     if isinstance(x, torch.Tensor):
         return f(x)
-    if isinstance(x, dict):
+    if type(x) is dict:
         return {k: _map_tensors(f, v) for k, v in x.items()}
-    if isinstance(x, (tuple, list)):
-        items = [_map_tensors(f, v) for v in x]
-        return type(x)(*items) if hasattr(x, "_fields") else type(x)(items)
+    if type(x) in (tuple, list):
+        return type(x)(_map_tensors(f, v) for v in x)
+    if isinstance(x, tuple) and hasattr(x, "_make"):
+        return x._make(_map_tensors(f, v) for v in x)
     return x
 
 

@@ -146,6 +146,30 @@ def test_advantages_through_the_engine(form, device):
             assert float((got - p.grad.float() / 2).norm()) <= 3 * half * float(p.grad.float().norm()) + 1e-8, n
 
 
+def test_which_labels_are_cut():
+    import collections
+
+    from piper_b200.runtime.actor import DagExecutor, _map_tensors
+
+    class Executor:
+        a = type("Actor", (), {"num_microbatches": 2})
+        _microbatch = DagExecutor._microbatch
+        cut = DagExecutor._microbatch_labels
+
+    pair = collections.namedtuple("pair", "tokens advantages")
+    t, w, own = torch.arange(8).view(4, 2), torch.ones(6), collections.OrderedDict(tokens=torch.arange(4))
+    cut = Executor().cut
+    assert torch.equal(cut(t, 1), t[2:]) and cut(None, 1) is None and cut(3, 0) == 3
+    got = cut((torch.tensor(5), t, {"w": w, "t": [t, "name"]}, own), 1)
+    assert got[0] == 5 and torch.equal(got[1], t[2:]) and got[2]["w"] is w and torch.equal(got[2]["t"][0], t[2:])
+    assert got[2]["t"][1] == "name" and got[3] is own
+    got = cut(pair(t, w), 0)
+    assert type(got) is pair and torch.equal(got.tokens, t[:2]) and got.advantages is w
+    assert cut((), 0) == () and _map_tensors(lambda x: x + 1, own) is own
+    odd = torch.arange(3)
+    assert cut((odd, odd), 0)[0] is odd                    # what is not divisible comes whole, as a single tensor does
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_policy_gradient_loss(device):
     from piper_b200.nn import cross_entropy_loss, policy_gradient_loss
