@@ -92,8 +92,8 @@ struct Sums {
   }
 };
 
-// The quick pass takes logits for at least `low`, a bf16 number of which low c2 is -2^30 or little above.  Its exponents fma(x, c2, -base)
-// keep what was lost when base = x c2 was rounded, half a unit of the last place: 64 at most for what is not below low, so a sum
+// What is not above `low`, a bf16 number of which low c2 is -2^30 or little above, has no weight in the quick pass.  Its exponents fma(x, c2,
+// -base) keep what was lost when base = x c2 was rounded, half a unit of the last place: 64 at most for what is above low / 2, so a sum
 // of a thread that has seen nothing but masked ids, whatever finite number they are masked by, is at most 2^64 times its length
 // until it is brought to the row's maximum, beside which it is 0.  A row whose maximum is not inside (low / 2, -low / 2), or whose
 // alternatives reach down to low, is read again by the exact pass.
@@ -223,7 +223,9 @@ __device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// A vector, no element below `low`, and the largest numbers of two halves of its elements, in the vector's own form.
+// A vector and the largest numbers of two halves of its elements, in the vector's own form.  bf16 elements are `low` at least, two in an
+// instruction; of fp32 ones the exponents are bounded in place of that, by a constant: 4096 rows of 128256 310 us, bounded by `low`
+// 328 (with alternatives, 2000 rows of 32003, 70 and 67).
 template <class T>
 struct Vec;
 template <>
@@ -243,9 +245,8 @@ template <>
 struct Vec<float> {
   float4 u;
   float most;
-  __device__ __forceinline__ Vec(const uint4& v, float low) {
-    u = make_float4(max_nan(__uint_as_float(v.x), low), max_nan(__uint_as_float(v.y), low), max_nan(__uint_as_float(v.z), low),
-                    max_nan(__uint_as_float(v.w), low));
+  __device__ __forceinline__ Vec(const uint4& v, float) {
+    u = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
     most = fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w));
   }
   __device__ __forceinline__ void also(const Vec& o) { most = fmaxf(most, o.most); }
@@ -271,8 +272,12 @@ struct QuickSums {
     base = to;
     top = x;
   }
+  // ANY: x may be below low, or -inf
+  template <bool ANY>
   __device__ __forceinline__ void add(float x, float c2) {
-    const float a = fmaf(x, c2, -base), w = ex2(a);
+    float a = fmaf(x, c2, -base);
+    if (ANY) a = max_nan(a, -200.f);                          // 2^-200 is 0 here, and so is 0 times -200
+    const float w = ex2(a);
     s += w;
     t = fmaf(w, a, t);
   }
@@ -314,7 +319,7 @@ struct Pass {
       second = fmaxf(second, fminf(x, m));
       m = fmaxf(m, x);
       if (x > v.top) v.raise(x, c2);
-      v.add(x, c2);
+      v.template add<false>(x, c2);
     };
     singles(sp.head, head, single);
     int best = -1, span = 0;               // the vectors from `best`, `span` apart at most, among which the largest element is
@@ -340,12 +345,12 @@ struct Pass {
       float f[VEC<T>];
       first.elements(f);
 #pragma unroll
-      for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
+      for (int q = 0; q < VEC<T>; ++q) v.template add<sizeof(T) == 4>(f[q], c2);
 #pragma unroll
       for (int j = 0; j < AHEAD - 1; ++j) {
         rest[j].elements(f);
 #pragma unroll
-        for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
+        for (int q = 0; q < VEC<T>; ++q) v.template add<sizeof(T) == 4>(f[q], c2);
       }
     }
 #pragma unroll 1
@@ -363,7 +368,7 @@ struct Pass {
       float f[VEC<T>];
       x.elements(f);
 #pragma unroll
-      for (int q = 0; q < VEC<T>; ++q) v.add(f[q], c2);
+      for (int q = 0; q < VEC<T>; ++q) v.template add<sizeof(T) == 4>(f[q], c2);
     }
     if (TOP && best >= 0) {
       place.first = static_cast<uint32_t>(body - row) + static_cast<uint32_t>(best) * VEC<T>;
