@@ -15,10 +15,20 @@
 //   dQ:    stationary tile = 128 query rows of one head (Q, dO); streams 128-row K and V blocks; dQ = dS K.
 // No gradient is reduced with atomics, so they are reproducible.
 //
+// Packed batches (PACKED): sequences of any lengths lie one behind the other in T rows.  A table on the device (pack.cu) lists
+// their blocks of 128 rows, longest first, and the CTAs of a block find their sequence there.  Tiles begin with their
+// sequence, at any row; only the last block of a sequence reaches into what lies behind it, and of that nothing may get in:
+// keys there lie above the diagonal (scores replaced by -inf, score gradients by 0), rows that a product would contract over
+// are left out of it in steps of 16 and set to zero within a step, and results are stored row by row.  lse and delta are
+// kept by blocks, [Hq][128 * blocks], so that a block's are aligned whatever row it begins at.
+//
 // Every mbarrier wait is bounded (see ptx.cuh); on expiry a status code is
 // recorded and the CTA unwinds and frees its TMEM.
 #include "attention_sm100.h"
 
+#include <atomic>
+
+#include "packed.h"
 #include "ptx.cuh"
 
 namespace piper {
@@ -61,6 +71,38 @@ __device__ __forceinline__ void store_row_chunk_sw128(uint8_t* tile, int row, in
     *reinterpret_cast<uint4*>(rbase + phys * 16) =
         make_uint4(w[4 * q + 0], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
   }
+}
+
+// ----------------------------------------------------------- packed batches
+// What a CTA needs of a row of the table.
+struct PackedBlock {
+  int tok0;                    // first row of the sequence
+  int len;                     // its rows
+  int block;                   // block of 128 rows in it; query blocks have block + 1 key blocks
+  int pad0;                    // where its lse and delta begin
+};
+
+__device__ __forceinline__ PackedBlock packed_block(const int4* table, int entry) {
+  const int4 e = __ldg(table + 1 + entry);
+  return {e.x, e.y, e.z, e.w};
+}
+
+// Rows [from, to) of a tile of 64-column halves, `half` bytes apart, become zero (whole rows: the swizzle stays within them).
+// Called by a warp in front of the products that contract over these rows.
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int halves, int half, int from, int to, int lane) {
+  const int n = (to - from) * 8;
+  for (int h = 0; h < halves; ++h)
+    for (int i = lane; i < n; i += 32)
+      *reinterpret_cast<uint4*>(tile + h * half + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// 64 bytes of a row
+__device__ __forceinline__ void store_row_chunk(__nv_bfloat16* dst, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    reinterpret_cast<uint4*>(dst)[q] = make_uint4(w[4 * q + 0], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
 }
 
 // ================================================================= forward
@@ -106,11 +148,13 @@ struct FwdBars {
 
 // ONE: one tile per CTA, else tiles_per_cta, two.  A constant for the one case only: the loops of two tiles lose 0.6 % both to
 // the other case's decisions and with their own number as a constant (1 x 8192, 32 / 4 heads x 128, 523.5 and 526.6 us).
-template <int HD, bool ONE>
+// PACKED: S is the padded length 128 * B of lse, B the blocks in the table's memory; a CTA has one tile or, where the group is
+// even, two heads of the group on the same rows.  CTAs behind the last block's set the rows behind the last sequence to zero.
+template <int HD, bool ONE, bool PACKED>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_out,
                 float* __restrict__ lse, int S, int Hq, int Hkv, int B, int tiles_per_cta, float scale_log2,
-                int* status) {
+                int* status, const int4* __restrict__ table, __nv_bfloat16* __restrict__ out, int T) {
   using L = FwdSmem<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -120,22 +164,56 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
   const int lane = threadIdx.x & 31;
   // longest rows first over all heads: the kv head and the sequence vary fastest, the query blocks fall
   const int group = Hq / Hkv;
-  const int tiles = group * (S / 128);
-  const int pairs = (tiles + tiles_per_cta - 1) / tiles_per_cta;
-  const int gb = static_cast<int>(blockIdx.x) % (Hkv * B);
-  const int pair = pairs - 1 - static_cast<int>(blockIdx.x) / (Hkv * B);
-  const int g = gb % Hkv;
-  const int b = gb / Hkv;
-  const int t0 = pair * tiles_per_cta;
-  const bool two = !ONE && tiles_per_cta == 2 && t0 + 1 < tiles;
-  const int qblk0 = t0 / group, head0 = g * group + t0 % group;
-  const int qblk1 = (t0 + 1) / group, head1 = g * group + (t0 + 1) % group;
+  int g, b, qblk0, head0, qblk1, head1;
+  bool two;
+  long long tok0;
+  PackedBlock e = {0, 0, 0, 0};
+  int rem = 128;                               // rows of this block that belong to the sequence
+  if constexpr (PACKED) {
+    grid_wait(table);
+    const int4 header = __ldg(table);          // blocks, end of the last sequence, rows of the batch
+    if (header.z != T) {                       // a table of another batch
+      if (threadIdx.x == 0) report_bad_argument(status, 53, header.z, T);
+      return;
+    }
+    const int units = ONE ? Hq : Hkv * (group / 2);
+    const int entry = static_cast<int>(blockIdx.x) / units, u = static_cast<int>(blockIdx.x) % units;
+    if (entry >= header.x) {
+      const long long rest = static_cast<long long>(T - header.y) * Hq * HD / 8;
+      uint4* const dst = reinterpret_cast<uint4*>(out + static_cast<long long>(header.y) * Hq * HD);
+      const long long first = static_cast<long long>(blockIdx.x) - static_cast<long long>(header.x) * units;
+      const long long ctas = static_cast<long long>(gridDim.x) - static_cast<long long>(header.x) * units;
+      for (long long i = first * FWD_THREADS + threadIdx.x; i < rest; i += ctas * FWD_THREADS) dst[i] = make_uint4(0, 0, 0, 0);
+      return;
+    }
+    e = packed_block(table, entry);
+    g = u % Hkv;
+    b = 0;
+    two = !ONE;
+    qblk0 = qblk1 = e.block;
+    head0 = g * group + (ONE ? 1 : 2) * (u / Hkv);
+    head1 = head0 + 1;
+    tok0 = e.tok0;
+    rem = min(128, e.len - e.block * 128);
+  } else {
+    const int tiles = group * (S / 128);
+    const int pairs = (tiles + tiles_per_cta - 1) / tiles_per_cta;
+    const int gb = static_cast<int>(blockIdx.x) % (Hkv * B);
+    const int pair = pairs - 1 - static_cast<int>(blockIdx.x) / (Hkv * B);
+    g = gb % Hkv;
+    b = gb / Hkv;
+    const int t0 = pair * tiles_per_cta;
+    two = !ONE && tiles_per_cta == 2 && t0 + 1 < tiles;
+    qblk0 = t0 / group, head0 = g * group + t0 % group;
+    qblk1 = (t0 + 1) / group, head1 = g * group + (t0 + 1) % group;
+    tok0 = static_cast<long long>(b) * S;
+  }
+  const int v_steps = PACKED ? (rem + 15) / 16 : 8;      // of 16 keys, in the last key block of the tiles
   // one tile: its even key blocks take the place of tile A, the odd ones that of tile B, and the two are merged at the end
   const bool halves = ONE && qblk0 > 0;
   const int n0 = halves ? (qblk0 + 2) / 2 : qblk0 + 1;
   const int n1 = two ? qblk1 + 1 : halves ? (qblk0 + 1) / 2 : 0;     // n1 >= n0 where there are two tiles
   const int n_blocks = two ? n1 : qblk0 + 1;
-  const long long tok0 = static_cast<long long>(b) * S;
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->q_full, 1);
@@ -157,7 +235,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
-  grid_wait();
+  grid_wait(table);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -212,14 +290,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
       }
       umma_commit(&bars->s_full[t]);
     };
-    auto issue_pv = [&](int t, int st, int half, bool first) {
+    auto issue_pv = [&](int t, int st, int half, bool first, int steps) {
       const uint64_t dv = dv_base + (st * L::TILE >> 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int ks = half * 4 + k;
-        umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + ks * 8, dv + (ks * 2048 >> 4), idesc_pv,
-                     (first && ks == 0) ? 0u : 1u);
+        if (!PACKED || ks < steps)
+          umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + ks * 8, dv + (ks * 2048 >> 4), idesc_pv,
+                       (first && ks == 0) ? 0u : 1u);
       }
+    };
+    // V of the last key block: what lies behind the sequence becomes zero up to a step's end
+    auto clear_v = [&](int st) {
+      if (PACKED && rem < v_steps * 16)
+        zero_tile_rows(smem + L::KV_OFF + st * L::TILE, L::HALVES, 16384, rem, v_steps * 16, lane);
     };
     bool ok = await_all(&bars->q_full, 0, status);
     ok = ok && await_all(&bars->kv_full[0], 0, status);
@@ -249,15 +333,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
       for (int b = 0; b < n_blocks && ok; ++b) {
         const int t = b & 1, v_st = (2 * b + 1) % L::STAGES;
         const uint32_t p_ph = (b >> 1) & 1;
-        ok = entry(2 * b + 1) && await_all(&bars->p_full[t][0], p_ph, status);
-        if (!ok) break;
+        const int steps = b == n_blocks - 1 ? v_steps : 8;
+        if (!(ok = entry(2 * b + 1))) break;
+        if (b == n_blocks - 1) clear_v(v_st);
+        if (!(ok = await_all(&bars->p_full[t][0], p_ph, status))) break;
         tc_fence_after();
-        if (elect_one()) issue_pv(t, v_st, 0, b < 2);
+        if (elect_one()) issue_pv(t, v_st, 0, b < 2, steps);
         __syncwarp();
         if (!(ok = await_all(&bars->p_full[t][1], p_ph, status))) break;
         tc_fence_after();
         if (elect_one()) {
-          issue_pv(t, v_st, 1, false);
+          issue_pv(t, v_st, 1, false, steps);
           if (b + 2 >= n_blocks) umma_commit(&bars->o_done[t]);
           umma_commit(&bars->kv_empty[v_st]);
         }
@@ -275,7 +361,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
       const uint32_t k_ph = ph;
       if (++st == L::STAGES) { st = 0; ph ^= 1; }
       const bool more = j + 1 < n_blocks;
+      const int steps = more ? 8 : v_steps;
       ok = await_all(&bars->kv_full[v_st], v_ph, status);
+      if (PACKED && ok && !more) clear_v(v_st);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int nt = t ? n1 : n0;
@@ -284,13 +372,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
         ok = await_all(&bars->p_full[t][0], j & 1, status);
         if (!ok) continue;
         tc_fence_after();
-        if (elect_one()) issue_pv(t, v_st, 0, j == 0);
+        if (elect_one()) issue_pv(t, v_st, 0, j == 0, steps);
         __syncwarp();
         ok = await_all(&bars->p_full[t][1], j & 1, status);
         if (!ok) continue;
         tc_fence_after();
         if (elect_one()) {
-          issue_pv(t, v_st, 1, false);
+          issue_pv(t, v_st, 1, false, steps);
           if (j == nt - 1) umma_commit(&bars->o_done[t]);
           if (last_user) umma_commit(&bars->kv_empty[v_st]);
         }
@@ -434,13 +522,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
           if (halves) v = fma2(make_float2(__uint_as_float(r2[2 * i]), __uint_as_float(r2[2 * i + 1])), fb, v);
           w[i] = pack_bf16x2(v.x, v.y);
         }
+        if (PACKED && rem < 128) {
+          if (row < rem) store_row_chunk(out + ((tok0 + qblk * 128 + row) * Hq + head) * HD + c * 32, w);
+          continue;
+        }
         store_row_chunk_sw128(obuf + (c >> 1) * 16384, row, (c & 1) * 4, w);
       }
-      lse[(static_cast<long long>(b) * Hq + head) * S + qblk * 128 + row] =
+      lse[(static_cast<long long>(b) * Hq + head) * S + (PACKED ? e.pad0 : 0) + qblk * 128 + row] =
           m_run * (scale_log2 * 0.6931471805599453f) + logf(l_run);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && (!PACKED || rem == 128)) {
         for (int h = 0; h < L::HALVES; ++h)
           tma_store_2d_bulk(&tmap_out, obuf + h * 16384 + (warp & 3) * 32 * 128, head * HD + 64 * h,
                             static_cast<int>(tok0) + qblk * 128 + (warp & 3) * 32);
@@ -491,6 +583,48 @@ attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __re
   }
 }
 
+// The same by the blocks of a packed batch, delta[h, pad0 + i] for row i of a sequence; and the rows of d_qkv behind the last
+// sequence become zero.
+template <int HD>
+__global__ void __launch_bounds__(256)
+attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta,
+                         int* __restrict__ arrived, int n_arrived, const int4* __restrict__ table, __nv_bfloat16* __restrict__ d_qkv,
+                         int T, int S, int Hq, int Hkv) {
+  grid_begin(o, d_o, table);
+  const long long thread = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, threads = static_cast<long long>(gridDim.x) * 256;
+  for (long long i = thread; i < n_arrived; i += threads) arrived[i] = 0;
+  constexpr int LANES = HD / 8;
+  const int wl = threadIdx.x & 31;
+  const int lane = wl & (LANES - 1);
+  const unsigned mask = ((1u << LANES) - 1u) << (wl & ~(LANES - 1));
+  const int4 header = __ldg(table);
+  if (header.z != T) return;
+  const long long total = static_cast<long long>(header.x) * 128 * Hq;
+  for (long long gi = thread / LANES; gi < total; gi += threads / LANES) {
+    const unsigned r = static_cast<unsigned>(gi / Hq), h = static_cast<unsigned>(gi - static_cast<long long>(r) * Hq);
+    const PackedBlock e = packed_block(table, r / 128);
+    const int i = e.block * 128 + static_cast<int>(r % 128);
+    if (i >= e.len) continue;
+    const long long at = (static_cast<long long>(e.tok0 + i) * Hq + h) * HD + 8 * lane;
+    const uint4 a = *reinterpret_cast<const uint4*>(o + at);
+    const uint4 b = *reinterpret_cast<const uint4*>(d_o + at);
+    const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&a);
+    const __nv_bfloat162* bp = reinterpret_cast<const __nv_bfloat162*>(&b);
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = __bfloat1622float2(ap[k]), y = __bfloat1622float2(bp[k]);
+      s += x.x * y.x + x.y * y.y;
+    }
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) s += __shfl_xor_sync(mask, s, off);
+    if (lane == 0) delta[static_cast<long long>(h) * S + e.pad0 + i] = s;
+  }
+  const long long row = static_cast<long long>(Hq + 2 * Hkv) * HD / 8, rest = (T - header.y) * row;
+  uint4* const dst = reinterpret_cast<uint4*>(d_qkv) + header.y * row;
+  for (long long i = thread; i < rest; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
+}
+
 // The dK/dV pass streams 64-row tiles through two tensor memory stages (dK, dV and two 64-wide pairs of S' and dP' fill
 // it).  Warps 0-7 turn the even tiles' scores into probabilities and score gradients, warps 8-15 the odd tiles' (four warps
 // per 32 columns), so each group has the MMAs of two tiles' time for its work; warp 16: TMA, warp 17: MMA.  P' and dS' (bf16) replace their
@@ -536,13 +670,14 @@ struct BwdBars {
 // dK and dV of key block xb of kv head g.  The query heads of the group may be split over `parts` CTAs; each accumulates over
 // its own and leaves its sums in `partial` ([part][slice of 64 columns][column][row]), and the one that finishes last
 // (by `arrived`, no CTA waits) adds them in the order of the parts, so the gradients are reproducible.
-template <int HD>
+template <int HD, bool PACKED>
 __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, const CUtensorMap* tmap_qkv_y,
                                              const CUtensorMap* tmap_do_y, const CUtensorMap* tmap_dqkv,
                                              const float* __restrict__ lse, const float* __restrict__ delta, int xb,
                                              int g, int b, int part, int parts, float* __restrict__ partial,
                                              int* __restrict__ arrived, int S, int Hq, int Hkv, float scale,
-                                             float scale_log2, int* status) {
+                                             float scale_log2, int* status, const PackedBlock e,
+                                             __nv_bfloat16* __restrict__ d_qkv) {
   using L = BwdSmem<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -552,10 +687,13 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
   const int lane = threadIdx.x & 31;
   const int heads = Hq / Hkv / parts;          // query heads of this CTA
   const int head0 = g * (Hq / Hkv) + part * heads;
-  const int tok0 = b * S;
+  const int tok0 = PACKED ? e.tok0 : b * S;
 
-  // for each of its query heads streams q tiles i in [2*xb, S/64 - 1]
-  const int tiles_per_head = S / 64 - 2 * xb;
+  // for each of its query heads streams q tiles i in [2*xb, y_tiles - 1]; of the last one y_rem rows belong to the sequence
+  const int y_tiles = PACKED ? (e.len + 63) / 64 : S / 64;
+  const int y_rem = PACKED ? e.len - (y_tiles - 1) * 64 : 64;
+  const int y_steps = (y_rem + 15) / 16;       // of 16 rows
+  const int tiles_per_head = y_tiles - 2 * xb;
   const int n_iter = tiles_per_head * heads;
 
   if (threadIdx.x == 0) {
@@ -615,11 +753,11 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
           tma_load_2d(y1, tmap_qkv_y, &bars->y_full[st], hh * HD + 64 * h, yrow);
           tma_load_2d(y2, tmap_do_y, &bars->y_full[st], hh * HD + 64 * h, yrow);
         }
-        const long long idx = (static_cast<long long>(b) * Hq + hh) * S + ti * 64;
+        const long long idx = (static_cast<long long>(b) * Hq + hh) * S + (PACKED ? e.pad0 : 0) + ti * 64;
         uint8_t* v = smem + L::VEC_OFF + st * 2 * L::VEC_BYTES;
         bulk_load(v, lse + idx, L::VEC_BYTES, &bars->y_full[st]);
         bulk_load(v + L::VEC_BYTES, delta + idx, L::VEC_BYTES, &bars->y_full[st]);
-        if (++ti == S / 64) { ti = 2 * xb; ++hh; }
+        if (++ti == y_tiles) { ti = 2 * xb; ++hh; }
       }
       grid_launch();
       if (it < n_iter) {
@@ -645,16 +783,27 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
         umma_bf16_ss(tmem_d, dx + (((ks / 4) * 16384 + (ks % 4) * 32) >> 4),
                      dy + (((ks / 4) * L::Y_HALF + (ks % 4) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
     };
-    auto issue_acc = [&](uint32_t tmem_d, uint32_t tmem_a, uint64_t dy, bool first) {
+    auto issue_acc = [&](uint32_t tmem_d, uint32_t tmem_a, uint64_t dy, bool first, int steps) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)       // contraction over the 64 streamed rows
-        umma_bf16_ts(tmem_d, tmem_a + (ks / 2) * 32 + (ks % 2) * 8, dy + (ks * 2048 >> 4), idesc_acc,
-                     (first && ks == 0) ? 0u : 1u);
+        if (!PACKED || ks < steps)
+          umma_bf16_ts(tmem_d, tmem_a + (ks / 2) * 32 + (ks % 2) * 8, dy + (ks * 2048 >> 4), idesc_acc,
+                       (first && ks == 0) ? 0u : 1u);
     };
+    // Q and dO of a head's last tile: what lies behind the sequence becomes zero up to a step's end
+    int in_head = 0;                       // tiles of this head whose scores have been asked for
+    auto clear_y = [&](int st) {
+      if (!PACKED || ++in_head < tiles_per_head) return;
+      in_head = 0;
+      if (y_rem < y_steps * 16)
+        zero_tile_rows(smem + L::Y_OFF + st * 2 * L::Y_TILE, 2 * L::HALVES, L::Y_HALF, y_rem, y_steps * 16, lane);
+    };
+    int acc_in_head = 0;
     bool ok = await_all(&bars->x_full, 0, status);
     for (int i = 0; i < 2 && i < n_iter && ok; ++i) {
       ok = await_all(&bars->y_full[i], 0, status);
       if (!ok) break;
+      clear_y(i);
       tc_fence_after();
       if (elect_one()) {
         const uint64_t y = dyk + (i * 2 * L::Y_TILE >> 4);
@@ -673,12 +822,18 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       const bool more = i + 2 < n_iter;
       const uint64_t yn = dyn + (st * 2 * L::Y_TILE >> 4);
       const uint64_t yk2 = dyk + (st2 * 2 * L::Y_TILE >> 4);
+      int steps = 4;
+      if (PACKED && ++acc_in_head == tiles_per_head) {
+        acc_in_head = 0;
+        steps = y_steps;
+      }
       if (!(ok = await_all(&bars->p_full[ss], ph, status))) break;
       tc_fence_after();
-      if (elect_one()) issue_acc(tmem_acc2, tmem_base + ss * 64, yn + (L::Y_TILE >> 4), i == 0);
+      if (elect_one()) issue_acc(tmem_acc2, tmem_base + ss * 64, yn + (L::Y_TILE >> 4), i == 0, steps);
       __syncwarp();
       if (more) {
         if (!(ok = await_all(&bars->y_full[st2], ((i + 2) / L::Y_STAGES) & 1, status))) break;
+        clear_y(st2);
         tc_fence_after();
         if (elect_one()) {
           issue_scores(tmem_base + ss * 64, dx1, yk2);
@@ -689,7 +844,7 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       if (!(ok = await_all(&bars->ds_full[ss], ph, status))) break;
       tc_fence_after();
       if (elect_one()) {
-        issue_acc(tmem_acc1, tmem_base + 128 + ss * 64, yn, i == 0);
+        issue_acc(tmem_acc1, tmem_base + 128 + ss * 64, yn, i == 0, steps);
         umma_commit(&bars->y_empty[st]);
         if (more) {
           issue_scores(tmem_base + 128 + ss * 64, dx2, yk2 + (L::Y_TILE >> 4));
@@ -714,7 +869,8 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
     const float2 sl2 = make_float2(scale_log2, scale_log2);
     constexpr float kNegLog2e = -1.4426950408889634f;
     const float2 neg_one = make_float2(-1.f, -1.f);
-    int ti = 2 * xb + wg;   // tiles_per_head is even: the parity of ti is wg throughout
+    int ti = 2 * xb + wg;   // unless PACKED, tiles_per_head is even: the parity of ti is wg throughout
+    if (PACKED && ti >= y_tiles) ti -= tiles_per_head;
     bool ok = true;
     for (int it = wg; it < n_iter; it += 2) {
       const uint32_t ph = (it >> 1) & 1;
@@ -727,6 +883,11 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       for (int c = 0; c < 4; ++c) {
         const float2 l2 = *reinterpret_cast<const float2*>(vl + 8 * c);
         nl[c] = make_float2(l2.x * kNegLog2e, l2.y * kNegLog2e);
+        if (PACKED && ti == y_tiles - 1) {     // probabilities of zero behind the sequence
+          const int y = ch * 32 + 8 * c + c0;
+          if (y >= y_rem) nl[c].x = -INFINITY;
+          if (y + 1 >= y_rem) nl[c].y = -INFINITY;
+        }
       }
       if (!await_all(&bars->s_full[wg], ph, status)) { ok = false; break; }
       tc_fence_after();
@@ -763,7 +924,14 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       warp_arrive(&bars->p_full[wg], lane);
       float2 dl[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) dl[c] = *reinterpret_cast<const float2*>(vd + 8 * c);
+      for (int c = 0; c < 4; ++c) {
+        dl[c] = *reinterpret_cast<const float2*>(vd + 8 * c);
+        if (PACKED && ti == y_tiles - 1) {
+          const int y = ch * 32 + 8 * c + c0;
+          if (y >= y_rem) dl[c].x = 0.f;
+          if (y + 1 >= y_rem) dl[c].y = 0.f;
+        }
+      }
       if (!await_all(&bars->dp_full[wg], ph, status)) { ok = false; break; }
       tc_fence_after();
       uint32_t dv[2][16];
@@ -786,7 +954,11 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       tc_fence_before();
       warp_arrive(&bars->ds_full[wg], lane);
       ti += 2;
-      if (ti >= S / 64) ti = 2 * xb + wg;
+      if constexpr (PACKED) {
+        while (ti >= y_tiles) ti -= tiles_per_head;
+      } else if (ti >= y_tiles) {
+        ti = 2 * xb + wg;
+      }
     }
     done = ok && await_all(&bars->acc_full, 0, status);
   }
@@ -824,6 +996,8 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
     const int h = is_k ? slice : slice - L::HALVES;
     uint8_t* obuf = smem + (is_k ? L::X1_OFF : L::X2_OFF) + h * 16384;
     const float sc = is_k ? scale : 1.f;
+    const int col = (Hq + (is_k ? 0 : Hkv) + g) * HD + 64 * h;
+    const int x_rem = PACKED ? min(128, e.len - xb * 128) : 128;
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
       uint32_t r[32], w[16];
@@ -842,13 +1016,17 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * sc, __uint_as_float(r[2 * i + 1]) * sc);
+      if (PACKED && x_rem < 128) {
+        if (row < x_rem)
+          store_row_chunk(d_qkv + static_cast<long long>(tok0 + xb * 128 + row) * (Hq + 2 * Hkv) * HD + col + c * 32, w);
+        continue;
+      }
       store_row_chunk_sw128(obuf, row, c * 4, w);
     }
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) {
-      tma_store_2d_bulk(tmap_dqkv, obuf + (warp & 3) * 32 * 128, (Hq + (is_k ? 0 : Hkv) + g) * HD + 64 * h,
-                        tok0 + xb * 128 + (warp & 3) * 32);
+    if (lane == 0 && (!PACKED || x_rem == 128)) {
+      tma_store_2d_bulk(tmap_dqkv, obuf + (warp & 3) * 32 * 128, col, tok0 + xb * 128 + (warp & 3) * 32);
       bulk_commit_group();
       bulk_wait_group<0>();
     }
@@ -888,11 +1066,12 @@ struct DqBars {
   uint32_t tmem_base;
 };
 
-template <int HD>
+template <int HD, bool PACKED>
 __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const CUtensorMap* tmap_do_x,
                                             const CUtensorMap* tmap_dqkv, const float* __restrict__ lse,
                                             const float* __restrict__ delta, int xb, int hy, int b, int S, int Hq,
-                                            int Hkv, float scale, float scale_log2, int* status) {
+                                            int Hkv, float scale, float scale_log2, int* status, const PackedBlock e,
+                                            __nv_bfloat16* __restrict__ d_qkv) {
   using L = DqSmem<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -901,8 +1080,10 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int lane = threadIdx.x & 31;
   const int g = hy / (Hq / Hkv);
-  const int tok0 = b * S;
+  const int tok0 = PACKED ? e.tok0 : b * S;
   const int n_blocks = xb + 1;
+  const int rem = PACKED ? min(128, e.len - xb * 128) : 128;     // rows of the last block that belong to the sequence
+  const int k_steps = (rem + 15) / 16;                           // of 16 keys
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->x_full, 1);
@@ -985,6 +1166,8 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
     auto s_block = [&](int j) -> bool {
       const int st = j % L::K_STAGES;
       if (!await_all(&bars->k_full[st], (j / L::K_STAGES) & 1, status)) return false;
+      if (PACKED && j == xb && rem < k_steps * 16)               // the keys behind the sequence, up to a step's end
+        zero_tile_rows(smem + L::K_OFF + st * L::TILE, L::HALVES, 16384, rem, k_steps * 16, lane);
       tc_fence_after();
       if (elect_one()) {
         issue_scores(tmem_base + (j & 1) * 128, dq, dk + (st * L::TILE >> 4));
@@ -1013,8 +1196,9 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
         const uint64_t kn = dkn + ((i % L::K_STAGES) * L::TILE >> 4);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks)     // dS of 32 keys each at columns 256, 288, 320, 352
-          umma_bf16_ts(tmem_base + 384, tmem_base + 256 + (ks / 2) * 32 + (ks % 2) * 8, kn + (ks * 2048 >> 4), idesc_acc,
-                       (i == 0 && ks == 0) ? 0u : 1u);
+          if (!PACKED || i < xb || ks < k_steps)
+            umma_bf16_ts(tmem_base + 384, tmem_base + 256 + (ks / 2) * 32 + (ks % 2) * 8, kn + (ks * 2048 >> 4), idesc_acc,
+                         (i == 0 && ks == 0) ? 0u : 1u);
         umma_commit(&bars->k_empty[i % L::K_STAGES]);
         if (i == n_blocks - 1) umma_commit(&bars->acc_full);
       }
@@ -1029,7 +1213,7 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t td = tmem_base + lane_sel + 256 + wg * 32;
     const float2 sl2 = make_float2(scale_log2, scale_log2);
-    const long long idx = (static_cast<long long>(b) * Hq + hy) * S + xb * 128 + row;
+    const long long idx = (static_cast<long long>(b) * Hq + hy) * S + (PACKED ? e.pad0 : 0) + xb * 128 + row;
     const float nl = lse[idx] * -1.4426950408889634f, ndl = -delta[idx];
     const float2 nl2 = make_float2(nl, nl), ndl2 = make_float2(ndl, ndl);
     bool ok = true;
@@ -1056,6 +1240,12 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
       uint32_t dv[32], dw[16];
       tmem_ld_32x32(td, dv);
       tmem_ld_wait();
+      if (PACKED && j == xb) {
+        // V behind the sequence may hold anything, 0 times which need not be 0
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (wg * 32 + i > row) dv[i] = 0;
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float2 d = add2(make_float2(__uint_as_float(dv[2 * i]), __uint_as_float(dv[2 * i + 1])), ndl2);
@@ -1080,11 +1270,16 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
+        if (PACKED && rem < 128) {
+          if (row < rem)
+            store_row_chunk(d_qkv + static_cast<long long>(tok0 + xb * 128 + row) * (Hq + 2 * Hkv) * HD + hy * HD + 64 * wg + c * 32, w);
+          continue;
+        }
         store_row_chunk_sw128(obuf, row, c * 4, w);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && (!PACKED || rem == 128)) {
         tma_store_2d_bulk(tmap_dqkv, obuf + (warp & 3) * 32 * 128, hy * HD + 64 * wg,
                           tok0 + xb * 128 + (warp & 3) * 32);
         bulk_commit_group();
@@ -1104,7 +1299,8 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
 // One launch for both passes.  They are independent (dK/dV and dQ go to different columns of d_qkv) and hold a whole
 // SM per CTA; the dK/dV CTAs are few and of very different lengths (with grouped heads up to group x S/64 tiles),
 // so they start first, longest first, and the many shorter dQ CTAs fill the SMs they leave.
-template <int HD>
+// PACKED: S is the padded length 128 * B of lse and delta, B the blocks in the table's memory.
+template <int HD, bool PACKED>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 128} over packed qkv
                 const __grid_constant__ CUtensorMap tmap_qkv_y,   // box {64, 64}  over packed qkv
@@ -1113,22 +1309,42 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 12
                 const __grid_constant__ CUtensorMap tmap_dqkv,    // box {64, 32}  over d_qkv
                 const float* __restrict__ lse, const float* __restrict__ delta, int B, int S, int Hq, int Hkv,
                 int parts, float* __restrict__ partial, int* __restrict__ arrived, float scale, float scale_log2,
-                int* status) {
+                int* status, const int4* __restrict__ table, __nv_bfloat16* __restrict__ d_qkv, int T) {
+  int idx = blockIdx.x;
+  if constexpr (PACKED) {
+    grid_wait(lse, delta, table);
+    const int n_kv = B * Hkv * parts;
+    const int entry = idx < n_kv ? idx / parts / Hkv : (idx - n_kv) / Hq;
+    const int4 header = __ldg(table);
+    if (entry >= header.x || header.z != T) return;
+    const PackedBlock e = packed_block(table, entry);
+    if (idx < n_kv) {
+      // of a sequence of n blocks, key block n - 1 - i has as many query blocks as query block i has key blocks
+      const int part = idx % parts;
+      idx /= parts;
+      attn_dkv_cta<HD, true>(&tmap_qkv_x, &tmap_qkv_y, &tmap_do_y, &tmap_dqkv, lse, delta, (e.len + 127) / 128 - 1 - e.block,
+                             idx % Hkv, 0, part, parts, partial + static_cast<long long>(idx) * parts * HD * 256, arrived + idx, S,
+                             Hq, Hkv, scale, scale_log2, status, e, d_qkv);
+    } else {
+      attn_dq_cta<HD, true>(&tmap_qkv_x, &tmap_do_x, &tmap_dqkv, lse, delta, e.block, (idx - n_kv) % Hq, 0, S, Hq, Hkv, scale,
+                            scale_log2, status, e, d_qkv);
+    }
+    return;
+  }
   const int blocks = S / 128;
   const int n_kv = blocks * Hkv * B * parts;
-  int idx = blockIdx.x;
   if (idx < n_kv) {
     const int part = idx % parts;
     idx /= parts;
     const int hb = idx % (Hkv * B);
-    attn_dkv_cta<HD>(&tmap_qkv_x, &tmap_qkv_y, &tmap_do_y, &tmap_dqkv, lse, delta, idx / (Hkv * B), hb % Hkv, hb / Hkv,
-                     part, parts, partial + static_cast<long long>(idx) * parts * HD * 256, arrived + idx, S, Hq, Hkv,
-                     scale, scale_log2, status);
+    attn_dkv_cta<HD, false>(&tmap_qkv_x, &tmap_qkv_y, &tmap_do_y, &tmap_dqkv, lse, delta, idx / (Hkv * B), hb % Hkv, hb / Hkv,
+                            part, parts, partial + static_cast<long long>(idx) * parts * HD * 256, arrived + idx, S, Hq, Hkv,
+                            scale, scale_log2, status, {}, nullptr);
   } else {
     idx -= n_kv;
     const int hb = idx % (Hq * B);
-    attn_dq_cta<HD>(&tmap_qkv_x, &tmap_do_x, &tmap_dqkv, lse, delta, blocks - 1 - idx / (Hq * B), hb % Hq, hb / Hq, S,
-                    Hq, Hkv, scale, scale_log2, status);
+    attn_dq_cta<HD, false>(&tmap_qkv_x, &tmap_do_x, &tmap_dqkv, lse, delta, blocks - 1 - idx / (Hq * B), hb % Hq, hb / Hq, S,
+                           Hq, Hkv, scale, scale_log2, status, {}, nullptr);
   }
 }
 
@@ -1166,7 +1382,8 @@ static int attn_fwd_impl(const CUtensorMap& tm, const CUtensorMap& to, float* ls
                          float softmax_scale, int num_sms, int* status, cudaStream_t st) {
   static bool cfg = false;
   if (!cfg) {
-    if (set_smem(attn_fwd_kernel<HD, true>, FwdSmem<HD>::TOTAL) || set_smem(attn_fwd_kernel<HD, false>, FwdSmem<HD>::TOTAL))
+    if (set_smem(attn_fwd_kernel<HD, true, false>, FwdSmem<HD>::TOTAL) ||
+        set_smem(attn_fwd_kernel<HD, false, false>, FwdSmem<HD>::TOTAL))
       return -2;
     cfg = true;
   }
@@ -1175,9 +1392,9 @@ static int attn_fwd_impl(const CUtensorMap& tm, const CUtensorMap& to, float* ls
   const int tiles_per_cta = attn_tiles_per_cta(B, S, Hq, num_sms);
   const long long ctas = (per_head + tiles_per_cta - 1) / tiles_per_cta * Hkv * B;
   if (ctas > 0x7fffffffll) return -1;
-  launch_overlapped(tiles_per_cta == 1 ? attn_fwd_kernel<HD, true> : attn_fwd_kernel<HD, false>, static_cast<unsigned>(ctas),
-                    FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse, S, Hq, Hkv, B, tiles_per_cta, scale_log2,
-                    status);
+  launch_overlapped(tiles_per_cta == 1 ? attn_fwd_kernel<HD, true, false> : attn_fwd_kernel<HD, false, false>,
+                    static_cast<unsigned>(ctas), FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse, S, Hq, Hkv, B, tiles_per_cta,
+                    scale_log2, status, nullptr, nullptr, 0);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -1237,7 +1454,7 @@ static int attn_bwd_impl(const void* qkv, const void* out, const void* d_out, co
   constexpr int smem = DqSmem<HD>::TOTAL > BwdSmem<HD>::TOTAL ? DqSmem<HD>::TOTAL : BwdSmem<HD>::TOTAL;
   static bool cfg = false;
   if (!cfg) {
-    if (set_smem(attn_bwd_kernel<HD>, smem)) return -2;
+    if (set_smem(attn_bwd_kernel<HD, false>, smem)) return -2;
     cfg = true;
   }
   // scratch: a counter per key block, padded to 16 bytes, and the parts' sums
@@ -1250,9 +1467,9 @@ static int attn_bwd_impl(const void* qkv, const void* out, const void* d_out, co
       static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(d_out), delta, arrived,
       parts > 1 ? n_kv : 0, T, S, Hq);
   if (cudaGetLastError() != cudaSuccess) return -3;
-  launch_overlapped(attn_bwd_kernel<HD>, static_cast<unsigned>(n_kv * parts + S / 128 * Hq * B), BWD_THREADS, smem, st,
+  launch_overlapped(attn_bwd_kernel<HD, false>, static_cast<unsigned>(n_kv * parts + S / 128 * Hq * B), BWD_THREADS, smem, st,
       tqx, tqy, tdx, tdy, tdq, lse, delta, B, S, Hq, Hkv, parts, partial, arrived, softmax_scale,
-      softmax_scale * 1.4426950408889634f, status);
+      softmax_scale * 1.4426950408889634f, status, nullptr, nullptr, 0);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -1270,6 +1487,121 @@ int attn_bwd(const void* qkv, const void* out, const void* d_out, const float* l
   if (hd == 128)
     return attn_bwd_impl<128>(qkv, out, d_out, lse, delta, scratch, d_qkv, B, S, Hq, Hkv, softmax_scale, num_sms, status, st);
   return attn_bwd_impl<64>(qkv, out, d_out, lse, delta, scratch, d_qkv, B, S, Hq, Hkv, softmax_scale, num_sms, status, st);
+}
+
+// ------------------------------------------------------------ packed batches
+// Once per kernel and device.
+template <typename K>
+static int set_smem_here(K kern, int bytes, std::atomic<bool>* configured) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return -2;
+  if (configured[device].load()) return 0;
+  const int rc = set_smem(kern, bytes);
+  if (rc == 0) configured[device].store(true);
+  return rc;
+}
+
+// The same costs as above, for `blocks` blocks of 128 rows, the longest sequence of `longest` blocks and `work` pairs of a query
+// and a key block.
+static int packed_tiles_per_cta(const PackedShape& p, int num_sms) {
+  const long long tiles = static_cast<long long>(p.Hq) * p.blocks;
+  return p.Hq / p.Hkv % 2 != 0 || tiles <= num_sms || p.Hq * p.work <= (p.longest - 1) * num_sms ? 1 : 2;
+}
+
+static int packed_parts(const PackedShape& p, int num_sms) {
+  const long long group = p.Hq / p.Hkv;
+  auto cost = [&](long long parts) {
+    const long long work = (p.Hq * p.work * 5800 + p.blocks * (p.Hkv * parts + p.Hq) * 6000) / num_sms;
+    const long long longest = group / parts * 2 * p.longest * 1600 + 6000 + (parts > 1 ? 3000 + 3000 * parts : 0);
+    return work > longest ? work : longest;
+  };
+  int best = 1;
+  for (int parts = 2; parts <= 8 && group % parts == 0; parts *= 2)
+    if (cost(parts) * 100 < cost(best) * 97) best = parts;
+  return best;
+}
+
+static bool packed_ok(const PackedShape& p) {
+  return p.Hq > 0 && p.Hkv > 0 && p.Hq % p.Hkv == 0 && (p.hd == 64 || p.hd == 128) && p.T >= 0 && p.T <= kMaxPackedTokens &&
+         p.blocks >= 0 && p.blocks * 128 <= INT32_MAX - 128 && static_cast<long long>(p.T) * (p.Hq + 2 * p.Hkv) <= INT32_MAX &&
+         p.blocks * (p.Hkv * 8ll + p.Hq) <= INT32_MAX - 64;
+}
+
+template <int HD>
+static int attn_packed_fwd_impl(const PackedShape& p, const void* qkv, void* out, float* lse, float softmax_scale, int num_sms,
+                                int* status, cudaStream_t st) {
+  const uint64_t W = static_cast<uint64_t>(p.Hq + 2 * p.Hkv) * HD, Wo = static_cast<uint64_t>(p.Hq) * HD;
+  CUtensorMap tm, to;
+  int rc;
+  if ((rc = make_tmap_2d_bf16(&tm, qkv, W, p.T, W * 2, 64, 128)) != 0) return rc;
+  if ((rc = make_tmap_2d_bf16(&to, out, Wo, p.T, Wo * 2, 64, 32)) != 0) return rc;
+  const bool one = packed_tiles_per_cta(p, num_sms) == 1;
+  const auto kern = one ? attn_fwd_kernel<HD, true, true> : attn_fwd_kernel<HD, false, true>;
+  static std::atomic<bool> configured[2][64];
+  if (set_smem_here(kern, FwdSmem<HD>::TOTAL, configured[one])) return -2;
+  const long long units = one ? p.Hq : p.Hq / 2;
+  launch_overlapped(kern, static_cast<unsigned>(p.blocks * units + 32), FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse,
+                    static_cast<int>(p.blocks) * 128, p.Hq, p.Hkv, static_cast<int>(p.blocks), one ? 1 : 2,
+                    softmax_scale * 1.4426950408889634f, status, reinterpret_cast<const int4*>(p.table),
+                    static_cast<__nv_bfloat16*>(out), p.T);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+int attn_packed_fwd(const PackedShape& p, const void* qkv, void* out, float* lse, float softmax_scale, int num_sms, int* status,
+                    cudaStream_t st) {
+  if (!packed_ok(p)) return -1;
+  if (p.T == 0) return 0;
+  return p.hd == 128 ? attn_packed_fwd_impl<128>(p, qkv, out, lse, softmax_scale, num_sms, status, st)
+                     : attn_packed_fwd_impl<64>(p, qkv, out, lse, softmax_scale, num_sms, status, st);
+}
+
+// scratch: delta, a counter per key block and kv head padded to 16 bytes, and the parts' sums
+long long attn_packed_bwd_floats(const PackedShape& p, int num_sms) {
+  const long long parts = packed_parts(p, num_sms), n_kv = p.blocks * p.Hkv;
+  return p.blocks * 128 * p.Hq + (parts == 1 ? 0 : (n_kv + 3) / 4 * 4 + n_kv * parts * p.hd * 256);
+}
+
+template <int HD>
+static int attn_packed_bwd_impl(const PackedShape& p, const void* qkv, const void* out, const void* d_out, const float* lse,
+                                float* scratch, void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st) {
+  const uint64_t W = static_cast<uint64_t>(p.Hq + 2 * p.Hkv) * HD, Wo = static_cast<uint64_t>(p.Hq) * HD;
+  if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(lse) |
+        reinterpret_cast<uintptr_t>(scratch)) & 15u) != 0)
+    return -1;
+  CUtensorMap tqx, tqy, tdx, tdy, tdq;
+  int rc;
+  if ((rc = make_tmap_2d_bf16(&tqx, qkv, W, p.T, W * 2, 64, 128)) != 0) return rc;
+  if ((rc = make_tmap_2d_bf16(&tqy, qkv, W, p.T, W * 2, 64, 64)) != 0) return rc;
+  if ((rc = make_tmap_2d_bf16(&tdx, d_out, Wo, p.T, Wo * 2, 64, 128)) != 0) return rc;
+  if ((rc = make_tmap_2d_bf16(&tdy, d_out, Wo, p.T, Wo * 2, 64, 64)) != 0) return rc;
+  if ((rc = make_tmap_2d_bf16(&tdq, d_qkv, W, p.T, W * 2, 64, 32)) != 0) return rc;
+  constexpr int smem = DqSmem<HD>::TOTAL > BwdSmem<HD>::TOTAL ? DqSmem<HD>::TOTAL : BwdSmem<HD>::TOTAL;
+  static std::atomic<bool> configured[64];
+  if (set_smem_here(attn_bwd_kernel<HD, true>, smem, configured)) return -2;
+  const int S = static_cast<int>(p.blocks) * 128, parts = packed_parts(p, num_sms);
+  const long long n_kv = p.blocks * p.Hkv;
+  float* const delta = scratch;
+  int* const arrived = reinterpret_cast<int*>(scratch + static_cast<long long>(S) * p.Hq);
+  float* const partial = scratch + static_cast<long long>(S) * p.Hq + (n_kv + 3) / 4 * 4;
+  const int4* const table = reinterpret_cast<const int4*>(p.table);
+  const long long delta_blocks = (static_cast<long long>(p.T) * p.Hq * (HD / 8) + 255) / 256;
+  launch_overlapped(attn_delta_packed_kernel<HD>, static_cast<unsigned>(delta_blocks < 148 * 16 ? delta_blocks : 148 * 16), 256, 0, st,
+                    static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(d_out), delta, arrived,
+                    parts > 1 ? static_cast<int>(n_kv) : 0, table, static_cast<__nv_bfloat16*>(d_qkv), p.T, S, p.Hq, p.Hkv);
+  if (cudaGetLastError() != cudaSuccess) return -3;
+  if (p.blocks == 0) return 0;
+  launch_overlapped(attn_bwd_kernel<HD, true>, static_cast<unsigned>(n_kv * parts + p.blocks * p.Hq), BWD_THREADS, smem, st, tqx, tqy,
+                    tdx, tdy, tdq, lse, delta, static_cast<int>(p.blocks), S, p.Hq, p.Hkv, parts, partial, arrived, softmax_scale,
+                    softmax_scale * 1.4426950408889634f, status, table, static_cast<__nv_bfloat16*>(d_qkv), p.T);
+  return cudaGetLastError() == cudaSuccess ? 0 : -3;
+}
+
+int attn_packed_bwd(const PackedShape& p, const void* qkv, const void* out, const void* d_out, const float* lse, float* scratch,
+                    void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st) {
+  if (!packed_ok(p)) return -1;
+  if (p.T == 0) return 0;
+  return p.hd == 128 ? attn_packed_bwd_impl<128>(p, qkv, out, d_out, lse, scratch, d_qkv, softmax_scale, num_sms, status, st)
+                     : attn_packed_bwd_impl<64>(p, qkv, out, d_out, lse, scratch, d_qkv, softmax_scale, num_sms, status, st);
 }
 
 }  // namespace piper

@@ -416,6 +416,7 @@ int64_t attn_bwd_parts(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t sm
 #include "bindings_moe.inc"
 #include "bindings_fused.inc"
 #include "bindings_tuning.inc"
+#include "bindings_packed.inc"
 #include "bindings_ops.inc"
 
 TORCH_LIBRARY(piper_c, m) {
@@ -452,5 +453,6 @@ TORCH_LIBRARY(piper_c, m) {
   register_moe_ops(m);
   register_fused_ops(m);
   register_tuning_ops(m);
+  register_packed_ops(m);
   register_native_ops(m);
 }

@@ -23,7 +23,8 @@ enum : int {
 // Records a rejected argument: the status word is the first of four ints; the first kernel to fail also leaves
 // (tag of the check, two values that describe it) in the other three.  Tags: 21-24 expert exchange (region
 // overflow, expert index, row count, segment range), 31-35 permutation kernels (permute, its gradient, combine,
-// its gradient, padding), 41 embedding.
+// its gradient, padding), 41 embedding, 51-53 packed batches (offsets, number of blocks, table of another batch), 61 balance (expert
+// index).
 __device__ __forceinline__ void report_bad_argument(int* status, int tag, long long a, long long b) {
   if (status != nullptr && atomicCAS(status, 0, kStatusBadArgument) == 0) {
     status[1] = tag;

@@ -20,7 +20,7 @@ import torch.nn as nn
 
 from .. import ops
 from ..api import annotate
-from ..nn import Attention, Embedding, FeedForward, Linear, RMSNorm
+from ..nn import Attention, Embedding, FeedForward, Linear, RMSNorm, packed_rope
 
 
 @dataclass
@@ -63,7 +63,7 @@ class TransformerBlock(nn.Module):
         self.ffn_norm = RMSNorm(cfg.dim, cfg.norm_eps)
         self.feed_forward = FeedForward(cfg.dim, cfg.ffn_hidden, cfg.fp8)
 
-    def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor], cos, sin, batch: int, seq: int):
+    def forward(self, h: torch.Tensor, delta: Optional[torch.Tensor], cos, sin, batch: int, seq: int, sequences=None):
         """``h`` is the residual stream and ``delta`` a branch output not yet added to it.
 
         Returns the new ``(h, delta)``; the pending add is folded into the next RMSNorm.
@@ -72,7 +72,7 @@ class TransformerBlock(nn.Module):
             y = self.attention_norm(h)
         else:
             y, h = self.attention_norm(delta, h)
-        a = self.attention(y, cos, sin, batch, seq)
+        a = self.attention(y, cos, sin, batch, seq, sequences)
         y, h = self.ffn_norm(a, h)
         return h, self.feed_forward(y)
 
@@ -120,8 +120,12 @@ class Transformer(nn.Module):
         c = self.const_attrs(self.cfg, seq_len or self.seq_len, self.rope_cos.device)
         self.rope_cos, self.rope_sin = c["rope_cos"].float(), c["rope_sin"].float()
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, sequences: Optional[ops.PackedSequences] = None) -> torch.Tensor:
+        """``sequences``: the tokens, row by row, are a packed batch (``ops.pack_sequences``), none longer than the rotary tables."""
         batch, seq = tokens.shape
+        cos, sin = self.rope_cos, self.rope_sin
+        if sequences is not None:
+            cos, sin = packed_rope(cos, sin, sequences)
         n = len(self.layers)
         h = delta = None
         out = None
@@ -135,7 +139,7 @@ class Transformer(nn.Module):
                 if stage == 0:
                     h = self.tok_embeddings(tokens.reshape(-1))
                 for i in range(lo, hi):
-                    h, delta = self.layers[i](h, delta, self.rope_cos, self.rope_sin, batch, seq)
+                    h, delta = self.layers[i](h, delta, cos, sin, batch, seq, sequences)
                 if stage == self.num_stages - 1:
                     y, h = self.norm(delta, h)
                     out = self.output(y).view(batch, seq, -1)

@@ -17,7 +17,7 @@ import torch.nn as nn
 
 from .. import ops
 from ..api import annotate
-from ..nn import Attention, Embedding, FeedForward, Linear, RMSNorm
+from ..nn import Attention, Embedding, FeedForward, Linear, RMSNorm, packed_rope
 from ..ops import moe as moe_ops
 
 PP_TAG = "PP"
@@ -47,6 +47,9 @@ class Qwen3Config:
     # the initial logits so that the load over experts is near-uniform from the first step.  0 disables it.
     router_jitter_std: float = 0.0
     fp8: bool = False               # projections of attention and of dense MLPs in 8 bits, see nn.Linear
+    # Weight of every layer's balance loss beside the model's own loss, in its gradients alone: the loss that is returned does
+    # not contain it.  0 leaves it out.
+    balance_coef: float = 0.0
 
 
 QWEN3_CONFIGS = {
@@ -86,7 +89,7 @@ class GroupedExperts(nn.Module):
 class MoE(nn.Module):
     def __init__(self, cfg: Qwen3Config) -> None:
         super().__init__()
-        self.top_k, self.renorm = cfg.top_k, cfg.norm_topk_prob
+        self.top_k, self.renorm, self.balance_coef = cfg.top_k, cfg.norm_topk_prob, cfg.balance_coef
         self.gate = Linear(cfg.dim, cfg.num_experts)
         self.experts = GroupedExperts(cfg.dim, cfg.moe_hidden, cfg.num_experts)
 
@@ -95,6 +98,8 @@ class MoE(nn.Module):
         if jitter is not None:
             logits = logits + jitter
         weights, idx, counts = moe_ops.moe_route(logits, self.top_k, self.renorm)
+        if self.balance_coef:
+            weights = moe_ops.moe_attach_loss(weights, moe_ops.moe_balance_loss(logits, idx).loss, self.balance_coef)
         rows, pos, g_start, g_len, ep_counts = moe_ops.moe_dispatch(x, idx, counts)
         with annotate(EP_TAG):
             out_rows = self.experts(rows, ep_counts)
@@ -111,12 +116,12 @@ class Qwen3Block(nn.Module):
         self.moe = MoE(cfg) if cfg.moe_enabled else None
         self.feed_forward = None if cfg.moe_enabled else FeedForward(cfg.dim, cfg.ffn_hidden, cfg.fp8)
 
-    def forward(self, h, delta, cos, sin, batch: int, seq: int, jitter=None):
+    def forward(self, h, delta, cos, sin, batch: int, seq: int, jitter=None, sequences=None):
         if delta is None:
             y = self.attention_norm(h)
         else:
             y, h = self.attention_norm(delta, h)
-        a = self.attention(y, cos, sin, batch, seq)
+        a = self.attention(y, cos, sin, batch, seq, sequences)
         y, h = self.ffn_norm(a, h)
         return h, (self.moe(y, jitter) if self.moe is not None else self.feed_forward(y))
 
@@ -157,8 +162,12 @@ class PiperQwen3Model(nn.Module):
         if self.use_jitter:
             self.router_jitter = c["router_jitter"].to(self.rope_cos.device)
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
+    def forward(self, tokens: torch.Tensor, sequences: Optional[ops.PackedSequences] = None) -> torch.Tensor:
+        """``sequences``: the tokens, row by row, are a packed batch (``ops.pack_sequences``), none longer than the rotary tables."""
         batch, seq = tokens.shape
+        cos, sin = self.rope_cos, self.rope_sin
+        if sequences is not None:
+            cos, sin = packed_rope(cos, sin, sequences)
         n = len(self.layers)
         h = delta = out = None
         jitter = None
@@ -170,7 +179,7 @@ class PiperQwen3Model(nn.Module):
                 if stage == 0:
                     h = self.tok_embeddings(tokens.reshape(-1))
                 for i in range(lo, hi):
-                    h, delta = self.layers[i](h, delta, self.rope_cos, self.rope_sin, batch, seq, jitter)
+                    h, delta = self.layers[i](h, delta, cos, sin, batch, seq, jitter, sequences)
                 if stage == self.num_stages - 1:
                     y, h = self.norm(delta, h)
                     out = self.output(y).view(batch, seq, -1)

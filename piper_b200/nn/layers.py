@@ -63,15 +63,31 @@ class Attention(nn.Module):
         self.q_norm = RMSNorm(head_dim, norm_eps) if qk_norm else None
         self.k_norm = RMSNorm(head_dim, norm_eps) if qk_norm else None
 
-    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, batch: int, seq: int) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, batch: int, seq: int,
+                sequences: Optional[ops.PackedSequences] = None) -> torch.Tensor:
+        """``sequences``: the ``batch * seq`` rows are a packed batch, ``cos`` and ``sin`` have a row for each of them (``packed_rope``)."""
+        if sequences is not None:
+            seq = batch * seq
         qkv = self.wqkv(x)
         qw = self.q_norm.weight if self.q_norm is not None else None
         kw = self.k_norm.weight if self.k_norm is not None else None
         qkv = ops.qk_rope(qkv, cos, sin, qw, kw, seq, self.n_heads, self.n_kv_heads, self.head_dim,
                           self.rope_interleaved, self.norm_eps)
-        out = ops.attention(qkv, batch, seq, self.n_heads, self.n_kv_heads, self.head_dim,
-                            1.0 / math.sqrt(self.head_dim))
+        scale = 1.0 / math.sqrt(self.head_dim)
+        if sequences is not None:
+            out = ops.packed_attention(qkv, sequences, self.n_heads, self.n_kv_heads, self.head_dim, scale)
+        else:
+            out = ops.attention(qkv, batch, seq, self.n_heads, self.n_kv_heads, self.head_dim, scale)
         return self.wo(out)
+
+
+def packed_rope(cos: torch.Tensor, sin: torch.Tensor, sequences: ops.PackedSequences) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows of the rotary tables for the tokens of a packed batch, whose positions begin with their sequence.  Tokens that the tables
+    have no row for get NaN, not some other position."""
+    at = sequences.positions()
+    beyond = (at >= cos.shape[0]).unsqueeze(1)
+    at = at.clamp(max=cos.shape[0] - 1)
+    return cos[at].masked_fill(beyond, math.nan), sin[at].masked_fill(beyond, math.nan)
 
 
 class FeedForward(nn.Module):
@@ -115,3 +131,19 @@ def policy_gradient_loss(output: torch.Tensor, tokens: torch.Tensor, advantages:
     if entropy_coef:
         gain = gain + entropy_coef * torch.where(counted, r.entropy, 0)
     return -gain.sum() / counted.sum().clamp(min=1)
+
+
+def clipped_policy_loss(output: torch.Tensor, tokens: torch.Tensor, advantages: torch.Tensor, old_logprob: torch.Tensor, *,
+                        ref_logprob: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                        sequences: Optional[ops.PackedSequences] = None, clip: tuple = (0.2, 0.2), kl_coef: float = 0.0,
+                        temperature: float = 1.0, ignore_index: int = -100) -> torch.Tensor:
+    """``ops.clipped_policy_loss`` of the tokens' log probabilities under ``[.., V]`` logits at ``temperature``.  Tokens that are
+    ``ignore_index`` or no ids do not count, nor those that ``mask`` leaves out."""
+    flat, V = tokens.reshape(-1), output.shape[-1]
+    r = ops.token_logprobs(output.reshape(-1, V), flat, temperature=temperature, ignore_index=ignore_index)
+    counted = (flat != ignore_index) & (flat >= 0) & (flat < V)
+    if mask is not None:
+        counted = counted & mask.reshape(-1)
+    return ops.clipped_policy_loss(r.logprob, old_logprob.reshape(-1), advantages.reshape(-1),
+                                   ref_logprob=None if ref_logprob is None else ref_logprob.reshape(-1), mask=counted,
+                                   sequences=sequences, clip=clip, kl_coef=kl_coef).loss

@@ -15,13 +15,13 @@ combine and their gradients are one kernel each and the expert GEMMs are ragged.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
 
 from . import core, native
-from .registry import custom_op, host_op
+from .registry import custom_op, host_op, once_differentiable
 from .core import _is_native, _require_bf16, grad_sinks, wgrad_store
 
 PAD = 128
@@ -99,6 +99,139 @@ def _route_backward(ctx, dw, _didx, _dcounts):
 
 
 moe_route.register_autograd(_route_backward, setup_context=_route_setup)
+
+
+# ------------------------------------------------------------ balance loss
+MAX_BALANCE_EXPERTS = 256
+
+
+class BalanceLoss(NamedTuple):
+    """``loss`` fp32 of no dimension, differentiable; ``counts`` int32 [E]: choices of every expert by the tokens that count;
+    ``prob`` fp32 [E]: its mean probability over them."""
+
+    loss: Tensor
+    counts: Tensor
+    prob: Tensor
+
+
+def _probabilities(logits: Tensor) -> Tensor:
+    """Softmax in fp64; rows without a finite logit become 0."""
+    x = logits.double()
+    top = x.amax(1, keepdim=True)
+    e = torch.exp(x - torch.where(top == -float("inf"), torch.zeros_like(top), top))
+    total = e.sum(1, keepdim=True)
+    return torch.where(total == 0, e, e / total)
+
+
+@custom_op("piper::moe_balance_fwd")
+def moe_balance_fwd(logits: Tensor, idx: Tensor, mask: Optional[Tensor]) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(loss, counts, prob, what the gradient of a probability is, up to that of the loss)."""
+    T, E = logits.shape
+    if _is_native(logits):
+        def empty(*shape, dtype=torch.float32):
+            return torch.empty(shape, dtype=dtype, device=logits.device)
+
+        loss, counts, prob, factor = empty(), empty(E, dtype=torch.int32), empty(E), empty(E)
+        scratch = empty(native.lib().balance_ctas(T, E) * 2 * (E + 1))
+        native.lib().balance_fwd(logits.contiguous(), idx.contiguous(), None if mask is None else mask.contiguous(), loss, counts,
+                                 prob, factor, scratch, native.status_tensor(logits.device))
+        return loss, counts, prob, factor
+    on = torch.ones(T, dtype=torch.bool) if mask is None else mask
+    n = max(1, int(on.sum()))
+    chosen = idx[on].reshape(-1).long()
+    if bool(((chosen < 0) | (chosen >= E)).any()):
+        raise ValueError(f"moe_balance_loss: idx holds what is no expert of {E}")
+    counts = torch.bincount(chosen, minlength=E)
+    prob = _probabilities(logits[on]).sum(0) / n
+    share = counts.double() * (E / (n * idx.shape[1]))
+    return (share * prob).sum().float(), counts.to(torch.int32), prob.float(), (share / n).float()
+
+
+@moe_balance_fwd.register_fake
+def _(logits, idx, mask):
+    E = logits.shape[1]
+    return (logits.new_empty((), dtype=torch.float32), logits.new_empty((E,), dtype=torch.int32),
+            logits.new_empty((E,), dtype=torch.float32), logits.new_empty((E,), dtype=torch.float32))
+
+
+def _balance_setup(ctx, inputs, output):
+    logits, idx, mask = inputs
+    _loss, counts, prob, factor = output
+    ctx.mark_non_differentiable(counts, prob, factor)
+    ctx.save_for_backward(logits, idx, mask, factor)
+
+
+def _balance_backward(ctx, d_loss, _d_counts, _d_prob, _d_factor):
+    logits, idx, mask, factor = ctx.saved_tensors
+    if d_loss is None:
+        return torch.zeros_like(logits), None, None
+    if _is_native(logits):
+        d = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        native.lib().balance_bwd(logits.contiguous(), idx.contiguous(), None if mask is None else mask.contiguous(), factor,
+                                 d_loss.to(torch.float32).contiguous(), d)
+    else:
+        with torch.no_grad():
+            p, c = _probabilities(logits), factor.double() * d_loss.double()
+            d = p * (c - (p * c).sum(1, keepdim=True))
+            if mask is not None:
+                d = torch.where(mask.unsqueeze(1), d, 0.0)
+            d = d.to(logits.dtype)
+    return once_differentiable("moe_balance_loss", d, logits), None, None
+
+
+moe_balance_fwd.register_autograd(_balance_backward, setup_context=_balance_setup)
+moe_balance_fwd = moe_balance_fwd.overload
+
+
+def moe_balance_loss(logits: Tensor, idx: Tensor, *, mask: Optional[Tensor] = None) -> BalanceLoss:
+    """E sum_e f_e P_e of a router: f_e the share of the choices ``idx`` (int32 [T, k], as ``moe_route`` gives) that went to expert
+    e, P_e its mean probability under ``logits`` [T, E], both over the tokens that count (``mask``, bool [T]).  1 where all
+    experts get the same, 0 without a token that counts.
+
+    Logits are bf16 or fp32, at most 256 experts; the choices have no gradient, and nothing at tokens that do not count reaches a
+    result.  A row of -inf alone has no probabilities and no gradient.  The gradient has no derivative of its own.  On
+    a GPU a choice that is no expert is left out, and the next status check raises.
+    """
+    if not logits.is_cuda:                           # on a GPU the op makes these checks by itself
+        if not logits.is_floating_point():
+            raise TypeError(f"moe_balance_loss: logits must be floating point, got {logits.dtype}")
+        if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_BALANCE_EXPERTS:
+            raise ValueError(f"moe_balance_loss: logits must be [T, E] with 1 to {MAX_BALANCE_EXPERTS} experts, got {tuple(logits.shape)}")
+        T, E = logits.shape
+        if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape[0] != T or not 1 <= idx.shape[1] <= E:
+            raise ValueError(f"moe_balance_loss: idx must be int32 [{T}, 1 to {E}], got {idx.dtype} {tuple(idx.shape)}")
+        if idx.device != logits.device:
+            raise ValueError(f"moe_balance_loss: idx is on {idx.device}, logits on {logits.device}")
+        if mask is not None and (mask.dtype != torch.bool or mask.shape != (T,) or mask.device != logits.device):
+            raise ValueError(f"moe_balance_loss: mask must be bool [{T}] on {logits.device}, got {mask.dtype} {tuple(mask.shape)} on "
+                             f"{mask.device}")
+    return BalanceLoss(*moe_balance_fwd(logits, idx, mask)[:3])
+
+
+@custom_op("piper::moe_attach_loss")
+def moe_attach_loss(weights: Tensor, loss: Tensor, coef: float) -> Tensor:
+    """The routing weights as they are; in the backward pass ``loss`` gets the gradient ``coef``, as if coef x loss had been added to
+    what the pass began with.  So a stage's auxiliary loss need not travel to the last stage."""
+    return weights.clone()
+
+
+@moe_attach_loss.register_fake
+def _(weights, loss, coef):
+    return torch.empty_like(weights)
+
+
+def _attach_setup(ctx, inputs, output):
+    _weights, loss, coef = inputs
+    ctx.coef, ctx.like = coef, (loss.shape, loss.dtype, loss.device)
+
+
+def _attach_backward(ctx, d_weights):
+    shape, dtype, device = ctx.like
+    return d_weights, torch.full(shape, ctx.coef, dtype=dtype, device=device), None
+
+
+moe_attach_loss.register_autograd(_attach_backward, setup_context=_attach_setup)
+moe_attach_loss = moe_attach_loss.overload
 
 
 # -------------------------------------------------------------- group table

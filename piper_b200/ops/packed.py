@@ -1,0 +1,222 @@
+"""Packed batches: sequences of any lengths, one behind the other in a batch of tokens, and causal attention within each of them.
+
+What fine-tuning on conversations and replies wants in place of ``attention``, whose sequences all have one length, a multiple of
+128.  ``pack_sequences`` lays out a batch once; every layer, forward and backward, and ``clipped_policy_loss`` take the result.
+Kernels: ``csrc/pack.cu``, ``csrc/attention_sm100.cu``.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+from torch import Tensor
+
+from . import native
+from .core import _is_native, _require_bf16
+from .registry import custom_op, once_differentiable
+
+BLOCK = 128                      # rows of a query or key block
+MAX_TOKENS = 1 << 21
+
+
+class PackedSequences(NamedTuple):
+    """Where the sequences of a packed batch lie.  ``longest`` (blocks of the longest sequence) and ``work`` (pairs of a query and a
+    key block) only choose launch shapes: where the offsets are on a GPU, they are those of equal sequences."""
+
+    offsets: Tensor              # int32 [n + 1]: sequence i has rows offsets[i] to offsets[i + 1]
+    table: Tensor                # int32 [blocks + 1, 4]: see _table_ref
+    tokens: int                  # rows of the batch, those behind the last sequence included
+    longest: int
+    work: int
+
+    def positions(self) -> Tensor:
+        """int64 [tokens]: a token's place in its sequence, 0 behind the last one."""
+        at = torch.arange(self.tokens, device=self.offsets.device)
+        of = torch.searchsorted(self.offsets, at, right=True) - 1
+        inside = at < self.offsets[-1]
+        return torch.where(inside, at - self.offsets[of.clamp(min=0)], 0)
+
+
+def _blocks(n: int) -> int:
+    return (n + BLOCK - 1) // BLOCK
+
+
+def _table_ref(offsets: list, tokens: int, blocks: int) -> Tensor:
+    """Row 0: blocks in use, end of the last sequence, tokens, 0.  Then, for every block of 128 rows, those with most blocks of their
+    sequence in front of them first: first row of the sequence, its rows, place of the block in it, and 128 times the
+    number of blocks of the sequences before."""
+    rows, before = [], 0
+    for a, b in zip(offsets, offsets[1:]):
+        rows += [(a, b - a, i, before * BLOCK) for i in range(_blocks(b - a))]
+        before += _blocks(b - a)
+    rows.sort(key=lambda r: (-r[2], -_blocks(r[1]), r[0]))
+    table = torch.zeros(blocks + 1, 4, dtype=torch.int32)
+    table[0] = torch.tensor([len(rows), offsets[-1], tokens, 0])
+    if rows:
+        table[1:len(rows) + 1] = torch.tensor(rows, dtype=torch.int32)
+    return table
+
+
+def _check_offsets(offsets: list, tokens: int) -> None:
+    if offsets[0] != 0 or any(b < a for a, b in zip(offsets, offsets[1:])) or offsets[-1] > tokens:
+        raise ValueError(f"pack_sequences: offsets must rise from 0 to at most {tokens}")
+
+
+@custom_op("piper::pack_table")
+def pack_table(offsets: Tensor, tokens: int, blocks: int) -> Tensor:
+    if _is_native(offsets):
+        table = torch.empty((blocks + 1, 4), dtype=torch.int32, device=offsets.device)
+        native.lib().pack_table(offsets, tokens, table, native.status_tensor(offsets.device))
+        return table
+    values = offsets.tolist()
+    _check_offsets(values, tokens)
+    return _table_ref(values, tokens, blocks)
+
+
+@pack_table.register_fake
+def _(offsets, tokens, blocks):
+    return offsets.new_empty((blocks + 1, 4), dtype=torch.int32)
+
+
+pack_table = pack_table.overload
+
+
+def pack_sequences(offsets: Tensor, tokens: int, device: Optional[torch.device] = None) -> PackedSequences:
+    """Lays out a batch of ``tokens`` rows in which sequence i has rows ``offsets[i]`` to ``offsets[i + 1]`` (int32 or int64 [n + 1],
+    rising from 0; sequences may be empty).  Rows behind the last sequence belong to none.
+
+    Offsets in host memory are checked here and give exact launch shapes; ``device`` is where the batch is.  Offsets
+    on a GPU stay there, nothing waits for them: if they do not rise from 0 to at most ``tokens``, the batch counts as empty and the
+    next status check raises.
+    """
+    if offsets.dim() != 1 or offsets.numel() < 1 or offsets.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"pack_sequences: offsets must be int32 or int64 [n + 1], got {offsets.dtype} {tuple(offsets.shape)}")
+    if not 0 <= tokens <= MAX_TOKENS:
+        raise ValueError(f"pack_sequences: 0 to {MAX_TOKENS} tokens, got {tokens}")
+    n = offsets.numel() - 1
+    if offsets.device.type == "cpu":
+        values = offsets.tolist()
+        _check_offsets(values, tokens)
+        counts = [_blocks(b - a) for a, b in zip(values, values[1:])]
+        blocks, longest, work = sum(counts), max(counts, default=0), sum(c * (c + 1) // 2 for c in counts)
+        offsets = offsets.to(device=device if device is not None else "cpu", dtype=torch.int32)
+    else:
+        if device is not None and torch.empty(0, device=device).device != offsets.device:
+            raise ValueError(f"pack_sequences: offsets are on {offsets.device}, not on {device}")
+        blocks = (tokens + (BLOCK - 1) * min(n, tokens)) // BLOCK
+        longest = _blocks(-(-tokens // max(n, 1)))
+        work = max(n, 1) * longest * (longest + 1) // 2
+        if offsets.dtype != torch.int32:     # what does not fit becomes an offset that is refused
+            offsets = offsets.clamp(-1, (1 << 31) - 1).to(torch.int32)
+    offsets = offsets.contiguous()
+    return PackedSequences(offsets, pack_table(offsets, tokens, blocks), tokens, longest, work)
+
+
+# --------------------------------------------------------------------------
+# attention
+# --------------------------------------------------------------------------
+
+
+def _sequences(table: Tensor) -> list:
+    """(first row, rows, place of lse) of the sequences in a table on the CPU."""
+    rows = table.tolist()
+    return [(a, n, at) for a, n, i, at in rows[1:rows[0][0] + 1] if i == 0]
+
+
+def _attention_ref(q: Tensor, k: Tensor, v: Tensor, scale: float) -> tuple[Tensor, Tensor]:
+    """[H, n, hd] in fp32 -> (out, lse)."""
+    s = (q @ k.transpose(-1, -2)) * scale
+    n = q.shape[1]
+    s = s.masked_fill(torch.ones(n, n, dtype=torch.bool).triu(1), float("-inf"))
+    return torch.softmax(s, -1) @ v, torch.logsumexp(s, -1)
+
+
+def _heads(x: Tensor, Hq: int, Hkv: int, hd: int) -> tuple[Tensor, Tensor, Tensor]:
+    """Rows of qkv as [H, n, hd] each, keys and values repeated over their group."""
+    x = x.float().view(x.shape[0], Hq + 2 * Hkv, hd).transpose(0, 1)
+    return x[:Hq], x[Hq:Hq + Hkv].repeat_interleave(Hq // Hkv, 0), x[Hq + Hkv:].repeat_interleave(Hq // Hkv, 0)
+
+
+@custom_op("piper::packed_attention_fwd")
+def packed_attention_fwd(qkv: Tensor, table: Tensor, longest: int, work: int, Hq: int, Hkv: int, hd: int,
+                         scale: float) -> tuple[Tensor, Tensor]:
+    """qkv [T, (Hq + 2 Hkv) * hd] -> (out [T, Hq * hd], lse [Hq, 128 * blocks], by the blocks of the table)."""
+    T, padded = qkv.shape[0], (table.shape[0] - 1) * BLOCK
+    if _is_native(qkv):
+        _require_bf16(qkv)
+        out = torch.empty((T, Hq * hd), dtype=qkv.dtype, device=qkv.device)
+        lse = torch.empty((Hq, padded), dtype=torch.float32, device=qkv.device)
+        native.lib().attn_packed_fwd(_aligned(qkv), table, out, lse, longest, work, Hq, Hkv, hd, scale,
+                                     native.status_tensor(qkv.device))
+        return out, lse
+    out, lse = torch.zeros(T, Hq * hd, dtype=qkv.dtype), torch.zeros(Hq, padded)
+    for a, n, at in _sequences(table):
+        o, lse[:, at:at + n] = _attention_ref(*_heads(qkv[a:a + n], Hq, Hkv, hd), scale)
+        out[a:a + n] = o.transpose(0, 1).reshape(n, Hq * hd).to(qkv.dtype)
+    return out, lse
+
+
+def _aligned(t: Tensor) -> Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+@packed_attention_fwd.register_fake
+def _(qkv, table, longest, work, Hq, Hkv, hd, scale):
+    return (qkv.new_empty((qkv.shape[0], Hq * hd)),
+            qkv.new_empty((Hq, (table.shape[0] - 1) * BLOCK), dtype=torch.float32))
+
+
+def _setup(ctx, inputs, output):
+    qkv, table, longest, work, Hq, Hkv, hd, scale = inputs
+    out, lse = output
+    ctx.cfg = (longest, work, Hq, Hkv, hd, scale)
+    ctx.mark_non_differentiable(lse)
+    ctx.save_for_backward(qkv, table, out, lse)
+
+
+def _backward(ctx, dout, _dlse):
+    longest, work, Hq, Hkv, hd, scale = ctx.cfg
+    qkv, table, out, lse = ctx.saved_tensors
+    none = (None,) * 7
+    if dout is None:
+        return torch.zeros_like(qkv), *none
+    if _is_native(qkv):
+        qc = _aligned(qkv)
+        dqkv = torch.empty_like(qc)
+        floats = native.lib().attn_packed_bwd_floats(table.shape[0] - 1, longest, work, Hq, Hkv, hd)
+        scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device)
+        native.lib().attn_packed_bwd(qc, table, _aligned(out), _aligned(dout), _aligned(lse), scratch, dqkv, longest, work, Hq,
+                                     Hkv, hd, scale, native.status_tensor(qkv.device))
+        return once_differentiable("packed_attention", dqkv, qkv), *none
+    dqkv = torch.zeros_like(qkv, memory_format=torch.contiguous_format)
+    for a, n, _at in _sequences(table):
+        with torch.enable_grad():
+            rows = qkv[a:a + n].detach().float().requires_grad_(True)
+            o, _ = _attention_ref(*_heads(rows, Hq, Hkv, hd), scale)
+            (g,) = torch.autograd.grad(o, rows, dout[a:a + n].float().view(n, Hq, hd).transpose(0, 1))
+        dqkv[a:a + n] = g.to(qkv.dtype)
+    return once_differentiable("packed_attention", dqkv, qkv), *none
+
+
+packed_attention_fwd.register_autograd(_backward, setup_context=_setup)
+packed_attention_fwd = packed_attention_fwd.overload
+
+
+def packed_attention(qkv: Tensor, sequences: PackedSequences, Hq: int, Hkv: int, hd: int, scale: float) -> Tensor:
+    """Causal grouped-query attention within every sequence of a packed batch: ``qkv`` [tokens, (Hq + 2 Hkv) * hd] -> [tokens, Hq *
+    hd].  Rows behind the last sequence give zeros and get a gradient of zero, whatever stands in them.
+
+    bf16 and heads of 64 or 128 on a GPU.  What stands in one sequence, infinities and NaN included, does not reach another.
+    The gradient has no derivative of its own.
+    """
+    if qkv.dim() != 2 or qkv.shape[0] != sequences.tokens:
+        raise ValueError(f"packed_attention: qkv is {tuple(qkv.shape)}, the batch has {sequences.tokens} tokens")
+    if qkv.is_cuda:                              # the op makes the checks below by itself
+        return packed_attention_fwd(qkv, sequences.table, sequences.longest, sequences.work, Hq, Hkv, hd, scale)[0]
+    if Hq < 1 or Hkv < 1 or Hq % Hkv or qkv.shape[1] != (Hq + 2 * Hkv) * hd:
+        raise ValueError(f"packed_attention: qkv must be [T, (Hq + 2 Hkv) * hd] with whole groups of heads, got "
+                         f"{tuple(qkv.shape)} for {Hq} / {Hkv} heads of {hd}")
+    if sequences.table.device != qkv.device:
+        raise ValueError(f"packed_attention: sequences are on {sequences.table.device}, qkv on {qkv.device}")
+    return packed_attention_fwd(qkv, sequences.table, sequences.longest, sequences.work, Hq, Hkv, hd, scale)[0]

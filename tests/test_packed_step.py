@@ -1,0 +1,138 @@
+"""A policy update on a packed batch: rotary positions, attention, log probabilities, the clipped loss within sequences and the
+routers' balance losses together, in the bundled models."""
+import pytest
+import torch
+
+from piper_b200 import nn, ops
+from piper_b200.ops import native
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+LENS = [130, 1, 77, 45]
+T = sum(LENS) + 3
+VOCAB = 512
+
+
+def _model(kind, device, balance_coef=0.0, max_len=160):
+    from piper_b200.models.llama3 import LlamaConfig, Transformer
+    from piper_b200.models.qwen3 import PiperQwen3Model, Qwen3Config
+    if kind == "llama":
+        cfg = LlamaConfig(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=VOCAB, ffn_hidden=256, rope_theta=10000.0)
+        model = Transformer(cfg, max_len, 1)
+    else:
+        cfg = Qwen3Config(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=64, vocab_size=VOCAB, num_experts=8, top_k=2,
+                          moe_hidden=128, balance_coef=balance_coef)
+        model = PiperQwen3Model(cfg, 1, max_len)
+    g = torch.Generator().manual_seed(0)
+    with torch.no_grad():
+        for name, p in sorted(model.named_parameters()):
+            p.copy_(torch.ones(p.shape) if p.dim() == 1 else torch.randn(p.shape, generator=g) * p.shape[-1] ** -0.5)
+    model = model.to(device)
+    if device == "cuda":
+        model = model.to(torch.bfloat16)
+    consts = type(model).const_attrs(cfg, max_len, device)
+    model.rope_cos, model.rope_sin = consts["rope_cos"], consts["rope_sin"]
+    return model
+
+
+def _batch(device):
+    g = torch.Generator().manual_seed(1)
+    tokens = torch.randint(0, VOCAB, (1, T), generator=g)
+    offsets = torch.tensor([0] + LENS).cumsum(0)
+    return tokens.to(device), offsets, ops.pack_sequences(offsets, T, device=device)
+
+
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+def test_packed_sequences_are_sequences_by_themselves(kind):
+    """On the CPU, in fp32: logits and gradients of a packed batch are those of its sequences one after the other."""
+    model = _model(kind, "cpu")
+    tokens, offsets, s = _batch("cpu")
+    g = torch.Generator().manual_seed(2)
+    up = torch.randn(T, VOCAB, generator=g)
+    up[sum(LENS):] = 0
+    out = model(tokens, s).view(T, VOCAB)
+    names = [n for n, _ in model.named_parameters()]
+    grads = torch.autograd.grad(out, list(model.parameters()), up)
+    want, sums = [], [torch.zeros_like(p) for p in model.parameters()]
+    for a, b in zip(offsets.tolist(), offsets.tolist()[1:]):
+        o = model(tokens[:, a:b]).view(b - a, VOCAB)
+        want.append(o.detach())
+        for acc, d in zip(sums, torch.autograd.grad(o, list(model.parameters()), up[a:b])):
+            acc += d
+    want = torch.cat(want)
+    # fp32 sums in another order: some 20 operations deep over at most 256 terms each, below 2^-24 x 20 x 256 of the largest
+    depth = 2.0 ** -24 * 20 * 256
+    assert float((out[:sum(LENS)].detach() - want).abs().max()) <= depth * float(want.abs().max())
+    for n, a, b in zip(names, grads, sums):
+        assert float((a - b).abs().max()) <= depth * float(b.abs().max()), n
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+def test_logits_of_a_sequence_do_not_depend_on_the_others(kind, device):
+    model = _model(kind, device)
+    tokens, offsets, s = _batch(device)
+    with torch.no_grad():
+        first = model(tokens, s).view(T, VOCAB)
+        other = tokens.clone()
+        a, b = int(offsets[2]), int(offsets[3])
+        other[0, a:b] = (other[0, a:b] + 1) % VOCAB
+        second = model(other, s).view(T, VOCAB)
+    end = int(offsets[-1])
+    assert torch.equal(first[:a], second[:a]) and torch.equal(first[b:end], second[b:end])
+    assert not torch.equal(first[a:b], second[a:b]) and bool(torch.isfinite(first[:end].float()).all())
+    if device == "cuda":
+        native.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+def test_a_policy_update(kind, device):
+    """Forward, loss and backward; tokens without advantage and without KL term leave no gradient, and balance losses add theirs to
+    the routers alone."""
+    model = _model(kind, device)
+    tokens, offsets, s = _batch(device)
+    target = torch.roll(tokens, -1, 1).reshape(-1)
+    g = torch.Generator().manual_seed(3)
+    with torch.no_grad():
+        old = ops.token_logprobs(model(tokens, s).view(T, VOCAB), target).logprob
+    old = old + (torch.randn(T, generator=g) * 0.1).to(device)
+    adv = torch.randn(T, generator=g).to(device)
+    mask = torch.ones(T, dtype=torch.bool, device=device)
+    mask[offsets[1:].to(device) - 1] = False              # the last token of a sequence predicts none
+
+    def step(m, advantages, kl_coef):
+        loss = nn.clipped_policy_loss(m(tokens, s), target, advantages, old, ref_logprob=old, mask=mask, sequences=s, kl_coef=kl_coef)
+        m.zero_grad()
+        loss.backward()
+        return loss.detach(), {n: p.grad.clone() for n, p in m.named_parameters()}
+
+    loss, grads = step(model, adv, 0.1)
+    assert bool(torch.isfinite(loss)) and all(bool(torch.isfinite(d.float()).all()) for d in grads.values())
+    assert all(bool(d.any()) for n, d in grads.items() if "gate" not in n)
+    only = torch.zeros_like(adv)
+    a, b = int(offsets[2]), int(offsets[3])
+    only[a:b] = adv[a:b]
+    _, grads = step(model, only, 0.0)
+    table = grads["tok_embeddings.weight"]
+    seen = torch.zeros(VOCAB, dtype=torch.bool, device=device)
+    seen[tokens[0, a:b]] = True
+    assert not bool(table[~seen].any()) and bool(table[tokens[0, a]].any())
+    if kind == "qwen":
+        zero, none = step(model, torch.zeros_like(adv), 0.0)
+        assert float(zero) == 0 and not any(bool(d.any()) for d in none.values())
+        balanced = _model(kind, device, balance_coef=0.5)
+        zero, some = step(balanced, torch.zeros_like(adv), 0.0)
+        assert float(zero) == 0 and bool(some["layers.1.moe.gate.weight"].any())
+        assert not bool(some["output.weight"].any()) and not bool(some["layers.1.moe.experts.w2"].any())
+    if device == "cuda":
+        native.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_positions_that_the_tables_lack_are_nan(device):
+    _tokens, offsets, s = _batch(device)
+    cos, sin = ops.rope_tables(64, 100, 10000.0, device)
+    c, d = nn.packed_rope(cos, sin, s)
+    at = s.positions()
+    assert bool(torch.isnan(c[at >= 100]).all()) and bool(torch.isnan(d[at >= 100]).all()) and int((at >= 100).sum()) == 30
+    assert torch.equal(c[at < 100], cos[at[at < 100]]) and torch.equal(d[at < 100], sin[at[at < 100]])
