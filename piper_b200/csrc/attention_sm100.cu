@@ -18,9 +18,10 @@
 // Packed batches (PACKED): sequences of any lengths lie one behind the other in T rows.  A table on the device (pack.cu) lists
 // their blocks of 128 rows, longest first, and the CTAs of a block find their sequence there.  Tiles begin with their
 // sequence, at any row; only the last block of a sequence reaches into what lies behind it, and of that nothing may get in:
-// keys there lie above the diagonal (scores replaced by -inf, score gradients by 0), rows that a product would contract over
-// are left out of it in steps of 16 and set to zero within a step, and results are stored row by row.  lse and delta are
-// kept by blocks, [Hq][128 * blocks], so that a block's are aligned whatever row it begins at.
+// keys there lie above the diagonal, where scores are replaced by -inf, rows that a product would contract over
+// are set to zero in shared memory (V as well where score gradients need a finite dP beside P = 0) or left out in steps of 16,
+// and results are stored row by row.  lse and delta are kept by blocks, [Hq][128 * blocks], so that a block's are aligned
+// whatever row it begins at; behind the sequence lse is infinite, which makes probabilities 0, and delta 0.
 //
 // Every mbarrier wait is bounded (see ptx.cuh); on expiry a status code is
 // recorded and the CTA unwinds and frees its TMEM.
@@ -87,6 +88,12 @@ __device__ __forceinline__ PackedBlock packed_block(const int4* table, int entry
   return {e.x, e.y, e.z, e.w};
 }
 
+// The same, known to the compiler as equal for a warp's lanes.
+__device__ __forceinline__ PackedBlock uniform(const PackedBlock& e) {
+  return {__shfl_sync(0xffffffffu, e.tok0, 0), __shfl_sync(0xffffffffu, e.len, 0), __shfl_sync(0xffffffffu, e.block, 0),
+          __shfl_sync(0xffffffffu, e.pad0, 0)};
+}
+
 // Rows [from, to) of a tile of 64-column halves, `half` bytes apart, become zero (whole rows: the swizzle stays within them).
 // Called by a warp in front of the products that contract over these rows.
 __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int halves, int half, int from, int to, int lane) {
@@ -96,6 +103,26 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int halves, int ha
       *reinterpret_cast<uint4*>(tile + h * half + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
+}
+
+// What rounding to bf16 takes from an output, in 128ths of the rounded number's last bit: with it the backward pass has dO . O to
+// 15 bits of O instead of 8.  Error of d_qkv against 64 bits (2-norm, 16384 tokens, 32 / 8 heads x 128): 2.7e-3 without it and
+// 2.4e-3 with it, of which the last rounding is 1.7e-3; a byte an output, kept where a gradient is wanted.
+constexpr uint32_t kExponent = 0x7f800000u;
+// Lost bits of two values, in the low bytes of x and y: a sum with 1.5 x 2^23 is rounded to whole numbers.  Below 2^-118 they are
+// any, and with_what_was_lost leaves them out.
+__device__ __forceinline__ float2 lost_by_rounding(float2 v, uint32_t rounded) {
+  const uint32_t x = rounded << 16, y = rounded & 0xffff0000u;
+  const float2 off = add2(v, make_float2(-__uint_as_float(x), -__uint_as_float(y)));
+  return fma2(off, make_float2(__uint_as_float((268u << 23) - (x & kExponent)), __uint_as_float((268u << 23) - (y & kExponent))),
+              make_float2(12582912.f, 12582912.f));
+}
+// lost: four bytes, each with its highest bit turned over, of which this is byte i.  (A conversion of every byte: 15 us more at
+// 16384 x 4096.)
+__device__ __forceinline__ float with_what_was_lost(float rounded, uint32_t lost, int i) {
+  const uint32_t e = __float_as_uint(rounded) & kExponent;
+  const float bits = __uint_as_float(__byte_perm(lost, 0x4b000000u, 0x7650 + i)) - 8388736.f;
+  return e < 16u << 23 ? rounded : fmaf(bits, __uint_as_float(e - (14u << 23)), rounded);
 }
 
 // 64 bytes of a row
@@ -154,7 +181,8 @@ template <int HD, bool ONE, bool PACKED>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_out,
                 float* __restrict__ lse, int S, int Hq, int Hkv, int B, int tiles_per_cta, float scale_log2,
-                int* status, const int4* __restrict__ table, __nv_bfloat16* __restrict__ out, int T) {
+                int* status, const int4* __restrict__ table, __nv_bfloat16* __restrict__ out, signed char* __restrict__ rest,
+                int T) {
   using L = FwdSmem<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -171,13 +199,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
   int rem = 128;                               // rows of this block that belong to the sequence
   if constexpr (PACKED) {
     grid_wait(table);
+    const int units = ONE ? Hq : Hkv * (group / 2);
+    const int entry = static_cast<int>(blockIdx.x) / units, u = static_cast<int>(blockIdx.x) % units;
     const int4 header = __ldg(table);          // blocks, end of the last sequence, rows of the batch
+    e = uniform(packed_block(table, min(entry, B - 1)));    // with the header, not behind it
     if (header.z != T) {                       // a table of another batch
       if (threadIdx.x == 0) report_bad_argument(status, 53, header.z, T);
       return;
     }
-    const int units = ONE ? Hq : Hkv * (group / 2);
-    const int entry = static_cast<int>(blockIdx.x) / units, u = static_cast<int>(blockIdx.x) % units;
     if (entry >= header.x) {
       const long long rest = static_cast<long long>(T - header.y) * Hq * HD / 8;
       uint4* const dst = reinterpret_cast<uint4*>(out + static_cast<long long>(header.y) * Hq * HD);
@@ -186,7 +215,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
       for (long long i = first * FWD_THREADS + threadIdx.x; i < rest; i += ctas * FWD_THREADS) dst[i] = make_uint4(0, 0, 0, 0);
       return;
     }
-    e = packed_block(table, entry);
     g = u % Hkv;
     b = 0;
     two = !ONE;
@@ -292,12 +320,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
     };
     auto issue_pv = [&](int t, int st, int half, bool first, int steps) {
       const uint64_t dv = dv_base + (st * L::TILE >> 4);
+      if (PACKED && steps < 8) {
+#pragma unroll 1
+        for (int ks = half * 4; ks < min(steps, half * 4 + 4); ++ks)
+          umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + ks * 8, dv + (ks * 2048 >> 4), idesc_pv,
+                       (first && ks == 0) ? 0u : 1u);
+        return;
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int ks = half * 4 + k;
-        if (!PACKED || ks < steps)
-          umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + ks * 8, dv + (ks * 2048 >> 4), idesc_pv,
-                       (first && ks == 0) ? 0u : 1u);
+        umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + ks * 8, dv + (ks * 2048 >> 4), idesc_pv,
+                     (first && ks == 0) ? 0u : 1u);
       }
     };
     // V of the last key block: what lies behind the sequence becomes zero up to a step's end
@@ -514,13 +548,29 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if (!ONE) {
-            w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
-            continue;
+          float2 v = make_float2(__uint_as_float(r[2 * i]) * inv, __uint_as_float(r[2 * i + 1]) * inv);
+          if (ONE) {
+            v = mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), fa);
+            if (halves) v = fma2(make_float2(__uint_as_float(r2[2 * i]), __uint_as_float(r2[2 * i + 1])), fb, v);
           }
-          float2 v = mul2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), fa);
-          if (halves) v = fma2(make_float2(__uint_as_float(r2[2 * i]), __uint_as_float(r2[2 * i + 1])), fb, v);
           w[i] = pack_bf16x2(v.x, v.y);
+          r[2 * i] = __float_as_uint(v.x);
+          r[2 * i + 1] = __float_as_uint(v.y);
+        }
+        if (PACKED && rest != nullptr) {
+          uint32_t lost[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 a = lost_by_rounding(make_float2(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])), w[2 * i]);
+            const float2 b = lost_by_rounding(make_float2(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])), w[2 * i + 1]);
+            lost[i] = __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040),
+                                  __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
+          }
+          if (row < rem) {
+            uint4* const dst = reinterpret_cast<uint4*>(rest + ((tok0 + qblk * 128 + row) * Hq + head) * HD + c * 32);
+            dst[0] = make_uint4(lost[0], lost[1], lost[2], lost[3]);
+            dst[1] = make_uint4(lost[4], lost[5], lost[6], lost[7]);
+          }
         }
         if (PACKED && rem < 128) {
           if (row < rem) store_row_chunk(out + ((tok0 + qblk * 128 + row) * Hq + head) * HD + c * 32, w);
@@ -528,8 +578,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
         }
         store_row_chunk_sw128(obuf + (c >> 1) * 16384, row, (c & 1) * 4, w);
       }
-      lse[(static_cast<long long>(b) * Hq + head) * S + (PACKED ? e.pad0 : 0) + qblk * 128 + row] =
-          m_run * (scale_log2 * 0.6931471805599453f) + logf(l_run);
+      float log_sum = m_run * (scale_log2 * 0.6931471805599453f) + logf(l_run);
+      if (PACKED && row >= rem) log_sum = INFINITY;      // probabilities of zero in the backward pass
+      lse[(static_cast<long long>(b) * Hq + head) * S + (PACKED ? e.pad0 : 0) + qblk * 128 + row] = log_sum;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0 && (!PACKED || rem == 128)) {
@@ -586,11 +637,12 @@ attn_delta_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __re
 // The same by the blocks of a packed batch, delta[h, pad0 + i] for row i of a sequence; and the rows of d_qkv behind the last
 // sequence become zero.
 template <int HD>
-__global__ void __launch_bounds__(256)
-attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta,
-                         int* __restrict__ arrived, int n_arrived, const int4* __restrict__ table, __nv_bfloat16* __restrict__ d_qkv,
-                         int T, int S, int Hq, int Hkv) {
-  grid_begin(o, d_o, table);
+__global__ void __launch_bounds__(256, 8)
+attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const signed char* __restrict__ rest,
+                         const __nv_bfloat16* __restrict__ d_o, float* __restrict__ delta, int* __restrict__ arrived, int n_arrived,
+                         const int4* __restrict__ table, __nv_bfloat16* __restrict__ d_qkv, int T, int S, int Hq, int Hkv) {
+  const bool exact = rest != nullptr;
+  grid_begin(o, rest, d_o, table);
   const long long thread = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x, threads = static_cast<long long>(gridDim.x) * 256;
   for (long long i = thread; i < n_arrived; i += threads) arrived[i] = 0;
   constexpr int LANES = HD / 8;
@@ -599,30 +651,43 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat1
   const unsigned mask = ((1u << LANES) - 1u) << (wl & ~(LANES - 1));
   const int4 header = __ldg(table);
   if (header.z != T) return;
-  const long long total = static_cast<long long>(header.x) * 128 * Hq;
-  for (long long gi = thread / LANES; gi < total; gi += threads / LANES) {
-    const unsigned r = static_cast<unsigned>(gi / Hq), h = static_cast<unsigned>(gi - static_cast<long long>(r) * Hq);
-    const PackedBlock e = packed_block(table, r / 128);
-    const int i = e.block * 128 + static_cast<int>(r % 128);
-    if (i >= e.len) continue;
-    const long long at = (static_cast<long long>(e.tok0 + i) * Hq + h) * HD + 8 * lane;
-    const uint4 a = *reinterpret_cast<const uint4*>(o + at);
-    const uint4 b = *reinterpret_cast<const uint4*>(d_o + at);
-    const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&a);
-    const __nv_bfloat162* bp = reinterpret_cast<const __nv_bfloat162*>(&b);
-    float s = 0.f;
+  // all heads of a row, or of several rows, at a time
+  constexpr int GROUPS = 256 / LANES;
+  const int group = threadIdx.x / LANES, at_once = Hq < GROUPS ? GROUPS / Hq : 1, own = group / Hq < at_once ? group / Hq : -1;
+  const int rows = header.x * 128;
+  for (int r0 = blockIdx.x * at_once; r0 < rows; r0 += gridDim.x * at_once) {
+    const int r = r0 + own;
+    if (at_once > 1 && (own < 0 || r >= rows)) continue;
+    const PackedBlock e = packed_block(table, (at_once > 1 ? r : r0) / 128);
+    const int i = e.block * 128 + (at_once > 1 ? r : r0) % 128;
+    for (int h = at_once > 1 ? group % Hq : group; h < Hq; h += GROUPS) {
+      float* const to = delta + static_cast<long long>(h) * S + e.pad0 + i;
+      if (i >= e.len) {                        // beside probabilities of zero
+        if (lane == 0) *to = 0.f;
+        continue;
+      }
+      const long long at = (static_cast<long long>(e.tok0 + i) * Hq + h) * HD + 8 * lane;
+      const uint4 a = *reinterpret_cast<const uint4*>(o + at);
+      const uint4 b = *reinterpret_cast<const uint4*>(d_o + at);
+      const uint2 l = exact ? *reinterpret_cast<const uint2*>(rest + at) : make_uint2(0, 0);
+      const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&a);
+      const __nv_bfloat162* bp = reinterpret_cast<const __nv_bfloat162*>(&b);
+      const uint32_t lw[2] = {l.x ^ 0x80808080u, l.y ^ 0x80808080u};
+      float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 x = __bfloat1622float2(ap[k]), y = __bfloat1622float2(bp[k]);
-      s += x.x * y.x + x.y * y.y;
+      for (int k = 0; k < 4; ++k) {
+        const float2 x = __bfloat1622float2(ap[k]), y = __bfloat1622float2(bp[k]);
+        s = fmaf(exact ? with_what_was_lost(x.x, lw[k / 2], 2 * (k & 1)) : x.x, y.x, s);
+        s = fmaf(exact ? with_what_was_lost(x.y, lw[k / 2], 2 * (k & 1) + 1) : x.y, y.y, s);
+      }
+#pragma unroll
+      for (int off = LANES / 2; off > 0; off >>= 1) s += __shfl_xor_sync(mask, s, off);
+      if (lane == 0) *to = s;
     }
-#pragma unroll
-    for (int off = LANES / 2; off > 0; off >>= 1) s += __shfl_xor_sync(mask, s, off);
-    if (lane == 0) delta[static_cast<long long>(h) * S + e.pad0 + i] = s;
   }
-  const long long row = static_cast<long long>(Hq + 2 * Hkv) * HD / 8, rest = (T - header.y) * row;
+  const long long row = static_cast<long long>(Hq + 2 * Hkv) * HD / 8, behind = (T - header.y) * row;
   uint4* const dst = reinterpret_cast<uint4*>(d_qkv) + header.y * row;
-  for (long long i = thread; i < rest; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
+  for (long long i = thread; i < behind; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
 }
 
 // The dK/dV pass streams 64-row tiles through two tensor memory stages (dK, dV and two 64-wide pairs of S' and dP' fill
@@ -639,6 +704,10 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat1
 // This kernel at 3 x 1408, 32 / 8 x 64: 139 us by rows, 128 us so; 1 x 4096, 32 / 8 x 128, which is short of power: 382 and 375 us.
 constexpr int BWD_THREADS = 576;
 constexpr int BWD_TMA_WARP = 16, BWD_MMA_WARP = 17;
+// Packed batches: one more warp stands between the copy of a sequence's last rows and its users and sets the rows behind them to zero
+// (by the MMA warp itself, which leaves out steps of 16 of them, the kernel takes 437 us instead of 406 at 1 x 4096, 32 / 8 x 128,
+// where no row is behind: its loop has no cycles to spare).
+constexpr int BWD_PACKED_THREADS = BWD_THREADS + 32, BWD_TAIL_WARP = 18;
 
 template <int HD>
 struct BwdSmem {
@@ -663,6 +732,7 @@ struct BwdBars {
   uint64_t p_full[2];                 // P' stands in the place of S'
   uint64_t ds_full[2];                // dS' stands in the place of dP'
   uint64_t acc_full;
+  uint64_t tail_full[4];              // PACKED: a head's last tile has landed, rows behind the sequence with it
   uint32_t tmem_base;
   int last;                           // this CTA has to add the parts
 };
@@ -692,7 +762,6 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
   // for each of its query heads streams q tiles i in [2*xb, y_tiles - 1]; of the last one y_rem rows belong to the sequence
   const int y_tiles = PACKED ? (e.len + 63) / 64 : S / 64;
   const int y_rem = PACKED ? e.len - (y_tiles - 1) * 64 : 64;
-  const int y_steps = (y_rem + 15) / 16;       // of 16 rows
   const int tiles_per_head = y_tiles - 2 * xb;
   const int n_iter = tiles_per_head * heads;
 
@@ -701,6 +770,7 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
     for (int i = 0; i < L::Y_STAGES; ++i) {
       mbar_init(&bars->y_full[i], 1);
       mbar_init(&bars->y_empty[i], 1);
+      mbar_init(&bars->tail_full[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
@@ -746,17 +816,18 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
         if (!await(&bars->y_empty[st], ((it / L::Y_STAGES) & 1) ^ 1, status)) break;
         const int yrow = tok0 + ti * 64;
         uint8_t* yb = smem + L::Y_OFF + st * 2 * L::Y_TILE;
-        mbar_arrive_expect_tx(&bars->y_full[st], 2 * L::Y_TILE + 2 * L::VEC_BYTES);
+        uint64_t* const full = PACKED && ti == y_tiles - 1 && y_rem < 64 ? &bars->tail_full[st] : &bars->y_full[st];
+        mbar_arrive_expect_tx(full, 2 * L::Y_TILE + 2 * L::VEC_BYTES);
         for (int h = 0; h < L::HALVES; ++h) {
           uint8_t* y1 = yb + h * L::Y_HALF;
           uint8_t* y2 = y1 + L::Y_TILE;
-          tma_load_2d(y1, tmap_qkv_y, &bars->y_full[st], hh * HD + 64 * h, yrow);
-          tma_load_2d(y2, tmap_do_y, &bars->y_full[st], hh * HD + 64 * h, yrow);
+          tma_load_2d(y1, tmap_qkv_y, full, hh * HD + 64 * h, yrow);
+          tma_load_2d(y2, tmap_do_y, full, hh * HD + 64 * h, yrow);
         }
         const long long idx = (static_cast<long long>(b) * Hq + hh) * S + (PACKED ? e.pad0 : 0) + ti * 64;
         uint8_t* v = smem + L::VEC_OFF + st * 2 * L::VEC_BYTES;
-        bulk_load(v, lse + idx, L::VEC_BYTES, &bars->y_full[st]);
-        bulk_load(v + L::VEC_BYTES, delta + idx, L::VEC_BYTES, &bars->y_full[st]);
+        bulk_load(v, lse + idx, L::VEC_BYTES, full);
+        bulk_load(v + L::VEC_BYTES, delta + idx, L::VEC_BYTES, full);
         if (++ti == y_tiles) { ti = 2 * xb; ++hh; }
       }
       grid_launch();
@@ -765,6 +836,18 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
         await(&bars->x_full, 0, nullptr);
         for (int jj = it - 1; jj >= 0 && jj > it - 1 - L::Y_STAGES; --jj)
           await(&bars->y_full[jj % L::Y_STAGES], (jj / L::Y_STAGES) & 1, nullptr);
+      }
+    }
+  } else if (PACKED && warp == BWD_TAIL_WARP) {
+    // --------------------------------- rows behind the sequence, set to zero
+    if (y_rem < 64) {
+      uint32_t phases = 0;                     // of tail_full, a bit each
+      for (int hh = 1; hh <= heads; ++hh) {
+        const int st = (hh * tiles_per_head - 1) % L::Y_STAGES;
+        if (!await_all(&bars->tail_full[st], phases >> st & 1, status)) break;
+        phases ^= 1u << st;
+        zero_tile_rows(smem + L::Y_OFF + st * 2 * L::Y_TILE, 2 * L::HALVES, L::Y_HALF, y_rem, 64, lane);
+        if (lane == 0) mbar_arrive(&bars->y_full[st]);
       }
     }
   } else if (warp == BWD_MMA_WARP) {
@@ -783,27 +866,16 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
         umma_bf16_ss(tmem_d, dx + (((ks / 4) * 16384 + (ks % 4) * 32) >> 4),
                      dy + (((ks / 4) * L::Y_HALF + (ks % 4) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
     };
-    auto issue_acc = [&](uint32_t tmem_d, uint32_t tmem_a, uint64_t dy, bool first, int steps) {
+    auto issue_acc = [&](uint32_t tmem_d, uint32_t tmem_a, uint64_t dy, bool first) {
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)       // contraction over the 64 streamed rows
-        if (!PACKED || ks < steps)
-          umma_bf16_ts(tmem_d, tmem_a + (ks / 2) * 32 + (ks % 2) * 8, dy + (ks * 2048 >> 4), idesc_acc,
-                       (first && ks == 0) ? 0u : 1u);
+        umma_bf16_ts(tmem_d, tmem_a + (ks / 2) * 32 + (ks % 2) * 8, dy + (ks * 2048 >> 4), idesc_acc,
+                     (first && ks == 0) ? 0u : 1u);
     };
-    // Q and dO of a head's last tile: what lies behind the sequence becomes zero up to a step's end
-    int in_head = 0;                       // tiles of this head whose scores have been asked for
-    auto clear_y = [&](int st) {
-      if (!PACKED || ++in_head < tiles_per_head) return;
-      in_head = 0;
-      if (y_rem < y_steps * 16)
-        zero_tile_rows(smem + L::Y_OFF + st * 2 * L::Y_TILE, 2 * L::HALVES, L::Y_HALF, y_rem, y_steps * 16, lane);
-    };
-    int acc_in_head = 0;
     bool ok = await_all(&bars->x_full, 0, status);
     for (int i = 0; i < 2 && i < n_iter && ok; ++i) {
       ok = await_all(&bars->y_full[i], 0, status);
       if (!ok) break;
-      clear_y(i);
       tc_fence_after();
       if (elect_one()) {
         const uint64_t y = dyk + (i * 2 * L::Y_TILE >> 4);
@@ -822,18 +894,12 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       const bool more = i + 2 < n_iter;
       const uint64_t yn = dyn + (st * 2 * L::Y_TILE >> 4);
       const uint64_t yk2 = dyk + (st2 * 2 * L::Y_TILE >> 4);
-      int steps = 4;
-      if (PACKED && ++acc_in_head == tiles_per_head) {
-        acc_in_head = 0;
-        steps = y_steps;
-      }
       if (!(ok = await_all(&bars->p_full[ss], ph, status))) break;
       tc_fence_after();
-      if (elect_one()) issue_acc(tmem_acc2, tmem_base + ss * 64, yn + (L::Y_TILE >> 4), i == 0, steps);
+      if (elect_one()) issue_acc(tmem_acc2, tmem_base + ss * 64, yn + (L::Y_TILE >> 4), i == 0);
       __syncwarp();
       if (more) {
         if (!(ok = await_all(&bars->y_full[st2], ((i + 2) / L::Y_STAGES) & 1, status))) break;
-        clear_y(st2);
         tc_fence_after();
         if (elect_one()) {
           issue_scores(tmem_base + ss * 64, dx1, yk2);
@@ -844,7 +910,7 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       if (!(ok = await_all(&bars->ds_full[ss], ph, status))) break;
       tc_fence_after();
       if (elect_one()) {
-        issue_acc(tmem_acc1, tmem_base + 128 + ss * 64, yn, i == 0, steps);
+        issue_acc(tmem_acc1, tmem_base + 128 + ss * 64, yn, i == 0);
         umma_commit(&bars->y_empty[st]);
         if (more) {
           issue_scores(tmem_base + 128 + ss * 64, dx2, yk2 + (L::Y_TILE >> 4));
@@ -883,11 +949,6 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       for (int c = 0; c < 4; ++c) {
         const float2 l2 = *reinterpret_cast<const float2*>(vl + 8 * c);
         nl[c] = make_float2(l2.x * kNegLog2e, l2.y * kNegLog2e);
-        if (PACKED && ti == y_tiles - 1) {     // probabilities of zero behind the sequence
-          const int y = ch * 32 + 8 * c + c0;
-          if (y >= y_rem) nl[c].x = -INFINITY;
-          if (y + 1 >= y_rem) nl[c].y = -INFINITY;
-        }
       }
       if (!await_all(&bars->s_full[wg], ph, status)) { ok = false; break; }
       tc_fence_after();
@@ -924,14 +985,7 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
       warp_arrive(&bars->p_full[wg], lane);
       float2 dl[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        dl[c] = *reinterpret_cast<const float2*>(vd + 8 * c);
-        if (PACKED && ti == y_tiles - 1) {
-          const int y = ch * 32 + 8 * c + c0;
-          if (y >= y_rem) dl[c].x = 0.f;
-          if (y + 1 >= y_rem) dl[c].y = 0.f;
-        }
-      }
+      for (int c = 0; c < 4; ++c) dl[c] = *reinterpret_cast<const float2*>(vd + 8 * c);
       if (!await_all(&bars->dp_full[wg], ph, status)) { ok = false; break; }
       tc_fence_after();
       uint32_t dv[2][16];
@@ -1063,6 +1117,7 @@ struct DqBars {
   uint64_t k_full[3], k_empty[3], v_full[2], v_empty[2];
   uint64_t s_full[2], dp_full, ds_full;
   uint64_t acc_full;
+  uint64_t tail_full[2];              // PACKED: K and V of the last block have landed, rows behind the sequence with them
   uint32_t tmem_base;
 };
 
@@ -1083,7 +1138,6 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
   const int tok0 = PACKED ? e.tok0 : b * S;
   const int n_blocks = xb + 1;
   const int rem = PACKED ? min(128, e.len - xb * 128) : 128;     // rows of the last block that belong to the sequence
-  const int k_steps = (rem + 15) / 16;                           // of 16 keys
 
   if (threadIdx.x == 0) {
     mbar_init(&bars->x_full, 1);
@@ -1095,6 +1149,7 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
       mbar_init(&bars->v_full[i], 1);
       mbar_init(&bars->v_empty[i], 1);
       mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->tail_full[i], 1);
     }
     mbar_init(&bars->dp_full, 1);
     mbar_init(&bars->ds_full, 16);             // one arrival per softmax warp
@@ -1127,16 +1182,18 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
       for (; vj < n_blocks; ++vj) {
         if (!await(&bars->k_empty[kj % L::K_STAGES], ((kj / L::K_STAGES) & 1) ^ 1, status)) break;
         const int ks = kj % L::K_STAGES;
-        mbar_arrive_expect_tx(&bars->k_full[ks], L::TILE);
+        const bool tail = PACKED && vj == xb && rem < 128;
+        uint64_t* const k_full = tail ? &bars->tail_full[0] : &bars->k_full[ks];
+        mbar_arrive_expect_tx(k_full, L::TILE);
         for (int h = 0; h < L::HALVES; ++h)
-          tma_load_2d(smem + L::K_OFF + ks * L::TILE + h * 16384, tmap_qkv_x, &bars->k_full[ks],
-                      (Hq + g) * HD + 64 * h, tok0 + kj * 128);
+          tma_load_2d(smem + L::K_OFF + ks * L::TILE + h * 16384, tmap_qkv_x, k_full, (Hq + g) * HD + 64 * h, tok0 + kj * 128);
         ++kj;
         if (!await(&bars->v_empty[vj & 1], ((vj >> 1) & 1) ^ 1, status)) break;
-        mbar_arrive_expect_tx(&bars->v_full[vj & 1], L::TILE);
+        uint64_t* const v_full = tail ? &bars->tail_full[1] : &bars->v_full[vj & 1];
+        mbar_arrive_expect_tx(v_full, L::TILE);
         for (int h = 0; h < L::HALVES; ++h)
-          tma_load_2d(smem + L::V_OFF + (vj & 1) * L::TILE + h * 16384, tmap_qkv_x, &bars->v_full[vj & 1],
-                      (Hq + Hkv + g) * HD + 64 * h, tok0 + vj * 128);
+          tma_load_2d(smem + L::V_OFF + (vj & 1) * L::TILE + h * 16384, tmap_qkv_x, v_full, (Hq + Hkv + g) * HD + 64 * h,
+                      tok0 + vj * 128);
       }
       grid_launch();
       if (vj < n_blocks) {
@@ -1145,6 +1202,16 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
         for (int j = kj - 1; j >= 0 && j >= kj - L::K_STAGES; --j)
           await(&bars->k_full[j % L::K_STAGES], (j / L::K_STAGES) & 1, nullptr);
         for (int j = vj - 1; j >= 0 && j >= vj - 2; --j) await(&bars->v_full[j & 1], (j >> 1) & 1, nullptr);
+      }
+    }
+  } else if (PACKED && warp == BWD_TAIL_WARP) {
+    // --------------------------------- rows behind the sequence, set to zero
+    if (rem < 128 && await_all(&bars->tail_full[0], 0, status)) {
+      zero_tile_rows(smem + L::K_OFF + xb % L::K_STAGES * L::TILE, L::HALVES, 16384, rem, 128, lane);
+      if (lane == 0) mbar_arrive(&bars->k_full[xb % L::K_STAGES]);
+      if (await_all(&bars->tail_full[1], 0, status)) {
+        zero_tile_rows(smem + L::V_OFF + (xb & 1) * L::TILE, L::HALVES, 16384, rem, 128, lane);
+        if (lane == 0) mbar_arrive(&bars->v_full[xb & 1]);
       }
     }
   } else if (warp == BWD_MMA_WARP) {
@@ -1166,8 +1233,6 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
     auto s_block = [&](int j) -> bool {
       const int st = j % L::K_STAGES;
       if (!await_all(&bars->k_full[st], (j / L::K_STAGES) & 1, status)) return false;
-      if (PACKED && j == xb && rem < k_steps * 16)               // the keys behind the sequence, up to a step's end
-        zero_tile_rows(smem + L::K_OFF + st * L::TILE, L::HALVES, 16384, rem, k_steps * 16, lane);
       tc_fence_after();
       if (elect_one()) {
         issue_scores(tmem_base + (j & 1) * 128, dq, dk + (st * L::TILE >> 4));
@@ -1196,9 +1261,8 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
         const uint64_t kn = dkn + ((i % L::K_STAGES) * L::TILE >> 4);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks)     // dS of 32 keys each at columns 256, 288, 320, 352
-          if (!PACKED || i < xb || ks < k_steps)
-            umma_bf16_ts(tmem_base + 384, tmem_base + 256 + (ks / 2) * 32 + (ks % 2) * 8, kn + (ks * 2048 >> 4), idesc_acc,
-                         (i == 0 && ks == 0) ? 0u : 1u);
+          umma_bf16_ts(tmem_base + 384, tmem_base + 256 + (ks / 2) * 32 + (ks % 2) * 8, kn + (ks * 2048 >> 4), idesc_acc,
+                       (i == 0 && ks == 0) ? 0u : 1u);
         umma_commit(&bars->k_empty[i % L::K_STAGES]);
         if (i == n_blocks - 1) umma_commit(&bars->acc_full);
       }
@@ -1240,12 +1304,6 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
       uint32_t dv[32], dw[16];
       tmem_ld_32x32(td, dv);
       tmem_ld_wait();
-      if (PACKED && j == xb) {
-        // V behind the sequence may hold anything, 0 times which need not be 0
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (wg * 32 + i > row) dv[i] = 0;
-      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float2 d = add2(make_float2(__uint_as_float(dv[2 * i]), __uint_as_float(dv[2 * i + 1])), ndl2);
@@ -1301,7 +1359,7 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
 // so they start first, longest first, and the many shorter dQ CTAs fill the SMs they leave.
 // PACKED: S is the padded length 128 * B of lse and delta, B the blocks in the table's memory.
 template <int HD, bool PACKED>
-__global__ void __launch_bounds__(BWD_THREADS, 1)
+__global__ void __launch_bounds__(PACKED ? BWD_PACKED_THREADS : BWD_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 128} over packed qkv
                 const __grid_constant__ CUtensorMap tmap_qkv_y,   // box {64, 64}  over packed qkv
                 const __grid_constant__ CUtensorMap tmap_do_x,    // box {64, 128} over dO [T, Hq*hd]
@@ -1316,8 +1374,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 12
     const int n_kv = B * Hkv * parts;
     const int entry = idx < n_kv ? idx / parts / Hkv : (idx - n_kv) / Hq;
     const int4 header = __ldg(table);
+    const PackedBlock e = uniform(packed_block(table, entry));      // with the header, not behind it
     if (entry >= header.x || header.z != T) return;
-    const PackedBlock e = packed_block(table, entry);
     if (idx < n_kv) {
       // of a sequence of n blocks, key block n - 1 - i has as many query blocks as query block i has key blocks
       const int part = idx % parts;
@@ -1394,7 +1452,7 @@ static int attn_fwd_impl(const CUtensorMap& tm, const CUtensorMap& to, float* ls
   if (ctas > 0x7fffffffll) return -1;
   launch_overlapped(tiles_per_cta == 1 ? attn_fwd_kernel<HD, true, false> : attn_fwd_kernel<HD, false, false>,
                     static_cast<unsigned>(ctas), FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse, S, Hq, Hkv, B, tiles_per_cta,
-                    scale_log2, status, nullptr, nullptr, 0);
+                    scale_log2, status, nullptr, nullptr, nullptr, 0);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -1528,8 +1586,8 @@ static bool packed_ok(const PackedShape& p) {
 }
 
 template <int HD>
-static int attn_packed_fwd_impl(const PackedShape& p, const void* qkv, void* out, float* lse, float softmax_scale, int num_sms,
-                                int* status, cudaStream_t st) {
+static int attn_packed_fwd_impl(const PackedShape& p, const void* qkv, void* out, float* lse, signed char* rest, float softmax_scale,
+                                int num_sms, int* status, cudaStream_t st) {
   const uint64_t W = static_cast<uint64_t>(p.Hq + 2 * p.Hkv) * HD, Wo = static_cast<uint64_t>(p.Hq) * HD;
   CUtensorMap tm, to;
   int rc;
@@ -1543,16 +1601,16 @@ static int attn_packed_fwd_impl(const PackedShape& p, const void* qkv, void* out
   launch_overlapped(kern, static_cast<unsigned>(p.blocks * units + 32), FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse,
                     static_cast<int>(p.blocks) * 128, p.Hq, p.Hkv, static_cast<int>(p.blocks), one ? 1 : 2,
                     softmax_scale * 1.4426950408889634f, status, reinterpret_cast<const int4*>(p.table),
-                    static_cast<__nv_bfloat16*>(out), p.T);
+                    static_cast<__nv_bfloat16*>(out), rest, p.T);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-int attn_packed_fwd(const PackedShape& p, const void* qkv, void* out, float* lse, float softmax_scale, int num_sms, int* status,
-                    cudaStream_t st) {
+int attn_packed_fwd(const PackedShape& p, const void* qkv, void* out, float* lse, signed char* rest, float softmax_scale, int num_sms,
+                    int* status, cudaStream_t st) {
   if (!packed_ok(p)) return -1;
   if (p.T == 0) return 0;
-  return p.hd == 128 ? attn_packed_fwd_impl<128>(p, qkv, out, lse, softmax_scale, num_sms, status, st)
-                     : attn_packed_fwd_impl<64>(p, qkv, out, lse, softmax_scale, num_sms, status, st);
+  return p.hd == 128 ? attn_packed_fwd_impl<128>(p, qkv, out, lse, rest, softmax_scale, num_sms, status, st)
+                     : attn_packed_fwd_impl<64>(p, qkv, out, lse, rest, softmax_scale, num_sms, status, st);
 }
 
 // scratch: delta, a counter per key block and kv head padded to 16 bytes, and the parts' sums
@@ -1562,11 +1620,11 @@ long long attn_packed_bwd_floats(const PackedShape& p, int num_sms) {
 }
 
 template <int HD>
-static int attn_packed_bwd_impl(const PackedShape& p, const void* qkv, const void* out, const void* d_out, const float* lse,
-                                float* scratch, void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st) {
+static int attn_packed_bwd_impl(const PackedShape& p, const void* qkv, const void* out, const signed char* rest, const void* d_out,
+                                const float* lse, float* scratch, void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st) {
   const uint64_t W = static_cast<uint64_t>(p.Hq + 2 * p.Hkv) * HD, Wo = static_cast<uint64_t>(p.Hq) * HD;
   if (((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(lse) |
-        reinterpret_cast<uintptr_t>(scratch)) & 15u) != 0)
+        reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(rest)) & 15u) != 0)
     return -1;
   CUtensorMap tqx, tqy, tdx, tdy, tdq;
   int rc;
@@ -1584,24 +1642,24 @@ static int attn_packed_bwd_impl(const PackedShape& p, const void* qkv, const voi
   int* const arrived = reinterpret_cast<int*>(scratch + static_cast<long long>(S) * p.Hq);
   float* const partial = scratch + static_cast<long long>(S) * p.Hq + (n_kv + 3) / 4 * 4;
   const int4* const table = reinterpret_cast<const int4*>(p.table);
-  const long long delta_blocks = (static_cast<long long>(p.T) * p.Hq * (HD / 8) + 255) / 256;
-  launch_overlapped(attn_delta_packed_kernel<HD>, static_cast<unsigned>(delta_blocks < 148 * 16 ? delta_blocks : 148 * 16), 256, 0, st,
-                    static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(d_out), delta, arrived,
+  const long long delta_ctas = p.blocks * 64 + 8;        // some for the rows behind the last sequence
+  launch_overlapped(attn_delta_packed_kernel<HD>, static_cast<unsigned>(delta_ctas < 148 * 8 ? delta_ctas : 148 * 8), 256, 0, st,
+                    static_cast<const __nv_bfloat16*>(out), rest, static_cast<const __nv_bfloat16*>(d_out), delta, arrived,
                     parts > 1 ? static_cast<int>(n_kv) : 0, table, static_cast<__nv_bfloat16*>(d_qkv), p.T, S, p.Hq, p.Hkv);
   if (cudaGetLastError() != cudaSuccess) return -3;
   if (p.blocks == 0) return 0;
-  launch_overlapped(attn_bwd_kernel<HD, true>, static_cast<unsigned>(n_kv * parts + p.blocks * p.Hq), BWD_THREADS, smem, st, tqx, tqy,
+  launch_overlapped(attn_bwd_kernel<HD, true>, static_cast<unsigned>(n_kv * parts + p.blocks * p.Hq), BWD_PACKED_THREADS, smem, st, tqx, tqy,
                     tdx, tdy, tdq, lse, delta, static_cast<int>(p.blocks), S, p.Hq, p.Hkv, parts, partial, arrived, softmax_scale,
                     softmax_scale * 1.4426950408889634f, status, table, static_cast<__nv_bfloat16*>(d_qkv), p.T);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
-int attn_packed_bwd(const PackedShape& p, const void* qkv, const void* out, const void* d_out, const float* lse, float* scratch,
-                    void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st) {
+int attn_packed_bwd(const PackedShape& p, const void* qkv, const void* out, const signed char* rest, const void* d_out,
+                    const float* lse, float* scratch, void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st) {
   if (!packed_ok(p)) return -1;
   if (p.T == 0) return 0;
-  return p.hd == 128 ? attn_packed_bwd_impl<128>(p, qkv, out, d_out, lse, scratch, d_qkv, softmax_scale, num_sms, status, st)
-                     : attn_packed_bwd_impl<64>(p, qkv, out, d_out, lse, scratch, d_qkv, softmax_scale, num_sms, status, st);
+  return p.hd == 128 ? attn_packed_bwd_impl<128>(p, qkv, out, rest, d_out, lse, scratch, d_qkv, softmax_scale, num_sms, status, st)
+                     : attn_packed_bwd_impl<64>(p, qkv, out, rest, d_out, lse, scratch, d_qkv, softmax_scale, num_sms, status, st);
 }
 
 }  // namespace piper

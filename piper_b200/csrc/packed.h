@@ -22,14 +22,15 @@ struct PackedShape {
   int Hq, Hkv, hd;
 };
 
-// qkv [T, (Hq + 2 Hkv) hd] bf16 -> out [T, Hq hd] bf16 and lse [Hq, 128 blocks] fp32 (natural log).
-int attn_packed_fwd(const PackedShape& p, const void* qkv, void* out, float* lse, float softmax_scale, int num_sms, int* status,
-                    cudaStream_t st);
+// qkv [T, (Hq + 2 Hkv) hd] bf16 -> out [T, Hq hd] bf16, lse [Hq, 128 blocks] fp32 (natural log) and, unless null, rest [T, Hq hd]:
+// what rounding has taken from out, for the backward pass.
+int attn_packed_fwd(const PackedShape& p, const void* qkv, void* out, float* lse, signed char* rest, float softmax_scale, int num_sms,
+                    int* status, cudaStream_t st);
 
-// d_qkv is overwritten whole.  scratch: attn_packed_bwd_floats(), 16-byte aligned as out, d_out and lse are.
+// d_qkv is overwritten whole.  rest may be null.  scratch: attn_packed_bwd_floats(); all 16-byte aligned.
 long long attn_packed_bwd_floats(const PackedShape& p, int num_sms);
-int attn_packed_bwd(const PackedShape& p, const void* qkv, const void* out, const void* d_out, const float* lse, float* scratch,
-                    void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st);
+int attn_packed_bwd(const PackedShape& p, const void* qkv, const void* out, const signed char* rest, const void* d_out,
+                    const float* lse, float* scratch, void* d_qkv, float softmax_scale, int num_sms, int* status, cudaStream_t st);
 
 // Clipped policy loss.  logprob, old, adv, ref (or null) [T] fp32, mask [T] bytes or null; table null: one mean over all tokens.
 struct PolicyArgs {

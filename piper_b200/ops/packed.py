@@ -138,22 +138,24 @@ def _heads(x: Tensor, Hq: int, Hkv: int, hd: int) -> tuple[Tensor, Tensor, Tenso
 
 
 @custom_op("piper::packed_attention_fwd")
-def packed_attention_fwd(qkv: Tensor, table: Tensor, longest: int, work: int, Hq: int, Hkv: int, hd: int,
-                         scale: float) -> tuple[Tensor, Tensor]:
-    """qkv [T, (Hq + 2 Hkv) * hd] -> (out [T, Hq * hd], lse [Hq, 128 * blocks], by the blocks of the table)."""
+def packed_attention_fwd(qkv: Tensor, table: Tensor, longest: int, work: int, Hq: int, Hkv: int, hd: int, scale: float,
+                         keep: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """qkv [T, (Hq + 2 Hkv) * hd] -> (out [T, Hq * hd], lse [Hq, 128 * blocks], by the blocks of the table, and, if ``keep`` and on a
+    GPU, what rounding has taken from out, int8 [T, Hq * hd]).  The formula keeps it."""
     T, padded = qkv.shape[0], (table.shape[0] - 1) * BLOCK
     if _is_native(qkv):
         _require_bf16(qkv)
         out = torch.empty((T, Hq * hd), dtype=qkv.dtype, device=qkv.device)
         lse = torch.empty((Hq, padded), dtype=torch.float32, device=qkv.device)
-        native.lib().attn_packed_fwd(_aligned(qkv), table, out, lse, longest, work, Hq, Hkv, hd, scale,
+        rest = torch.empty((T if keep else 0, Hq * hd), dtype=torch.int8, device=qkv.device)
+        native.lib().attn_packed_fwd(_aligned(qkv), table, out, lse, rest, longest, work, Hq, Hkv, hd, scale,
                                      native.status_tensor(qkv.device))
-        return out, lse
+        return out, lse, rest
     out, lse = torch.zeros(T, Hq * hd, dtype=qkv.dtype), torch.zeros(Hq, padded)
     for a, n, at in _sequences(table):
         o, lse[:, at:at + n] = _attention_ref(*_heads(qkv[a:a + n], Hq, Hkv, hd), scale)
         out[a:a + n] = o.transpose(0, 1).reshape(n, Hq * hd).to(qkv.dtype)
-    return out, lse
+    return out, lse, torch.empty((0, Hq * hd), dtype=torch.int8)
 
 
 def _aligned(t: Tensor) -> Tensor:
@@ -162,23 +164,25 @@ def _aligned(t: Tensor) -> Tensor:
 
 
 @packed_attention_fwd.register_fake
-def _(qkv, table, longest, work, Hq, Hkv, hd, scale):
+def _(qkv, table, longest, work, Hq, Hkv, hd, scale, keep):
     return (qkv.new_empty((qkv.shape[0], Hq * hd)),
-            qkv.new_empty((Hq, (table.shape[0] - 1) * BLOCK), dtype=torch.float32))
+            qkv.new_empty((Hq, (table.shape[0] - 1) * BLOCK), dtype=torch.float32),
+            qkv.new_empty((qkv.shape[0] if keep else 0, Hq * hd), dtype=torch.int8))
 
 
-def _setup(ctx, inputs, output):
-    qkv, table, longest, work, Hq, Hkv, hd, scale = inputs
-    out, lse = output
+def _forward(ctx, qkv, table, longest, work, Hq, Hkv, hd, scale, _keep):
+    out, lse, rest = packed_attention_fwd(qkv, table, longest, work, Hq, Hkv, hd, scale, True)
+    ctx.set_materialize_grads(False)
     ctx.cfg = (longest, work, Hq, Hkv, hd, scale)
-    ctx.mark_non_differentiable(lse)
-    ctx.save_for_backward(qkv, table, out, lse)
+    ctx.mark_non_differentiable(lse, rest)
+    ctx.save_for_backward(qkv, table, out, lse, rest)
+    return out, lse, rest
 
 
-def _backward(ctx, dout, _dlse):
+def _backward(ctx, dout, _dlse, _drest):
     longest, work, Hq, Hkv, hd, scale = ctx.cfg
-    qkv, table, out, lse = ctx.saved_tensors
-    none = (None,) * 7
+    qkv, table, out, lse, rest = ctx.saved_tensors
+    none = (None,) * 8
     if dout is None:
         return torch.zeros_like(qkv), *none
     if _is_native(qkv):
@@ -186,7 +190,7 @@ def _backward(ctx, dout, _dlse):
         dqkv = torch.empty_like(qc)
         floats = native.lib().attn_packed_bwd_floats(table.shape[0] - 1, longest, work, Hq, Hkv, hd)
         scratch = torch.empty(floats, dtype=torch.float32, device=qkv.device)
-        native.lib().attn_packed_bwd(qc, table, _aligned(out), _aligned(dout), _aligned(lse), scratch, dqkv, longest, work, Hq,
+        native.lib().attn_packed_bwd(qc, table, _aligned(out), _aligned(rest), _aligned(dout), _aligned(lse), scratch, dqkv, longest, work, Hq,
                                      Hkv, hd, scale, native.status_tensor(qkv.device))
         return once_differentiable("packed_attention", dqkv, qkv), *none
     dqkv = torch.zeros_like(qkv, memory_format=torch.contiguous_format)
@@ -199,7 +203,7 @@ def _backward(ctx, dout, _dlse):
     return once_differentiable("packed_attention", dqkv, qkv), *none
 
 
-packed_attention_fwd.register_autograd(_backward, setup_context=_setup)
+packed_attention_fwd.register_autograd(_backward, forward=_forward)
 packed_attention_fwd = packed_attention_fwd.overload
 
 
@@ -213,10 +217,10 @@ def packed_attention(qkv: Tensor, sequences: PackedSequences, Hq: int, Hkv: int,
     if qkv.dim() != 2 or qkv.shape[0] != sequences.tokens:
         raise ValueError(f"packed_attention: qkv is {tuple(qkv.shape)}, the batch has {sequences.tokens} tokens")
     if qkv.is_cuda:                              # the op makes the checks below by itself
-        return packed_attention_fwd(qkv, sequences.table, sequences.longest, sequences.work, Hq, Hkv, hd, scale)[0]
+        return packed_attention_fwd(qkv, sequences.table, sequences.longest, sequences.work, Hq, Hkv, hd, scale, False)[0]
     if Hq < 1 or Hkv < 1 or Hq % Hkv or qkv.shape[1] != (Hq + 2 * Hkv) * hd:
         raise ValueError(f"packed_attention: qkv must be [T, (Hq + 2 Hkv) * hd] with whole groups of heads, got "
                          f"{tuple(qkv.shape)} for {Hq} / {Hkv} heads of {hd}")
     if sequences.table.device != qkv.device:
         raise ValueError(f"packed_attention: sequences are on {sequences.table.device}, qkv on {qkv.device}")
-    return packed_attention_fwd(qkv, sequences.table, sequences.longest, sequences.work, Hq, Hkv, hd, scale)[0]
+    return packed_attention_fwd(qkv, sequences.table, sequences.longest, sequences.work, Hq, Hkv, hd, scale, False)[0]

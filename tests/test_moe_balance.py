@@ -244,7 +244,15 @@ def test_a_model_with_a_balance_loss(device):
     route = torch.autograd.grad((layers[0](x) * dy).sum(), layers[0].gate.weight)[0].double().abs()
     tol = half * 4 * (size.cpu() + grads[0].abs() + grads[1].abs() + route.cpu()) + half * 4 * _route_size(layers[0], x, dy)
     assert bool(((grads[1] - grads[0] - want).abs() <= tol).all())
-    assert float(want.abs().max()) > 10 * float(tol.min())
+    if device == "cpu":                          # in bf16 the roundings of the model's own gradient are larger than what is added to it
+        assert float(want.abs().max()) > 10 * float(tol.min())
+    # nothing of the model's own: the gradient of the balance loss alone
+    layers[1].zero_grad()
+    (layers[1](x) * torch.zeros_like(dy)).sum().backward()
+    got = layers[1].gate.weight.grad.double().cpu()
+    assert bool(((got - want).abs() <= half * 4 * size.cpu() + half * want.abs()).all())
+    worst, least = float((half * 4 * size.cpu() + half * want.abs()).max()), float(want.abs().max())
+    assert least > 4 * worst
 
 
 def _route_size(layer, x, dy):
