@@ -175,8 +175,8 @@ struct FwdBars {
 
 // ONE: one tile per CTA, else tiles_per_cta, two.  A constant for the one case only: the loops of two tiles lose 0.6 % both to
 // the other case's decisions and with their own number as a constant (1 x 8192, 32 / 4 heads x 128, 523.5 and 526.6 us).
-// PACKED: S is the padded length 128 * B of lse, B the blocks in the table's memory; a CTA has one tile or, where the group is
-// even, two heads of the group on the same rows.  CTAs behind the last block's set the rows behind the last sequence to zero.
+// PACKED: S is the padded length 128 * B of lse, B the blocks in the table's memory; a CTA has one tile or two heads of the group
+// (the last of an odd one by itself) on the same rows.  CTAs behind the last block's set the rows behind the last sequence to zero.
 template <int HD, bool ONE, bool PACKED>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_out,
@@ -199,7 +199,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
   int rem = 128;                               // rows of this block that belong to the sequence
   if constexpr (PACKED) {
     grid_wait(table);
-    const int units = ONE ? Hq : Hkv * (group / 2);
+    const int units = ONE ? Hq : Hkv * ((group + 1) / 2);
     const int entry = static_cast<int>(blockIdx.x) / units, u = static_cast<int>(blockIdx.x) % units;
     const int4 header = __ldg(table);          // blocks, end of the last sequence, rows of the batch
     e = uniform(packed_block(table, min(entry, B - 1)));    // with the header, not behind it
@@ -217,7 +217,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
     }
     g = u % Hkv;
     b = 0;
-    two = !ONE;
+    two = !ONE && 2 * (u / Hkv) + 1 < group;
     qblk0 = qblk1 = e.block;
     head0 = g * group + (ONE ? 1 : 2) * (u / Hkv);
     head1 = head0 + 1;
@@ -1563,19 +1563,22 @@ static int set_smem_here(K kern, int bytes, std::atomic<bool>* configured) {
 // and a key block.
 static int packed_tiles_per_cta(const PackedShape& p, int num_sms) {
   const long long tiles = static_cast<long long>(p.Hq) * p.blocks;
-  return p.Hq / p.Hkv % 2 != 0 || tiles <= num_sms || p.Hq * p.work <= (p.longest - 1) * num_sms ? 1 : 2;
+  return p.Hq == p.Hkv || tiles <= num_sms || p.Hq * p.work <= (p.longest - 1) * num_sms ? 1 : 2;
 }
 
+// Batches of few blocks lose more by the exchange of the parts' sums than the costs above say.  One CTA per key block against the
+// split, us of both kernels: 572 tokens in one sequence, 64 / 8 x 128 82 and 57 in four; not split: 496 in six, 64 / 8 x 128 47 and
+// 53, 8923 in fourteen, 4 / 2 x 64 45 and 55, 8192 in forty, 32 / 4 x 128 419 and 444.
 static int packed_parts(const PackedShape& p, int num_sms) {
   const long long group = p.Hq / p.Hkv;
   auto cost = [&](long long parts) {
     const long long work = (p.Hq * p.work * 5800 + p.blocks * (p.Hkv * parts + p.Hq) * 6000) / num_sms;
-    const long long longest = group / parts * 2 * p.longest * 1600 + 6000 + (parts > 1 ? 3000 + 3000 * parts : 0);
+    const long long longest = group / parts * 2 * p.longest * 1600 + 6000 + (parts > 1 ? 8000 + 6000 * parts : 0);
     return work > longest ? work : longest;
   };
   int best = 1;
   for (int parts = 2; parts <= 8 && group % parts == 0; parts *= 2)
-    if (cost(parts) * 100 < cost(best) * 97) best = parts;
+    if (cost(parts) * 100 < cost(best) * 85) best = parts;
   return best;
 }
 
@@ -1597,7 +1600,7 @@ static int attn_packed_fwd_impl(const PackedShape& p, const void* qkv, void* out
   const auto kern = one ? attn_fwd_kernel<HD, true, true> : attn_fwd_kernel<HD, false, true>;
   static std::atomic<bool> configured[2][64];
   if (set_smem_here(kern, FwdSmem<HD>::TOTAL, configured[one])) return -2;
-  const long long units = one ? p.Hq : p.Hq / 2;
+  const long long units = one ? p.Hq : static_cast<long long>(p.Hkv) * ((p.Hq / p.Hkv + 1) / 2);
   launch_overlapped(kern, static_cast<unsigned>(p.blocks * units + 32), FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse,
                     static_cast<int>(p.blocks) * 128, p.Hq, p.Hkv, static_cast<int>(p.blocks), one ? 1 : 2,
                     softmax_scale * 1.4426950408889634f, status, reinterpret_cast<const int4*>(p.table),

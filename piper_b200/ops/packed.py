@@ -99,7 +99,8 @@ def pack_sequences(offsets: Tensor, tokens: int, device: Optional[torch.device] 
         _check_offsets(values, tokens)
         counts = [_blocks(b - a) for a, b in zip(values, values[1:])]
         blocks, longest, work = sum(counts), max(counts, default=0), sum(c * (c + 1) // 2 for c in counts)
-        offsets = offsets.to(device=device if device is not None else "cpu", dtype=torch.int32)
+        # a copy of what was checked; nothing waits for its way to the device
+        offsets = torch.tensor(values, dtype=torch.int32).to("cpu" if device is None else device, non_blocking=True)
     else:
         if device is not None and torch.empty(0, device=device).device != offsets.device:
             raise ValueError(f"pack_sequences: offsets are on {offsets.device}, not on {device}")

@@ -2,6 +2,7 @@
 routers' balance losses together, in the bundled models."""
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from piper_b200 import nn, ops
 from piper_b200.ops import native
@@ -136,3 +137,98 @@ def test_positions_that_the_tables_lack_are_nan(device):
     at = s.positions()
     assert bool(torch.isnan(c[at >= 100]).all()) and bool(torch.isnan(d[at >= 100]).all()) and int((at >= 100).sum()) == 30
     assert torch.equal(c[at < 100], cos[at[at < 100]]) and torch.equal(d[at < 100], sin[at[at < 100]])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_balance_losses_through_the_engine(device):
+    """Two pipeline stages, two microbatches: every stage's routers get the gradient of their balance losses, the losses that come back
+    are the model's own."""
+    from piper_b200 import piper_exec_dag, piper_setup
+    from piper_b200.models.qwen3 import PiperQwen3Model, Qwen3Config
+    from piper_b200.runtime.storage import init_tensor
+
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    cfg = Qwen3Config(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=64, vocab_size=VOCAB, num_experts=8, top_k=2,
+                      moe_hidden=128, balance_coef=1.5)
+    g = torch.Generator().manual_seed(5)
+    x, y = (torch.randint(0, VOCAB, (4, 128), generator=g) for _ in range(2))
+    schedule = [{"op": "place", "filter": {"PP": i}, "devices": [0]} for i in range(2)] + \
+        [{"op": "split", "filter": {}, "dim_name": "MB", "num_microbatches": 2}]
+    actor = piper_setup(PiperQwen3Model, (cfg, 2, 128), optim_fn=torch.optim.AdamW, example_inputs=[x], example_outputs=y,
+                        model_dtype=dtype, const_attrs=PiperQwen3Model.const_attrs(cfg, 128), schedule_directives=schedule,
+                        device=device)
+    actor.debug_keep_grads = True
+    model = PiperQwen3Model(cfg, 2, 128).to(device).to(dtype)
+    consts = PiperQwen3Model.const_attrs(cfg, 128, device)
+    model.rope_cos, model.rope_sin = consts["rope_cos"], consts["rope_sin"]
+    with torch.no_grad():
+        for n, p in model.named_parameters():
+            p.copy_(init_tensor(n, p.shape, dtype, torch.device(device)))
+    losses = [float(v) for v in piper_exec_dag(nn.cross_entropy_loss)]
+    got = {k: v.float() for k, v in actor.last_grads.items()}
+    want = []
+    for a, b in zip(x.to(device).split(2), y.to(device).split(2)):
+        loss = nn.cross_entropy_loss(model(a), b)
+        want.append(float(loss.detach()))
+        loss.backward()
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -20
+    # the same ops on the same microbatches: weight gradients of both summed in another order, two roundings of autograd's sum
+    assert all(abs(a - b) <= 2.0 ** -20 * abs(b) for a, b in zip(losses, want)), (losses, want)
+    for n, p in model.named_parameters():
+        a, b = got[n], p.grad.float() / 2
+        assert float((a - b).norm()) <= 3 * half * float(b.norm()) + 1e-8, n
+    plain = PiperQwen3Model(Qwen3Config(**{**cfg.__dict__, "balance_coef": 0.0}), 2, 128).to(device).to(dtype)
+    plain.load_state_dict(model.state_dict())
+    plain.rope_cos, plain.rope_sin = model.rope_cos, model.rope_sin
+    nn.cross_entropy_loss(plain(x.to(device)), y.to(device)).backward()
+    for i in range(2):                           # both stages' routers differ from those without balance losses
+        a, b = got[f"layers.{i}.moe.gate.weight"], plain.layers[i].moe.gate.weight.grad.float()
+        assert float((a - b).norm()) > 0.05 * float(a.norm())
+    if device == "cuda":
+        native.check_status()
+
+
+def test_full_graph_capture_records_the_ops():
+    s = ops.pack_sequences(torch.tensor([0, 5, 14]), 16)
+    g = torch.Generator().manual_seed(6)
+    qkv, new, old, adv = (torch.randn(*shape, generator=g) for shape in ((16, 4 * 8), (16,), (16,), (16,)))
+    logits = torch.randn(16, 4, generator=g)
+    idx = torch.randint(0, 4, (16, 2), generator=g, dtype=torch.int32)
+
+    def f(qkv, new, logits):
+        out = ops.packed_attention(qkv, s, 2, 1, 8, 0.3).square().sum()
+        loss = ops.clipped_policy_loss(new, old, adv, ref_logprob=old, sequences=s, kl_coef=0.1).loss
+        return out + loss + ops.moe.moe_balance_loss(logits, idx).loss
+
+    leaves = [t.requires_grad_(True) for t in (qkv, new, logits)]
+    want = torch.autograd.grad(f(*leaves), leaves)
+    # the graph of the forward pass, as the engine records it; a tracer of backward passes would need formulas that do not read tables
+    compiled = torch.compile(f, backend="eager", fullgraph=True)
+    for a, b in zip(torch.autograd.grad(compiled(*leaves), leaves), want):
+        assert torch.allclose(a, b)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_under_recomputing_checkpoints(device):
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    s = ops.pack_sequences(torch.tensor([0, 70, 200]), 210, device=device)
+    g = torch.Generator().manual_seed(7)
+    qkv = torch.randn(210, 4 * 64, generator=g).to(dtype).to(device).requires_grad_(True)
+    new, old, adv = (torch.randn(210, generator=g).to(device) for _ in range(3))
+    new.requires_grad_(True)
+    logits = torch.randn(210, 8, generator=g).to(dtype).to(device).requires_grad_(True)
+
+    def block(qkv, new, logits):
+        _w, idx, _c = ops.moe.moe_route(logits * 1.0, 2, True)
+        out = ops.packed_attention(qkv * 1.0, s, 2, 1, 64, 0.125).float().sum()
+        loss = ops.clipped_policy_loss(new * 1.0, old, adv, sequences=s).loss
+        return out + loss + ops.moe.moe_balance_loss(logits * 1.0, idx).loss
+
+    leaves = [qkv, new, logits]
+    want = torch.autograd.grad(block(*leaves), leaves)
+    for reentrant in (False, True):
+        out = torch.utils.checkpoint.checkpoint(block, *leaves, use_reentrant=reentrant)
+        for t in leaves:
+            t.grad = None
+        out.backward()
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
