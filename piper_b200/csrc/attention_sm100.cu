@@ -75,17 +75,96 @@ __device__ __forceinline__ void store_row_chunk_sw128(uint8_t* tile, int row, in
 }
 
 // ----------------------------------------------------------- packed batches
+// Short sequences: neighbours that fit one block share it.  A row then sees the keys from the first row of its own sequence on; what
+// is masked has a probability of exactly 0 and, chosen so, a score gradient of 0.  But a product contracts over all rows of the
+// block, and 0 times an infinity or NaN of another sequence is NaN: rows whose results are not finite are computed again, of
+// their own sequence alone, by a thread each (repair_*), so that nothing of one sequence reaches another here either.
+// 2,563 tokens in 91 sequences: 93 blocks without groups, 26 with.  Batches with groups have kernels of their own (kGroups): what
+// they do in addition takes 7 % of the time of those without (1 x 4096, 32 / 8 heads x 128, backward 406 and 432 us).
+enum Mode : int { kEqual = 0, kPacked = 1, kGroups = 2 };       // sequences of one length; packed; packed with groups
+
 // What a CTA needs of a row of the table.
 struct PackedBlock {
   int tok0;                    // first row of the sequence
   int len;                     // its rows
   int block;                   // block of 128 rows in it; query blocks have block + 1 key blocks
-  int pad0;                    // where its lse and delta begin
+  int pad0;                    // where its lse and delta begin; kGroup is added for a group
+  __device__ int place() const { return pad0 & ~kGroup; }
+  __device__ bool group() const { return (pad0 & kGroup) != 0; }
 };
 
 __device__ __forceinline__ PackedBlock packed_block(const int4* table, int entry) {
   const int4 e = __ldg(table + 1 + entry);
   return {e.x, e.y, e.z, e.w};
+}
+
+// First and last row, in the group, of the sequence of row i of a group.
+__device__ __forceinline__ uchar2 own_rows(const uchar2* own, const PackedBlock& e, int i) { return __ldg(own + e.place() + i); }
+
+__device__ __forceinline__ bool not_finite(uint32_t bits) { return (bits & 0x7f800000u) == 0x7f800000u; }
+
+template <int HD>
+__device__ float dot_rows(const __nv_bfloat16* a, const __nv_bfloat16* b) {
+  float s = 0.f;
+  for (int d = 0; d < HD; ++d) s = fmaf(__bfloat162float(a[d]), __bfloat162float(b[d]), s);
+  return s;
+}
+
+// A row of queries of one head against keys k, v [n] of its sequence, `stride` elements apart.
+template <int HD>
+__device__ __noinline__ void repair_out(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v, int n, long long stride,
+                                        float scale, __nv_bfloat16* out, signed char* rest, float* lse) {
+  float top = -INFINITY, sum = 0.f;
+  bool nan = false;
+  for (int j = 0; j < n; ++j) {
+    const float s = dot_rows<HD>(q, k + j * stride) * scale;
+    nan |= isnan(s);
+    top = fmaxf(top, s);
+  }
+  for (int j = 0; j < n; ++j) sum += expf(dot_rows<HD>(q, k + j * stride) * scale - top);
+  if (nan) sum = NAN;
+  for (int d = 0; d < HD; ++d) {
+    float o = 0.f;
+    for (int j = 0; j < n; ++j)
+      o = fmaf(expf(dot_rows<HD>(q, k + j * stride) * scale - top), __bfloat162float(v[j * stride + d]), o);
+    out[d] = __float2bfloat16(o / sum);
+    if (rest != nullptr) rest[d] = 0;
+  }
+  *lse = top + logf(sum);
+}
+
+// 64 columns of the gradient of that row of queries: d_out, out row's delta and lse, columns `k64` of the keys.
+template <int HD>
+__device__ __noinline__ void repair_dq(const __nv_bfloat16* q, const __nv_bfloat16* d_out, const __nv_bfloat16* k,
+                                       const __nv_bfloat16* v, int n, long long stride, int k64, float scale, float lse, float delta,
+                                       __nv_bfloat16* dq) {
+  for (int d = 0; d < 64; ++d) {
+    float s = 0.f;
+    for (int j = 0; j < n; ++j) {
+      const float p = expf(dot_rows<HD>(q, k + j * stride) * scale - lse);
+      s = fmaf(p * (dot_rows<HD>(d_out, v + j * stride) - delta), __bfloat162float(k[j * stride + k64 + d]), s);
+    }
+    dq[d] = __float2bfloat16(s * scale);
+  }
+}
+
+// 64 columns from `c64` of the gradient of a row of keys (is_k) or values: queries q, d_out [n] of its sequence from that row on, of
+// `heads` heads; lse and delta [heads][n], `padded` apart.
+template <int HD>
+__device__ __noinline__ void repair_dkv(const __nv_bfloat16* k, const __nv_bfloat16* v, const __nv_bfloat16* q, const __nv_bfloat16* d_out,
+                                        int n, int heads, long long q_stride, long long o_stride, bool is_k, int c64, float scale,
+                                        const float* lse, const float* delta, long long padded, __nv_bfloat16* out) {
+  for (int d = 0; d < 64; ++d) {
+    float s = 0.f;
+    for (int h = 0; h < heads; ++h)
+      for (int i = 0; i < n; ++i) {
+        const __nv_bfloat16 *qi = q + i * q_stride + h * HD, *di = d_out + i * o_stride + h * HD;
+        const float p = expf(dot_rows<HD>(qi, k) * scale - lse[h * padded + i]);
+        if (is_k) s = fmaf(p * (dot_rows<HD>(di, v) - delta[h * padded + i]) * scale, __bfloat162float(qi[c64 + d]), s);
+        else s = fmaf(p, __bfloat162float(di[c64 + d]), s);
+      }
+    out[d] = __float2bfloat16(s);
+  }
 }
 
 // The same, known to the compiler as equal for a warp's lanes.
@@ -177,13 +256,14 @@ struct FwdBars {
 // the other case's decisions and with their own number as a constant (1 x 8192, 32 / 4 heads x 128, 523.5 and 526.6 us).
 // PACKED: S is the padded length 128 * B of lse, B the blocks in the table's memory; a CTA has one tile or two heads of the group
 // (the last of an odd one by itself) on the same rows.  CTAs behind the last block's set the rows behind the last sequence to zero.
-template <int HD, bool ONE, bool PACKED>
+template <int HD, bool ONE, int MODE>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant__ CUtensorMap tmap_out,
                 float* __restrict__ lse, int S, int Hq, int Hkv, int B, int tiles_per_cta, float scale_log2,
-                int* status, const int4* __restrict__ table, __nv_bfloat16* __restrict__ out, signed char* __restrict__ rest,
-                int T) {
+                int* status, const int4* __restrict__ table, const uchar2* __restrict__ own,
+                const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ out, signed char* __restrict__ rest, int T) {
   using L = FwdSmem<HD>;
+  constexpr bool PACKED = MODE != kEqual, GROUPS = MODE == kGroups;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -198,7 +278,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
   PackedBlock e = {0, 0, 0, 0};
   int rem = 128;                               // rows of this block that belong to the sequence
   if constexpr (PACKED) {
-    grid_wait(table);
+    grid_wait(table, own, qkv);
     const int units = ONE ? Hq : Hkv * ((group + 1) / 2);
     const int entry = static_cast<int>(blockIdx.x) / units, u = static_cast<int>(blockIdx.x) % units;
     const int4 header = __ldg(table);          // blocks, end of the last sequence, rows of the batch
@@ -263,7 +343,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
     tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish();
   }
-  grid_wait(table);
+  grid_wait(table, own, qkv);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -457,6 +537,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 128; ++i)
           if (i > row) sv[i / 32][i % 32] = 0xff800000u;
+        if (GROUPS && e.group()) {
+          const int first = row < rem ? own_rows(own, e, row).x : 0;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i < first) sv[i / 32][i % 32] = 0xff800000u;
+        }
       }
       float mx[4];
 #pragma unroll
@@ -538,6 +624,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
       // the tile's Q operand has been read for the last time; its buffer takes the output, 32 rows per warp
       tc_fence_after();
       const float inv = 1.f / l_run;
+      bool bad = false;
       const float2 fa = make_float2(wa * inv, wa * inv), fb = make_float2(wb * inv, wb * inv);
       uint8_t* obuf = smem + L::Q_OFF + t * L::TILE;
 #pragma unroll
@@ -556,6 +643,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
           w[i] = pack_bf16x2(v.x, v.y);
           r[2 * i] = __float_as_uint(v.x);
           r[2 * i + 1] = __float_as_uint(v.y);
+          if (GROUPS) bad |= not_finite(r[2 * i]) || not_finite(r[2 * i + 1]);
         }
         if (PACKED && rest != nullptr) {
           uint32_t lost[8];
@@ -572,7 +660,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
             dst[1] = make_uint4(lost[4], lost[5], lost[6], lost[7]);
           }
         }
-        if (PACKED && rem < 128) {
+        if (PACKED && (rem < 128 || (GROUPS && e.group()))) {
           if (row < rem) store_row_chunk(out + ((tok0 + qblk * 128 + row) * Hq + head) * HD + c * 32, w);
           continue;
         }
@@ -580,10 +668,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
       }
       float log_sum = m_run * (scale_log2 * 0.6931471805599453f) + logf(l_run);
       if (PACKED && row >= rem) log_sum = INFINITY;      // probabilities of zero in the backward pass
-      lse[(static_cast<long long>(b) * Hq + head) * S + (PACKED ? e.pad0 : 0) + qblk * 128 + row] = log_sum;
+      float* const lse_at = lse + (static_cast<long long>(b) * Hq + head) * S + (PACKED ? e.place() : 0) + qblk * 128 + row;
+      *lse_at = log_sum;
+      if (GROUPS && e.group() && bad && row < rem) {
+        const int first = own_rows(own, e, row).x;
+        const long long stride = static_cast<long long>(Hq + 2 * Hkv) * HD, o = ((tok0 + row) * Hq + head) * HD;
+        const __nv_bfloat16* k = qkv + (tok0 + first) * stride + static_cast<long long>(Hq + g) * HD;
+        repair_out<HD>(qkv + (tok0 + row) * stride + head * HD, k, k + static_cast<long long>(Hkv) * HD, row + 1 - first, stride,
+                       scale_log2 * 0.6931471805599453f, out + o, rest == nullptr ? nullptr : rest + o, lse_at);
+      }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && (!PACKED || rem == 128)) {
+      if (lane == 0 && (!PACKED || (rem == 128 && !(GROUPS && e.group())))) {
         for (int h = 0; h < L::HALVES; ++h)
           tma_store_2d_bulk(&tmap_out, obuf + h * 16384 + (warp & 3) * 32 * 128, head * HD + 64 * h,
                             static_cast<int>(tok0) + qblk * 128 + (warp & 3) * 32);
@@ -661,7 +757,7 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const signed char*
     const PackedBlock e = packed_block(table, (at_once > 1 ? r : r0) / 128);
     const int i = e.block * 128 + (at_once > 1 ? r : r0) % 128;
     for (int h = at_once > 1 ? group % Hq : group; h < Hq; h += GROUPS) {
-      float* const to = delta + static_cast<long long>(h) * S + e.pad0 + i;
+      float* const to = delta + static_cast<long long>(h) * S + e.place() + i;
       if (i >= e.len) {                        // beside probabilities of zero
         if (lane == 0) *to = 0.f;
         continue;
@@ -689,6 +785,13 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const signed char*
   uint4* const dst = reinterpret_cast<uint4*>(d_qkv) + header.y * row;
   for (long long i = thread; i < behind; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
 }
+
+// What the backward CTAs of a packed batch need beside tensor maps.
+struct PackedArgs {
+  const uchar2* own;
+  const __nv_bfloat16 *qkv, *d_out;
+  __nv_bfloat16* d_qkv;
+};
 
 // The dK/dV pass streams 64-row tiles through two tensor memory stages (dK, dV and two 64-wide pairs of S' and dP' fill
 // it).  Warps 0-7 turn the even tiles' scores into probabilities and score gradients, warps 8-15 the odd tiles' (four warps
@@ -740,15 +843,15 @@ struct BwdBars {
 // dK and dV of key block xb of kv head g.  The query heads of the group may be split over `parts` CTAs; each accumulates over
 // its own and leaves its sums in `partial` ([part][slice of 64 columns][column][row]), and the one that finishes last
 // (by `arrived`, no CTA waits) adds them in the order of the parts, so the gradients are reproducible.
-template <int HD, bool PACKED>
+template <int HD, int MODE>
 __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, const CUtensorMap* tmap_qkv_y,
                                              const CUtensorMap* tmap_do_y, const CUtensorMap* tmap_dqkv,
                                              const float* __restrict__ lse, const float* __restrict__ delta, int xb,
                                              int g, int b, int part, int parts, float* __restrict__ partial,
                                              int* __restrict__ arrived, int S, int Hq, int Hkv, float scale,
-                                             float scale_log2, int* status, const PackedBlock e,
-                                             __nv_bfloat16* __restrict__ d_qkv) {
+                                             float scale_log2, int* status, const PackedBlock e, const PackedArgs& args) {
   using L = BwdSmem<HD>;
+  constexpr bool PACKED = MODE != kEqual, GROUPS = MODE == kGroups;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -824,7 +927,7 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
           tma_load_2d(y1, tmap_qkv_y, full, hh * HD + 64 * h, yrow);
           tma_load_2d(y2, tmap_do_y, full, hh * HD + 64 * h, yrow);
         }
-        const long long idx = (static_cast<long long>(b) * Hq + hh) * S + (PACKED ? e.pad0 : 0) + ti * 64;
+        const long long idx = (static_cast<long long>(b) * Hq + hh) * S + (PACKED ? e.place() : 0) + ti * 64;
         uint8_t* v = smem + L::VEC_OFF + st * 2 * L::VEC_BYTES;
         bulk_load(v, lse + idx, L::VEC_BYTES, full);
         bulk_load(v + L::VEC_BYTES, delta + idx, L::VEC_BYTES, full);
@@ -966,6 +1069,16 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
           for (int i = 0; i < 16; ++i)
             if (xpos + 16 * h + 8 * ((i >> 1) & 1) > ypos0 + 8 * (i >> 2) + c0 + (i & 1)) sv[h][i] = 0xff800000u;
       }
+      if (GROUPS && e.group()) {               // queries behind the key's own sequence
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uchar2 a = own_rows(args.own, e, min(xpos + 16 * h, e.len - 1));
+          const uchar2 b2 = own_rows(args.own, e, min(xpos + 16 * h + 8, e.len - 1));
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (ypos0 + 8 * (i >> 2) + c0 + (i & 1) > ((i >> 1) & 1 ? b2.y : a.y)) sv[h][i] = 0xff800000u;
+        }
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -1000,6 +1113,7 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
           const uint32_t* p = &sv[h][2 * i];
           float2 d = fma2(dl[i >> 1], neg_one, make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])));
           d = mul2(d, make_float2(__uint_as_float(p[0]), __uint_as_float(p[1])));
+          if (GROUPS && e.group()) d = make_float2(p[0] == 0 ? 0.f : d.x, p[1] == 0 ? 0.f : d.y);
           w[i] = pack_bf16x2(d.x, d.y);
         }
         tmem_st_16x128b_x4(td + h * kUpper, w);
@@ -1052,6 +1166,7 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
     const float sc = is_k ? scale : 1.f;
     const int col = (Hq + (is_k ? 0 : Hkv) + g) * HD + 64 * h;
     const int x_rem = PACKED ? min(128, e.len - xb * 128) : 128;
+    bool bad = false;
 #pragma unroll 1
     for (int c = 0; c < 2; ++c) {
       uint32_t r[32], w[16];
@@ -1070,16 +1185,27 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * sc, __uint_as_float(r[2 * i + 1]) * sc);
-      if (PACKED && x_rem < 128) {
+      if (PACKED && (x_rem < 128 || (GROUPS && e.group()))) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) bad |= GROUPS && not_finite(r[i]);
         if (row < x_rem)
-          store_row_chunk(d_qkv + static_cast<long long>(tok0 + xb * 128 + row) * (Hq + 2 * Hkv) * HD + col + c * 32, w);
+          store_row_chunk(args.d_qkv + static_cast<long long>(tok0 + xb * 128 + row) * (Hq + 2 * Hkv) * HD + col + c * 32, w);
         continue;
       }
       store_row_chunk_sw128(obuf, row, c * 4, w);
     }
+    if (GROUPS && e.group() && bad && row < x_rem) {
+      const int n = own_rows(args.own, e, row).y + 1 - row, head = g * (Hq / Hkv);
+      const long long stride = static_cast<long long>(Hq + 2 * Hkv) * HD, at = static_cast<long long>(head) * S + e.place() + row;
+      const __nv_bfloat16* q = args.qkv + (tok0 + row) * stride;
+      repair_dkv<HD>(q + (Hq + g) * HD, q + (Hq + Hkv + g) * HD, q + head * HD,
+                     args.d_out + (static_cast<long long>(tok0 + row) * Hq + head) * HD, n, Hq / Hkv, stride,
+                     static_cast<long long>(Hq) * HD, is_k, 64 * h, scale, lse + at, delta + at, S,
+                     args.d_qkv + (tok0 + row) * stride + col);
+    }
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0 && (!PACKED || x_rem == 128)) {
+    if (lane == 0 && (!PACKED || (x_rem == 128 && !(GROUPS && e.group())))) {
       tma_store_2d_bulk(tmap_dqkv, obuf + (warp & 3) * 32 * 128, col, tok0 + xb * 128 + (warp & 3) * 32);
       bulk_commit_group();
       bulk_wait_group<0>();
@@ -1121,13 +1247,14 @@ struct DqBars {
   uint32_t tmem_base;
 };
 
-template <int HD, bool PACKED>
+template <int HD, int MODE>
 __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const CUtensorMap* tmap_do_x,
                                             const CUtensorMap* tmap_dqkv, const float* __restrict__ lse,
                                             const float* __restrict__ delta, int xb, int hy, int b, int S, int Hq,
                                             int Hkv, float scale, float scale_log2, int* status, const PackedBlock e,
-                                            __nv_bfloat16* __restrict__ d_qkv) {
+                                            const PackedArgs& args) {
   using L = DqSmem<HD>;
+  constexpr bool PACKED = MODE != kEqual, GROUPS = MODE == kGroups;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -1277,7 +1404,7 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t td = tmem_base + lane_sel + 256 + wg * 32;
     const float2 sl2 = make_float2(scale_log2, scale_log2);
-    const long long idx = (static_cast<long long>(b) * Hq + hy) * S + (PACKED ? e.pad0 : 0) + xb * 128 + row;
+    const long long idx = (static_cast<long long>(b) * Hq + hy) * S + (PACKED ? e.place() : 0) + xb * 128 + row;
     const float nl = lse[idx] * -1.4426950408889634f, ndl = -delta[idx];
     const float2 nl2 = make_float2(nl, nl), ndl2 = make_float2(ndl, ndl);
     bool ok = true;
@@ -1292,6 +1419,12 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           if (wg * 32 + i > row) sv[i] = 0xff800000u;
+        if (GROUPS && e.group()) {
+          const int first = row < rem ? own_rows(args.own, e, row).x : 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (wg * 32 + i < first) sv[i] = 0xff800000u;
+        }
       }
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
@@ -1308,6 +1441,7 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
       for (int i = 0; i < 16; ++i) {
         float2 d = add2(make_float2(__uint_as_float(dv[2 * i]), __uint_as_float(dv[2 * i + 1])), ndl2);
         d = mul2(d, make_float2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])));
+        if (GROUPS && e.group()) d = make_float2(sv[2 * i] == 0 ? 0.f : d.x, sv[2 * i + 1] == 0 ? 0.f : d.y);
         dw[i] = pack_bf16x2(d.x, d.y);
       }
       tmem_st_32x16(td, dw);                   // over columns this thread has already read
@@ -1320,6 +1454,7 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
       tc_fence_after();
       const uint32_t ta = tmem_base + lane_sel + 384 + wg * 64;
       uint8_t* obuf = smem + L::X1_OFF + wg * 16384;
+      bool bad = false;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t r[32], w[16];
@@ -1328,16 +1463,26 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           w[i] = pack_bf16x2(__uint_as_float(r[2 * i]) * scale, __uint_as_float(r[2 * i + 1]) * scale);
-        if (PACKED && rem < 128) {
+        if (PACKED && (rem < 128 || (GROUPS && e.group()))) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) bad |= GROUPS && not_finite(r[i]);
           if (row < rem)
-            store_row_chunk(d_qkv + static_cast<long long>(tok0 + xb * 128 + row) * (Hq + 2 * Hkv) * HD + hy * HD + 64 * wg + c * 32, w);
+            store_row_chunk(args.d_qkv + static_cast<long long>(tok0 + xb * 128 + row) * (Hq + 2 * Hkv) * HD + hy * HD + 64 * wg + c * 32, w);
           continue;
         }
         store_row_chunk_sw128(obuf, row, c * 4, w);
       }
+      if (GROUPS && e.group() && bad && row < rem) {
+        const int first = own_rows(args.own, e, row).x;
+        const long long stride = static_cast<long long>(Hq + 2 * Hkv) * HD, at = (tok0 + row) * stride + hy * HD;
+        const __nv_bfloat16* k = args.qkv + (tok0 + first) * stride + static_cast<long long>(Hq + g) * HD;
+        repair_dq<HD>(args.qkv + at, args.d_out + (static_cast<long long>(tok0 + row) * Hq + hy) * HD, k,
+                      k + static_cast<long long>(Hkv) * HD, row + 1 - first, stride, 64 * wg, scale, lse[idx], delta[idx],
+                      args.d_qkv + at + 64 * wg);
+      }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0 && (!PACKED || rem == 128)) {
+      if (lane == 0 && (!PACKED || (rem == 128 && !(GROUPS && e.group())))) {
         tma_store_2d_bulk(tmap_dqkv, obuf + (warp & 3) * 32 * 128, hy * HD + 64 * wg,
                           tok0 + xb * 128 + (warp & 3) * 32);
         bulk_commit_group();
@@ -1358,8 +1503,8 @@ __device__ __forceinline__ void attn_dq_cta(const CUtensorMap* tmap_qkv_x, const
 // SM per CTA; the dK/dV CTAs are few and of very different lengths (with grouped heads up to group x S/64 tiles),
 // so they start first, longest first, and the many shorter dQ CTAs fill the SMs they leave.
 // PACKED: S is the padded length 128 * B of lse and delta, B the blocks in the table's memory.
-template <int HD, bool PACKED>
-__global__ void __launch_bounds__(PACKED ? BWD_PACKED_THREADS : BWD_THREADS, 1)
+template <int HD, int MODE>
+__global__ void __launch_bounds__(MODE != kEqual ? BWD_PACKED_THREADS : BWD_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 128} over packed qkv
                 const __grid_constant__ CUtensorMap tmap_qkv_y,   // box {64, 64}  over packed qkv
                 const __grid_constant__ CUtensorMap tmap_do_x,    // box {64, 128} over dO [T, Hq*hd]
@@ -1367,10 +1512,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 12
                 const __grid_constant__ CUtensorMap tmap_dqkv,    // box {64, 32}  over d_qkv
                 const float* __restrict__ lse, const float* __restrict__ delta, int B, int S, int Hq, int Hkv,
                 int parts, float* __restrict__ partial, int* __restrict__ arrived, float scale, float scale_log2,
-                int* status, const int4* __restrict__ table, __nv_bfloat16* __restrict__ d_qkv, int T) {
+                int* status, const int4* __restrict__ table, const uchar2* __restrict__ own,
+                const __nv_bfloat16* __restrict__ qkv, const __nv_bfloat16* __restrict__ d_out,
+                __nv_bfloat16* __restrict__ d_qkv, int T) {
   int idx = blockIdx.x;
-  if constexpr (PACKED) {
-    grid_wait(lse, delta, table);
+  if constexpr (MODE != kEqual) {
+    grid_wait(lse, delta, table, own, qkv, d_out);
+    const PackedArgs args = {own, qkv, d_out, d_qkv};
     const int n_kv = B * Hkv * parts;
     const int entry = idx < n_kv ? idx / parts / Hkv : (idx - n_kv) / Hq;
     const int4 header = __ldg(table);
@@ -1380,12 +1528,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 12
       // of a sequence of n blocks, key block n - 1 - i has as many query blocks as query block i has key blocks
       const int part = idx % parts;
       idx /= parts;
-      attn_dkv_cta<HD, true>(&tmap_qkv_x, &tmap_qkv_y, &tmap_do_y, &tmap_dqkv, lse, delta, (e.len + 127) / 128 - 1 - e.block,
+      attn_dkv_cta<HD, MODE>(&tmap_qkv_x, &tmap_qkv_y, &tmap_do_y, &tmap_dqkv, lse, delta, (e.len + 127) / 128 - 1 - e.block,
                              idx % Hkv, 0, part, parts, partial + static_cast<long long>(idx) * parts * HD * 256, arrived + idx, S,
-                             Hq, Hkv, scale, scale_log2, status, e, d_qkv);
+                             Hq, Hkv, scale, scale_log2, status, e, args);
     } else {
-      attn_dq_cta<HD, true>(&tmap_qkv_x, &tmap_do_x, &tmap_dqkv, lse, delta, e.block, (idx - n_kv) % Hq, 0, S, Hq, Hkv, scale,
-                            scale_log2, status, e, d_qkv);
+      attn_dq_cta<HD, MODE>(&tmap_qkv_x, &tmap_do_x, &tmap_dqkv, lse, delta, e.block, (idx - n_kv) % Hq, 0, S, Hq, Hkv, scale,
+                            scale_log2, status, e, args);
     }
     return;
   }
@@ -1395,14 +1543,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 12
     const int part = idx % parts;
     idx /= parts;
     const int hb = idx % (Hkv * B);
-    attn_dkv_cta<HD, false>(&tmap_qkv_x, &tmap_qkv_y, &tmap_do_y, &tmap_dqkv, lse, delta, idx / (Hkv * B), hb % Hkv, hb / Hkv,
+    attn_dkv_cta<HD, kEqual>(&tmap_qkv_x, &tmap_qkv_y, &tmap_do_y, &tmap_dqkv, lse, delta, idx / (Hkv * B), hb % Hkv, hb / Hkv,
                             part, parts, partial + static_cast<long long>(idx) * parts * HD * 256, arrived + idx, S, Hq, Hkv,
-                            scale, scale_log2, status, {}, nullptr);
+                            scale, scale_log2, status, {}, {});
   } else {
     idx -= n_kv;
     const int hb = idx % (Hq * B);
-    attn_dq_cta<HD, false>(&tmap_qkv_x, &tmap_do_x, &tmap_dqkv, lse, delta, blocks - 1 - idx / (Hq * B), hb % Hq, hb / Hq, S,
-                           Hq, Hkv, scale, scale_log2, status, {}, nullptr);
+    attn_dq_cta<HD, kEqual>(&tmap_qkv_x, &tmap_do_x, &tmap_dqkv, lse, delta, blocks - 1 - idx / (Hq * B), hb % Hq, hb / Hq, S,
+                           Hq, Hkv, scale, scale_log2, status, {}, {});
   }
 }
 
@@ -1440,8 +1588,8 @@ static int attn_fwd_impl(const CUtensorMap& tm, const CUtensorMap& to, float* ls
                          float softmax_scale, int num_sms, int* status, cudaStream_t st) {
   static bool cfg = false;
   if (!cfg) {
-    if (set_smem(attn_fwd_kernel<HD, true, false>, FwdSmem<HD>::TOTAL) ||
-        set_smem(attn_fwd_kernel<HD, false, false>, FwdSmem<HD>::TOTAL))
+    if (set_smem(attn_fwd_kernel<HD, true, kEqual>, FwdSmem<HD>::TOTAL) ||
+        set_smem(attn_fwd_kernel<HD, false, kEqual>, FwdSmem<HD>::TOTAL))
       return -2;
     cfg = true;
   }
@@ -1450,9 +1598,9 @@ static int attn_fwd_impl(const CUtensorMap& tm, const CUtensorMap& to, float* ls
   const int tiles_per_cta = attn_tiles_per_cta(B, S, Hq, num_sms);
   const long long ctas = (per_head + tiles_per_cta - 1) / tiles_per_cta * Hkv * B;
   if (ctas > 0x7fffffffll) return -1;
-  launch_overlapped(tiles_per_cta == 1 ? attn_fwd_kernel<HD, true, false> : attn_fwd_kernel<HD, false, false>,
+  launch_overlapped(tiles_per_cta == 1 ? attn_fwd_kernel<HD, true, kEqual> : attn_fwd_kernel<HD, false, kEqual>,
                     static_cast<unsigned>(ctas), FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse, S, Hq, Hkv, B, tiles_per_cta,
-                    scale_log2, status, nullptr, nullptr, nullptr, 0);
+                    scale_log2, status, nullptr, nullptr, nullptr, nullptr, nullptr, 0);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -1512,7 +1660,7 @@ static int attn_bwd_impl(const void* qkv, const void* out, const void* d_out, co
   constexpr int smem = DqSmem<HD>::TOTAL > BwdSmem<HD>::TOTAL ? DqSmem<HD>::TOTAL : BwdSmem<HD>::TOTAL;
   static bool cfg = false;
   if (!cfg) {
-    if (set_smem(attn_bwd_kernel<HD, false>, smem)) return -2;
+    if (set_smem(attn_bwd_kernel<HD, kEqual>, smem)) return -2;
     cfg = true;
   }
   // scratch: a counter per key block, padded to 16 bytes, and the parts' sums
@@ -1525,9 +1673,9 @@ static int attn_bwd_impl(const void* qkv, const void* out, const void* d_out, co
       static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(d_out), delta, arrived,
       parts > 1 ? n_kv : 0, T, S, Hq);
   if (cudaGetLastError() != cudaSuccess) return -3;
-  launch_overlapped(attn_bwd_kernel<HD, false>, static_cast<unsigned>(n_kv * parts + S / 128 * Hq * B), BWD_THREADS, smem, st,
+  launch_overlapped(attn_bwd_kernel<HD, kEqual>, static_cast<unsigned>(n_kv * parts + S / 128 * Hq * B), BWD_THREADS, smem, st,
       tqx, tqy, tdx, tdy, tdq, lse, delta, B, S, Hq, Hkv, parts, partial, arrived, softmax_scale,
-      softmax_scale * 1.4426950408889634f, status, nullptr, nullptr, 0);
+      softmax_scale * 1.4426950408889634f, status, nullptr, nullptr, nullptr, nullptr, nullptr, 0);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -1597,14 +1745,17 @@ static int attn_packed_fwd_impl(const PackedShape& p, const void* qkv, void* out
   if ((rc = make_tmap_2d_bf16(&tm, qkv, W, p.T, W * 2, 64, 128)) != 0) return rc;
   if ((rc = make_tmap_2d_bf16(&to, out, Wo, p.T, Wo * 2, 64, 32)) != 0) return rc;
   const bool one = packed_tiles_per_cta(p, num_sms) == 1;
-  const auto kern = one ? attn_fwd_kernel<HD, true, true> : attn_fwd_kernel<HD, false, true>;
-  static std::atomic<bool> configured[2][64];
-  if (set_smem_here(kern, FwdSmem<HD>::TOTAL, configured[one])) return -2;
+  const bool groups = p.own != nullptr;
+  const auto kern = groups ? (one ? attn_fwd_kernel<HD, true, kGroups> : attn_fwd_kernel<HD, false, kGroups>)
+                           : (one ? attn_fwd_kernel<HD, true, kPacked> : attn_fwd_kernel<HD, false, kPacked>);
+  static std::atomic<bool> configured[4][64];
+  if (set_smem_here(kern, FwdSmem<HD>::TOTAL, configured[2 * groups + one])) return -2;
   const long long units = one ? p.Hq : static_cast<long long>(p.Hkv) * ((p.Hq / p.Hkv + 1) / 2);
   launch_overlapped(kern, static_cast<unsigned>(p.blocks * units + 32), FWD_THREADS, FwdSmem<HD>::TOTAL, st, tm, to, lse,
                     static_cast<int>(p.blocks) * 128, p.Hq, p.Hkv, static_cast<int>(p.blocks), one ? 1 : 2,
                     softmax_scale * 1.4426950408889634f, status, reinterpret_cast<const int4*>(p.table),
-                    static_cast<__nv_bfloat16*>(out), rest, p.T);
+                    reinterpret_cast<const uchar2*>(p.own), static_cast<const __nv_bfloat16*>(qkv), static_cast<__nv_bfloat16*>(out),
+                    rest, p.T);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
@@ -1637,8 +1788,10 @@ static int attn_packed_bwd_impl(const PackedShape& p, const void* qkv, const voi
   if ((rc = make_tmap_2d_bf16(&tdy, d_out, Wo, p.T, Wo * 2, 64, 64)) != 0) return rc;
   if ((rc = make_tmap_2d_bf16(&tdq, d_qkv, W, p.T, W * 2, 64, 32)) != 0) return rc;
   constexpr int smem = DqSmem<HD>::TOTAL > BwdSmem<HD>::TOTAL ? DqSmem<HD>::TOTAL : BwdSmem<HD>::TOTAL;
-  static std::atomic<bool> configured[64];
-  if (set_smem_here(attn_bwd_kernel<HD, true>, smem, configured)) return -2;
+  const bool groups = p.own != nullptr;
+  const auto kern = groups ? attn_bwd_kernel<HD, kGroups> : attn_bwd_kernel<HD, kPacked>;
+  static std::atomic<bool> configured[2][64];
+  if (set_smem_here(kern, smem, configured[groups])) return -2;
   const int S = static_cast<int>(p.blocks) * 128, parts = packed_parts(p, num_sms);
   const long long n_kv = p.blocks * p.Hkv;
   float* const delta = scratch;
@@ -1651,9 +1804,10 @@ static int attn_packed_bwd_impl(const PackedShape& p, const void* qkv, const voi
                     parts > 1 ? static_cast<int>(n_kv) : 0, table, static_cast<__nv_bfloat16*>(d_qkv), p.T, S, p.Hq, p.Hkv);
   if (cudaGetLastError() != cudaSuccess) return -3;
   if (p.blocks == 0) return 0;
-  launch_overlapped(attn_bwd_kernel<HD, true>, static_cast<unsigned>(n_kv * parts + p.blocks * p.Hq), BWD_PACKED_THREADS, smem, st, tqx, tqy,
+  launch_overlapped(kern, static_cast<unsigned>(n_kv * parts + p.blocks * p.Hq), BWD_PACKED_THREADS, smem, st, tqx, tqy,
                     tdx, tdy, tdq, lse, delta, static_cast<int>(p.blocks), S, p.Hq, p.Hkv, parts, partial, arrived, softmax_scale,
-                    softmax_scale * 1.4426950408889634f, status, table, static_cast<__nv_bfloat16*>(d_qkv), p.T);
+                    softmax_scale * 1.4426950408889634f, status, table, reinterpret_cast<const uchar2*>(p.own),
+                    static_cast<const __nv_bfloat16*>(qkv), static_cast<const __nv_bfloat16*>(d_out), static_cast<__nv_bfloat16*>(d_qkv), p.T);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 

@@ -11,11 +11,21 @@ constexpr int kMaxPackedTokens = 1 << 21;      // two counters per 128 of them f
 // The table of a packed batch: [blocks + 1] rows of four ints.  Row 0: blocks in use, end of the last sequence, T, 0.  Then, for
 // every block of 128 rows of a sequence, those with most blocks in front of them first: first row of the sequence, its rows, place of the
 // block in the sequence, and 128 times the number of blocks of the sequences before (where lse and the like of it begin).
+// own, unless null: neighbouring sequences that fit one block together count as one sequence, a group, with kGroup added to the
+// fourth number, and of row i of a group own [blocks * 128][2] has the first and last row of its sequence in the group, at the place that
+// lse begins at plus i.  Groups are formed within kGroupChunks parts of the sequences, of group_chunk(n) each.
 // cu: n + 1 ints on the device, cu[0] == 0, rising, none above T; otherwise the table is empty and `status` set.
-int pack_table(const int* cu, int n, int T, int blocks, int* table, int* status, cudaStream_t st);
+// scratch: 2 n ints with own, else unused.
+constexpr int kGroup = 1, kGroupChunks = 32;
+inline __host__ __device__ int group_chunk(int n) {
+  const int c = (n + kGroupChunks - 1) / kGroupChunks;
+  return c > 64 ? c : 64;
+}
+int pack_table(const int* cu, int n, int T, int blocks, int* table, unsigned char* own, int* scratch, int* status, cudaStream_t st);
 
 struct PackedShape {
   const int* table;
+  const unsigned char* own;    // null for a table without groups
   int T;
   long long blocks;            // that the table has memory for
   long long longest, work;     // about: blocks of the longest sequence, pairs of a query and a key block; choose launch shapes only
