@@ -128,7 +128,7 @@ __device__ __noinline__ void repair_out(const __nv_bfloat16* q, const __nv_bfloa
     for (int j = 0; j < n; ++j)
       o = fmaf(expf(dot_rows<HD>(q, k + j * stride) * scale - top), __bfloat162float(v[j * stride + d]), o);
     out[d] = __float2bfloat16(o / sum);
-    if (rest != nullptr) rest[d] = 0;
+    if (rest != nullptr) rest[d / 32 * 4096 + d % 32] = 0;       // see lost_at
   }
   *lse = top + logf(sum);
 }
@@ -202,6 +202,13 @@ __device__ __forceinline__ float with_what_was_lost(float rounded, uint32_t lost
   const uint32_t e = __float_as_uint(rounded) & kExponent;
   const float bits = __uint_as_float(__byte_perm(lost, 0x4b000000u, 0x7650 + i)) - 8388736.f;
   return e < 16u << 23 ? rounded : fmaf(bits, __uint_as_float(e - (14u << 23)), rounded);
+}
+
+// These bytes lie by blocks of 128 rows and pieces of 32 columns, so that neighbouring lanes, which have neighbouring rows, write
+// neighbouring bytes (row by row the forward kernel takes 243 us instead of 234 at 16 x 1024, 32 / 8 heads x 128).
+template <int HD>
+__device__ __forceinline__ long long lost_at(int padded_row, int head, int Hq, int piece) {
+  return (((static_cast<long long>(padded_row >> 7) * Hq + head) * (HD / 32) + piece) * 128 + (padded_row & 127)) * 32;
 }
 
 // 64 bytes of a row
@@ -655,7 +662,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
                                   __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
           }
           if (row < rem) {
-            uint4* const dst = reinterpret_cast<uint4*>(rest + ((tok0 + qblk * 128 + row) * Hq + head) * HD + c * 32);
+            uint4* const dst = reinterpret_cast<uint4*>(rest + lost_at<HD>(e.place() + qblk * 128 + row, head, Hq, c));
             dst[0] = make_uint4(lost[0], lost[1], lost[2], lost[3]);
             dst[1] = make_uint4(lost[4], lost[5], lost[6], lost[7]);
           }
@@ -675,7 +682,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
         const long long stride = static_cast<long long>(Hq + 2 * Hkv) * HD, o = ((tok0 + row) * Hq + head) * HD;
         const __nv_bfloat16* k = qkv + (tok0 + first) * stride + static_cast<long long>(Hq + g) * HD;
         repair_out<HD>(qkv + (tok0 + row) * stride + head * HD, k, k + static_cast<long long>(Hkv) * HD, row + 1 - first, stride,
-                       scale_log2 * 0.6931471805599453f, out + o, rest == nullptr ? nullptr : rest + o, lse_at);
+                       scale_log2 * 0.6931471805599453f, out + o,
+                       rest == nullptr ? nullptr : rest + lost_at<HD>(e.place() + row, head, Hq, 0), lse_at);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -765,7 +773,7 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const signed char*
       const long long at = (static_cast<long long>(e.tok0 + i) * Hq + h) * HD + 8 * lane;
       const uint4 a = *reinterpret_cast<const uint4*>(o + at);
       const uint4 b = *reinterpret_cast<const uint4*>(d_o + at);
-      const uint2 l = exact ? *reinterpret_cast<const uint2*>(rest + at) : make_uint2(0, 0);
+      const uint2 l = exact ? *reinterpret_cast<const uint2*>(rest + lost_at<HD>(e.place() + i, h, Hq, lane / 4) + lane % 4 * 8) : make_uint2(0, 0);
       const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&a);
       const __nv_bfloat162* bp = reinterpret_cast<const __nv_bfloat162*>(&b);
       const uint32_t lw[2] = {l.x ^ 0x80808080u, l.y ^ 0x80808080u};

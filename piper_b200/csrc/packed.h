@@ -32,8 +32,8 @@ struct PackedShape {
   int Hq, Hkv, hd;
 };
 
-// qkv [T, (Hq + 2 Hkv) hd] bf16 -> out [T, Hq hd] bf16, lse [Hq, 128 blocks] fp32 (natural log) and, unless null, rest [T, Hq hd]:
-// what rounding has taken from out, for the backward pass.
+// qkv [T, (Hq + 2 Hkv) hd] bf16 -> out [T, Hq hd] bf16, lse [Hq, 128 blocks] fp32 (natural log) and, unless null, rest
+// [128 blocks, Hq hd]: what rounding has taken from out, for the backward pass, in an order of its own.
 int attn_packed_fwd(const PackedShape& p, const void* qkv, void* out, float* lse, signed char* rest, float softmax_scale, int num_sms,
                     int* status, cudaStream_t st);
 

@@ -204,13 +204,13 @@ def _heads(x: Tensor, Hq: int, Hkv: int, hd: int) -> tuple[Tensor, Tensor, Tenso
 def packed_attention_fwd(qkv: Tensor, tiles: Tensor, own: Tensor, longest: int, work: int, Hq: int, Hkv: int, hd: int,
                          scale: float, keep: bool) -> tuple[Tensor, Tensor, Tensor]:
     """qkv [T, (Hq + 2 Hkv) * hd] -> (out [T, Hq * hd], lse [Hq, 128 * blocks], by the blocks of the tiles, and, if ``keep`` and on a
-    GPU, what rounding has taken from out, int8 [T, Hq * hd]).  The formula keeps it."""
+    GPU, what rounding has taken from out, int8 [128 * blocks, Hq * hd] in the kernels' own order).  The formula keeps it."""
     T, padded = qkv.shape[0], (tiles.shape[0] - 1) * BLOCK
     if _is_native(qkv):
         _require_bf16(qkv)
         out = torch.empty((T, Hq * hd), dtype=qkv.dtype, device=qkv.device)
         lse = torch.empty((Hq, padded), dtype=torch.float32, device=qkv.device)
-        rest = torch.empty((T if keep else 0, Hq * hd), dtype=torch.int8, device=qkv.device)
+        rest = torch.empty((padded if keep else 0, Hq * hd), dtype=torch.int8, device=qkv.device)
         native.lib().attn_packed_fwd(_aligned(qkv), tiles, own, out, lse, rest, longest, work, Hq, Hkv, hd, scale,
                                      native.status_tensor(qkv.device))
         return out, lse, rest
@@ -230,7 +230,7 @@ def _aligned(t: Tensor) -> Tensor:
 def _(qkv, tiles, own, longest, work, Hq, Hkv, hd, scale, keep):
     return (qkv.new_empty((qkv.shape[0], Hq * hd)),
             qkv.new_empty((Hq, (tiles.shape[0] - 1) * BLOCK), dtype=torch.float32),
-            qkv.new_empty((qkv.shape[0] if keep else 0, Hq * hd), dtype=torch.int8))
+            qkv.new_empty(((tiles.shape[0] - 1) * BLOCK if keep else 0, Hq * hd), dtype=torch.int8))
 
 
 def _forward(ctx, qkv, tiles, own, longest, work, Hq, Hkv, hd, scale, _keep):
