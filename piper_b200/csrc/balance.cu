@@ -15,7 +15,7 @@
 namespace piper {
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int CLUSTER = 8;
 
@@ -84,15 +84,21 @@ __device__ void sum_rows(const BalanceArgs& a, int lanes, void* scratch) {
   const long long step = static_cast<long long>(gridDim.x) * WARPS * per_warp;
   float sum[8] = {};
   int tokens = 0;
-  for (long long t0 = (static_cast<long long>(blockIdx.x) * WARPS + warp) * per_warp; t0 < a.T; t0 += step) {
-    const long long t = t0 + lane / lanes;
-    const bool on = t < a.T && (a.mask == nullptr || a.mask[t] != 0);
-    float x[8] = {};
-    if (on) load8<F32>(a.logits, t * a.E + e0, left, vector, x);
-    softmax8(x, lanes);
-    if (on) {
+  for (long long t0 = (static_cast<long long>(blockIdx.x) * WARPS + warp) * per_warp; t0 < a.T; t0 += 2 * step) {
+    const long long t[2] = {t0 + lane / lanes, t0 + step + lane / lanes};     // two rows at a time: their loads overlap
+    bool on[2];
+    float x[2][8] = {};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += x[i];
+    for (int r = 0; r < 2; ++r) {
+      on[r] = t[r] < a.T && (a.mask == nullptr || a.mask[t[r]] != 0);
+      if (on[r]) load8<F32>(a.logits, t[r] * a.E + e0, left, vector, x[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      softmax8(x[r], lanes);
+      if (!on[r]) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += x[r][i];
       tokens += e0 == 0;
     }
   }
@@ -126,46 +132,50 @@ __device__ void sum_rows(const BalanceArgs& a, int lanes, void* scratch) {
   }
 }
 
+constexpr int ADD_THREADS = 1024;
+
 __device__ void add_rows(const BalanceArgs& a, int ctas, void* scratch, float* loss, int* counts, float* prob, float* factor) {
+  __shared__ double sums[ADD_THREADS];
+  __shared__ int chosen[ADD_THREADS];
   __shared__ double terms[kMaxBalanceExperts];
   __shared__ int tokens;
-  const int threads = blockDim.x;
-  if (threadIdx.x == 0) tokens = 0;
+  // Neighbouring threads have neighbouring experts (the last place: tokens that count) of one of `parts` shares of the CTAs.
+  const int width = a.E + 1, parts = blockDim.x / width;
+  const int part = threadIdx.x / width, e = threadIdx.x - part * width;
+  double p = 0.;
+  int count = 0;
+  if (part < parts) {
+    const float* s = sums_of(scratch, a.E, part) + e;
+    const long long step = 2ll * width * parts;
+#pragma unroll 8
+    for (int c = part; c < ctas; c += parts, s += step) {
+      p += s[0];
+      count += reinterpret_cast<const int*>(s)[width];
+    }
+    sums[threadIdx.x] = p;
+    chosen[threadIdx.x] = count;
+  }
   __syncthreads();
-  int own = 0;
-  for (int c = threadIdx.x; c < ctas; c += threads) own += reinterpret_cast<const int*>(sums_of(scratch, a.E, c))[2 * a.E + 1];
-  atomicAdd(&tokens, own);
+  if (threadIdx.x < width) {
+    for (int i = 1; i < parts; ++i) {
+      p += sums[i * width + e];
+      count += chosen[i * width + e];
+    }
+    if (e == a.E) tokens = count;
+  }
   __syncthreads();
   const double n = max(1, tokens);
-  // eight lanes an expert
-  const int part = threadIdx.x & 7;
-  for (int e0 = 0; e0 < a.E; e0 += threads / 8) {
-    const int e = e0 + threadIdx.x / 8;
-    double p = 0.;
-    int count = 0;
-    if (e < a.E)
-      for (int c = part; c < ctas; c += 8) {
-        const float* s = sums_of(scratch, a.E, c);
-        p += s[e];
-        count += reinterpret_cast<const int*>(s)[a.E + 1 + e];
-      }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-      p += __shfl_xor_sync(0xffffffffu, p, o);
-      count += __shfl_xor_sync(0xffffffffu, count, o);
-    }
-    if (e < a.E && part == 0) {
-      const double f = count * (a.E / (n * a.k));
-      counts[e] = count;
-      prob[e] = static_cast<float>(p / n);
-      factor[e] = static_cast<float>(f / n);
-      terms[e] = f * (p / n);
-    }
+  if (threadIdx.x < a.E) {
+    const double f = count * (a.E / (n * a.k));
+    counts[e] = count;
+    prob[e] = static_cast<float>(p / n);
+    factor[e] = static_cast<float>(f / n);
+    terms[e] = f * (p / n);
   }
   __syncthreads();
   if (threadIdx.x >= 32) return;
   double sum = 0.;
-  for (int e = threadIdx.x; e < a.E; e += 32) sum += terms[e];
+  for (int i = threadIdx.x; i < a.E; i += 32) sum += terms[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (threadIdx.x == 0) *loss = static_cast<float>(sum);
@@ -187,7 +197,7 @@ __global__ void __launch_bounds__(THREADS) balance_sums_kernel(const BalanceArgs
   sum_rows<F32>(a, lanes, scratch);
 }
 
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(ADD_THREADS)
 balance_add_kernel(const BalanceArgs a, int ctas, void* scratch, float* loss, int* counts, float* prob, float* factor) {
   grid_begin();
   add_rows(a, ctas, scratch, loss, counts, prob, factor);
@@ -287,7 +297,7 @@ int balance_fwd(const BalanceArgs& a, float* loss, int* counts, float* prob, flo
   }
   launch_overlapped(a.f32 ? balance_sums_kernel<true> : balance_sums_kernel<false>, ctas, THREADS, 0, st, a, lanes, scratch);
   if (cudaGetLastError() != cudaSuccess) return -3;
-  launch_overlapped(balance_add_kernel, 1, 1024, 0, st, a, ctas, scratch, loss, counts, prob, factor);
+  launch_overlapped(balance_add_kernel, 1, ADD_THREADS, 0, st, a, ctas, scratch, loss, counts, prob, factor);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 

@@ -126,8 +126,10 @@ pack_table_kernel(const int* __restrict__ cu, int n, int T, int blocks, int4* ta
   // of the sequences of v blocks the first comes behind all of more: next[v - 1] = cnt[v]
   for (int i = threadIdx.x; i < m; i += PACK_THREADS) next[i] = i + 1 < m ? base[i + 1] : 0;
   __syncthreads();
+  const int some = m > 0 ? base[0] : 0;        // sequences that have rows; read before the next sums
+  __syncthreads();
   const int used = sum_from_the_end(base, m, false, warp_sums);
-  if (threadIdx.x == 0) table[0] = make_int4(used <= blocks ? used : 0, used <= blocks ? cu[n] : 0, T, 0);
+  if (threadIdx.x == 0) table[0] = used <= blocks ? make_int4(used, cu[n], T, some) : make_int4(0, 0, T, 0);
   if (used > blocks) {                         // the caller's memory is for fewer: its number did not come from these sequences
     if (threadIdx.x == 0) report_bad_argument(status, 52, used, blocks);
     return;

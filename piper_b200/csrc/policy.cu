@@ -157,37 +157,46 @@ __device__ void add_blocks(const PolicyArgs& a, const int4* table, const Sums* s
       s.count += b.count;
     }
   } else {
-    // Entries of place 0 are the sequences; a warp adds the blocks of one.  The lanes of a warp look for the next ones together.
-    for (long long i0 = warp * 32; i0 < used; i0 += warps * 32) {
-      const int4 e = i0 + lane < used ? __ldg(table + 1 + i0 + lane) : make_int4(0, 0, 1, 0);
-      unsigned found = __ballot_sync(0xffffffffu, e.z == 0);
-      while (found != 0) {
-        const int j = __ffs(found) - 1;
-        found &= found - 1;
-        const int len = __shfl_sync(0xffffffffu, e.y, j), place = __shfl_sync(0xffffffffu, e.w, j) / 128;
-        Sums q = {0., 0., 0, 0, 0.};
-        for (int b = lane; b < (len + 127) / 128; b += 32) {
-          const Sums v = sums[place + b];
-          q.loss += v.loss;
-          q.kl += v.kl;
-          q.clipped += v.clipped;
-          q.count += v.count;
-        }
-        q.loss = warp_sum(q.loss);
-        q.kl = warp_sum(q.kl);
-        q.clipped = warp_sum(q.clipped);
-        q.count = warp_sum(q.count);
-        if (lane != 0) continue;
-        out.weight[1 + place] = q.count > 0 ? 1.f / static_cast<float>(q.count) : 0.f;
-        if (q.count == 0) continue;
-        s.loss += q.loss / q.count;
-        s.kl += q.kl / q.count;
-        s.clipped += q.clipped;
-        s.count += q.count;
-        ++sequences;
+    // The last entries, of place 0, are the sequences, those of most blocks first.  Long ones take a warp each, the others eight lanes.
+    const int some = used > 0 ? __ldg(table).w : 0;
+    const int4* const first = table + 1 + used - some;
+    auto add = [&](const int4& e, int lanes, unsigned mask) {
+      const int own = lane & (lanes - 1), place = e.w / 128, blocks = (e.y + 127) / 128;
+      Sums q = {0., 0., 0, 0, 0.};
+      for (int b = own; b < blocks; b += lanes) {
+        const Sums v = sums[place + b];
+        q.loss += v.loss;
+        q.kl += v.kl;
+        q.clipped += v.clipped;
+        q.count += v.count;
       }
-      __syncwarp();
+      for (int o = lanes / 2; o > 0; o >>= 1) {
+        q.loss += __shfl_xor_sync(mask, q.loss, o);
+        q.kl += __shfl_xor_sync(mask, q.kl, o);
+        q.clipped += __shfl_xor_sync(mask, q.clipped, o);
+        q.count += __shfl_xor_sync(mask, q.count, o);
+      }
+      if (own != 0) return;
+      out.weight[1 + place] = q.count > 0 ? 1.f / static_cast<float>(q.count) : 0.f;
+      if (q.count == 0) return;
+      s.loss += q.loss / q.count;
+      s.kl += q.kl / q.count;
+      s.clipped += q.clipped;
+      s.count += q.count;
+      ++sequences;
+    };
+    constexpr int kLong = 64 * 128;
+    for (int i = warp; i < some; i += warps) {
+      const int4 e = __ldg(first + i);
+      if (e.y <= kLong) break;
+      add(e, 32, 0xffffffffu);
     }
+    __syncwarp();
+    for (int i = threadIdx.x / 8; i < some; i += blockDim.x / 8) {
+      const int4 e = __ldg(first + i);
+      if (e.y <= kLong) add(e, 8, 0xffu << (lane & 24));
+    }
+    __syncwarp();
   }
   s.loss = warp_sum(s.loss);
   s.kl = warp_sum(s.kl);

@@ -44,8 +44,8 @@ def _blocks(n: int) -> int:
 
 
 def _table_ref(offsets: list, tokens: int, blocks: int, marks: Optional[list] = None) -> Tensor:
-    """Row 0: blocks in use, end of the last sequence, tokens, 0.  Then, for every block of 128 rows, those with most blocks of their
-    sequence in front of them first: first row of the sequence, its rows, place of the block in it, and 128 times the
+    """Row 0: blocks in use, end of the last sequence, tokens, sequences that have rows.  Then, for every block of 128 rows, those with
+    most blocks of their sequence in front of them first: first row of the sequence, its rows, place of the block in it, and 128 times the
     number of blocks of the sequences before, the sequence's mark added."""
     rows, before = [], 0
     for s, (a, b) in enumerate(zip(offsets, offsets[1:])):
@@ -53,7 +53,7 @@ def _table_ref(offsets: list, tokens: int, blocks: int, marks: Optional[list] = 
         before += _blocks(b - a)
     rows.sort(key=lambda r: (-r[2], -_blocks(r[1]), r[0]))
     table = torch.zeros(blocks + 1, 4, dtype=torch.int32)
-    table[0] = torch.tensor([len(rows), offsets[-1], tokens, 0])
+    table[0] = torch.tensor([len(rows), offsets[-1], tokens, sum(r[2] == 0 for r in rows)])
     if rows:
         table[1:len(rows) + 1] = torch.tensor(rows, dtype=torch.int32)
     return table

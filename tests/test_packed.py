@@ -93,7 +93,7 @@ def test_table_on_the_cpu(lens, behind):
     T = sum(lens) + behind
     s = ops.pack_sequences(_offsets(lens), T)
     rows = s.table.tolist()
-    assert rows[0] == [sum((n + 127) // 128 for n in lens), sum(lens), T, 0] and len(rows) == rows[0][0] + 1
+    assert rows[0] == [sum((n + 127) // 128 for n in lens), sum(lens), T, sum(n > 0 for n in lens)] and len(rows) == rows[0][0] + 1
     blocks, at = {}, 0
     for a, n in zip(_offsets(lens).tolist(), lens):
         for i in range((n + 127) // 128):
