@@ -110,6 +110,8 @@ __device__ float dot_rows(const __nv_bfloat16* a, const __nv_bfloat16* b) {
   return s;
 }
 
+// The following are for rows of groups that hold what is not finite, 32 columns at a time.
+//
 // A row of queries of one head against keys k, v [n] of its sequence, `stride` elements apart.
 template <int HD>
 __device__ __noinline__ void repair_out(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v, int n, long long stride,
@@ -123,47 +125,58 @@ __device__ __noinline__ void repair_out(const __nv_bfloat16* q, const __nv_bfloa
   }
   for (int j = 0; j < n; ++j) sum += expf(dot_rows<HD>(q, k + j * stride) * scale - top);
   if (nan) sum = NAN;
-  for (int d = 0; d < HD; ++d) {
-    float o = 0.f;
-    for (int j = 0; j < n; ++j)
-      o = fmaf(expf(dot_rows<HD>(q, k + j * stride) * scale - top), __bfloat162float(v[j * stride + d]), o);
-    out[d] = __float2bfloat16(o / sum);
-    if (rest != nullptr) rest[d / 32 * 4096 + d % 32] = 0;       // see lost_at
+  for (int c = 0; c < HD; c += 32) {
+    float o[32] = {};
+    for (int j = 0; j < n; ++j) {
+      const float p = expf(dot_rows<HD>(q, k + j * stride) * scale - top);
+#pragma unroll
+      for (int d = 0; d < 32; ++d) o[d] = fmaf(p, __bfloat162float(v[j * stride + c + d]), o[d]);
+    }
+#pragma unroll
+    for (int d = 0; d < 32; ++d) {
+      out[c + d] = __float2bfloat16(o[d] / sum);
+      if (rest != nullptr) rest[c / 32 * 4096 + d] = 0;          // see lost_at
+    }
   }
   *lse = top + logf(sum);
 }
 
-// 64 columns of the gradient of that row of queries: d_out, out row's delta and lse, columns `k64` of the keys.
+// 64 columns, from c64, of the gradient of that row of queries, with its output gradient, lse and delta.
 template <int HD>
 __device__ __noinline__ void repair_dq(const __nv_bfloat16* q, const __nv_bfloat16* d_out, const __nv_bfloat16* k,
-                                       const __nv_bfloat16* v, int n, long long stride, int k64, float scale, float lse, float delta,
+                                       const __nv_bfloat16* v, int n, long long stride, int c64, float scale, float lse, float delta,
                                        __nv_bfloat16* dq) {
-  for (int d = 0; d < 64; ++d) {
-    float s = 0.f;
+  for (int c = c64; c < c64 + 64; c += 32) {
+    float s[32] = {};
     for (int j = 0; j < n; ++j) {
-      const float p = expf(dot_rows<HD>(q, k + j * stride) * scale - lse);
-      s = fmaf(p * (dot_rows<HD>(d_out, v + j * stride) - delta), __bfloat162float(k[j * stride + k64 + d]), s);
+      const float ds = expf(dot_rows<HD>(q, k + j * stride) * scale - lse) * (dot_rows<HD>(d_out, v + j * stride) - delta);
+#pragma unroll
+      for (int d = 0; d < 32; ++d) s[d] = fmaf(ds, __bfloat162float(k[j * stride + c + d]), s[d]);
     }
-    dq[d] = __float2bfloat16(s * scale);
+#pragma unroll
+    for (int d = 0; d < 32; ++d) dq[c - c64 + d] = __float2bfloat16(s[d] * scale);
   }
 }
 
-// 64 columns from `c64` of the gradient of a row of keys (is_k) or values: queries q, d_out [n] of its sequence from that row on, of
-// `heads` heads; lse and delta [heads][n], `padded` apart.
+// 64 columns, from c64, of the gradient of a row of keys (is_k) or values: queries q and output gradients [n] of its sequence from that
+// row on, of `heads` heads; lse and delta [heads][n], `padded` apart.
 template <int HD>
 __device__ __noinline__ void repair_dkv(const __nv_bfloat16* k, const __nv_bfloat16* v, const __nv_bfloat16* q, const __nv_bfloat16* d_out,
                                         int n, int heads, long long q_stride, long long o_stride, bool is_k, int c64, float scale,
                                         const float* lse, const float* delta, long long padded, __nv_bfloat16* out) {
-  for (int d = 0; d < 64; ++d) {
-    float s = 0.f;
+  for (int c = c64; c < c64 + 64; c += 32) {
+    float s[32] = {};
     for (int h = 0; h < heads; ++h)
       for (int i = 0; i < n; ++i) {
         const __nv_bfloat16 *qi = q + i * q_stride + h * HD, *di = d_out + i * o_stride + h * HD;
-        const float p = expf(dot_rows<HD>(qi, k) * scale - lse[h * padded + i]);
-        if (is_k) s = fmaf(p * (dot_rows<HD>(di, v) - delta[h * padded + i]) * scale, __bfloat162float(qi[c64 + d]), s);
-        else s = fmaf(p, __bfloat162float(di[c64 + d]), s);
+        float f = expf(dot_rows<HD>(qi, k) * scale - lse[h * padded + i]);
+        if (is_k) f *= (dot_rows<HD>(di, v) - delta[h * padded + i]) * scale;
+        const __nv_bfloat16* const x = (is_k ? qi : di) + c;
+#pragma unroll
+        for (int d = 0; d < 32; ++d) s[d] = fmaf(f, __bfloat162float(x[d]), s[d]);
       }
-    out[d] = __float2bfloat16(s);
+#pragma unroll
+    for (int d = 0; d < 32; ++d) out[c - c64 + d] = __float2bfloat16(s[d]);
   }
 }
 
@@ -288,11 +301,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
     grid_wait(table, own, qkv);
     const int units = ONE ? Hq : Hkv * ((group + 1) / 2);
     const int entry = static_cast<int>(blockIdx.x) / units, u = static_cast<int>(blockIdx.x) % units;
-    const int4 header = __ldg(table);          // blocks, end of the last sequence, rows of the batch
+    int4 header = __ldg(table);                // blocks, end of the last sequence, rows of the batch
     e = uniform(packed_block(table, min(entry, B - 1)));    // with the header, not behind it
-    if (header.z != T) {                       // a table of another batch
+    if (header.z != T) {                       // a table of another batch: all rows are behind it
       if (threadIdx.x == 0) report_bad_argument(status, 53, header.z, T);
-      return;
+      header.x = header.y = 0;
     }
     if (entry >= header.x) {
       const long long rest = static_cast<long long>(T - header.y) * Hq * HD / 8;
@@ -753,8 +766,8 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const signed char*
   const int wl = threadIdx.x & 31;
   const int lane = wl & (LANES - 1);
   const unsigned mask = ((1u << LANES) - 1u) << (wl & ~(LANES - 1));
-  const int4 header = __ldg(table);
-  if (header.z != T) return;
+  int4 header = __ldg(table);
+  if (header.z != T) header.x = header.y = 0;
   // all heads of a row, or of several rows, at a time
   constexpr int GROUPS = 256 / LANES;
   const int group = threadIdx.x / LANES, at_once = Hq < GROUPS ? GROUPS / Hq : 1, own = group / Hq < at_once ? group / Hq : -1;

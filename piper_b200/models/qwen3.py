@@ -93,13 +93,16 @@ class MoE(nn.Module):
         self.gate = Linear(cfg.dim, cfg.num_experts)
         self.experts = GroupedExperts(cfg.dim, cfg.moe_hidden, cfg.num_experts)
 
-    def forward(self, x: torch.Tensor, jitter: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, jitter: Optional[torch.Tensor] = None,
+                counted: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``counted`` (bool [T]): tokens that the balance loss is about, all without it."""
         logits = self.gate(x)
         if jitter is not None:
             logits = logits + jitter
         weights, idx, counts = moe_ops.moe_route(logits, self.top_k, self.renorm)
         if self.balance_coef:
-            weights = moe_ops.moe_attach_loss(weights, moe_ops.moe_balance_loss(logits, idx).loss, self.balance_coef)
+            weights = moe_ops.moe_attach_loss(weights, moe_ops.moe_balance_loss(logits, idx, mask=counted).loss,
+                                              self.balance_coef)
         rows, pos, g_start, g_len, ep_counts = moe_ops.moe_dispatch(x, idx, counts)
         with annotate(EP_TAG):
             out_rows = self.experts(rows, ep_counts)
@@ -116,14 +119,14 @@ class Qwen3Block(nn.Module):
         self.moe = MoE(cfg) if cfg.moe_enabled else None
         self.feed_forward = None if cfg.moe_enabled else FeedForward(cfg.dim, cfg.ffn_hidden, cfg.fp8)
 
-    def forward(self, h, delta, cos, sin, batch: int, seq: int, jitter=None, sequences=None):
+    def forward(self, h, delta, cos, sin, batch: int, seq: int, jitter=None, sequences=None, counted=None):
         if delta is None:
             y = self.attention_norm(h)
         else:
             y, h = self.attention_norm(delta, h)
         a = self.attention(y, cos, sin, batch, seq, sequences)
         y, h = self.ffn_norm(a, h)
-        return h, (self.moe(y, jitter) if self.moe is not None else self.feed_forward(y))
+        return h, (self.moe(y, jitter, counted) if self.moe is not None else self.feed_forward(y))
 
 
 class PiperQwen3Model(nn.Module):
@@ -170,16 +173,20 @@ class PiperQwen3Model(nn.Module):
             cos, sin = packed_rope(cos, sin, sequences)
         n = len(self.layers)
         h = delta = out = None
-        jitter = None
-        if self.use_jitter:
+        jitter = counted = None
+        if self.use_jitter and sequences is not None:
+            jitter = self.router_jitter[sequences.positions().clamp(max=self.router_jitter.shape[0] - 1)]
+        elif self.use_jitter:
             jitter = self.router_jitter if batch == 1 else self.router_jitter.repeat(batch, 1)
+        if sequences is not None and self.cfg.balance_coef:
+            counted = sequences.inside()
         for stage in range(self.num_stages):
             lo, hi = stage * n // self.num_stages, (stage + 1) * n // self.num_stages
             with annotate(PP_TAG):
                 if stage == 0:
                     h = self.tok_embeddings(tokens.reshape(-1))
                 for i in range(lo, hi):
-                    h, delta = self.layers[i](h, delta, cos, sin, batch, seq, jitter, sequences)
+                    h, delta = self.layers[i](h, delta, cos, sin, batch, seq, jitter, sequences, counted)
                 if stage == self.num_stages - 1:
                     y, h = self.norm(delta, h)
                     out = self.output(y).view(batch, seq, -1)

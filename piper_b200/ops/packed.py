@@ -6,6 +6,7 @@ Kernels: ``csrc/pack.cu``, ``csrc/attention_sm100.cu``.
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -31,12 +32,15 @@ class PackedSequences(NamedTuple):
     longest: int
     work: int
 
+    def inside(self) -> Tensor:
+        """bool [tokens]: whether a token belongs to a sequence."""
+        return torch.arange(self.tokens, device=self.offsets.device) < self.offsets[-1]
+
     def positions(self) -> Tensor:
         """int64 [tokens]: a token's place in its sequence, 0 behind the last one."""
         at = torch.arange(self.tokens, device=self.offsets.device)
         of = torch.searchsorted(self.offsets, at, right=True) - 1
-        inside = at < self.offsets[-1]
-        return torch.where(inside, at - self.offsets[of.clamp(min=0)], 0)
+        return torch.where(self.inside(), at - self.offsets[of.clamp(min=0)], 0)
 
 
 def _blocks(n: int) -> int:
@@ -285,6 +289,8 @@ def packed_attention(qkv: Tensor, sequences: PackedSequences, Hq: int, Hkv: int,
     if Hq < 1 or Hkv < 1 or Hq % Hkv or qkv.shape[1] != (Hq + 2 * Hkv) * hd:
         raise ValueError(f"packed_attention: qkv must be [T, (Hq + 2 Hkv) * hd] with whole groups of heads, got "
                          f"{tuple(qkv.shape)} for {Hq} / {Hkv} heads of {hd}")
+    if not 0 < scale < math.inf:
+        raise ValueError(f"packed_attention: scale must be above 0, got {scale}")
     if sequences.tiles.device != qkv.device:
         raise ValueError(f"packed_attention: sequences are on {sequences.tiles.device}, qkv on {qkv.device}")
     return packed_attention_fwd(qkv, sequences.tiles, sequences.own, sequences.longest, sequences.work, Hq, Hkv, hd, scale,

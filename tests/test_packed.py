@@ -171,7 +171,8 @@ def test_attention_refuses_what_does_not_fit(device):
     x = torch.zeros(7, 256, dtype=torch.bfloat16, device=device)
     calls = [lambda: ops.packed_attention(x[:6], s, 2, 1, 64, 1.0), lambda: ops.packed_attention(x, s, 3, 2, 64, 1.0),
              lambda: ops.packed_attention(x, s, 2, 0, 64, 1.0), lambda: ops.packed_attention(x.view(7, 4, 64), s, 2, 1, 64, 1.0),
-             lambda: ops.packed_attention(x, s, 2, 2, 64, 1.0)]
+             lambda: ops.packed_attention(x, s, 2, 2, 64, 1.0), lambda: ops.packed_attention(x, s, 2, 1, 64, 0.0),
+             lambda: ops.packed_attention(x, s, 2, 1, 64, -1.0), lambda: ops.packed_attention(x, s, 2, 1, 64, float("nan"))]
     if device == "cuda":
         calls += [lambda: ops.packed_attention(x, s, 14, 1, 16, 1.0), lambda: ops.packed_attention(x.float(), s, 2, 1, 64, 1.0),
                   lambda: ops.packed_attention(x, ops.pack_sequences(_offsets([3, 4]), 7), 2, 1, 64, 1.0)]
@@ -370,6 +371,36 @@ def test_attention_on_other_streams_and_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(out[0], w[0]) and torch.equal(out[1], w[1])
     native.check_status()
+
+
+@pytest.mark.gpu
+def test_batches_of_more_than_2_to_the_31_elements():
+    """The last sequences of a batch whose rows lie beyond 2^31 elements, and the rows behind them."""
+    Hq, Hkv, hd, tail = 64, 8, 128, [300, 40, 50, 513]
+    lens = [777] * 360 + tail
+    T = sum(lens) + 100
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * hd, generator=g, device="cuda", dtype=torch.bfloat16)
+    dout = torch.randn(T, Hq * hd, generator=g, device="cuda", dtype=torch.bfloat16)
+    first = sum(lens) - sum(tail)
+    assert first * qkv.shape[1] > 2 ** 31
+    out, d = _pass(qkv, dout, ops.pack_sequences(_offsets(lens), T, device="cuda"), Hq, Hkv, hd)
+    want = _definition(qkv[first:first + sum(tail)], dout[first:first + sum(tail)], tail, Hq, Hkv, hd, hd ** -0.5)
+    _close(out[first:first + sum(tail)], *want[:2])
+    _close(d[first:first + sum(tail)], *want[2:])
+    assert not bool(out[sum(lens):].any()) and not bool(d[sum(lens):].any())
+
+
+@pytest.mark.gpu
+def test_a_table_of_another_batch_gives_zeros_and_an_error():
+    a, b = ops.pack_sequences(_offsets([100, 60]), 200, device="cuda"), ops.pack_sequences(_offsets([130, 5]), 190, device="cuda")
+    qkv, dout = _inputs(200, 4, 2, 64, "cuda", 0)
+    x = qkv.requires_grad_(True)
+    out = ops.packed_attention(x, a._replace(tiles=b.tiles, own=b.own), 4, 2, 64, 0.125)
+    (d,) = torch.autograd.grad(out, x, dout)
+    assert not bool(out.any()) and not bool(d.any())
+    with pytest.raises(native.PiperKernelError):
+        native.check_status()
 
 
 @pytest.mark.gpu

@@ -67,6 +67,38 @@ def test_packed_sequences_are_sequences_by_themselves(kind):
         assert float((a - b).abs().max()) <= depth * float(b.abs().max()), n
 
 
+def test_jitter_and_balance_loss_of_a_packed_batch_are_those_of_its_sequences():
+    """The frozen router noise goes by a token's place in its sequence, and tokens behind the last sequence do not count."""
+    from piper_b200.models.qwen3 import PiperQwen3Model, Qwen3Config
+    cfg = Qwen3Config(dim=64, n_layers=1, n_heads=2, n_kv_heads=1, head_dim=32, vocab_size=VOCAB, num_experts=8, top_k=2, moe_hidden=32,
+                      balance_coef=3.0, router_jitter_std=1.0)
+    model = PiperQwen3Model(cfg, 1, 130)
+    torch.manual_seed(0)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.copy_(torch.randn(p.shape) * 0.1)
+    consts = PiperQwen3Model.const_attrs(cfg, 130)
+    model.rope_cos, model.rope_sin, model.router_jitter = consts["rope_cos"], consts["rope_sin"], consts["router_jitter"].float()
+    tokens, offsets, s = _batch("cpu")
+    with torch.no_grad():
+        out = model(tokens, s).view(T, VOCAB)
+        for a, b in zip(offsets.tolist(), offsets.tolist()[1:]):
+            alone = ops.pack_sequences(torch.tensor([0, b - a]), b - a)
+            # fp32 sums in another order, as above
+            want = model(tokens[:, a:b], alone).view(b - a, VOCAB)
+            assert float((out[a:b] - want).abs().max()) <= 2.0 ** -24 * 20 * 256 * float(want.abs().max())
+
+    def gate_gradient(toks):                     # of the balance loss alone
+        model.zero_grad()
+        (model(toks, s) * 0.0).sum().backward()
+        return model.layers[0].moe.gate.weight.grad.clone()
+
+    first = gate_gradient(tokens)
+    other = tokens.clone()
+    other[0, sum(LENS):] = (other[0, sum(LENS):] + 1) % VOCAB
+    assert bool(first.any()) and torch.equal(first, gate_gradient(other))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("kind", ["llama", "qwen"])
 def test_logits_of_a_sequence_do_not_depend_on_the_others(kind, device):
