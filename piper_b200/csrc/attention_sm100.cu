@@ -180,12 +180,6 @@ __device__ __noinline__ void repair_dkv(const __nv_bfloat16* k, const __nv_bfloa
   }
 }
 
-// The same, known to the compiler as equal for a warp's lanes.
-__device__ __forceinline__ PackedBlock uniform(const PackedBlock& e) {
-  return {__shfl_sync(0xffffffffu, e.tok0, 0), __shfl_sync(0xffffffffu, e.len, 0), __shfl_sync(0xffffffffu, e.block, 0),
-          __shfl_sync(0xffffffffu, e.pad0, 0)};
-}
-
 // Rows [from, to) of a tile of 64-column halves, `half` bytes apart, become zero (whole rows: the swizzle stays within them).
 // Called by a warp in front of the products that contract over these rows.
 __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int halves, int half, int from, int to, int lane) {
@@ -302,7 +296,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
     const int units = ONE ? Hq : Hkv * ((group + 1) / 2);
     const int entry = static_cast<int>(blockIdx.x) / units, u = static_cast<int>(blockIdx.x) % units;
     int4 header = __ldg(table);                // blocks, end of the last sequence, rows of the batch
-    e = uniform(packed_block(table, min(entry, B - 1)));    // with the header, not behind it
+    e = packed_block(table, min(entry, B - 1));    // with the header, not behind it
     if (header.z != T) {                       // a table of another batch: all rows are behind it
       if (threadIdx.x == 0) report_bad_argument(status, 53, header.z, T);
       header.x = header.y = 0;
@@ -1543,7 +1537,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmap_qkv_x,   // box {64, 12
     const int n_kv = B * Hkv * parts;
     const int entry = idx < n_kv ? idx / parts / Hkv : (idx - n_kv) / Hq;
     const int4 header = __ldg(table);
-    const PackedBlock e = uniform(packed_block(table, entry));      // with the header, not behind it
+    const PackedBlock e = packed_block(table, entry);      // with the header, not behind it
     if (entry >= header.x || header.z != T) return;
     if (idx < n_kv) {
       // of a sequence of n blocks, key block n - 1 - i has as many query blocks as query block i has key blocks

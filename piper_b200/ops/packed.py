@@ -18,19 +18,26 @@ from .registry import custom_op, once_differentiable
 
 BLOCK = 128                      # rows of a query or key block
 MAX_TOKENS = 1 << 21
+# Short neighbours share blocks where that saves a fifth of some 5,800 cycles a pair of a query and a key block and 7,500 a block, and where
+# the query blocks of all heads are more than two for each of 148 SMs.  Time of both passes with groups, of that without, by that
+# share of cycles, on 340 to 16,000 tokens in up to 871 sequences: 1.0-1.06 at 0.9 and above, 0.90-1.03 at 0.77 to 0.9, 0.24-0.76 below; with
+# 112 blocks of all heads 1.16 at 0.29.
+GROUP_GAIN = 1.25
+GROUP_BLOCKS = 296
 
 
 class PackedSequences(NamedTuple):
-    """Where the sequences of a packed batch lie.  ``longest`` (blocks of the longest sequence) and ``work`` (pairs of a query and a
-    key block) only choose launch shapes: where the offsets are on a GPU, they are those of equal sequences."""
+    """Where the sequences of a packed batch lie.  ``longest`` (blocks of the longest sequence), ``work`` and ``tile_work`` (pairs of a
+    query and a key block) only choose launch shapes: where the offsets are on a GPU, they are those of equal sequences."""
 
     offsets: Tensor              # int32 [n + 1]: sequence i has rows offsets[i] to offsets[i + 1]
     table: Tensor                # int32 [blocks + 1, 4]: blocks of the sequences, see _table_ref
-    tiles: Tensor                # the same for attention: of sequences or, if ``own`` is not empty, of groups of short ones too
-    own: Tensor                  # uint8 [128 * blocks, 2]: see _groups_ref
+    tiles: Optional[Tensor]      # the same with groups of short sequences, if there are enough of them, and
+    own: Optional[Tensor]        # uint8 [128 * blocks, 2]: see _groups_ref
     tokens: int                  # rows of the batch, those behind the last sequence included
     longest: int
     work: int
+    tile_work: int
 
     def inside(self) -> Tensor:
         """bool [tokens]: whether a token belongs to a sequence."""
@@ -143,10 +150,9 @@ def pack_sequences(offsets: Tensor, tokens: int, device: Optional[torch.device] 
         _check_offsets(values, tokens)
         ends = [values[g[0]] for g in _groups(values)] + [values[-1]]
         counts, fewer = ([_blocks(b - a) for a, b in zip(v, v[1:])] for v in (values, ends))
-        blocks, (work, less) = sum(counts), (sum(c * (c + 1) // 2 for c in v) for v in (counts, fewer))
-        # in cycles of the backward pass, of the kernels with groups too: batches that gain 10 %
-        grouped = 1.1 * (less * 5800 + sum(fewer) * 7500) < work * 5800 + blocks * 7500
-        tiles, work, longest = (sum(fewer), less, max(fewer)) if grouped else (blocks, work, max(counts, default=0))
+        blocks, tiles, longest = sum(counts), sum(fewer), max(counts, default=0)
+        work, tile_work = (sum(c * (c + 1) // 2 for c in v) for v in (counts, fewer))
+        grouped = GROUP_GAIN * (tile_work * 5800 + tiles * 7500) < work * 5800 + blocks * 7500
         # a copy of what was checked; nothing waits for its way to the device
         offsets = torch.tensor(values, dtype=torch.int32).to("cpu" if device is None else device, non_blocking=True)
     else:
@@ -155,16 +161,14 @@ def pack_sequences(offsets: Tensor, tokens: int, device: Optional[torch.device] 
         blocks = (tokens + (BLOCK - 1) * min(n, tokens)) // BLOCK
         grouped = tokens < n * BLOCK // 2
         # two neighbouring groups have more than 128 rows together, but at long sequences and the ends of the 32 parts
-        tiles = min(blocks, 3 * tokens // BLOCK + 33) if grouped else blocks
+        tiles = min(blocks, 3 * tokens // BLOCK + 33)
         longest = _blocks(-(-tokens // max(n, 1)))
-        work = min(max(n, 1), tiles) * longest * (longest + 1) // 2
+        work, tile_work = (min(max(n, 1), b) * longest * (longest + 1) // 2 for b in (blocks, tiles))
         if offsets.dtype != torch.int32:     # what does not fit becomes an offset that is refused
             offsets = offsets.clamp(-1, (1 << 31) - 1).to(torch.int32)
     offsets = offsets.contiguous()
-    table, own = pack_table(offsets, tokens, blocks, False)
-    # where groups are many: csrc/attention_sm100.cu
-    pair = pack_table(offsets, tokens, tiles, True) if grouped else (table, own)
-    return PackedSequences(offsets, table, *pair, tokens, longest, work)
+    pair = pack_table(offsets, tokens, tiles, True) if grouped else (None, None)
+    return PackedSequences(offsets, pack_table(offsets, tokens, blocks, False)[0], *pair, tokens, longest, work, tile_work)
 
 
 # --------------------------------------------------------------------------
@@ -205,7 +209,7 @@ def _heads(x: Tensor, Hq: int, Hkv: int, hd: int) -> tuple[Tensor, Tensor, Tenso
 
 
 @custom_op("piper::packed_attention_fwd")
-def packed_attention_fwd(qkv: Tensor, tiles: Tensor, own: Tensor, longest: int, work: int, Hq: int, Hkv: int, hd: int,
+def packed_attention_fwd(qkv: Tensor, tiles: Tensor, own: Optional[Tensor], longest: int, work: int, Hq: int, Hkv: int, hd: int,
                          scale: float, keep: bool) -> tuple[Tensor, Tensor, Tensor]:
     """qkv [T, (Hq + 2 Hkv) * hd] -> (out [T, Hq * hd], lse [Hq, 128 * blocks], by the blocks of the tiles, and, if ``keep`` and on a
     GPU, what rounding has taken from out, int8 [128 * blocks, Hq * hd] in the kernels' own order).  The formula keeps it."""
@@ -283,15 +287,16 @@ def packed_attention(qkv: Tensor, sequences: PackedSequences, Hq: int, Hkv: int,
     """
     if qkv.dim() != 2 or qkv.shape[0] != sequences.tokens:
         raise ValueError(f"packed_attention: qkv is {tuple(qkv.shape)}, the batch has {sequences.tokens} tokens")
+    tiles, own, work = sequences.table, None, sequences.work
+    if sequences.own is not None and Hq * (tiles.shape[0] - 1) > GROUP_BLOCKS:
+        tiles, own, work = sequences.tiles, sequences.own, sequences.tile_work
     if qkv.is_cuda:                              # the op makes the checks below by itself
-        return packed_attention_fwd(qkv, sequences.tiles, sequences.own, sequences.longest, sequences.work, Hq, Hkv, hd, scale,
-                                    False)[0]
+        return packed_attention_fwd(qkv, tiles, own, sequences.longest, work, Hq, Hkv, hd, scale, False)[0]
     if Hq < 1 or Hkv < 1 or Hq % Hkv or qkv.shape[1] != (Hq + 2 * Hkv) * hd:
         raise ValueError(f"packed_attention: qkv must be [T, (Hq + 2 Hkv) * hd] with whole groups of heads, got "
                          f"{tuple(qkv.shape)} for {Hq} / {Hkv} heads of {hd}")
     if not 0 < scale < math.inf:
         raise ValueError(f"packed_attention: scale must be above 0, got {scale}")
-    if sequences.tiles.device != qkv.device:
-        raise ValueError(f"packed_attention: sequences are on {sequences.tiles.device}, qkv on {qkv.device}")
-    return packed_attention_fwd(qkv, sequences.tiles, sequences.own, sequences.longest, sequences.work, Hq, Hkv, hd, scale,
-                                    False)[0]
+    if tiles.device != qkv.device:
+        raise ValueError(f"packed_attention: sequences are on {tiles.device}, qkv on {qkv.device}")
+    return packed_attention_fwd(qkv, tiles, own, sequences.longest, work, Hq, Hkv, hd, scale, False)[0]

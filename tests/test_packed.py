@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from piper_b200 import ops
-from piper_b200.ops import native
+from piper_b200.ops import native, packed
 from piper_b200.ops.packed import _table_ref
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -116,18 +116,16 @@ def test_table_on_the_gpu(lens, behind):
     here = ops.pack_sequences(_offsets(lens), T, device="cuda")                  # offsets from the host
     there = ops.pack_sequences(_offsets(lens).cuda(), T)                          # offsets that are on the GPU
     native.check_status()
-    assert torch.equal(here.table.cpu(), want.table) and here[4:] == want[4:]
+    assert torch.equal(here.table.cpu(), want.table) and here[4:] == want[4:] and (here.own is None) == (want.own is None)
     used = want.table.shape[0]
     assert there.table.shape[0] >= used and torch.equal(there.table[:used].cpu(), want.table)
-    if want.own.numel():                         # rows of blocks that are no groups are not written
+    if want.own is not None:                     # rows of blocks that are no groups are not written
         used = want.tiles.shape[0]
-        for s in (here, there):
+        for s in (here, there) if there.own is not None else (here,):
             assert s.own.shape[0] == 128 * (s.tiles.shape[0] - 1) and torch.equal(s.tiles[:used].cpu(), want.tiles)
             for _a, n, _i, at in want.tiles[1:].tolist():
                 if at % 2:
                     assert torch.equal(s.own[at - 1:at - 1 + n].cpu(), want.own[at - 1:at - 1 + n])
-    else:
-        assert torch.equal(here.tiles, here.table) and here.own.numel() == 0
     assert torch.equal(there.positions().cpu(), want.positions())
 
 
@@ -136,15 +134,16 @@ def test_table_on_the_gpu(lens, behind):
 def test_short_neighbours_share_blocks(lens):
     """Every row of a sequence is in one block, in one piece; a block has a sequence or a group of whole ones; no two neighbouring
     groups of one part of the sequences would fit one block."""
-    s = ops.pack_sequences(_offsets(lens), sum(lens))
     at = _offsets(lens).tolist()
-    from piper_b200.ops.packed import _groups, _sequences
-    assert sorted((a, n) for a, n, _ in _sequences(s.tiles, s.own)) == [(a, n) for a, n in zip(at, lens) if n]
-    places = sorted((p, p + n) for _a, n, p in _sequences(s.tiles, s.own))
+    from piper_b200.ops.packed import _groups, _groups_ref, _sequences
+    tiles, own = _groups_ref(at, sum(lens), len(lens) + sum(lens) // 128)
+    assert sorted((a, n) for a, n, _ in _sequences(tiles, own)) == [(a, n) for a, n in zip(at, lens) if n]
+    places = sorted((p, p + n) for _a, n, p in _sequences(tiles, own))
     assert all(b <= c for (_, b), (c, _) in zip(places, places[1:]))
     groups = _groups(at)
     assert [i for g in groups for i in g] == [i for i, n in enumerate(lens) if n]
-    assert bool(s.own.numel()) == (len(groups) * 10 < 8 * sum(n > 0 for n in lens))          # of these, none is near the border
+    s = ops.pack_sequences(_offsets(lens), sum(lens))                        # of these, none is near the border
+    assert (s.own is not None) == (s.tiles is not None) == (len(groups) * 10 < 7 * sum(n > 0 for n in lens))
     chunk = max(64, -(-len(lens) // 32))
     for g, h in zip(groups, groups[1:]):
         assert len(g) == 1 or at[g[-1] + 1] - at[g[0]] <= 128
@@ -206,13 +205,20 @@ CASES = [
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("lens,Hq,Hkv,hd", CASES, ids=lambda v: str(v).replace(" ", ""))
-def test_attention(lens, Hq, Hkv, hd, device):
+def test_attention(lens, Hq, Hkv, hd, device, monkeypatch):
     if device == "cpu" and (sum(lens) * Hq > 2000 or len(lens) > 12):
         pytest.skip("long on the CPU")
     T = sum(lens) + 3
     qkv, dout = _inputs(T, Hq, Hkv, hd, device, len(lens) + hd)
     want = _definition(qkv, dout, lens, Hq, Hkv, hd, hd ** -0.5)
     out, d = _pass(qkv, dout, ops.pack_sequences(_offsets(lens), T, device=device), Hq, Hkv, hd)
+    _close(out, *want[:2])
+    _close(d, *want[2:])
+    monkeypatch.setattr(packed, "GROUP_GAIN", 0.0)         # groups wherever there are any
+    monkeypatch.setattr(packed, "GROUP_BLOCKS", 0)
+    s = ops.pack_sequences(_offsets(lens), T, device=device)
+    assert s.own is not None
+    out, d = _pass(qkv, dout, s, Hq, Hkv, hd)
     _close(out, *want[:2])
     _close(d, *want[2:])
     if device == "cuda":                                   # launch shapes of a batch that the host does not know
@@ -276,15 +282,17 @@ def test_nothing_of_a_sequence_reaches_another(device, hd, value):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
-def test_nothing_of_a_sequence_reaches_others_of_its_block(device, hd, value):
+def test_nothing_of_a_sequence_reaches_others_of_its_block(device, hd, value, monkeypatch):
     """Sequences that share a block: what is not finite in one of them, in all of its row or in queries, keys, values or output gradients
     alone, leaves the others as exact as they were, and does what it does to its own."""
     if device == "cpu" and (hd != 64 or value == value):
         pytest.skip("one of them on the CPU")
     lens = [40, 50, 1, 37, 100, 28, 130, 10, 20, 64]
     T, Hq, Hkv = sum(lens) + 2, 4, 2
+    monkeypatch.setattr(packed, "GROUP_BLOCKS", 0)
     qkv, dout = _inputs(T, Hq, Hkv, hd, device, 6)
     s = ops.pack_sequences(_offsets(lens), T, device=device)
+    assert s.own is not None
     want = _definition(qkv, dout, lens, Hq, Hkv, hd, hd ** -0.5)
     at = _offsets(lens).tolist()
     for bad in (1, 2, 4, 8):
@@ -374,6 +382,42 @@ def test_attention_on_other_streams_and_in_a_graph():
 
 
 @pytest.mark.gpu
+def test_groups_in_a_graph_whose_offsets_change():
+    """Short sequences with offsets on the GPU, in groups: captured with their layout, replayed with other offsets, on two streams at once."""
+    Hq, Hkv, hd, T, n = 32, 8, 64, 700, 40
+    rng = random.Random(2)
+    batches = []
+    for _ in range(3):
+        cuts = sorted(rng.randrange(0, T + 1) for _ in range(n - 1))
+        batches.append([b - a for a, b in zip([0, *cuts], [*cuts, T])])
+    qkv, dout = _inputs(T, Hq, Hkv, hd, "cuda", 9)
+    assert ops.pack_sequences(_offsets(batches[0]).cuda(), T).own is not None
+    want = [_definition(qkv, dout, b, Hq, Hkv, hd, hd ** -0.5) for b in batches]
+    offsets = [_offsets(batches[0]).int().cuda() for _ in range(2)]
+    x = qkv.detach().clone().requires_grad_(True)
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in range(2)]
+    for o in offsets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.packed_attention(x, ops.pack_sequences(o, T), Hq, Hkv, hd, hd ** -0.5)
+            outs.append((out, *torch.autograd.grad(out, x, dout)))
+        graphs.append(graph)
+    for i in range(3):
+        for j in range(2):
+            offsets[j].copy_(_offsets(batches[(i + j) % 3]))
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for j in range(2):
+            w = want[(i + j) % 3]
+            _close(outs[j][0].detach(), *w[:2])
+            _close(outs[j][1], *w[2:])
+    native.check_status()
+
+
+@pytest.mark.gpu
 def test_batches_of_more_than_2_to_the_31_elements():
     """The last sequences of a batch whose rows lie beyond 2^31 elements, and the rows behind them."""
     Hq, Hkv, hd, tail = 64, 8, 128, [300, 40, 50, 513]
@@ -396,7 +440,7 @@ def test_a_table_of_another_batch_gives_zeros_and_an_error():
     a, b = ops.pack_sequences(_offsets([100, 60]), 200, device="cuda"), ops.pack_sequences(_offsets([130, 5]), 190, device="cuda")
     qkv, dout = _inputs(200, 4, 2, 64, "cuda", 0)
     x = qkv.requires_grad_(True)
-    out = ops.packed_attention(x, a._replace(tiles=b.tiles, own=b.own), 4, 2, 64, 0.125)
+    out = ops.packed_attention(x, a._replace(table=b.table), 4, 2, 64, 0.125)
     (d,) = torch.autograd.grad(out, x, dout)
     assert not bool(out.any()) and not bool(d.any())
     with pytest.raises(native.PiperKernelError):
