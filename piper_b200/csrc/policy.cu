@@ -8,8 +8,9 @@
 // differences (the latter by its series near 0, where its terms cancel); sums are in 64 bits and in a fixed order.
 //
 // Some 20 bytes a token: bound by launches and latency.  One warp sums 128 tokens (of a block of the table, or just the next ones), one
-// CTA adds the blocks' sums.  Up to kClusterBlocks blocks all of that is one launch of one cluster, whose first CTA adds
-// behind a cluster barrier; above, more SMs than a cluster has pay for a second launch.
+// CTA adds the blocks' sums, those of sequences first where there is a table.  us on the device, forward, without and with 1,000
+// tokens a sequence: 4,096 tokens 6.0 and 6.8 (one launch), 65,536 4.8 and 6.6, 131,072 5.3 and 8.7, of which the bytes are 0.4;
+// the gradient 4 to 7.
 #include "packed.h"
 
 #include "ptx.cuh"
@@ -18,7 +19,6 @@ namespace piper {
 namespace {
 
 constexpr int THREADS = 1024;
-constexpr int CLUSTER = 8;
 
 struct Sums {                  // of the tokens that count
   double loss, kl;
@@ -223,13 +223,12 @@ __device__ void add_blocks(const PolicyArgs& a, const int4* table, const Sums* s
   out.weight[0] = static_cast<float>(1. / n);
 }
 
-__global__ void __launch_bounds__(THREADS) policy_cluster_kernel(const PolicyArgs a, const PolicyOut out, Sums* sums) {
+__global__ void __launch_bounds__(THREADS) policy_one_kernel(const PolicyArgs a, const PolicyOut out, Sums* sums) {
   grid_begin();
   const int4* const table = reinterpret_cast<const int4*>(a.table);
   sum_blocks(a, table, sums);
-  __threadfence();
-  cluster_sync();
-  if (blockIdx.x == 0) add_blocks(a, table, sums, out);
+  __syncthreads();
+  add_blocks(a, table, sums, out);
 }
 
 __global__ void __launch_bounds__(256) policy_sums_kernel(const PolicyArgs a, Sums* sums) {
@@ -268,28 +267,18 @@ __global__ void __launch_bounds__(256) policy_bwd_kernel(const PolicyArgs a, con
     d[t] = 0.f;
 }
 
-// One cluster up to here.
-constexpr long long kClusterBlocks = 512;
+// One CTA does all up to here, a block a warp.  us on the device in one launch and in two, of which the second costs the host 2.5: 128
+// tokens 4.2 and 4.0, 1,024 4.5 and 4.3, 4,096 6.0 and 4.4.  (One cluster of eight CTAs: 16,384 tokens 6.1 and 4.5, 65,536 8.9 and
+// 4.8.)
+constexpr long long kOneCtaBlocks = THREADS / 32;
 
 }  // namespace
 
 int policy_fwd(const PolicyArgs& a, const PolicyOut& out, void* scratch, int num_sms, cudaStream_t st) {
   if (a.T < 0 || a.blocks < 0 || a.blocks > INT32_MAX / 128 || (a.table != nullptr && a.T > kMaxPackedTokens)) return -1;
   Sums* const sums = static_cast<Sums*>(scratch);
-  if (a.blocks <= kClusterBlocks) {
-    cudaLaunchConfig_t cfg = {};
-    const int ctas = a.blocks <= THREADS / 32 ? 1 : CLUSTER;
-    cfg.gridDim = ctas;
-    cfg.blockDim = THREADS;
-    cfg.stream = st;
-    cudaLaunchAttribute attrs[2];
-    attrs[0].id = cudaLaunchAttributeClusterDimension;
-    attrs[0].val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
-    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attrs[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attrs;
-    cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, policy_cluster_kernel, a, out, sums);
+  if (a.blocks <= kOneCtaBlocks) {
+    launch_overlapped(policy_one_kernel, 1, THREADS, 0, st, a, out, sums);
     return cudaGetLastError() == cudaSuccess ? 0 : -3;
   }
   const long long ctas = (a.blocks + 7) / 8;

@@ -1,6 +1,6 @@
 """Clipped policy loss with a KL term, on the log probabilities that ``token_logprobs`` gives.
 
-``csrc/policy.cu`` has the formulas; one launch forward for up to 65,536 tokens, two above, one backward.
+``csrc/policy.cu`` has the formulas; one launch forward for up to 4,096 tokens, two above, one backward.
 """
 from __future__ import annotations
 

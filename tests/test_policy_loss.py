@@ -104,8 +104,8 @@ def test_loss_and_gradient(T, lens, kl_coef, device):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,lens", [(65536, None), (65537, None), (70000, [30000, 1, 39000]), (66000, [100] * 650), (300000, None)])
-def test_both_sides_of_the_cluster_limit(T, lens):
+@pytest.mark.parametrize("T,lens", [(4096, None), (4097, None), (4000, [2000, 1, 1999]), (4096, [7] * 500), (65536, None), (70000, [30000, 1, 39000]), (66000, [100] * 650), (300000, None)])
+def test_both_sides_of_the_limit_of_one_launch(T, lens):
     new, old, adv, ref, mask = _inputs(T, "cuda", 1)
     s = None if lens is None else ops.pack_sequences(_offsets(lens), T, device="cuda")
     x = new.clone().requires_grad_(True)
