@@ -302,11 +302,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap, const __grid_constant_
       header.x = header.y = 0;
     }
     if (entry >= header.x) {
-      const long long rest = static_cast<long long>(T - header.y) * Hq * HD / 8;
+      const long long behind = static_cast<long long>(T - header.y) * Hq * HD / 8;
       uint4* const dst = reinterpret_cast<uint4*>(out + static_cast<long long>(header.y) * Hq * HD);
       const long long first = static_cast<long long>(blockIdx.x) - static_cast<long long>(header.x) * units;
       const long long ctas = static_cast<long long>(gridDim.x) - static_cast<long long>(header.x) * units;
-      for (long long i = first * FWD_THREADS + threadIdx.x; i < rest; i += ctas * FWD_THREADS) dst[i] = make_uint4(0, 0, 0, 0);
+      for (long long i = first * FWD_THREADS + threadIdx.x; i < behind; i += ctas * FWD_THREADS) dst[i] = make_uint4(0, 0, 0, 0);
       return;
     }
     g = u % Hkv;
@@ -780,7 +780,8 @@ attn_delta_packed_kernel(const __nv_bfloat16* __restrict__ o, const signed char*
       const long long at = (static_cast<long long>(e.tok0 + i) * Hq + h) * HD + 8 * lane;
       const uint4 a = *reinterpret_cast<const uint4*>(o + at);
       const uint4 b = *reinterpret_cast<const uint4*>(d_o + at);
-      const uint2 l = exact ? *reinterpret_cast<const uint2*>(rest + lost_at<HD>(e.place() + i, h, Hq, lane / 4) + lane % 4 * 8) : make_uint2(0, 0);
+      const uint2 l = exact ? *reinterpret_cast<const uint2*>(rest + lost_at<HD>(e.place() + i, h, Hq, lane / 4) + lane % 4 * 8)
+                            : make_uint2(0, 0);
       const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&a);
       const __nv_bfloat162* bp = reinterpret_cast<const __nv_bfloat162*>(&b);
       const uint32_t lw[2] = {l.x ^ 0x80808080u, l.y ^ 0x80808080u};

@@ -282,8 +282,8 @@ def packed_attention(qkv: Tensor, sequences: PackedSequences, Hq: int, Hkv: int,
     """Causal grouped-query attention within every sequence of a packed batch: ``qkv`` [tokens, (Hq + 2 Hkv) * hd] -> [tokens, Hq *
     hd].  Rows behind the last sequence give zeros and get a gradient of zero, whatever stands in them.
 
-    bf16 and heads of 64 or 128 on a GPU.  What stands in one sequence, infinities and NaN included, does not reach another.
-    The gradient has no derivative of its own.
+    bf16 and heads of 64 or 128 on a GPU; ``scale`` above 0.  What stands in one sequence, infinities and NaN included, does not reach
+    another.  The gradient has no derivative of its own; for it a byte an output is kept beside ``qkv`` and the output.
     """
     if qkv.dim() != 2 or qkv.shape[0] != sequences.tokens:
         raise ValueError(f"packed_attention: qkv is {tuple(qkv.shape)}, the batch has {sequences.tokens} tokens")
