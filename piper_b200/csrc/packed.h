@@ -9,8 +9,9 @@ namespace piper {
 constexpr int kMaxPackedTokens = 1 << 21;      // two counters per 128 of them fit the shared memory of a CTA
 
 // The table of a packed batch: [blocks + 1] rows of four ints.  Row 0: blocks in use, end of the last sequence, T, sequences
-// that have rows (whose first blocks come last).  Then, for every block of 128 rows of a sequence, those with most blocks in front of them first: first row of the sequence, its rows, place of the
-// block in the sequence, and 128 times the number of blocks of the sequences before (where lse and the like of it begin).
+// that have rows (whose first blocks come last).  Then, for every block of 128 rows of a sequence, those with most blocks in front of
+// them first: first row of the sequence, its rows, place of the block in the sequence, and 128 times the number of blocks of the
+// sequences before (where lse and the like of it begin).
 // own, unless null: neighbouring sequences that fit one block together count as one sequence, a group, with kGroup added to the
 // fourth number, and of row i of a group own [blocks * 128][2] has the first and last row of its sequence in the group, at the place that
 // lse begins at plus i.  Groups are formed within kGroupChunks parts of the sequences, of group_chunk(n) each.

@@ -48,7 +48,7 @@ class Qwen3Config:
     router_jitter_std: float = 0.0
     fp8: bool = False               # projections of attention and of dense MLPs in 8 bits, see nn.Linear
     # Weight of every layer's balance loss beside the model's own loss, in its gradients alone: the loss that is returned does
-    # not contain it.  0 leaves it out.
+    # not contain it, and factors of that loss (of a microbatch's share, say) do not apply to it.  0 leaves it out.
     balance_coef: float = 0.0
 
 

@@ -210,8 +210,8 @@ def moe_balance_loss(logits: Tensor, idx: Tensor, *, mask: Optional[Tensor] = No
 
 @custom_op("piper::moe_attach_loss")
 def moe_attach_loss(weights: Tensor, loss: Tensor, coef: float) -> Tensor:
-    """The routing weights as they are; in the backward pass ``loss`` gets the gradient ``coef``, as if coef x loss had been added to
-    what the pass began with.  So a stage's auxiliary loss need not travel to the last stage."""
+    """The routing weights as they are; in a backward pass that reaches them ``loss`` gets the gradient ``coef``, as if coef x loss had
+    been added to what the pass began with, whatever factor that had.  So a stage's auxiliary loss need not travel to the last stage."""
     return weights.clone()
 
 

@@ -211,8 +211,8 @@ def _heads(x: Tensor, Hq: int, Hkv: int, hd: int) -> tuple[Tensor, Tensor, Tenso
 @custom_op("piper::packed_attention_fwd")
 def packed_attention_fwd(qkv: Tensor, tiles: Tensor, own: Optional[Tensor], longest: int, work: int, Hq: int, Hkv: int, hd: int,
                          scale: float, keep: bool) -> tuple[Tensor, Tensor, Tensor]:
-    """qkv [T, (Hq + 2 Hkv) * hd] -> (out [T, Hq * hd], lse [Hq, 128 * blocks], by the blocks of the tiles, and, if ``keep`` and on a
-    GPU, what rounding has taken from out, int8 [128 * blocks, Hq * hd] in the kernels' own order).  The formula keeps it."""
+    """qkv [T, (Hq + 2 Hkv) * hd] -> (out [T, Hq * hd], lse [Hq, 128 * blocks], by the blocks of the tiles, and, if ``keep``, what
+    rounding has taken from out, int8 [128 * blocks, Hq * hd] in the kernels' own order, which only they use).  The formula keeps it."""
     T, padded = qkv.shape[0], (tiles.shape[0] - 1) * BLOCK
     if _is_native(qkv):
         _require_bf16(qkv)
@@ -226,7 +226,7 @@ def packed_attention_fwd(qkv: Tensor, tiles: Tensor, own: Optional[Tensor], long
     for a, n, at in _sequences(tiles, own):
         o, lse[:, at:at + n] = _attention_ref(*_heads(qkv[a:a + n], Hq, Hkv, hd), scale)
         out[a:a + n] = o.transpose(0, 1).reshape(n, Hq * hd).to(qkv.dtype)
-    return out, lse, torch.empty((0, Hq * hd), dtype=torch.int8)
+    return out, lse, torch.zeros((padded if keep else 0, Hq * hd), dtype=torch.int8)
 
 
 def _aligned(t: Tensor) -> Tensor:

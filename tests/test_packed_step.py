@@ -264,3 +264,25 @@ def test_under_recomputing_checkpoints(device):
             t.grad = None
         out.backward()
         assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("grouped", [False, True])
+def test_ops_keep_to_their_schemas(grouped, device):
+    """Schemas, fake bodies and registrations of the ops, as the dispatcher's own check sees them."""
+    from piper_b200.ops import packed
+    offsets = torch.tensor([0, 3, 9], dtype=torch.int32).to(device)
+    tiles, own = packed.pack_table(offsets, 12, 3, grouped)
+    g = torch.Generator().manual_seed(8)
+    qkv, new, old, adv, logits = (torch.randn(*shape, generator=g).to(device) for shape in ((12, 256), (12,), (12,), (12,), (12, 4)))
+    qkv = qkv.to(torch.bfloat16).requires_grad_(True)
+    idx = torch.zeros(12, 2, dtype=torch.int32, device=device)
+    weights, loss = (torch.ones(shape, device=device, requires_grad=True) for shape in ((3, 2), ()))
+    calls = [(torch.ops.piper.packed_attention_fwd, (qkv, tiles, own if grouped else None, 1, 2, 2, 1, 64, 0.3, grouped)),
+             (torch.ops.piper.clipped_policy_fwd, (new.requires_grad_(True), old, adv, old, adv > 0, None if grouped else tiles, 0.8, 1.2, 0.1)),
+             (torch.ops.piper.moe_balance_fwd, (logits.requires_grad_(True), idx, adv > 0 if grouped else None)),
+             (torch.ops.piper.moe_attach_loss, (weights, loss, 0.5))]
+    if device == "cpu":                          # on a GPU rows of the table's memory that are not in use are not written
+        calls.append((torch.ops.piper.pack_table, (offsets, 12, 3, grouped)))
+    for op, args in calls:
+        torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))

@@ -157,7 +157,7 @@ def test_nothing_counts(T, device):
 
 @pytest.mark.parametrize("device", DEVICES)
 def test_borders_and_extremes(device):
-    """A ratio at a border by fp32 rounding is judged by its exact difference; ratios that overflow are clipped or infinite."""
+    """A ratio at a border by fp32 rounding goes by its exact difference; ratios that overflow are clipped or infinite."""
     high, low = math.log(1.2), math.log(0.8)
     old = torch.tensor([-2.0, -2.0, -2.0, -2.0, -300.0, -300.0, -1.0, -1.0, -100.0])
     new = torch.tensor([0.0] * 9)
