@@ -175,7 +175,7 @@ class PiperQwen3Model(nn.Module):
         h = delta = out = None
         jitter = counted = None
         if self.use_jitter and sequences is not None:
-            jitter = self.router_jitter[sequences.positions().clamp(max=self.router_jitter.shape[0] - 1)]
+            jitter = self.router_jitter[sequences.positions().clamp(0, self.router_jitter.shape[0] - 1)]
         elif self.use_jitter:
             jitter = self.router_jitter if batch == 1 else self.router_jitter.repeat(batch, 1)
         if sequences is not None and self.cfg.balance_coef:

@@ -85,8 +85,8 @@ def packed_rope(cos: torch.Tensor, sin: torch.Tensor, sequences: ops.PackedSeque
     """Rows of the rotary tables for the tokens of a packed batch, whose positions begin with their sequence.  Tokens that the tables
     have no row for get NaN, not some other position."""
     at = sequences.positions()
-    beyond = (at >= cos.shape[0]).unsqueeze(1)
-    at = at.clamp(max=cos.shape[0] - 1)
+    beyond = ((at < 0) | (at >= cos.shape[0])).unsqueeze(1)
+    at = at.clamp(0, cos.shape[0] - 1)
     return cos[at].masked_fill(beyond, math.nan), sin[at].masked_fill(beyond, math.nan)
 
 

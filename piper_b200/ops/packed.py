@@ -41,7 +41,8 @@ class PackedSequences(NamedTuple):
 
     def inside(self) -> Tensor:
         """bool [tokens]: whether a token belongs to a sequence."""
-        return torch.arange(self.tokens, device=self.offsets.device) < self.offsets[-1]
+        # by the table, where all is behind the last sequence if offsets on a GPU do not rise from 0 to at most `tokens`
+        return torch.arange(self.tokens, device=self.offsets.device) < self.table[0, 1]
 
     def positions(self) -> Tensor:
         """int64 [tokens]: a token's place in its sequence, 0 behind the last one."""

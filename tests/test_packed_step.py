@@ -286,3 +286,59 @@ def test_ops_keep_to_their_schemas(grouped, device):
         calls.append((torch.ops.piper.pack_table, (offsets, 12, 3, grouped)))
     for op, args in calls:
         torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+
+
+def _empty_for(offsets, tokens):
+    """The layout that a GPU gives for offsets which do not rise from 0 to at most ``tokens``: their batch counts as empty."""
+    from piper_b200.ops import packed
+    s = ops.pack_sequences(torch.tensor([0, tokens]), tokens)
+    return s._replace(offsets=torch.tensor(offsets, dtype=torch.int32), table=packed._table_ref([0, 0], tokens, 3))
+
+
+BAD_OFFSETS = [[1000, 1100], [5, 300], [0, 300, 200], [0, 301], [0, -5, 3], [-40, 300]]
+
+
+@pytest.mark.parametrize("offsets", BAD_OFFSETS)
+def test_bad_offsets_look_up_nothing_out_of_range(offsets):
+    """No token of such a batch belongs to a sequence; each has position 0, so all tables have a row for it."""
+    s = _empty_for(offsets, 300)
+    assert not bool(s.inside().any()) and not bool(s.positions().any())
+    cos, sin = ops.rope_tables(64, 100, 10000.0, "cpu")
+    c, d = nn.packed_rope(cos, sin, s)
+    assert torch.equal(c, cos[:1].expand(300, -1)) and torch.equal(d, sin[:1].expand(300, -1))
+
+
+@pytest.mark.parametrize("offsets", [[5, 300], [1000, 1100]])
+def test_positions_below_zero_are_nan(offsets):
+    """A table that calls tokens in front of the first offset its own: no row of the rotary tables is theirs, from the end neither."""
+    s = ops.pack_sequences(torch.tensor([0, 300]), 300)._replace(offsets=torch.tensor(offsets, dtype=torch.int32))
+    cos, sin = ops.rope_tables(64, 400, 10000.0, "cpu")
+    c, d = nn.packed_rope(cos, sin, s)
+    first = min(offsets[0], 300)
+    assert bool(torch.isnan(c[:first]).all()) and bool(torch.isnan(d[:first]).all())
+    assert torch.equal(c[first:], cos[:300 - first]) and torch.equal(d[first:], sin[:300 - first])
+
+
+@pytest.mark.parametrize("kind", ["llama", "qwen"])
+def test_a_model_takes_bad_offsets_as_an_empty_batch(kind):
+    model = _model(kind, "cpu", balance_coef=0.5)
+    if kind == "qwen":
+        model.use_jitter, model.router_jitter = True, torch.randn(160, 8)
+    tokens = torch.zeros(1, 300, dtype=torch.int64)
+    for bad in (_empty_for([1000, 1100], 300),
+                ops.pack_sequences(torch.tensor([0, 300]), 300)._replace(offsets=torch.tensor([1000, 1100], dtype=torch.int32))):
+        assert model(tokens, bad).shape == (1, 300, VOCAB)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offsets", BAD_OFFSETS)
+def test_a_model_takes_bad_offsets_on_the_gpu_as_an_empty_batch(offsets):
+    model = _model("qwen", "cuda", balance_coef=0.5)
+    s = ops.pack_sequences(torch.tensor(offsets, device="cuda"), 300)
+    assert not bool(s.inside().any()) and not bool(s.positions().any())
+    tokens = torch.zeros(1, 300, dtype=torch.int64, device="cuda")
+    logits = model(tokens, s)
+    assert bool(torch.isfinite(logits.float()).all())
+    with pytest.raises(native.PiperKernelError):
+        native.check_status()
+    native.check_status()
