@@ -223,28 +223,33 @@ __device__ void add_blocks(const PolicyArgs& a, const int4* table, const Sums* s
   out.weight[0] = static_cast<float>(1. / n);
 }
 
+// The table is read by __ldg, often right behind the launch that writes it: by the pointer that comes out of the wait alone.
+__device__ __forceinline__ const int4* begin_with_table(const PolicyArgs& a) {
+  const int4* table = reinterpret_cast<const int4*>(a.table);
+  grid_begin(table);
+  return a.table == nullptr ? nullptr : table;
+}
+
 __global__ void __launch_bounds__(THREADS) policy_one_kernel(const PolicyArgs a, const PolicyOut out, Sums* sums) {
-  grid_begin();
-  const int4* const table = reinterpret_cast<const int4*>(a.table);
+  const int4* const table = begin_with_table(a);
   sum_blocks(a, table, sums);
   __syncthreads();
   add_blocks(a, table, sums, out);
 }
 
 __global__ void __launch_bounds__(256) policy_sums_kernel(const PolicyArgs a, Sums* sums) {
-  grid_begin();
-  sum_blocks(a, reinterpret_cast<const int4*>(a.table), sums);
+  const int4* const table = begin_with_table(a);
+  sum_blocks(a, table, sums);
 }
 
 __global__ void __launch_bounds__(THREADS) policy_add_kernel(const PolicyArgs a, const PolicyOut out, Sums* sums) {
-  grid_begin();
-  add_blocks(a, reinterpret_cast<const int4*>(a.table), sums, out);
+  const int4* const table = begin_with_table(a);
+  add_blocks(a, table, sums, out);
 }
 
 __global__ void __launch_bounds__(256) policy_bwd_kernel(const PolicyArgs a, const float* weight, const float* d_loss,
                                                          float* d) {
-  grid_begin();
-  const int4* const table = reinterpret_cast<const int4*>(a.table);
+  const int4* const table = begin_with_table(a);
   const int lane = threadIdx.x & 31;
   const long long used = blocks_in_use(a, table), warps = static_cast<long long>(gridDim.x) * (blockDim.x / 32);
   const float up = *d_loss * weight[0];
