@@ -32,9 +32,9 @@ struct Token {
   bool clipped;
 };
 
-// e^u - 1 - u.  The series' next term is below 2^-26 of the sum where |u| < 0.5.
+// e^u - 1 - u.  The series' next term is below 2^-26 of the sum where |u| < 0.5.  At u = inf the difference would be NaN.
 __device__ __forceinline__ float exp_behind_linear(float u, float em1) {
-  if (fabsf(u) >= 0.5f) return em1 - u;
+  if (fabsf(u) >= 0.5f) return em1 == INFINITY ? em1 : em1 - u;
   float s = 1.f / 362880.f;
   s = fmaf(s, u, 1.f / 40320.f);
   s = fmaf(s, u, 1.f / 5040.f);

@@ -37,7 +37,7 @@ def _tokens_ref(logprob, old, adv, ref, low, high, kl_coef):
     if ref is not None:
         u = ref.double() - logprob.double()
         em1 = torch.expm1(u)
-        kl = torch.where(u.abs() < 1e-3, u * u * (0.5 + u * (1 / 6 + u / 24)), em1 - u)
+        kl = torch.where(u.abs() < 1e-3, u * u * (0.5 + u * (1 / 6 + u / 24)), torch.where(em1 == math.inf, em1, em1 - u))
         if kl_coef:
             loss, grad = loss + kl_coef * kl, grad - kl_coef * em1
     return loss, kl, grad, clipped

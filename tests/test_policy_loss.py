@@ -324,3 +324,31 @@ def test_from_logits(device):
     size = (want[3].abs() + 2.0 ** -23 * want[6]).unsqueeze(1) * (onehot + z.exp()) / 0.8
     off = (d.double().cpu().view(80, 97) - grad).abs()
     assert bool((off <= half * grad.abs() + 2.0 ** -18 * size + 1e-30).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens", [None, [2, 1]])
+def test_divergences_without_bound(lens, device):
+    """A token that counts and whose log probability is -inf, as a masked id's, is infinitely far from a reference that gives it one, not NaN."""
+    old, ref = torch.tensor([-1.0, -2.0, -3.0], device=device), torch.tensor([-1.5, -2.0, -2.5], device=device)
+    adv = torch.tensor([1.0, 0.0, -1.0], device=device)
+    s = None if lens is None else ops.pack_sequences(_offsets(lens), 3, device=device)
+    for at, value, grad in ((0, -INF, -INF), (1, -INF, -INF), (2, -INF, -INF), (0, INF, None), (1, INF, None)):
+        x, y = old.clone(), ref.clone()
+        if grad is None:                          # a reference of -inf: u = -inf, whose gradient is that of -u
+            y[at] = -INF
+        else:
+            x[at] = value
+        x.requires_grad_(True)
+        for kl_coef in (0.5, 0.0):
+            r = ops.clipped_policy_loss(x, old, adv, ref_logprob=y, sequences=s, kl_coef=kl_coef)
+            (d,) = torch.autograd.grad(r.loss, x)
+            assert float(r.kl) == INF
+            assert float(r.loss) == INF if kl_coef else math.isfinite(float(r.loss))
+            assert bool(torch.isfinite(d[torch.arange(3, device=device) != at]).all())
+            if kl_coef and grad is not None:
+                assert float(d[at]) == grad
+            else:
+                assert math.isfinite(float(d[at]))
+    if device == "cuda":
+        native.check_status()
