@@ -50,7 +50,7 @@ __device__ __forceinline__ Token token(const PolicyArgs& a, float logprob, float
   Token t = {0.f, 0.f, 0.f, false};
   if (adv != 0.f) {                            // or a NaN
     const double d = static_cast<double>(logprob) - static_cast<double>(old);
-    t.clipped = adv > 0.f ? d > a.log_high : d < a.log_low;
+    t.clipped = adv > 0.f ? d > a.log_high : adv < 0.f && d < a.log_low;      // a NaN has no border
     const float r = expf(static_cast<float>(d));
     t.loss = -adv * (t.clipped ? (adv > 0.f ? a.high : a.low) : r);
     t.grad = t.clipped ? 0.f : t.loss;

@@ -352,3 +352,20 @@ def test_divergences_without_bound(lens, device):
                 assert math.isfinite(float(d[at]))
     if device == "cuda":
         native.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("diff", [-1.0, 0.0, 1.0])
+def test_advantages_that_are_nan_leave_a_trace(diff, device):
+    """Below, between and above the borders: the loss and the token's gradient are NaN, and no border is its."""
+    old = torch.tensor([-2.0, -2.0, -2.0], device=device)
+    new = old + torch.tensor([0.1, diff, 0.1], device=device)
+    adv = torch.tensor([1.0, NAN, -1.0], device=device)
+    x = new.requires_grad_(True)
+    r = ops.clipped_policy_loss(x, old, adv)
+    (d,) = torch.autograd.grad(r.loss, x)
+    assert torch.isnan(r.loss) and torch.isnan(d).tolist() == [False, True, False] and float(r.clipped) == 0
+    on = torch.tensor([True, False, True], device=device)
+    r = ops.clipped_policy_loss(x, old, adv, mask=on)         # nor where the token does not count
+    (d,) = torch.autograd.grad(r.loss, x)
+    assert torch.isfinite(r.loss) and float(d[1]) == 0 and bool(torch.isfinite(d).all())
