@@ -296,7 +296,9 @@ int policy_fwd(const PolicyArgs& a, const PolicyOut& out, void* scratch, int num
 int policy_bwd(const PolicyArgs& a, const float* weight, const float* d_loss, float* d, int num_sms, cudaStream_t st) {
   if (a.T < 0 || a.blocks < 0 || a.blocks > INT32_MAX / 128 || (a.table != nullptr && a.T > kMaxPackedTokens)) return -1;
   if (a.T == 0) return 0;
-  const long long ctas = (a.T + 1023) / 1024;
+  // A warp for every block, of which short sequences have more than their tokens say (600 tokens in 500 sequences: CTAs by tokens
+  // 44 us, by blocks 2.3), and for every 128 tokens behind the last sequence.
+  const long long of_tokens = (a.T + 127) / 128, ctas = ((a.blocks > of_tokens ? a.blocks : of_tokens) + 7) / 8;
   launch_overlapped(policy_bwd_kernel, static_cast<unsigned>(ctas < 8ll * num_sms ? ctas : 8ll * num_sms), 256, 0, st, a, weight, d_loss,
                     d);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;

@@ -369,3 +369,27 @@ def test_advantages_that_are_nan_leave_a_trace(diff, device):
     r = ops.clipped_policy_loss(x, old, adv, mask=on)         # nor where the token does not count
     (d,) = torch.autograd.grad(r.loss, x)
     assert torch.isfinite(r.loss) and float(d[1]) == 0 and bool(torch.isfinite(d).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,lens", [(600, [1, 2, 0, 1] * 125), (700, [3] * 40 + [580]), (9000, None)])
+def test_the_gradient_has_a_warp_for_every_block(T, lens, tmp_path):
+    """Blocks are of 128 tokens or, in a packed batch, of a sequence: many short ones are more than their tokens would say."""
+    import json
+    new, old, adv, ref, mask = _inputs(T, "cuda", 10)
+    s = None if lens is None else ops.pack_sequences(_offsets(lens), T, device="cuda")
+    blocks = (T + 127) // 128 if lens is None else sum((n + 127) // 128 for n in lens)
+    x = new.requires_grad_(True)
+
+    def step():
+        r = ops.clipped_policy_loss(x, old, adv, ref_logprob=ref, mask=mask, sequences=s, kl_coef=0.05)
+        return r, torch.autograd.grad(r.loss, x)[0]
+
+    _check(*step(), _definition(new, old, adv, ref, mask, lens, (0.2, 0.2), 0.05))
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        step()
+        torch.cuda.synchronize()
+    prof.export_chrome_trace(str(tmp_path / "trace.json"))
+    grids = [e["args"]["grid"][0] for e in json.loads((tmp_path / "trace.json").read_text())["traceEvents"]
+             if e.get("cat") == "kernel" and "policy_bwd" in e["name"]]
+    assert grids and all(8 * g >= blocks for g in grids)
