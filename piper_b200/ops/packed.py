@@ -165,9 +165,8 @@ def pack_sequences(offsets: Tensor, tokens: int, device: Optional[torch.device] 
         tiles = min(blocks, 3 * tokens // BLOCK + 33)
         longest = _blocks(-(-tokens // max(n, 1)))
         work, tile_work = (min(max(n, 1), b) * longest * (longest + 1) // 2 for b in (blocks, tiles))
-        if offsets.dtype != torch.int32:     # what does not fit becomes an offset that is refused
-            offsets = offsets.clamp(-1, (1 << 31) - 1).to(torch.int32)
-    offsets = offsets.contiguous()
+        # a copy: the caller may fill the same buffer for the next batch; what does not fit becomes an offset that is refused
+        offsets = offsets.clamp(-1, (1 << 31) - 1).to(torch.int32).contiguous()
     pair = pack_table(offsets, tokens, tiles, True) if grouped else (None, None)
     return PackedSequences(offsets, pack_table(offsets, tokens, blocks, False)[0], *pair, tokens, longest, work, tile_work)
 

@@ -493,3 +493,15 @@ def test_attention_gradient_against_differences():
 
 def test_reference_table_is_the_ops():
     assert torch.equal(_table_ref([0, 130, 135], 140, 4)[:4], ops.pack_sequences(torch.tensor([0, 130, 135]), 140).table)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_a_layout_keeps_the_offsets_that_it_was_made_of(dtype, device):
+    """A program that fills the same buffer for its next batch changes nothing of this one."""
+    offsets = torch.tensor([0, 3, 10], dtype=dtype, device=device)
+    s = ops.pack_sequences(offsets, 12)
+    positions, inside = s.positions(), s.inside()
+    offsets.copy_(torch.tensor([0, 7, 12]))
+    assert torch.equal(s.positions(), positions) and torch.equal(s.inside(), inside)
+    assert s.positions().tolist() == [0, 1, 2, 0, 1, 2, 3, 4, 5, 6, 0, 0]
