@@ -1085,6 +1085,12 @@ __device__ __forceinline__ void attn_dkv_cta(const CUtensorMap* tmap_qkv_x, cons
           for (int i = 0; i < 16; ++i)
             if (xpos + 16 * h + 8 * ((i >> 1) & 1) > ypos0 + 8 * (i >> 2) + c0 + (i & 1)) sv[h][i] = 0xff800000u;
       }
+      // Queries behind the sequence: zeros, whose score with a key that is infinite is NaN.
+      if (PACKED && ypos0 + 32 > e.len) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (ypos0 + 8 * (i >> 2) + c0 + (i & 1) >= e.len) sv[0][i] = sv[1][i] = 0xff800000u;
+      }
       if (GROUPS && e.group()) {               // queries behind the key's own sequence
 #pragma unroll
         for (int h = 0; h < 2; ++h) {

@@ -505,3 +505,33 @@ def test_a_layout_keeps_the_offsets_that_it_was_made_of(dtype, device):
     offsets.copy_(torch.tensor([0, 7, 12]))
     assert torch.equal(s.positions(), positions) and torch.equal(s.inside(), inside)
     assert s.positions().tolist() == [0, 1, 2, 0, 1, 2, 3, 4, 5, 6, 0, 0]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("grouped", [False, True])
+@pytest.mark.parametrize("lens", [[64], [70], [128, 3], [333, 20, 30], [1, 200, 5]], ids=str)
+def test_keys_that_no_query_sees_by_their_scores(lens, grouped, hd, device, monkeypatch):
+    """A key of -inf where all queries are positive has probabilities of 0: outputs and the gradients of keys and values are those
+    beside a key whose scores are so far down that its probabilities are 0 too, whatever the sequence's length."""
+    if device == "cpu" and hd != 64:
+        pytest.skip("one of them on the CPU")
+    Hq, Hkv, T = 4, 2, sum(lens)
+    if grouped:
+        monkeypatch.setattr(packed, "GROUP_GAIN", 0.0)
+        monkeypatch.setattr(packed, "GROUP_BLOCKS", 0)
+    s = ops.pack_sequences(_offsets(lens), T, device=device)
+    qkv, dout = _inputs(T, Hq, Hkv, hd, device, 11)
+    x = qkv.view(T, Hq + 2 * Hkv, hd)
+    x[:, :Hq, 0] = x[:, :Hq, 0].abs() + 1
+    at = _offsets(lens).tolist()
+    results = []
+    for value in (-float("inf"), -2.0 ** 16):                # at most -2^16 / 2^4 beside scores below 2^7
+        for a, b in zip(at, at[1:]):
+            if b - a > 5:                                    # not the first key, which is all that the first query has
+                x[a + 5, Hq:Hq + Hkv, 0] = value
+        out, d = _pass(qkv, dout, s, Hq, Hkv, hd)
+        results.append((out, d.view(T, Hq + 2 * Hkv, hd)[:, Hq:]))
+    (out, d), (want, dwant) = results
+    assert bool(torch.isfinite(out.float()).all()) and bool(torch.isfinite(d.float()).all())
+    assert torch.equal(out, want) and torch.equal(d, dwant)
