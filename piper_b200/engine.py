@@ -27,6 +27,7 @@ import torch.distributed as dist
 from . import api
 from .compiler.dag import RECV, SEND, TrainingDAG
 from .compiler.schedule import derive_schedule_info, load_schedule_directives, stage_device_map
+from .ops import PackedSequences
 from .runtime.actor import PiperActor
 from .runtime.layout import ProcessGroups, RankLayout, init_distributed, make_layout
 from .runtime.storage import AdamConfig
@@ -120,6 +121,12 @@ def _adam_config(optim_fn, optim_kwargs: Optional[dict]) -> AdamConfig:
     return cfg
 
 
+def _check_inputs(inputs) -> None:
+    """Stages are traced without data, and microbatches are rows of the inputs: a packed batch's layout is neither traced nor cut."""
+    if any(isinstance(t, PackedSequences) for t in inputs or []):
+        raise TypeError("the layout of a packed batch (ops.pack_sequences) is no input of a pipeline's stages; call the model itself with it")
+
+
 def piper_setup(model_class, model_args=(), model_kwargs: Optional[dict] = None, optim_fn=None,
                 example_inputs: Optional[list] = None, example_outputs=None, activation_checkpointing: bool = False,
                 num_checkpoints: int = 1, model_dtype: torch.dtype = torch.bfloat16, use_inductor: bool = False,
@@ -139,6 +146,7 @@ def piper_setup(model_class, model_args=(), model_kwargs: Optional[dict] = None,
     per-actor ``runtime_env``, ``src/actor.py:57-64``); here it only checks that the process is being profiled.
     """
     del pg, temp_dir, pp_outer
+    _check_inputs(example_inputs)
     if nsight and not os.environ.get("NSYS_PROFILING_SESSION_ID"):
         logger.warning("nsight=True but this process does not run under nsys: start the job through "
                        "Coordinator(nsight=True) or the harness's --nsight")
@@ -255,6 +263,7 @@ def piper_exec_dag(loss_fn: Callable, log_stats: bool = False, step_timeout: Opt
     actors = piper_metadata.actors
     if not actors:
         raise RuntimeError("piper_exec_dag called before piper_setup")
+    _check_inputs(inputs)
     t0 = time.perf_counter()
     results: list = []
     for actor in actors.values():

@@ -342,3 +342,23 @@ def test_a_model_takes_bad_offsets_on_the_gpu_as_an_empty_batch(offsets):
     with pytest.raises(native.PiperKernelError):
         native.check_status()
     native.check_status()
+
+
+def test_the_engine_refuses_layouts_of_packed_batches():
+    """Stages are traced without data and batches cut into microbatches by rows: a layout is refused by name in front of both."""
+    from piper_b200 import piper_exec_dag, piper_setup
+    from piper_b200.models.llama3 import LlamaConfig, Transformer
+    cfg = LlamaConfig(dim=64, n_layers=2, n_heads=2, n_kv_heads=1, vocab_size=VOCAB, ffn_hidden=64, rope_theta=10000.0)
+    tokens, _offsets, s = _batch("cpu")
+    schedule = [{"op": "place", "filter": {"PP": 0}, "devices": [0]}, {"op": "split", "filter": {}, "dim_name": "MB", "num_microbatches": 1}]
+
+    def setup(inputs):
+        return piper_setup(Transformer, (cfg, T, 1), optim_fn=torch.optim.AdamW, example_inputs=inputs, example_outputs=tokens, device="cpu",
+                           model_dtype=torch.float32, const_attrs=Transformer.const_attrs(cfg, T), schedule_directives=schedule)
+
+    with pytest.raises(TypeError, match="packed batch"):
+        setup([tokens, s])
+    setup([tokens])
+    with pytest.raises(TypeError, match="packed batch"):
+        piper_exec_dag(nn.cross_entropy_loss, inputs=[tokens, s])
+    assert len(piper_exec_dag(nn.cross_entropy_loss, inputs=[tokens])) == 1
