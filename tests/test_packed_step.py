@@ -362,3 +362,29 @@ def test_the_engine_refuses_layouts_of_packed_batches():
     with pytest.raises(TypeError, match="packed batch"):
         piper_exec_dag(nn.cross_entropy_loss, inputs=[tokens, s])
     assert len(piper_exec_dag(nn.cross_entropy_loss, inputs=[tokens])) == 1
+
+
+@pytest.mark.gpu
+def test_packed_sequences_are_sequences_by_themselves_on_the_gpu():
+    """As on the CPU, in bf16: one by one, as batches of their own, the sequences give the same logits and sums of gradients, but for roundings.
+
+    A layer rounds some 9 times on the way (norms, projections, rotations, attention, its probabilities, SwiGLU, sums) and twice as often
+    on the way back, both passes do, and what a norm or an attention makes of an error is no larger relative to its size: of two layers
+    and the head by norms 2 x 20 x 2^-8 forward, three times that for gradients.  Another position, neighbour or mask is off by its own size."""
+    model = _model("llama", "cuda")
+    tokens, offsets, s = _batch("cuda")
+    up = torch.randn(T, VOCAB, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    up[sum(LENS):] = 0
+    params = list(model.parameters())
+    out = model(tokens, s).view(T, VOCAB)
+    grads = torch.autograd.grad(out, params, up)
+    sums = [torch.zeros_like(p, dtype=torch.float32) for p in params]
+    bound = 2 * 20 * 2.0 ** -8
+    for a, b in zip(offsets.tolist(), offsets.tolist()[1:]):
+        o = model(tokens[:, a:b], ops.pack_sequences(torch.tensor([0, b - a]), b - a, device="cuda")).view(b - a, VOCAB)
+        assert float((o - out[a:b]).float().norm()) <= bound * float(o.float().norm())
+        for acc, d in zip(sums, torch.autograd.grad(o, params, up[a:b])):
+            acc += d
+    for (name, _p), got, want in zip(model.named_parameters(), grads, sums):
+        assert float((got.float() - want).norm()) <= 3 * bound * float(want.norm()), name
+    native.check_status()
