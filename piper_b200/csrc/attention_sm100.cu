@@ -1730,7 +1730,8 @@ static int set_smem_here(K kern, int bytes, std::atomic<bool>* configured) {
 }
 
 // The same costs as above, for `blocks` blocks of 128 rows, the longest sequence of `longest` blocks and `work` pairs of a query
-// and a key block.
+// and a key block.  Two tiles are two heads of a group on the same rows; without groups of heads there is no second one, and pairs of
+// neighbouring query blocks, as equal sequences have them, are not built.
 static int packed_tiles_per_cta(const PackedShape& p, int num_sms) {
   const long long tiles = static_cast<long long>(p.Hq) * p.blocks;
   return p.Hq == p.Hkv || tiles <= num_sms || p.Hq * p.work <= (p.longest - 1) * num_sms ? 1 : 2;

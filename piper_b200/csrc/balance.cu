@@ -7,8 +7,9 @@
 // so a warp works on 256 / E rows at once, and each lane adds up the probabilities of its experts over its rows in fp32; choices are
 // counted in shared memory.  A CTA leaves its sums, one CTA adds those of all in a fixed order in 64 bits: behind a
 // cluster barrier where one cluster is enough for the rows, in a second launch otherwise.  Backward: the probabilities again, one
-// read and one write of the logits.  us on the device by ncu, cold: 16,384 x 128 bf16 8.3, 12 and 8 (0.7, 0 and 1.3 at the measured
-// bandwidth), 131,072 x 64 18, 10 and 16 (3.3, 0 and 5.1): launches and latencies, beside 66 us of the host.
+// read and one write of the logits.  us of the three kernels by themselves with cold caches (ncu): 16,384 x 128 bf16 8.4, 15.7 and 8.2
+// (0.7, 0 and 1.3 at the measured bandwidth), 131,072 x 64 18, 10 and 16 (3.3, 0 and 5.1); in a graph of 20 passes (launches overlap,
+// caches are warm) 15 forward and 6 backward, 19 and 13: launches and latencies, that of the one CTA that adds above all.
 #include "packed.h"
 
 #include "ptx.cuh"
@@ -260,8 +261,8 @@ bool takes(const BalanceArgs& a) {
   return a.E >= 1 && a.E <= kMaxBalanceExperts && a.k >= 1 && a.k <= a.E && a.T >= 0 && a.T * a.k <= INT32_MAX;
 }
 
-// Up to this many logits one cluster is enough.  us on the device as one cluster and in two launches, of which the second costs the
-// host 2.5: 512 x 8 7.1 and 7.4, 1,024 x 64 6.8 and 6.6, 2,048 x 64 8.6 and 7.0, 1,024 x 128 9.2 and 7.8.
+// Up to this many logits one cluster is enough.  us a pass in a graph of 20 as one cluster and in two launches, of which the second costs
+// the host 2.5: 512 x 8 7.1 and 7.4, 1,024 x 64 6.8 and 6.6, 2,048 x 64 8.6 and 7.0, 1,024 x 128 9.2 and 7.8.
 constexpr long long kClusterLogits = 1 << 16;
 
 long long row_ctas(long long T, int E) {

@@ -8,9 +8,9 @@
 // differences (the latter by its series near 0, where its terms cancel); sums are in 64 bits and in a fixed order.
 //
 // Some 20 bytes a token: bound by launches and latency.  One warp sums 128 tokens (of a block of the table, or just the next ones), one
-// CTA adds the blocks' sums, those of sequences first where there is a table.  us on the device, forward, without and with 1,000
-// tokens a sequence: 4,096 tokens 6.0 and 6.8 (one launch), 65,536 4.8 and 6.6, 131,072 5.3 and 8.7, of which the bytes are 0.4;
-// the gradient 4 to 7.
+// CTA adds the blocks' sums, those of sequences first where there is a table.  us a pass in a graph of 20 (launches overlap, caches are
+// warm), forward, without and with sequences of some 1,000 tokens: 1,024 tokens 3.8 and 4.7 (one launch), 65,536 4.8 and 6.7, 131,072 5.3
+// and 9.0, of which the bytes are 0.4; the gradient 2 to 4.  By itself and with cold caches (ncu) a launch takes 4 to 9.
 #include "packed.h"
 
 #include "ptx.cuh"
@@ -272,9 +272,9 @@ __global__ void __launch_bounds__(256) policy_bwd_kernel(const PolicyArgs a, con
     d[t] = 0.f;
 }
 
-// One CTA does all up to here, a block a warp.  us on the device in one launch and in two, of which the second costs the host 2.5: 128
-// tokens 4.2 and 4.0, 1,024 4.5 and 4.3, 4,096 6.0 and 4.4.  (One cluster of eight CTAs: 16,384 tokens 6.1 and 4.5, 65,536 8.9 and
-// 4.8.)
+// One CTA does all up to here, a block a warp.  us a pass in a graph of 20 in one launch and in two, of which the second costs the host
+// 2.5: 128 tokens 3.5 and 4.1, 1,024 3.8 and 4.4, 4,096 5.2 and 4.4.  (One cluster of eight CTAs: 16,384 tokens 6.1 and 4.5, 65,536 8.9
+// and 4.8.)
 constexpr long long kOneCtaBlocks = THREADS / 32;
 
 }  // namespace

@@ -283,7 +283,9 @@ def packed_attention(qkv: Tensor, sequences: PackedSequences, Hq: int, Hkv: int,
     hd].  Rows behind the last sequence give zeros and get a gradient of zero, whatever stands in them.
 
     bf16 and heads of 64 or 128 on a GPU; ``scale`` above 0.  What stands in one sequence, infinities and NaN included, does not reach
-    another.  The gradient has no derivative of its own; for it a byte an output is kept beside ``qkv`` and the output.
+    another.  The gradient has no derivative of its own; for it ``qkv``, the output, and a byte an output and a number a row and head are
+    kept, these two for whole blocks: by the batch's own number of them where the offsets were in host memory, by the most that
+    ``tokens`` rows in as many sequences can have where they were on a GPU.
     """
     if qkv.dim() != 2 or qkv.shape[0] != sequences.tokens:
         raise ValueError(f"packed_attention: qkv is {tuple(qkv.shape)}, the batch has {sequences.tokens} tokens")
