@@ -263,12 +263,13 @@ def piper_exec_dag(loss_fn: Callable, log_stats: bool = False, step_timeout: Opt
     actors = piper_metadata.actors
     if not actors:
         raise RuntimeError("piper_exec_dag called before piper_setup")
-    _check_inputs(inputs)
     t0 = time.perf_counter()
     results: list = []
     for actor in actors.values():
         if inputs is not None and actor.has_first_stage():
-            actor.load_input(list(inputs))
+            inputs = list(inputs)
+            _check_inputs(inputs)
+            actor.load_input(inputs)
         if labels is not None and actor.has_loss_stage():
             actor.load_labels(labels)
         if step_timeout is None:

@@ -388,3 +388,15 @@ def test_packed_sequences_are_sequences_by_themselves_on_the_gpu():
     for (name, _p), got, want in zip(model.named_parameters(), grads, sums):
         assert float((got.float() - want).norm()) <= 3 * bound * float(want.norm()), name
     native.check_status()
+
+
+def test_a_step_takes_its_inputs_from_an_iterator():
+    from piper_b200 import piper_exec_dag, piper_setup
+    from piper_b200.models.llama3 import LlamaConfig, Transformer
+    cfg = LlamaConfig(dim=64, n_layers=1, n_heads=2, n_kv_heads=1, vocab_size=VOCAB, ffn_hidden=64, rope_theta=10000.0)
+    tokens = torch.zeros(1, 128, dtype=torch.int64)
+    schedule = [{"op": "place", "filter": {"PP": 0}, "devices": [0]}, {"op": "split", "filter": {}, "dim_name": "MB", "num_microbatches": 1}]
+    piper_setup(Transformer, (cfg, 128, 1), optim_fn=torch.optim.AdamW, example_inputs=[tokens], example_outputs=tokens, device="cpu",
+                model_dtype=torch.float32, const_attrs=Transformer.const_attrs(cfg, 128), schedule_directives=schedule)
+    (first,) = piper_exec_dag(nn.cross_entropy_loss, inputs=iter([tokens + 1]))
+    assert bool(torch.isfinite(torch.as_tensor(first)).all())
